@@ -70,6 +70,21 @@ _SIGNATURES = {
     "dropkv_decode_attention": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
                                          _c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                                          _c_float, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_size, _c_vp]),
+    "dropkv_tree_workspace_bytes": (_c_size, [_c_i64] * 6),
+    "dropkv_tree_attention": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
+                                       _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64,
+                                       _c_vp, _c_i64, _c_i64, _c_i64, _c_int,
+                                       _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float,
+                                       _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_size, _c_vp]),
+    "dropkv_tree_commit": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp,
+                                    _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                    _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
+                                    _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp]),
+    "dropkv_norm_rope": (_c_int, [_c_vp] * 14 + [_c_int, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int,
+                                         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_vp]),
+    "dropkv_token_logprobs_workspace_bytes": (_c_size, [_c_i64] * 3),
+    "dropkv_token_logprobs": (_c_int, [_c_vp, _c_i64, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp,
+                                       _c_vp, _c_vp, _c_size, _c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -1,0 +1,274 @@
+// Queries and keys of new tokens made ready for the cache and the attention:
+// an RMS norm over each head (optional), the rotation by position, and K and V
+// stored where the caller keeps them, in one pass.  (The reference takes
+// rotated queries and keys from the model; patches/dropkv_transformers.patch:
+// 329-343.)
+//
+// For a head's row x of D values and the token's rows c, s of R values:
+//   y = x rsqrt(mean(x^2) + eps) w          (y = x without a weight)
+//   z_i       = y_i c_i - y_{i+R/2} s_i               i < R/2
+//   z_{i+R/2} = y_{i+R/2} c_{i+R/2} + y_i s_{i+R/2}
+//   z_i       = y_i                                   i >= R
+// in fp32, rounded once, at the store.
+//
+// Bound by memory: every row is read and written once.  A lane holds 8 values
+// of the first half and their partners of the second, so that a pair never
+// leaves the lane and the norm is a reduction over the row's D / 16 lanes.  A
+// wave takes several heads of one token, since c and s (as long as a row, and
+// in fp32 twice its bytes) are then loaded once for all of them.
+#include "dkv_common.h"
+#include "dkv_internal.h"
+
+#include <algorithm>
+
+namespace dkv {
+
+struct RopeArgs {
+  const void* src[3];  // q, k, v: row (b, h, l) at element b sb + h sh + l sl
+  void* dst[3];
+  int64_t s_sb[3], s_sh[3], s_sl[3], d_sb[3], d_sh[3], d_sl[3];
+  const void* w[2];  // norm weights of q and of k, or null
+  int w_f32;
+  const void* cos;  // row l of sequence b at element b c_sb + l c_sl; with positions, row `position` at position * c_sl
+  const void* sin;
+  int64_t c_sb, c_sl;
+  const int64_t* pos;
+  int64_t p_sb, P;
+  int L, Hq, Hk, Hv, D, R, tokens;
+  int per, chunks;  // heads (q, k and v, in that order) per wave; waves per token
+  float eps;
+};
+
+template <typename T>
+struct Vec8 {
+  T x[8];
+};
+
+template <typename T>
+__device__ __forceinline__ void load_vec8(const T* p, float* f) {
+  const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(__builtin_assume_aligned(p, 16));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(v.x[e]);
+}
+template <typename T>
+__device__ __forceinline__ void store_vec8(T* p, const float* f) {
+  Vec8<T> v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v.x[e] = static_cast<T>(f[e]);
+  *reinterpret_cast<Vec8<T>*>(__builtin_assume_aligned(p, 16)) = v;
+}
+
+// The token's row of the tables; false where its position is not in them.
+template <typename TC>
+__device__ __forceinline__ bool rope_row(const RopeArgs& a, int b, int l, const TC** c, const TC** s) {
+  int64_t off = (int64_t)b * a.c_sb + (int64_t)l * a.c_sl;
+  if (a.pos) {
+    const int64_t p = a.pos[(int64_t)b * a.p_sb + l];
+    if (p < 0 || p >= a.P) return false;
+    off = p * a.c_sl;
+  }
+  *c = static_cast<const TC*>(a.cos) + off;
+  *s = static_cast<const TC*>(a.sin) + off;
+  return true;
+}
+
+template <typename T, typename TC, int D>
+__global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
+  constexpr int LPR = D / 16, HPW = 64 / LPR;
+  const int wid = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+  const int token = wid / a.chunks, h0 = (wid - token * a.chunks) * a.per;
+  if (token >= a.tokens) return;
+  const int b = token / a.L, l = token - b * a.L;
+  const int c = lane % LPR;
+  const int R = a.R, pairs = R / 16;
+  // The lane's two runs of 8 values.
+  const bool turned = c < pairs;
+  const int i0 = turned ? 8 * c : R + 16 * (c - pairs), i1 = turned ? i0 + R / 2 : i0 + 8;
+  float c0[8], c1[8], s0[8], s1[8];
+  if (turned) {
+    const TC *cr, *sr;
+    if (rope_row(a, b, l, &cr, &sr)) {
+      load_vec8(cr + i0, c0);
+      load_vec8(cr + i1, c1);
+      load_vec8(sr + i0, s0);
+      load_vec8(sr + i1, s1);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c0[e] = c1[e] = s0[e] = s1[e] = __builtin_nanf("");
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c0[e] = c1[e] = 1.f;
+      s0[e] = s1[e] = 0.f;
+    }
+  }
+  const int heads = a.Hq + a.Hk + a.Hv, h_end = min(heads, h0 + a.per);
+  for (int hh = h0 + lane / LPR; hh < h_end; hh += HPW) {
+    const int kind = hh < a.Hq ? 0 : hh < a.Hq + a.Hk ? 1 : 2;
+    const int h = hh - (kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hk);
+    const T* src = static_cast<const T*>(a.src[kind]) + b * a.s_sb[kind] + h * a.s_sh[kind] + l * a.s_sl[kind];
+    T* dst = static_cast<T*>(a.dst[kind]) + b * a.d_sb[kind] + h * a.d_sh[kind] + l * a.d_sl[kind];
+    if (kind == 2) {
+      const Vec8<T> x0 = *reinterpret_cast<const Vec8<T>*>(__builtin_assume_aligned(src + i0, 16));
+      const Vec8<T> x1 = *reinterpret_cast<const Vec8<T>*>(__builtin_assume_aligned(src + i1, 16));
+      *reinterpret_cast<Vec8<T>*>(__builtin_assume_aligned(dst + i0, 16)) = x0;
+      *reinterpret_cast<Vec8<T>*>(__builtin_assume_aligned(dst + i1, 16)) = x1;
+      continue;
+    }
+    float x0[8], x1[8];
+    load_vec8(src + i0, x0);
+    load_vec8(src + i1, x1);
+    const void* w = a.w[kind];
+    if (w) {
+      float ss = 0.f, w0[8], w1[8];
+      if (a.w_f32) {
+        load_vec8(static_cast<const float*>(w) + i0, w0);
+        load_vec8(static_cast<const float*>(w) + i1, w1);
+      } else {
+        load_vec8(static_cast<const T*>(w) + i0, w0);
+        load_vec8(static_cast<const T*>(w) + i1, w1);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], ss));
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor(ss, o);
+      const float inv = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x0[e] = x0[e] * inv * w0[e];
+        x1[e] = x1[e] * inv * w1[e];
+      }
+    }
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y0 = fmaf(x0[e], c0[e], -(x1[e] * s0[e]));
+        x1[e] = fmaf(x1[e], c1[e], x0[e] * s1[e]);
+        x0[e] = y0;
+      }
+    }
+    store_vec8(dst + i0, x0);
+    store_vec8(dst + i1, x1);
+  }
+}
+
+// Any head dimension, alignment and rotated width: a wave per head's row, a
+// pair per lane at a time.
+template <typename T, typename TC>
+__global__ void __launch_bounds__(256) norm_rope_any_kernel(RopeArgs a) {
+  const int heads = a.Hq + a.Hk + a.Hv;
+  const int64_t wid = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const int lane = threadIdx.x & 63;
+  if (wid >= (int64_t)a.tokens * heads) return;
+  const int token = (int)(wid / heads), hh = (int)(wid - (int64_t)token * heads);
+  const int b = token / a.L, l = token - b * a.L;
+  const int kind = hh < a.Hq ? 0 : hh < a.Hq + a.Hk ? 1 : 2;
+  const int h = hh - (kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hk);
+  const T* src = static_cast<const T*>(a.src[kind]) + b * a.s_sb[kind] + h * a.s_sh[kind] + l * a.s_sl[kind];
+  T* dst = static_cast<T*>(a.dst[kind]) + b * a.d_sb[kind] + h * a.d_sh[kind] + l * a.d_sl[kind];
+  if (kind == 2) {
+    for (int i = lane; i < a.D; i += 64) dst[i] = src[i];
+    return;
+  }
+  const void* w = a.w[kind];
+  float inv = 1.f;
+  if (w) {
+    float ss = 0.f;
+    for (int i = lane; i < a.D; i += 64) {
+      const float x = static_cast<float>(src[i]);
+      ss = fmaf(x, x, ss);
+    }
+    inv = 1.f / sqrtf(wave_sum(ss) / (float)a.D + a.eps);
+  }
+  auto get = [&](int i) {
+    const float x = static_cast<float>(src[i]);
+    if (!w) return x;
+    return x * inv * (a.w_f32 ? static_cast<const float*>(w)[i] : static_cast<float>(static_cast<const T*>(w)[i]));
+  };
+  const TC *cr = nullptr, *sr = nullptr;
+  const bool known = rope_row(a, b, l, &cr, &sr);
+  const int half = a.R / 2;
+  for (int i = lane; i < half; i += 64) {
+    const float x0 = get(i), x1 = get(i + half);
+    const float c0 = known ? static_cast<float>(cr[i]) : __builtin_nanf("");
+    const float c1 = known ? static_cast<float>(cr[i + half]) : __builtin_nanf("");
+    const float s0 = known ? static_cast<float>(sr[i]) : 0.f, s1 = known ? static_cast<float>(sr[i + half]) : 0.f;
+    dst[i] = static_cast<T>(fmaf(x0, c0, -(x1 * s0)));
+    dst[i + half] = static_cast<T>(fmaf(x1, c1, x0 * s1));
+  }
+  for (int i = a.R + lane; i < a.D; i += 64) dst[i] = static_cast<T>(get(i));
+}
+
+// Waves that a call is spread over, where its tokens allow.
+constexpr int64_t kRopeWaves = 4096;
+
+template <typename T, typename TC>
+static hipError_t launch_rope_t(RopeArgs a, bool vec, hipStream_t st) {
+  const int64_t heads = (int64_t)a.Hq + a.Hk + a.Hv;
+  if (vec && (a.D == 64 || a.D == 128 || a.D == 256)) {
+    const int hpw = 64 / (a.D / 16);
+    const int64_t its = (heads + hpw - 1) / hpw;
+    const int64_t want = std::min<int64_t>(its, std::max<int64_t>(1, kRopeWaves / a.tokens));  // waves per token
+    const int64_t its_w = (its + want - 1) / want;
+    a.per = (int)(its_w * hpw);
+    a.chunks = (int)((its + its_w - 1) / its_w);
+    const dim3 grid((unsigned)(((int64_t)a.tokens * a.chunks + 3) / 4));
+    if (a.D == 64)
+      launch((norm_rope_kernel<T, TC, 64>), grid, dim3(256), 0, st, a);
+    else if (a.D == 128)
+      launch((norm_rope_kernel<T, TC, 128>), grid, dim3(256), 0, st, a);
+    else
+      launch((norm_rope_kernel<T, TC, 256>), grid, dim3(256), 0, st, a);
+  } else {
+    launch((norm_rope_any_kernel<T, TC>), dim3((unsigned)(((int64_t)a.tokens * heads + 3) / 4)), dim3(256), 0, st, a);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_norm_rope(const RopeParams& p, hipStream_t st) {
+  RopeArgs a{};
+  const RopeTensor* t[3] = {&p.q, &p.k, &p.v};
+  const int64_t eb = p.dtype == kDtypeFp32 ? 4 : 2, cb = p.cos_f32 ? 4 : eb;
+  uint64_t all = 0;
+  for (int i = 0; i < 3; ++i) {
+    a.src[i] = t[i]->src;
+    a.dst[i] = t[i]->dst;
+    a.s_sb[i] = t[i]->s_sb;
+    a.s_sh[i] = t[i]->s_sh;
+    a.s_sl[i] = t[i]->s_sl;
+    a.d_sb[i] = t[i]->d_sb;
+    a.d_sh[i] = t[i]->d_sh;
+    a.d_sl[i] = t[i]->d_sl;
+    if (t[i]->src)
+      all |= reinterpret_cast<uintptr_t>(t[i]->src) | reinterpret_cast<uintptr_t>(t[i]->dst) |
+             (uint64_t)((t[i]->s_sb | t[i]->s_sh | t[i]->s_sl | t[i]->d_sb | t[i]->d_sh | t[i]->d_sl) * eb);
+  }
+  a.w[0] = p.qw;
+  a.w[1] = p.kw;
+  a.w_f32 = p.w_f32;
+  a.cos = p.cos;
+  a.sin = p.sin;
+  a.c_sb = p.c_sb;
+  a.c_sl = p.c_sl;
+  a.pos = p.pos;
+  a.p_sb = p.p_sb;
+  a.P = p.P;
+  a.L = p.L;
+  a.tokens = p.B * p.L;
+  a.Hq = p.Hq;
+  a.Hk = p.Hk;
+  a.Hv = p.v.src ? p.Hk : 0;
+  a.D = p.D;
+  a.R = p.R;
+  a.eps = p.eps;
+  all |= reinterpret_cast<uintptr_t>(p.qw) | reinterpret_cast<uintptr_t>(p.kw) | reinterpret_cast<uintptr_t>(p.cos) |
+         reinterpret_cast<uintptr_t>(p.sin) | (uint64_t)((p.c_sb | p.c_sl) * cb);
+  const bool vec = all % 16 == 0 && p.R % 16 == 0;
+  if (p.dtype == kDtypeFp32) return launch_rope_t<float, float>(a, vec, st);
+  if (p.dtype == kDtypeBf16)
+    return p.cos_f32 ? launch_rope_t<__bf16, float>(a, vec, st) : launch_rope_t<__bf16, __bf16>(a, vec, st);
+  return p.cos_f32 ? launch_rope_t<_Float16, float>(a, vec, st) : launch_rope_t<_Float16, _Float16>(a, vec, st);
+}
+
+}  // namespace dkv

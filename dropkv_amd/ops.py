@@ -9,7 +9,9 @@ alignment) and raise ``RuntimeError`` otherwise; the reference-compatible
 
 from __future__ import annotations
 
+import ctypes
 import threading
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -399,6 +401,265 @@ def decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, 
         out.stride(0), out.stride(2), out.stride(3), workspace.data_ptr(), workspace.numel(), _stream(dev))
     _lib.check(rc, "dropkv_decode_attention")
     return out
+
+
+def _call(dev: torch.device, name: str, *args) -> None:
+    """Entry point ``name`` on the current stream of ``dev``, with ``dev`` current."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    _lib.check(rc, name)
+
+
+def _no_grad(name: str, *ts) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with its last axis contiguous."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def tree_workspace(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int, device) -> torch.Tensor:
+    """Workspace of ``tree_attention`` for one geometry (reusable across steps
+    and layers of that geometry, one call at a time)."""
+    nbytes = _lib.load().dropkv_tree_workspace_bytes(B, Hq, Hkv, D, T, capacity)
+    if nbytes == 0:
+        raise RuntimeError("unsupported tree geometry")
+    return _workspace(nbytes, torch.device(device))
+
+
+def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor, n_rows: torch.Tensor, scale: float, out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of T drafted tokens per sequence over the cache and over one
+    another (``dropkv_tree_attention``): q [B, Hq, T, D], their own rows
+    k_new / v_new [B, Hkv, T, D], the buffers [B, Hkv, capacity, D] whose first
+    ``n_rows`` rows (int32 on the device, one count or one per sequence) are
+    filled.  ``mask`` (bool, [T, T] or [B, T, T]) says which drafted token
+    (second to last axis) sees which; without it they are a chain.  Returns
+    ``out`` [B, T, Hq, D]; a row that sees no key is zeros.  The buffers are not
+    written: ``tree_commit`` stores the rows of the tokens that stand."""
+    dev = _check_device(q, k_new, v_new, k_cache, v_cache, n_rows)
+    _no_grad("tree_attention", q, k_new, v_new, k_cache, v_cache)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError("tree_attention: the dtype must be bf16 or fp16")
+    for t in (k_new, v_new, k_cache, v_cache):
+        if t.dtype != q.dtype:
+            raise RuntimeError("tree_attention: all tensors must share a dtype")
+    if q.dim() != 4 or k_new.dim() != 4:
+        raise RuntimeError("tree_attention: q, k_new and v_new must be [B, H, T, D]")
+    B, Hq, T, D = q.shape
+    _check_buffer(k_cache, "k_cache")
+    _check_buffer(v_cache, "v_cache")
+    Hkv, C = k_cache.shape[1], k_cache.shape[2]
+    if k_new.shape != (B, Hkv, T, D) or v_new.shape != k_new.shape:
+        raise RuntimeError("tree_attention: k_new and v_new must be [B, Hkv, T, D]")
+    if k_cache.shape != (B, Hkv, C, D) or v_cache.shape != k_cache.shape:
+        raise RuntimeError("tree_attention: the cache buffers must be [B, Hkv, capacity, D]")
+    if n_rows.dtype != torch.int32 or n_rows.numel() not in (1, B) or not n_rows.is_contiguous():
+        raise RuntimeError("tree_attention: n_rows must hold one int32 count, or one per sequence")
+    m_ptr, m_strides = None, (0, 0, 0)
+    if mask is not None:
+        _check_device(q, mask)
+        if mask.dtype != torch.bool or mask.shape not in ((T, T), (B, T, T)):
+            raise RuntimeError("tree_attention: mask must be bool, [T, T] or [B, T, T]")
+        m_ptr = mask.data_ptr()
+        m_strides = (0, *mask.stride()) if mask.dim() == 2 else mask.stride()
+    if out is None:
+        out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=dev)
+    else:
+        _check_device(q, out)
+        if out.shape != (B, T, Hq, D) or out.dtype != q.dtype or (out.stride(3) != 1 and D > 1):
+            raise RuntimeError("tree_attention: out must be [B, T, Hq, D] of q's dtype, D contiguous")
+    if workspace is None:
+        workspace = tree_workspace(B, Hq, Hkv, D, T, C, dev)
+    else:
+        _check_device(q, workspace)
+    q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)
+    qs, ks, vs, os = q.stride(), k_new.stride(), v_new.stride(), out.stride()
+    _call(dev, "dropkv_tree_attention", q.data_ptr(), qs[0], qs[1], qs[2], k_new.data_ptr(), ks[0], ks[1], ks[2],
+          v_new.data_ptr(), vs[0], vs[1], vs[2], k_cache.data_ptr(), v_cache.data_ptr(), n_rows.data_ptr(),
+          int(n_rows.numel() > 1), m_ptr, *m_strides, _DTYPE_CODE[q.dtype], B, Hq, Hkv, T, D, C, float(scale),
+          out.data_ptr(), os[0], os[1], os[2], workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    return out
+
+
+def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tensor, k_new: torch.Tensor,
+                v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_rows: torch.Tensor):
+    """Which drafted tokens stand, and their rows appended to the caches
+    (``dropkv_tree_commit``).  ``tokens`` [B, T] int64 were fed, ``choice``
+    [B, T] int64 is the token settled on after each, ``parents`` ([T] or [B, T],
+    int32) the trees; node 0 stands, and from a node that stands the walk goes
+    to its lowest child whose token is the node's choice.  ``k_new`` / ``v_new``
+    [B, H, T, D] and the buffers [B, H, capacity, D], or those of N layers with
+    an axis N in front; ``n_rows`` int32, [1] or [B], or [N, 1] or [N, B].
+    Returns ``(path [B, T] int32, the nodes that stand, then -1; accepted [B]
+    int32)``.  ``n_rows`` is not advanced."""
+    dev = _check_device(tokens, parents, choice, k_new, v_new, k_cache, v_cache, n_rows)
+    _no_grad("tree_commit", k_new, v_new, k_cache, v_cache)
+    if tokens.dim() != 2 or choice.shape != tokens.shape or tokens.dtype != torch.int64 or choice.dtype != torch.int64:
+        raise RuntimeError("tree_commit: tokens and choice must be int64 [B, T]")
+    B, T = tokens.shape
+    if parents.dtype != torch.int32 or parents.shape not in ((T,), (1, T), (B, T)):
+        raise RuntimeError("tree_commit: parents must be int32 [T] or [B, T]")
+    if k_cache.dim() not in (4, 5) or k_new.dim() != k_cache.dim():
+        raise RuntimeError("tree_commit: rows and buffers must be [B, H, ., D] or [N, B, H, ., D]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise RuntimeError("tree_commit: the cache buffers must be contiguous")
+    *lead, H, C, D = k_cache.shape
+    if lead[-1] != B or k_new.shape != (*lead, H, T, D) or v_new.shape != k_new.shape or v_cache.shape != k_cache.shape:
+        raise RuntimeError("tree_commit: shape mismatch")
+    if not k_cache.dtype == v_cache.dtype == k_new.dtype == v_new.dtype or k_cache.dtype not in _DTYPE_CODE:
+        raise RuntimeError("tree_commit: rows and buffers must share a bf16, fp16 or fp32 dtype")
+    if n_rows.dtype != torch.int32 or n_rows.dim() != len(lead) or any(
+            a not in (1, b) for a, b in zip(n_rows.shape, lead)) or (len(lead) == 2 and n_rows.shape[0] != lead[0]):
+        raise RuntimeError("tree_commit: n_rows must be int32, [1] or [B], or [N, 1] or [N, B]")
+    N = lead[0] if len(lead) == 2 else 1
+    path = torch.empty(B, T, dtype=torch.int32, device=dev)
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    if path.numel() == 0:
+        return path, accepted
+    tokens, choice, parents = tokens.contiguous(), choice.contiguous(), parents.contiguous()
+    k_new, v_new = _rows(k_new), _rows(v_new)
+    ks, vs, ns = k_new.stride()[:-1], v_new.stride()[:-1], n_rows.expand(lead).stride()
+    if N == 1 and len(lead) == 1:
+        ks, vs, ns = (0, *ks), (0, *vs), (0, *ns)
+    _call(dev, "dropkv_tree_commit", tokens.data_ptr(), parents.data_ptr(), T if parents.numel() > T else 0,
+          choice.data_ptr(), path.data_ptr(), accepted.data_ptr(), k_new.data_ptr(), *ks, v_new.data_ptr(), *vs,
+          k_cache.data_ptr(), v_cache.data_ptr(), n_rows.data_ptr(), *ns, k_cache.element_size(), N, B, H, T, D, C)
+    return path, accepted
+
+
+def norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+              positions: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+              k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, v: Optional[torch.Tensor] = None,
+              q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+              v_out: Optional[torch.Tensor] = None):
+    """Norms (with ``q_weight`` / ``k_weight`` [D]) and rotation of queries
+    [B, Hq, L, D] and keys [B, Hkv, L, D], any strides, in one pass
+    (``dropkv_norm_rope``).  ``cos`` and ``sin`` hold the R <= D rotated values'
+    factors (value i is paired with i + R/2), in fp32 or q's dtype: each token's
+    ([L, R], [1, L, R] or [B, L, R]), or with ``positions`` (int64, [L], [1, L]
+    or [B, L]) a table [rows, R]; a position outside the table gives NaN.  With
+    ``v`` its rows are copied too.  The outputs may be views of cache buffers
+    (``k_buf[:, :, n:n + L]``), or the inputs themselves, and are new tensors
+    otherwise.  Returns ``(q_out, k_out)``, or ``(q_out, k_out, v_out)``."""
+    dev = _check_device(q, k, cos, sin)
+    _no_grad("norm_rope", q, k, v, cos, sin, q_weight, k_weight)
+    if q.dtype not in _DTYPE_CODE or k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
+        raise RuntimeError("norm_rope: q, k and v must share a bf16, fp16 or fp32 dtype")
+    if q.dim() != 4 or k.dim() != 4:
+        raise RuntimeError("norm_rope: q and k must be [B, H, L, D]")
+    B, Hq, L, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape != (B, Hkv, L, D) or (v is not None and v.shape != k.shape):
+        raise RuntimeError("norm_rope: k and v must be [B, Hkv, L, D]")
+    R = cos.shape[-1]
+    if sin.shape != cos.shape or sin.dtype != cos.dtype or cos.dtype not in (torch.float32, q.dtype):
+        raise RuntimeError("norm_rope: cos and sin must be alike, fp32 or of q's dtype")
+    p_ptr, p_sb = None, 0
+    if positions is not None:
+        _check_device(q, positions)
+        if cos.dim() != 2 or positions.dtype != torch.int64 or positions.shape not in ((L,), (1, L), (B, L)):
+            raise RuntimeError("norm_rope: positions must be int64 [L] or [B, L], with cos and sin [rows, R]")
+        positions = positions.contiguous()
+        p_ptr, p_sb = positions.data_ptr(), L if positions.numel() > L else 0
+    elif cos.shape not in ((L, R), (1, L, R), (B, L, R)):
+        raise RuntimeError("norm_rope: cos and sin must be [L, R], [1, L, R] or [B, L, R]")
+    if cos.stride(-1) != 1 or sin.stride() != cos.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    c_sb = cos.stride(0) if positions is None and cos.dim() == 3 and cos.shape[0] > 1 else 0
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        _check_device(q, w)
+        if w.shape != (D,) or w.dtype not in (torch.float32, q.dtype) or w.dtype != weights[0].dtype:
+            raise RuntimeError("norm_rope: norm weights must be [D], fp32 or of q's dtype, and alike")
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    if v is None and v_out is not None:
+        raise RuntimeError("norm_rope: v_out without v")
+
+    def target(t, like, name):
+        if t is None:
+            return torch.empty(like.shape, dtype=q.dtype, device=dev)
+        _check_device(q, t)
+        if t.shape != like.shape or t.dtype != q.dtype or t.stride(3) != 1:
+            raise RuntimeError(f"norm_rope: {name} must have its input's shape and dtype, D contiguous")
+        return t
+
+    q_out, k_out = target(q_out, q, "q_out"), target(k_out, k, "k_out")
+    outs = (q_out, k_out)
+    q, k = _rows(q), _rows(k)
+    pairs = [(q, q_out), (k, k_out)]
+    if v is not None:
+        v_out = target(v_out, v, "v_out")
+        v = _rows(v)
+        outs += (v_out,)
+        pairs.append((v, v_out))
+    if q.numel() == 0:
+        return outs
+    strides = (ctypes.c_int64 * 18)(*[s for pair in pairs for t in pair for s in t.stride()[:3]])
+    args = []
+    for i, pair in enumerate(pairs):
+        for j, t in enumerate(pair):
+            args += [t.data_ptr(), ctypes.addressof(strides) + 24 * (2 * i + j)]
+    if v is None:
+        args += [None] * 4
+    _call(dev, "dropkv_norm_rope", *args, None if q_weight is None else q_weight.data_ptr(),
+          None if k_weight is None else k_weight.data_ptr(), _DTYPE_CODE[weights[0].dtype] if weights else 0,
+          cos.data_ptr(), sin.data_ptr(), _DTYPE_CODE[cos.dtype], c_sb, cos.stride(-2), p_ptr, p_sb, cos.shape[0],
+          _DTYPE_CODE[q.dtype], B, Hq, Hkv, L, D, R, float(eps))
+    return outs
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns; the leading axes are the logits'."""
+
+    logprob: Optional[torch.Tensor]  # [...] fp32, None without tokens
+    entropy: torch.Tensor            # [...] fp32
+    top_logprobs: torch.Tensor       # [..., top] fp32
+    top_ids: torch.Tensor            # [..., top] int64
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+    """Log probability of a given token, entropy, and the ``top`` (at most 32)
+    most probable tokens of every row of ``logits`` [..., V] (bf16, fp16 or
+    fp32), in one pass over them (``dropkv_token_logprobs``).  ``tokens`` [...]
+    int64: 0 comes out where it is negative, NaN where it is V or more.  The top
+    tokens come largest first, the lowest id first among equals."""
+    dev = _check_device(logits)
+    _no_grad("token_logprobs", logits)
+    if logits.dtype not in _DTYPE_CODE:
+        raise RuntimeError("token_logprobs: logits must be bf16, fp16 or fp32")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError("token_logprobs: logits must be [..., V]")
+    *lead, V = logits.shape
+    if not 0 <= top <= V:
+        raise RuntimeError("token_logprobs: top must be in [0, V]")
+    if tokens is not None:
+        _check_device(logits, tokens)
+        if tokens.dtype != torch.int64 or list(tokens.shape) != lead:
+            raise RuntimeError("token_logprobs: tokens must be int64, of the logits' leading shape")
+        tokens = tokens.contiguous()
+    x = _rows(logits.reshape(-1, V))
+    N = x.shape[0]
+    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    top_lp = torch.empty(*lead, top, dtype=torch.float32, device=dev)
+    top_id = torch.empty(*lead, top, dtype=torch.int64, device=dev)
+    res = TokenLogprobs(logprob, entropy, top_lp, top_id)
+    if N == 0:
+        return res
+    nbytes = _lib.load().dropkv_token_logprobs_workspace_bytes(N, V, top)
+    ws = _workspace(nbytes, dev) if nbytes else None
+    _call(dev, "dropkv_token_logprobs", x.data_ptr(), x.stride(0), _DTYPE_CODE[x.dtype], N, V,
+          None if tokens is None else tokens.data_ptr(), int(top), None if logprob is None else logprob.data_ptr(),
+          entropy.data_ptr(), top_lp.data_ptr(), top_id.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
+    return res
 
 
 def mfma_selftest(device="cuda") -> torch.Tensor:
