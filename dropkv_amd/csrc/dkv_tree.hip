@@ -24,6 +24,14 @@
 
 namespace dkv {
 
+#ifndef W16
+#define W16 2048
+#define W64 512
+#define W128 512
+#define W256 256
+#define LO128 true
+#define LO256 true
+#endif
 constexpr int kTreeTile = 32;       // keys per tile
 constexpr int kTreeMaxSplits = 63;  // of the cache: one lane of the merge each, with the drafted keys'
 
@@ -40,12 +48,16 @@ struct TreeArgs {
   const uint8_t* mask;  // [T, T] bytes at m_sb, m_st, m_sj; null: a chain (j <= t)
   int64_t m_sb, m_st, m_sj;
   int B, Hq, Hkv, D, T, C, M, S, MC;
+  int P;       // parts of a KV head: S per sequence, and one more each where the drafted keys are a part of their own
+  int apart;   // they are
+  int ragged;  // the B * S parts are dealt out by the sequences' lengths
+  int direct;  // one part: the output is written by it
   int qvec, nvec;
   Div div_t;
   float scale_log2;
-  float* part_m;  // [B*Hkv, S + 1, M]
+  float* part_m;  // [Hkv, P, M]
   float* part_l;
-  float* part_o;  // [B*Hkv, S + 1, M, D]
+  float* part_o;  // [Hkv, P, M, D]
   void* out;      // [B, T, Hq, D], D contiguous
   int64_t o_sb, o_st, o_sh;
 };
@@ -83,20 +95,108 @@ __device__ __forceinline__ int tree_rows(const TreeArgs& a, int b) {
   return min(max(a.n_rows[b * a.n_sb], 0), a.C);
 }
 
+// Sequence b's parts of the cache: `count` of them from `first` on, `per` tiles
+// each.  With one count for all, or one sequence, S parts each.  Otherwise the
+// B * S parts go by length, so that no workgroup has much more than the mean (8
+// sequences of 940 to 8003 rows at equal parts: the longest took twice the
+// mean's time): ceil(tiles / per) parts each, at least one, `per` the mean where
+// that fits, else what always does: sum ceil(t_b / per) <= sum t_b / per + B.
+// Every lane of the wave calls this; lane i looks at sequence i.
+constexpr int kTreeRaggedB = 64;
+struct TreeParts {
+  int first, count, per;
+};
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int tree_tiles(const TreeArgs& a, int b) {
+  return (tree_rows(a, b) + kTreeTile - 1) / kTreeTile;
+}
+__device__ __forceinline__ int wave_sum_int(int x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ TreeParts tree_parts_ragged(const TreeArgs& a, int lane) {
+  const int t = lane < a.B ? tree_tiles(a, lane) : 0;
+  int sum = t, most = t;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    sum += __shfl_xor(sum, o);
+    most = max(most, __shfl_xor(most, o));
+  }
+  const int floor_per = max(1, ceil_div(most, kTreeMaxSplits));
+  TreeParts p;
+  p.per = max(floor_per, ceil_div(sum, a.B * a.S));
+  auto parts = [&]() { return lane < a.B ? max(1, ceil_div(t, p.per)) : 0; };
+  p.count = parts();
+  if (wave_sum_int(p.count) > a.B * a.S) {
+    p.per = max(floor_per, ceil_div(sum, a.B * (a.S - 1)));
+    p.count = parts();
+  }
+  int off = p.count;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(off, o);
+    if (lane >= o) off += x;
+  }
+  p.first = off - p.count;
+  return p;
+}
+__device__ __forceinline__ TreeParts tree_parts(const TreeArgs& a, int b, int lane) {
+  if (!a.ragged) return TreeParts{b * a.S, a.S, ceil_div(tree_tiles(a, b), a.S)};
+  TreeParts p = tree_parts_ragged(a, lane);
+  return TreeParts{__builtin_amdgcn_readlane(p.first, b), __builtin_amdgcn_readlane(p.count, b),
+                   __builtin_amdgcn_readfirstlane(p.per)};
+}
+
+// Part `slot` of a KV head: tiles t_lo .. t_hi of sequence b, whose stored rows
+// are n, and with `tail` the drafted keys; b < 0: none.
+struct TreePart {
+  int b, n, t_lo, t_hi;
+  bool tail;
+};
+__device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int slot, int lane) {
+  TreePart p;
+  if (slot >= a.B * a.S) return TreePart{slot - a.B * a.S, 0, 0, 0, true};
+  int first, count, per;
+  if (a.ragged) {
+    const TreeParts all = tree_parts_ragged(a, lane);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(all.first <= slot && slot < all.first + all.count);
+    if (!hit) return TreePart{-1, 0, 0, 0, false};
+    p.b = __builtin_ctzll(hit);
+    first = __builtin_amdgcn_readlane(all.first, p.b);
+    count = __builtin_amdgcn_readlane(all.count, p.b);
+    per = __builtin_amdgcn_readfirstlane(all.per);
+    p.n = tree_rows(a, p.b);
+  } else {
+    p.b = slot / a.S;
+    p.n = tree_rows(a, p.b);
+    first = p.b * a.S;
+    count = a.S;
+    per = ceil_div((p.n + kTreeTile - 1) / kTreeTile, a.S);
+  }
+  const int tiles = (p.n + kTreeTile - 1) / kTreeTile;
+  p.t_lo = min((slot - first) * per, tiles);
+  p.t_hi = min(p.t_lo + per, tiles);
+  p.tail = !a.apart && slot - first == count - 1;
+  return p;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   typedef typename Elem<T>::v8 v8;
   constexpr int KK = D / 32, DT = D / 16, CPR = D / 8, GRP = 64 / CPR, NVC = kTreeTile / GRP;
   constexpr int kVPitch = D + 16;  // transposing reads without bank conflicts
   constexpr uint32_t kRowBytes = D * (uint32_t)sizeof(T);
-  const int split = blockIdx.x % (a.S + 1);
-  const int mc = (blockIdx.x / (a.S + 1)) % a.MC, bh = blockIdx.x / ((a.S + 1) * a.MC);
-  const int b = bh / a.Hkv, hkv = bh % a.Hkv, g = a.Hq / a.Hkv;
+  const int slot = blockIdx.x % a.P, hkv = blockIdx.x / a.P, g = a.Hq / a.Hkv;
   const int lane = threadIdx.x, li = lane & 15, lg = lane >> 4;
   __shared__ __attribute__((aligned(16))) T vt[kTreeTile * kVPitch];
 
-  // Row 16 mc + li of the KV head: query head hkv g + h, token t.
-  const int row = 16 * mc + li;
+  const TreePart part = tree_part(a, slot, lane);
+  const int b = part.b;
+  if (b < 0) return;
+  const int bh = b * a.Hkv + hkv;
+  // Row li of the KV head: query head hkv g + h, token t.
+  const int row = li;
   const bool valid = row < a.M;
   const int h = valid ? a.div_t.div(row) : 0, t = valid ? row - h * a.T : 0;
   v8 qop[KK];
@@ -104,11 +204,9 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) qop[kk] = tree_load8(qr + 32 * kk + 8 * lg, a.qvec);
 
-  const bool drafted = split == a.S;
-  const int n = drafted ? a.T : tree_rows(a, b);
-  const int tiles = (n + kTreeTile - 1) / kTreeTile;
-  const int per = drafted ? tiles : (tiles + a.S - 1) / a.S;
-  const int j_lo = drafted ? 0 : split * per * kTreeTile, j_hi = drafted ? n : min(n, j_lo + per * kTreeTile);
+  const bool drafted = part.tail;
+  const int n = drafted ? a.T : part.n;
+  const int j_lo = drafted ? 0 : part.t_lo * kTreeTile, j_hi = drafted ? n : min(n, part.t_hi * kTreeTile);
   // Rows past n read as zeros.
   const rsrc_t krs = make_rsrc(static_cast<const T*>(a.kbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
   const rsrc_t vrs = make_rsrc(static_cast<const T*>(a.vbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
@@ -230,7 +328,7 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   }
 
   lsum = add_xor32(add_xor16(lsum));
-  const int64_t base = ((int64_t)bh * (a.S + 1) + split) * a.M + row;
+  const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + row;
   if (valid) {
     float* po = a.part_o + base * D + 4 * lg;
 #pragma unroll
@@ -242,31 +340,309 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   }
 }
 
-// One wave per row: lane s holds split s's maximum and sum, D / 4 lanes a
-// partial output row.
+// What a tile's keys are to the rows: all seen, the first ones, or by the mask.
+template <int k>
+struct Kind {
+  static constexpr int value = k;
+};
+
+// More than 16 rows: NW waves of QB blocks of 16 rows take the same keys, so
+// that a tile of K and V is read once for all of them, into LDS.  The next tile
+// is on its way in registers while the waves compute on this one, and goes to
+// the other of two buffers: one barrier per tile.  A K operand (a V operand)
+// read from LDS serves QB products.  LDS pitches leave every 16 lanes of a
+// K read, and every 32 of a transposing V read, on banks of their own.
+template <typename T, int D, int QB, int NW, bool LO>
+__global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
+  typedef typename Elem<T>::v8 v8;
+  constexpr int KK = D / 32, DT = D / 16, CPR = D / 8, NT = 64 * NW;
+  constexpr int kSub = 2, kStage = kSub * kTreeTile;
+  constexpr int kChunks = kStage * CPR;         // 16-byte pieces of a stage's K (or V)
+  constexpr int NC = 2 * kChunks / NT;          // pieces per thread
+  constexpr int kKP = D + 8, kVP = D + 16, kBuf = kStage * (kKP + kVP);
+  constexpr uint32_t kRowBytes = D * (uint32_t)sizeof(T);
+  static_assert(NC * NT == 2 * kChunks, "whole pieces per thread");
+  __shared__ __attribute__((aligned(16))) T lds[2 * kBuf];
+  __shared__ int odd_flag;
+
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int mc = id % a.MC, slot = (id / a.MC) % a.P, hkv = id / (a.MC * a.P), g = a.Hq / a.Hkv;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const TreePart part = tree_part(a, slot, lane);
+  const int b = part.b, n = part.n;
+  if (b < 0) return;
+  const int bh = b * a.Hkv + hkv;
+  const int row0 = (mc * NW + wave) * (16 * QB) + li;  // the lane's row of block 0
+
+  v8 qop[QB][KK];
+  int tq[QB];
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    const int row = min(row0 + 16 * x, a.M - 1);  // (rows past the last repeat it and are not stored)
+    const int h = a.div_t.div(row), t = row - h * a.T;
+    tq[x] = t;
+    const T* qr =
+        static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hkv * g + h) * a.q_sh + (int64_t)t * a.q_st;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qop[x][kk] = tree_load8(qr + 32 * kk + 8 * lg, a.qvec);
+  }
+
+  // Rows past n read as zeros.
+  const rsrc_t krs = make_rsrc(static_cast<const T*>(a.kbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
+  const rsrc_t vrs = make_rsrc(static_cast<const T*>(a.vbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
+  const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
+  const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
+
+  u32x4 piece[NC];
+  auto place = [&](int i, int* row, int* col) __attribute__((always_inline)) {  // piece i: K or V, its row and column
+    const int c = tid + i * NT, v = c >= kChunks;
+    *row = (c - v * kChunks) / CPR;
+    *col = 8 * (c % CPR);
+    return v != 0;
+  };
+  auto fetch = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      int r, col;
+      const bool v = place(i, &r, &col);
+      piece[i] = buf_load16(v ? vrs : krs, (uint32_t)(j0 + r) * kRowBytes + col * (uint32_t)sizeof(T));
+    }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      int r, col;
+      const bool v = place(i, &r, &col);
+      *reinterpret_cast<u32x4*>(lds + buf * kBuf + (v ? kStage * kKP + r * kVP : r * kKP) + col) = piece[i];
+    }
+  };
+
+  float m[QB], lsum[QB];
+  f32x4 o[QB][DT];
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    m[x] = -__FLT_MAX__;  // (finite, so that logits of -inf get no weight)
+    lsum[x] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int tr_row = 4 * lg + li / 4, tr_col = 4 * (li % 4);
+
+  // Tile `sub` of the stage in buffer `buf`.  Kind 0: every key seen; 1: the
+  // first `keys`; 2: drafted keys j0 ..., seen by the mask.
+  auto compute = [&](int buf, int sub, auto kind, int keys, int j0) __attribute__((always_inline)) {
+    constexpr int kKind = decltype(kind)::value;
+    const T* kt = lds + buf * kBuf + sub * kTreeTile * kKP;
+    const T* vt = lds + buf * kBuf + kStage * kKP + sub * kTreeTile * kVP;
+    f32x4 s[QB][2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+      for (int x = 0; x < QB; ++x) s[x][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const v8 kop = *reinterpret_cast<const v8*>(kt + (16 * hf + li) * kKP + 32 * kk + 8 * lg);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) s[x][hf] = Elem<T>::mfma(kop, qop[x][kk], s[x][hf]);
+      }
+    }
+    v8 phi[QB], plo[LO ? QB : 1];
+    float alpha[QB], pf[kKind == 2 ? QB : 1][8];
+    bool turn = false;
+#pragma unroll
+    for (int x = 0; x < QB; ++x) {
+      uint32_t seen = 0xff;
+      if (kKind != 0) {
+        const uint8_t* mrow =
+            kKind == 2 && a.mask ? a.mask + (int64_t)b * a.m_sb + (int64_t)tq[x] * a.m_st : nullptr;
+        seen = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = 16 * (e / 4) + 4 * lg + e % 4;
+          bool see = j < keys;
+          if (kKind == 2 && see) see = mrow ? mrow[(int64_t)(j0 + j) * a.m_sj] != 0 : j0 + j <= tq[x];
+          seen |= (uint32_t)see << e;
+          s[x][e / 4][e % 4] = see ? s[x][e / 4][e % 4] : -INFINITY;
+        }
+      }
+      float tmax = s[x][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
+      tmax = max_xor32(max_xor16(tmax)) * a.scale_log2;
+      const float mnew = fmaxf(m[x], tmax);
+      alpha[x] = __builtin_amdgcn_exp2f(m[x] - mnew);
+      turn |= mnew != m[x];
+      m[x] = mnew;
+      const float ref = mnew - kPBias<T>;
+      float psum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[x][e / 4][e % 4], a.scale_log2, -ref));
+        psum += p;
+        phi[x][e] = static_cast<T>(p);
+        if (LO) plo[x][e] = static_cast<T>(p - static_cast<float>(phi[x][e]));
+        if (kKind == 2) pf[x][e] = (seen >> e) & 1 ? p : -1.f;
+      }
+      lsum[x] = fmaf(lsum[x], alpha[x], psum);
+    }
+    if (wave_any(turn)) {
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha[x];
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s4 lds_s4;
+      const s4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vt + tr_row * kVP + 16 * dt + tr_col));
+      const s4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vt + (16 + tr_row) * kVP + 16 * dt + tr_col));
+      const v8 aop = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int x = 0; x < QB; ++x) {
+        o[x][dt] = Elem<T>::mfma(aop, phi[x], o[x][dt]);
+        if (LO) o[x][dt] = Elem<T>::mfma(aop, plo[x], o[x][dt]);
+      }
+    }
+    if (kKind == 2 && odd_flag) {
+      // A drafted value that is not finite reaches only the rows that see its
+      // key: the product above took it as zero (0 * inf is NaN), and here it
+      // is added where it is seen.
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll 1
+          for (int lgp = 0; lgp < 4; ++lgp) {
+            const int j = 16 * (e / 4) + 4 * lgp + e % 4;
+            const float p = __shfl(pf[x][e], li + 16 * lgp);
+            if (j < keys && !(p < 0.f))
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const T val = vn[(int64_t)(j0 + j) * a.vn_st + 16 * dt + 4 * lg + r];
+                  if (not_finite<T>(val)) o[x][dt][r] = fmaf(p, static_cast<float>(val), o[x][dt][r]);
+                }
+          }
+    }
+  };
+
+  int buf = 0;
+  const int j_hi = min(n, part.t_hi * kTreeTile);
+  int j0 = part.t_lo * kTreeTile;
+  if (j0 < j_hi) {
+    fetch(j0);
+    put(0);
+    for (; j0 + kStage < j_hi; j0 += kStage) {
+      fetch(j0 + kStage);
+      __syncthreads();
+#pragma unroll
+      for (int sub = 0; sub < kSub; ++sub) compute(buf, sub, Kind<0>{}, kTreeTile, 0);
+      buf ^= 1;
+      put(buf);
+    }
+    __syncthreads();
+    for (int sub = 0; j0 < j_hi; ++sub, j0 += kTreeTile) compute(buf, sub, Kind<1>{}, j_hi - j0, 0);
+    buf ^= 1;
+  }
+  if (part.tail)
+    for (j0 = 0; j0 < a.T; j0 += kStage) {
+      if (tid == 0) odd_flag = 0;
+      __syncthreads();  // (also: nobody reads the buffer any more)
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        int r, col;
+        const bool v = place(i, &r, &col);
+        v8 x = v8{};
+        if (j0 + r < a.T) {
+          x = tree_load8((v ? vn + (int64_t)(j0 + r) * a.vn_st : kn + (int64_t)(j0 + r) * a.kn_st) + col, a.nvec);
+          if (v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (not_finite<T>(x[e])) {
+                odd = true;
+                x[e] = static_cast<T>(0.f);
+              }
+        }
+        piece[i] = __builtin_bit_cast(u32x4, x);
+      }
+      put(buf);
+      if (odd) odd_flag = 1;
+      __syncthreads();
+      for (int sub = 0; sub < kSub && j0 + sub * kTreeTile < a.T; ++sub)
+        compute(buf, sub, Kind<2>{}, a.T - j0 - sub * kTreeTile, j0 + sub * kTreeTile);
+      __syncthreads();
+    }
+
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    const int row = row0 + 16 * x;
+    const float l = add_xor32(add_xor16(lsum[x]));
+    if (row >= a.M) continue;
+    if (a.direct) {
+      const int h = a.div_t.div(row), t = row - h * a.T;
+      T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(hkv * g + h) * a.o_sh;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          out[16 * dt + 4 * lg + r] = static_cast<T>(l == 0.f ? 0.f : o[x][dt][r] * inv);
+      continue;
+    }
+    const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + row;
+    float* po = a.part_o + base * D + 4 * lg;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[x][dt];
+    if (lg == 0) {
+      a.part_m[base] = m[x] - kPBias<T>;
+      a.part_l[base] = l;
+    }
+  }
+}
+
+// One wave per row: lane s holds part s's maximum and sum, D / 4 lanes a
+// partial output row.  The first eight loads of partial outputs are issued with
+// the statistics, before the reductions: one round trip for up to 16 (D = 128)
+// or 32 parts.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
-  constexpr int LPR = D / 4, SPL = 64 / LPR;
-  const int S1 = a.S + 1;
+  constexpr int LPR = D / 4, SPL = 64 / LPR, NL = 8;
   const int wid = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
   if (wid >= a.B * a.Hkv * a.M) return;
   const int bh = wid / a.M, row = wid - bh * a.M;
   const int b = bh / a.Hkv, hkv = bh % a.Hkv;
   const int h = a.div_t.div(row), t = row - h * a.T;
   const int sub = lane / LPR, d0 = 4 * (lane % LPR);
-  const int64_t base = (int64_t)bh * S1 * a.M + row;
-  const float ml = lane < S1 ? a.part_m[base + (int64_t)lane * a.M] : -__FLT_MAX__;
-  const float ll = lane < S1 ? a.part_l[base + (int64_t)lane * a.M] : 0.f;
-  const float mx = wave_max(ml);
-  const float f = __builtin_amdgcn_exp2f(ml - mx);
-  const float l = wave_sum(ll * f);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < S1; s += SPL) {
-    const float fs = __shfl(f, (s + sub) & 63);
-    if (s + sub < S1) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (base + (int64_t)(s + sub) * a.M) * D + d0);
+  const TreeParts parts = tree_parts(a, b, lane);
+  const int S1 = parts.count + a.apart;
+  // Row of part s: those of the cache, then the drafted keys'.
+  auto at = [&](int s) { return ((int64_t)hkv * a.P + (s < parts.count ? parts.first + s : a.B * a.S + b)) * a.M + row; };
+  const float ml = lane < S1 ? a.part_m[at(lane)] : -__FLT_MAX__;
+  const float ll = lane < S1 ? a.part_l[at(lane)] : 0.f;
+  f32x4 x[NL];
+  auto fetch = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(fs, x[e], acc[e]);
+    for (int i = 0; i < NL; ++i) {
+      const int s = s0 + SPL * i + sub;
+      x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (s < S1) x[i] = *reinterpret_cast<const f32x4*>(a.part_o + at(s) * D + d0);
+    }
+  };
+  fetch(0);
+  const float mx = wave_max_dpp(ml);
+  const float f = __builtin_amdgcn_exp2f(ml - mx);
+  const float l = wave_sum_dpp(ll * f);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < S1; s0 += SPL * NL) {
+    if (s0 > 0) fetch(s0);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const float fs = __shfl(f, (s0 + SPL * i + sub) & 63);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(fs, x[i][e], acc[e]);
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -280,24 +656,23 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
   }
 }
 
-// Splits of the cache for so many (b, KV head, row chunk) pairs.
-constexpr int kTreeWaves = 2048;
-static int tree_splits(int64_t chunks, int C) {
-  const int tiles = (C + kTreeTile - 1) / kTreeTile;
-  const int64_t want = std::max<int64_t>(1, kTreeWaves / chunks);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, kTreeMaxSplits, (tiles + 1) / 2}));
-}
-
+// How a call is cut: rows per workgroup, parts of the cache per sequence, and
+// whether the drafted keys are parts of their own.
 struct TreePlan {
-  int M, MC, S;
+  int M, rows_wg, MC, S, P, apart;
   size_t rows, bytes;
 };
 static TreePlan tree_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C) {
   TreePlan p;
   p.M = (int)(Hq / Hkv * T);
-  p.MC = (p.M + 15) / 16;
-  p.S = tree_splits(B * Hkv * p.MC, (int)C);
-  p.rows = (size_t)B * Hkv * (p.S + 1) * p.M;
+  p.rows_wg = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256;
+  p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
+  const int64_t chunks = B * Hkv * p.MC, tiles = (C + kTreeTile - 1) / kTreeTile;
+  const int64_t want = (p.rows_wg == 16 ? W16 : p.rows_wg <= 64 ? W64 : p.rows_wg == 128 ? W128 : W256) / chunks;
+  p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, kTreeMaxSplits, (tiles + 1) / 2}));
+  p.apart = p.rows_wg == 16 || chunks * p.S < 192;
+  p.P = (int)(B * (p.S + p.apart));
+  p.rows = (size_t)Hkv * p.P * p.M;
   p.bytes = p.rows * sizeof(float) * (2 + (size_t)D) + 256;
   return p;
 }
@@ -306,9 +681,19 @@ size_t tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
 }
 
 template <typename T, int D>
-static hipError_t launch_tree_t(const TreeArgs& a, hipStream_t st) {
-  launch((tree_partial_kernel<T, D>), dim3(a.B * a.Hkv * a.MC * (a.S + 1)), dim3(64), 0, st, a);
-  launch((tree_merge_kernel<T, D>), dim3((a.B * a.Hkv * a.M + 3) / 4), dim3(256), 0, st, a);
+static hipError_t launch_tree_t(const TreeArgs& a, int rows_wg, hipStream_t st) {
+  const dim3 grid(a.Hkv * a.P * a.MC);
+  if (rows_wg == 16)
+    launch((tree_partial_kernel<T, D>), grid, dim3(64), 0, st, a);
+  else if (rows_wg == 32)
+    launch((tree_wide_kernel<T, D, 1, 2, true>), grid, dim3(128), 0, st, a);
+  else if (rows_wg == 64)
+    launch((tree_wide_kernel<T, D, 1, 4, true>), grid, dim3(256), 0, st, a);
+  else if (rows_wg == 128)
+    launch((tree_wide_kernel<T, D, 2, 4, LO128>), grid, dim3(256), 0, st, a);
+  else
+    launch((tree_wide_kernel<T, D, 2, 8, LO256>), grid, dim3(512), 0, st, a);
+  if (!a.direct) launch((tree_merge_kernel<T, D>), dim3((a.B * a.Hkv * a.M + 3) / 4), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -344,6 +729,10 @@ hipError_t launch_tree_attention(const TreeParams& p, hipStream_t st) {
   a.M = pl.M;
   a.MC = pl.MC;
   a.S = pl.S;
+  a.P = pl.P;
+  a.apart = pl.apart;
+  a.ragged = p.n_sb != 0 && p.B > 1 && p.B <= kTreeRaggedB && pl.S > 1;
+  a.direct = pl.S == 1 && !pl.apart;
   a.div_t = Div::of(p.T);
   a.scale_log2 = p.scale * 1.4426950408889634f;
   auto vec = [](const void* x, int64_t s0, int64_t s1, int64_t s2) {
@@ -360,11 +749,11 @@ hipError_t launch_tree_attention(const TreeParams& p, hipStream_t st) {
   a.o_st = p.o_st;
   a.o_sh = p.o_sh;
   if (p.dtype == kDtypeBf16) {
-    if (p.D == 64) return launch_tree_t<__bf16, 64>(a, st);
-    return launch_tree_t<__bf16, 128>(a, st);
+    if (p.D == 64) return launch_tree_t<__bf16, 64>(a, pl.rows_wg, st);
+    return launch_tree_t<__bf16, 128>(a, pl.rows_wg, st);
   }
-  if (p.D == 64) return launch_tree_t<_Float16, 64>(a, st);
-  return launch_tree_t<_Float16, 128>(a, st);
+  if (p.D == 64) return launch_tree_t<_Float16, 64>(a, pl.rows_wg, st);
+  return launch_tree_t<_Float16, 128>(a, pl.rows_wg, st);
 }
 
 // The walk, by one wave per sequence (lane i looks at nodes i, i + 64, ...).
