@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -19,6 +20,7 @@ DROPKV_FP32 = 3
 
 _c_i64 = ctypes.c_int64
 _c_vp = ctypes.c_void_p
+_c_char_p = ctypes.c_char_p
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
 _c_float = ctypes.c_float
@@ -71,23 +73,32 @@ _SIGNATURES = {
                                          _c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                                          _c_float, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_size, _c_vp]),
     "dropkv_tree_workspace_bytes": (_c_size, [_c_i64] * 6),
-    "dropkv_tree_attention": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
-                                       _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64,
-                                       _c_vp, _c_i64, _c_i64, _c_i64, _c_int,
-                                       _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float,
-                                       _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_size, _c_vp]),
-    "dropkv_tree_commit": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp,
-                                    _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
-                                    _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
-                                    _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp]),
-    "dropkv_norm_rope": (_c_int, [_c_vp] * 14 + [_c_int, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int,
-                                         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_vp]),
+    "dropkv_tree_attention": (_c_int, [_c_char_p, _c_vp]),
+    "dropkv_tree_commit": (_c_int, [_c_char_p, _c_vp]),
+    "dropkv_norm_rope": (_c_int, [_c_char_p, _c_vp]),
     "dropkv_token_logprobs_workspace_bytes": (_c_size, [_c_i64] * 3),
-    "dropkv_token_logprobs": (_c_int, [_c_vp, _c_i64, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp,
-                                       _c_vp, _c_vp, _c_size, _c_vp]),
+    "dropkv_token_logprobs": (_c_int, [_c_char_p, _c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
+
+# Argument structures (dropkv_*_args in include/dropkv_amd.h): fields of eight
+# bytes each, in the header's order.  ``ARGS[name].pack(...)`` makes the bytes
+# that the entry point reads (0 for a null pointer).
+ARG_FIELDS = {
+    "dropkv_tree_attention": "q q_sb q_sh q_st k_new kn_sb kn_sh kn_st v_new vn_sb vn_sh vn_st k_cache v_cache n_rows "
+                             "n_sb mask m_sb m_st m_sj dtype B Hq Hkv T D capacity scale:d out o_sb o_st o_sh "
+                             "workspace workspace_bytes",
+    "dropkv_tree_commit": "tokens parents p_sb choice path accepted k_new kn_sn kn_sb kn_sh kn_st v_new vn_sn vn_sb "
+                          "vn_sh vn_st k_cache v_cache n_rows n_sn n_sb elem_bytes N B H T D capacity",
+    "dropkv_norm_rope": "q q_sb q_sh q_sl q_out qo_sb qo_sh qo_sl k k_sb k_sh k_sl k_out ko_sb ko_sh ko_sl v v_sb v_sh "
+                        "v_sl v_out vo_sb vo_sh vo_sl q_w k_w w_dtype cos sin c_dtype c_sb c_sl positions p_sb c_rows "
+                        "dtype B Hq Hkv L D R eps:d",
+    "dropkv_token_logprobs": "logits row_stride dtype N V tokens top logprob entropy top_logprobs top_ids workspace "
+                             "workspace_bytes",
+}
+ARGS = {name: struct.Struct("@" + "".join("d" if f.endswith(":d") else "q" for f in fields.split()))
+        for name, fields in ARG_FIELDS.items()}
 
 # Size of the static per-GPU scratch of dropkv_evict_noalloc
 # (DROPKV_NOALLOC_SCRATCH_BYTES in include/dropkv_amd.h).

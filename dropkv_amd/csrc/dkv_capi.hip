@@ -539,161 +539,63 @@ size_t dropkv_tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D
   return dkv::tree_workspace_bytes(B, Hq, Hkv, D, T, capacity);
 }
 
-int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k_new, int64_t kn_sb,
-                          int64_t kn_sh, int64_t kn_st, const void* v_new, int64_t vn_sb, int64_t vn_sh,
-                          int64_t vn_st, const void* k_cache, const void* v_cache, const int32_t* n_rows,
-                          int64_t n_sb, const void* mask, int64_t m_sb, int64_t m_st, int64_t m_sj, int dtype,
-                          int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t capacity, float scale,
-                          void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, void* workspace,
-                          size_t workspace_bytes, void* stream) {
+int dropkv_tree_attention(const dropkv_tree_attention_args* a, void* stream) {
   (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
-  if (!q || !k_new || !v_new || !k_cache || !v_cache || !n_rows || !out || !workspace)
+  if (!a || !a->q || !a->k_new || !a->v_new || !a->k_cache || !a->v_cache || !a->n_rows || !a->out || !a->workspace)
     return fail(DROPKV_E_ARG, "null pointer argument");
-  if (dtype != DROPKV_BF16 && dtype != DROPKV_FP16) return fail(DROPKV_E_ARG, "dtype must be bf16 or fp16");
-  const int rc = check_tree_shape(B, Hq, Hkv, T, D, capacity);
+  if (a->dtype != DROPKV_BF16 && a->dtype != DROPKV_FP16) return fail(DROPKV_E_ARG, "dtype must be bf16 or fp16");
+  const int rc = check_tree_shape(a->B, a->Hq, a->Hkv, a->T, a->D, a->capacity);
   if (rc) return rc;
-  if (n_sb != 0 && n_sb != 1) return fail(DROPKV_E_ARG, "n_sb must be 0 or 1");
-  if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(DROPKV_E_ARG, "cache buffers must be 16-byte aligned");
-  const size_t need = dkv::tree_workspace_bytes(B, Hq, Hkv, D, T, capacity);
-  if (workspace_bytes < need)
-    return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
-  dkv::TreeParams p{};
-  p.q = q;
-  p.q_sb = q_sb;
-  p.q_sh = q_sh;
-  p.q_st = q_st;
-  p.k_new = k_new;
-  p.kn_sb = kn_sb;
-  p.kn_sh = kn_sh;
-  p.kn_st = kn_st;
-  p.v_new = v_new;
-  p.vn_sb = vn_sb;
-  p.vn_sh = vn_sh;
-  p.vn_st = vn_st;
-  p.k_cache = k_cache;
-  p.v_cache = v_cache;
-  p.n_rows = n_rows;
-  p.n_sb = (int)n_sb;
-  p.mask = static_cast<const uint8_t*>(mask);
-  p.m_sb = m_sb;
-  p.m_st = m_st;
-  p.m_sj = m_sj;
-  p.dtype = dtype;
-  p.B = (int)B;
-  p.Hq = (int)Hq;
-  p.Hkv = (int)Hkv;
-  p.T = (int)T;
-  p.D = (int)D;
-  p.C = (int)capacity;
-  p.scale = scale;
-  p.out = out;
-  p.o_sb = o_sb;
-  p.o_st = o_st;
-  p.o_sh = o_sh;
-  p.workspace = workspace;
+  if (a->n_sb != 0 && a->n_sb != 1) return fail(DROPKV_E_ARG, "n_sb must be 0 or 1");
+  if (!aligned16(a->k_cache) || !aligned16(a->v_cache))
+    return fail(DROPKV_E_ARG, "cache buffers must be 16-byte aligned");
+  const size_t need = dkv::tree_workspace_bytes(a->B, a->Hq, a->Hkv, a->D, a->T, a->capacity);
+  if (a->workspace_bytes < 0 || (size_t)a->workspace_bytes < need)
+    return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %lld", need,
+                (long long)a->workspace_bytes);
   timing_start(static_cast<hipStream_t>(stream));
-  return hip_status(dkv::launch_tree_attention(p, static_cast<hipStream_t>(stream)), "dropkv_tree_attention launch");
+  return hip_status(dkv::launch_tree_attention(*a, static_cast<hipStream_t>(stream)), "dropkv_tree_attention launch");
 }
 
-int dropkv_tree_commit(const int64_t* tokens, const int32_t* parents, int64_t p_sb, const int64_t* choice,
-                       int32_t* path, int32_t* accepted, const void* k_new, int64_t kn_sn, int64_t kn_sb,
-                       int64_t kn_sh, int64_t kn_st, const void* v_new, int64_t vn_sn, int64_t vn_sb, int64_t vn_sh,
-                       int64_t vn_st, void* k_cache, void* v_cache, const int32_t* n_rows, int64_t n_sn,
-                       int64_t n_sb, int64_t elem_bytes, int64_t N, int64_t B, int64_t H, int64_t T, int64_t D,
-                       int64_t capacity, void* stream) {
+int dropkv_tree_commit(const dropkv_tree_commit_args* a, void* stream) {
   (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
-  if (!tokens || !parents || !choice || !path || !accepted || !k_new || !v_new || !k_cache || !v_cache || !n_rows)
+  if (!a || !a->tokens || !a->parents || !a->choice || !a->path || !a->accepted || !a->k_new || !a->v_new ||
+      !a->k_cache || !a->v_cache || !a->n_rows)
     return fail(DROPKV_E_ARG, "null pointer argument");
-  if (elem_bytes != 2 && elem_bytes != 4) return fail(DROPKV_E_ARG, "elem_bytes must be 2 or 4");
-  if (N < 1 || B < 1 || H < 1 || D < 1 || capacity < 1) return fail(DROPKV_E_ARG, "N, B, H, D, capacity must be positive");
-  if (T < 1 || T > dkv::kTreeMaxT) return fail(DROPKV_E_UNSUPPORTED, "T must be in [1, %d]", (int)dkv::kTreeMaxT);
-  if (D > kMaxRowElems || capacity > INT32_MAX || (double)N * (double)B * (double)H > (double)INT32_MAX)
+  if (a->elem_bytes != 2 && a->elem_bytes != 4) return fail(DROPKV_E_ARG, "elem_bytes must be 2 or 4");
+  if (a->N < 1 || a->B < 1 || a->H < 1 || a->D < 1 || a->capacity < 1)
+    return fail(DROPKV_E_ARG, "N, B, H, D, capacity must be positive");
+  if (a->T < 1 || a->T > dkv::kTreeMaxT)
+    return fail(DROPKV_E_UNSUPPORTED, "T must be in [1, %d]", (int)dkv::kTreeMaxT);
+  if (a->D > kMaxRowElems || a->capacity > INT32_MAX || (double)a->N * (double)a->B * (double)a->H > (double)INT32_MAX)
     return fail(DROPKV_E_UNSUPPORTED, "D, capacity or N*B*H too large");
-  if (p_sb != 0 && p_sb < T) return fail(DROPKV_E_ARG, "p_sb must be 0 or at least T");
-  if (p_sb > INT32_MAX || n_sn < 0 || n_sn > INT32_MAX || n_sb < 0 || n_sb > INT32_MAX)
-    return fail(DROPKV_E_ARG, "strides of parents and n_rows out of range");
-  dkv::CommitParams p{};
-  p.tokens = tokens;
-  p.choice = choice;
-  p.parents = parents;
-  p.p_sb = (int)p_sb;
-  p.path = path;
-  p.accepted = accepted;
-  p.k_new = k_new;
-  p.kn_sn = kn_sn;
-  p.kn_sb = kn_sb;
-  p.kn_sh = kn_sh;
-  p.kn_st = kn_st;
-  p.v_new = v_new;
-  p.vn_sn = vn_sn;
-  p.vn_sb = vn_sb;
-  p.vn_sh = vn_sh;
-  p.vn_st = vn_st;
-  p.k_cache = k_cache;
-  p.v_cache = v_cache;
-  p.n_rows = n_rows;
-  p.n_sn = (int)n_sn;
-  p.n_sb = (int)n_sb;
-  p.elem_bytes = (int)elem_bytes;
-  p.N = (int)N;
-  p.B = (int)B;
-  p.H = (int)H;
-  p.T = (int)T;
-  p.D = (int)D;
-  p.C = (int)capacity;
+  if (a->p_sb != 0 && a->p_sb < a->T) return fail(DROPKV_E_ARG, "p_sb must be 0 or at least T");
+  if (a->n_s[0] < 0 || a->n_s[1] < 0) return fail(DROPKV_E_ARG, "strides of n_rows must not be negative");
   timing_start(static_cast<hipStream_t>(stream));
-  return hip_status(dkv::launch_tree_commit(p, static_cast<hipStream_t>(stream)), "dropkv_tree_commit launch");
+  return hip_status(dkv::launch_tree_commit(*a, static_cast<hipStream_t>(stream)), "dropkv_tree_commit launch");
 }
 
-int dropkv_norm_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* qo_strides, const void* k,
-                     const int64_t* k_strides, void* k_out, const int64_t* ko_strides, const void* v,
-                     const int64_t* v_strides, void* v_out, const int64_t* vo_strides, const void* q_w,
-                     const void* k_w, int w_dtype, const void* cos, const void* sin, int c_dtype, int64_t c_sb,
-                     int64_t c_sl, const int64_t* positions, int64_t p_sb, int64_t c_rows, int dtype, int64_t B,
-                     int64_t Hq, int64_t Hkv, int64_t L, int64_t D, int64_t R, float eps, void* stream) {
+int dropkv_norm_rope(const dropkv_norm_rope_args* a, void* stream) {
   (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
-  if (!q || !q_out || !k || !k_out || !cos || !sin || !q_strides || !qo_strides || !k_strides || !ko_strides)
+  if (!a || !a->q || !a->q_out || !a->k || !a->k_out || !a->cos || !a->sin || (a->v && !a->v_out))
     return fail(DROPKV_E_ARG, "null pointer argument");
-  if (v && (!v_out || !v_strides || !vo_strides)) return fail(DROPKV_E_ARG, "v without v_out or strides");
-  if (dtype != DROPKV_BF16 && dtype != DROPKV_FP16 && dtype != DROPKV_FP32)
+  if (a->dtype != DROPKV_BF16 && a->dtype != DROPKV_FP16 && a->dtype != DROPKV_FP32)
     return fail(DROPKV_E_ARG, "dtype must be bf16, fp16 or fp32");
-  if (c_dtype != DROPKV_FP32 && c_dtype != dtype) return fail(DROPKV_E_ARG, "c_dtype must be fp32 or the inputs' type");
-  if ((q_w || k_w) && w_dtype != DROPKV_FP32 && w_dtype != dtype)
+  if (a->c_dtype != DROPKV_FP32 && a->c_dtype != a->dtype)
+    return fail(DROPKV_E_ARG, "c_dtype must be fp32 or the inputs' type");
+  if ((a->q_w || a->k_w) && a->w_dtype != DROPKV_FP32 && a->w_dtype != a->dtype)
     return fail(DROPKV_E_ARG, "w_dtype must be fp32 or the inputs' type");
-  if (B < 0 || L < 0 || Hq < 1 || Hkv < 1) return fail(DROPKV_E_ARG, "invalid shape");
-  if (D < 2 || D > kMaxRowElems) return fail(DROPKV_E_UNSUPPORTED, "head dim must be in [2, %d]", (int)kMaxRowElems);
-  if (R < 2 || R > D || R % 2) return fail(DROPKV_E_ARG, "R must be even, in [2, D]");
-  if (positions && c_rows < 1) return fail(DROPKV_E_ARG, "c_rows must be positive");
-  if (!(eps >= 0.f)) return fail(DROPKV_E_ARG, "eps must not be negative");
-  if ((double)B * (double)L * ((double)Hq + 2.0 * (double)Hkv) > (double)INT32_MAX)
+  if (a->B < 0 || a->L < 0 || a->Hq < 1 || a->Hkv < 1) return fail(DROPKV_E_ARG, "invalid shape");
+  if (a->D < 2 || a->D > kMaxRowElems)
+    return fail(DROPKV_E_UNSUPPORTED, "head dim must be in [2, %d]", (int)kMaxRowElems);
+  if (a->R < 2 || a->R > a->D || a->R % 2) return fail(DROPKV_E_ARG, "R must be even, in [2, D]");
+  if (a->positions && a->c_rows < 1) return fail(DROPKV_E_ARG, "c_rows must be positive");
+  if (!(a->eps >= 0.)) return fail(DROPKV_E_ARG, "eps must not be negative");
+  if ((double)a->B * (double)a->L * ((double)a->Hq + 2.0 * (double)a->Hkv) > (double)INT32_MAX)
     return fail(DROPKV_E_UNSUPPORTED, "B*L*(Hq + 2*Hkv) above %d", INT32_MAX);
-  if (B * L == 0) return DROPKV_OK;
-  dkv::RopeParams p{};
-  p.q = dkv::RopeTensor{q, q_strides[0], q_strides[1], q_strides[2], q_out, qo_strides[0], qo_strides[1], qo_strides[2]};
-  p.k = dkv::RopeTensor{k, k_strides[0], k_strides[1], k_strides[2], k_out, ko_strides[0], ko_strides[1], ko_strides[2]};
-  if (v)
-    p.v = dkv::RopeTensor{v, v_strides[0], v_strides[1], v_strides[2], v_out, vo_strides[0], vo_strides[1], vo_strides[2]};
-  p.qw = q_w;
-  p.kw = k_w;
-  p.w_f32 = w_dtype == DROPKV_FP32;
-  p.cos = cos;
-  p.sin = sin;
-  p.cos_f32 = c_dtype == DROPKV_FP32;
-  p.c_sb = positions ? 0 : c_sb;
-  p.c_sl = c_sl;
-  p.pos = positions;
-  p.p_sb = p_sb;
-  p.P = c_rows;
-  p.dtype = dtype;
-  p.B = (int)B;
-  p.Hq = (int)Hq;
-  p.Hk = (int)Hkv;
-  p.L = (int)L;
-  p.D = (int)D;
-  p.R = (int)R;
-  p.eps = eps;
+  if (a->B * a->L == 0) return DROPKV_OK;
   timing_start(static_cast<hipStream_t>(stream));
-  return hip_status(dkv::launch_norm_rope(p, static_cast<hipStream_t>(stream)), "dropkv_norm_rope launch");
+  return hip_status(dkv::launch_norm_rope(*a, static_cast<hipStream_t>(stream)), "dropkv_norm_rope launch");
 }
 
 size_t dropkv_token_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top) {
@@ -701,29 +603,26 @@ size_t dropkv_token_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top) 
   return dkv::logprob_workspace_bytes(N, V, top);
 }
 
-int dropkv_token_logprobs(const void* logits, int64_t row_stride, int dtype, int64_t N, int64_t V,
-                          const int64_t* tokens, int64_t top, float* logprob, float* entropy, float* top_logprobs,
-                          int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
+int dropkv_token_logprobs(const dropkv_token_logprobs_args* a, void* stream) {
   (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
-  if (N == 0) return DROPKV_OK;
-  if (!logits || !entropy) return fail(DROPKV_E_ARG, "null pointer argument");
-  if (!tokens != !logprob) return fail(DROPKV_E_ARG, "tokens and logprob go together");
-  if (dtype != DROPKV_BF16 && dtype != DROPKV_FP16 && dtype != DROPKV_FP32)
+  if (!a) return fail(DROPKV_E_ARG, "null pointer argument");
+  if (a->N == 0) return DROPKV_OK;
+  if (!a->logits || !a->entropy) return fail(DROPKV_E_ARG, "null pointer argument");
+  if (!a->tokens != !a->logprob) return fail(DROPKV_E_ARG, "tokens and logprob go together");
+  if (a->dtype != DROPKV_BF16 && a->dtype != DROPKV_FP16 && a->dtype != DROPKV_FP32)
     return fail(DROPKV_E_ARG, "dtype must be bf16, fp16 or fp32");
-  if (N < 0 || V < 1) return fail(DROPKV_E_ARG, "V must be positive");
-  if (N > INT32_MAX || V > kMaxLk) return fail(DROPKV_E_UNSUPPORTED, "N or V too large");
-  if (top < 0 || top > V) return fail(DROPKV_E_ARG, "top must be in [0, V]");
-  if (top > dkv::logprob_max_top())
-    return fail(DROPKV_E_UNSUPPORTED, "top (%lld) above %lld", (long long)top, (long long)dkv::logprob_max_top());
-  if (top > 0 && (!top_logprobs || !top_ids)) return fail(DROPKV_E_ARG, "null top_logprobs/top_ids");
-  const size_t need = dkv::logprob_workspace_bytes(N, V, top);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  if (a->N < 0 || a->V < 1) return fail(DROPKV_E_ARG, "V must be positive");
+  if (a->N > INT32_MAX || a->V > kMaxLk) return fail(DROPKV_E_UNSUPPORTED, "N or V too large");
+  if (a->top < 0 || a->top > a->V) return fail(DROPKV_E_ARG, "top must be in [0, V]");
+  if (a->top > dkv::logprob_max_top())
+    return fail(DROPKV_E_UNSUPPORTED, "top (%lld) above %lld", (long long)a->top, (long long)dkv::logprob_max_top());
+  if (a->top > 0 && (!a->top_logprobs || !a->top_ids)) return fail(DROPKV_E_ARG, "null top_logprobs/top_ids");
+  const size_t need = dkv::logprob_workspace_bytes(a->N, a->V, a->top);
+  if (need && (!a->workspace || a->workspace_bytes < 0 || (size_t)a->workspace_bytes < need))
+    return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %lld", need,
+                (long long)a->workspace_bytes);
   timing_start(static_cast<hipStream_t>(stream));
-  return hip_status(dkv::launch_token_logprobs(dkv::LogprobParams{logits, row_stride, dtype, N, V, top, tokens, logprob,
-                                                                  entropy, top_logprobs, top_ids, workspace},
-                                               static_cast<hipStream_t>(stream)),
-                    "dropkv_token_logprobs launch");
+  return hip_status(dkv::launch_token_logprobs(*a, static_cast<hipStream_t>(stream)), "dropkv_token_logprobs launch");
 }
 
 int dropkv_selftest_mfma(float* out, void* stream) {

@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/dropkv_amd.h"
+
 namespace dkv {
 
 // Kernel timing (dropkv_timing_*): when enabled on the calling thread,
@@ -133,88 +135,17 @@ struct DecodeParams {
 size_t decode_workspace_bytes(int B, int Hq, int Hkv, int D, int C);
 hipError_t launch_decode_attention(const DecodeParams& p, hipStream_t st);
 
-// Attention of drafted tokens over the cache (dkv_tree.hip).
-struct TreeParams {
-  const void* q;  // [B, Hq, T, D] element strides, D contiguous
-  int64_t q_sb, q_sh, q_st;
-  const void* k_new;  // drafted K and V rows [B, Hkv, T, D], D contiguous
-  int64_t kn_sb, kn_sh, kn_st;
-  const void* v_new;
-  int64_t vn_sb, vn_sh, vn_st;
-  const void* k_cache;  // [B, Hkv, C, D] contiguous
-  const void* v_cache;
-  const int* n_rows;  // device: rows stored of sequence b at b * n_sb
-  int n_sb;
-  const uint8_t* mask;  // may be null: a chain
-  int64_t m_sb, m_st, m_sj;
-  int dtype, B, Hq, Hkv, T, D, C;
-  float scale;
-  void* out;  // [B, T, Hq, D] element strides, D contiguous
-  int64_t o_sb, o_st, o_sh;
-  void* workspace;
-};
-size_t tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C);
-hipError_t launch_tree_attention(const TreeParams& p, hipStream_t st);
-// The accepted path of each tree and its rows appended to the caches.
-struct CommitParams {
-  const int64_t* tokens;  // [B, T] contiguous
-  const int64_t* choice;
-  const int* parents;  // sequence b's at b * p_sb
-  int p_sb;
-  int* path;  // [B, T] contiguous
-  int* accepted;
-  const void* k_new;  // [N, B, H, T, D] element strides, D contiguous
-  int64_t kn_sn, kn_sb, kn_sh, kn_st;
-  const void* v_new;
-  int64_t vn_sn, vn_sb, vn_sh, vn_st;
-  void* k_cache;  // [N, B, H, C, D] contiguous
-  void* v_cache;
-  const int* n_rows;
-  int n_sn, n_sb;
-  int elem_bytes, N, B, H, T, D, C;
-};
+// Attention of drafted tokens over the cache, and the accepted path's rows
+// appended to it (dkv_tree.hip); norms and rotation (dkv_norm_rope.hip); log
+// probabilities (dkv_logprob.hip).  The arguments are the C ABI's, checked.
 constexpr int64_t kTreeMaxT = 256;
-hipError_t launch_tree_commit(const CommitParams& p, hipStream_t st);
-
-// Norms and rotation of queries and keys (dkv_norm_rope.hip).
-struct RopeTensor {
-  const void* src;  // [B, H, L, D] element strides, D contiguous
-  int64_t s_sb, s_sh, s_sl;
-  void* dst;
-  int64_t d_sb, d_sh, d_sl;
-};
-struct RopeParams {
-  RopeTensor q, k, v;  // v.src null: no values
-  const void* qw;      // may be null
-  const void* kw;
-  int w_f32;
-  const void* cos;
-  const void* sin;
-  int cos_f32;
-  int64_t c_sb, c_sl;
-  const int64_t* pos;  // may be null
-  int64_t p_sb, P;
-  int dtype, B, Hq, Hk, L, D, R;
-  float eps;
-};
-hipError_t launch_norm_rope(const RopeParams& p, hipStream_t st);
-
-// Log probabilities, entropy and top tokens of rows of logits (dkv_logprob.hip).
-struct LogprobParams {
-  const void* logits;  // [N, V], V contiguous
-  int64_t row_stride;
-  int dtype;
-  int64_t N, V, top;
-  const int64_t* tokens;  // [N] or null
-  float* logprob;         // [N] (tokens given)
-  float* entropy;         // [N]
-  float* top_logprobs;    // [N, top]
-  int64_t* top_ids;
-  void* workspace;
-};
+size_t tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C);
+hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_t st);
+hipError_t launch_tree_commit(const dropkv_tree_commit_args& p, hipStream_t st);
+hipError_t launch_norm_rope(const dropkv_norm_rope_args& p, hipStream_t st);
 int64_t logprob_max_top();
 size_t logprob_workspace_bytes(int64_t N, int64_t V, int64_t top);
-hipError_t launch_token_logprobs(const LogprobParams& p, hipStream_t st);
+hipError_t launch_token_logprobs(const dropkv_token_logprobs_args& p, hipStream_t st);
 
 size_t select_workspace_bytes(int64_t rows, int64_t Lk);
 // Workspace of a layer-call: the plan's, the scores and the selection's.

@@ -325,7 +325,7 @@ static LogprobPlan logprob_plan(int64_t N, int64_t V, int64_t top) {
   LogprobPlan p;
   p.S = (int)((tiles + per - 1) / per);
   p.seg = (int)std::min<int64_t>(per * kLpTile, INT32_MAX - kLpTile);
-  p.bytes = p.S == 1 ? 0 : (size_t)N * p.S * (3 * sizeof(float) + (size_t)top * sizeof(uint64_t)) + 256;
+  p.bytes = p.S == 1 ? 0 : kSyncBytes + (size_t)N * p.S * (3 * sizeof(float) + (size_t)top * sizeof(uint64_t)) + 256;
   return p;
 }
 size_t logprob_workspace_bytes(int64_t N, int64_t V, int64_t top) { return logprob_plan(N, V, top).bytes; }
@@ -344,7 +344,7 @@ static hipError_t launch_logprob_t(const LogprobArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t launch_token_logprobs(const LogprobParams& p, hipStream_t st) {
+hipError_t launch_token_logprobs(const dropkv_token_logprobs_args& p, hipStream_t st) {
   const LogprobPlan pl = logprob_plan(p.N, p.V, p.top);
   LogprobArgs a{};
   a.x = p.logits;
@@ -356,8 +356,8 @@ hipError_t launch_token_logprobs(const LogprobParams& p, hipStream_t st) {
   a.S = pl.S;
   a.seg = pl.seg;
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
-  a.keys = reinterpret_cast<uint64_t*>(ws);
-  a.part = reinterpret_cast<float*>(ws + (size_t)p.N * pl.S * p.top * sizeof(uint64_t));
+  a.keys = reinterpret_cast<uint64_t*>(ws + kSyncBytes);
+  a.part = reinterpret_cast<float*>(a.keys + (size_t)p.N * pl.S * p.top);
   a.logprob = p.logprob;
   a.entropy = p.entropy;
   a.top_lp = p.top_logprobs;

@@ -226,49 +226,50 @@ static hipError_t launch_rope_t(RopeArgs a, bool vec, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t launch_norm_rope(const RopeParams& p, hipStream_t st) {
+hipError_t launch_norm_rope(const dropkv_norm_rope_args& p, hipStream_t st) {
   RopeArgs a{};
-  const RopeTensor* t[3] = {&p.q, &p.k, &p.v};
-  const int64_t eb = p.dtype == kDtypeFp32 ? 4 : 2, cb = p.cos_f32 ? 4 : eb;
+  const int64_t eb = p.dtype == kDtypeFp32 ? 4 : 2, cb = p.c_dtype == kDtypeFp32 ? 4 : eb;
   uint64_t all = 0;
-  for (int i = 0; i < 3; ++i) {
-    a.src[i] = t[i]->src;
-    a.dst[i] = t[i]->dst;
-    a.s_sb[i] = t[i]->s_sb;
-    a.s_sh[i] = t[i]->s_sh;
-    a.s_sl[i] = t[i]->s_sl;
-    a.d_sb[i] = t[i]->d_sb;
-    a.d_sh[i] = t[i]->d_sh;
-    a.d_sl[i] = t[i]->d_sl;
-    if (t[i]->src)
-      all |= reinterpret_cast<uintptr_t>(t[i]->src) | reinterpret_cast<uintptr_t>(t[i]->dst) |
-             (uint64_t)((t[i]->s_sb | t[i]->s_sh | t[i]->s_sl | t[i]->d_sb | t[i]->d_sh | t[i]->d_sl) * eb);
-  }
-  a.w[0] = p.qw;
-  a.w[1] = p.kw;
-  a.w_f32 = p.w_f32;
+  auto tensor = [&](int i, const void* src, const int64_t* s, void* dst, const int64_t* d) {
+    a.src[i] = src;
+    a.dst[i] = dst;
+    a.s_sb[i] = s[0];
+    a.s_sh[i] = s[1];
+    a.s_sl[i] = s[2];
+    a.d_sb[i] = d[0];
+    a.d_sh[i] = d[1];
+    a.d_sl[i] = d[2];
+    all |= reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) |
+           (uint64_t)((s[0] | s[1] | s[2] | d[0] | d[1] | d[2]) * eb);
+  };
+  tensor(0, p.q, p.q_s, p.q_out, p.qo_s);
+  tensor(1, p.k, p.k_s, p.k_out, p.ko_s);
+  if (p.v) tensor(2, p.v, p.v_s, p.v_out, p.vo_s);
+  a.w[0] = p.q_w;
+  a.w[1] = p.k_w;
+  a.w_f32 = p.w_dtype == kDtypeFp32;
   a.cos = p.cos;
   a.sin = p.sin;
-  a.c_sb = p.c_sb;
+  a.c_sb = p.positions ? 0 : p.c_sb;
   a.c_sl = p.c_sl;
-  a.pos = p.pos;
+  a.pos = p.positions;
   a.p_sb = p.p_sb;
-  a.P = p.P;
-  a.L = p.L;
-  a.tokens = p.B * p.L;
-  a.Hq = p.Hq;
-  a.Hk = p.Hk;
-  a.Hv = p.v.src ? p.Hk : 0;
-  a.D = p.D;
-  a.R = p.R;
-  a.eps = p.eps;
-  all |= reinterpret_cast<uintptr_t>(p.qw) | reinterpret_cast<uintptr_t>(p.kw) | reinterpret_cast<uintptr_t>(p.cos) |
-         reinterpret_cast<uintptr_t>(p.sin) | (uint64_t)((p.c_sb | p.c_sl) * cb);
+  a.P = p.c_rows;
+  a.L = (int)p.L;
+  a.tokens = (int)(p.B * p.L);
+  a.Hq = (int)p.Hq;
+  a.Hk = (int)p.Hkv;
+  a.Hv = p.v ? (int)p.Hkv : 0;
+  a.D = (int)p.D;
+  a.R = (int)p.R;
+  a.eps = (float)p.eps;
+  all |= reinterpret_cast<uintptr_t>(p.q_w) | reinterpret_cast<uintptr_t>(p.k_w) | reinterpret_cast<uintptr_t>(p.cos) |
+         reinterpret_cast<uintptr_t>(p.sin) | (uint64_t)((a.c_sb | a.c_sl) * cb);
   const bool vec = all % 16 == 0 && p.R % 16 == 0;
   if (p.dtype == kDtypeFp32) return launch_rope_t<float, float>(a, vec, st);
   if (p.dtype == kDtypeBf16)
-    return p.cos_f32 ? launch_rope_t<__bf16, float>(a, vec, st) : launch_rope_t<__bf16, __bf16>(a, vec, st);
-  return p.cos_f32 ? launch_rope_t<_Float16, float>(a, vec, st) : launch_rope_t<_Float16, _Float16>(a, vec, st);
+    return cb == 4 ? launch_rope_t<__bf16, float>(a, vec, st) : launch_rope_t<__bf16, __bf16>(a, vec, st);
+  return cb == 4 ? launch_rope_t<_Float16, float>(a, vec, st) : launch_rope_t<_Float16, _Float16>(a, vec, st);
 }
 
 }  // namespace dkv

@@ -26,10 +26,20 @@ namespace dkv {
 
 #ifndef W16
 #define W16 2048
+#endif
+#ifndef W64
 #define W64 512
+#endif
+#ifndef W128
 #define W128 512
+#endif
+#ifndef W256
 #define W256 256
+#endif
+#ifndef LO128
 #define LO128 true
+#endif
+#ifndef LO256
 #define LO256 true
 #endif
 constexpr int kTreeTile = 32;       // keys per tile
@@ -673,7 +683,7 @@ static TreePlan tree_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t
   p.apart = p.rows_wg == 16 || chunks * p.S < 192;
   p.P = (int)(B * (p.S + p.apart));
   p.rows = (size_t)Hkv * p.P * p.M;
-  p.bytes = p.rows * sizeof(float) * (2 + (size_t)D) + 256;
+  p.bytes = kSyncBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
   return p;
 }
 size_t tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C) {
@@ -697,35 +707,35 @@ static hipError_t launch_tree_t(const TreeArgs& a, int rows_wg, hipStream_t st) 
   return hipGetLastError();
 }
 
-hipError_t launch_tree_attention(const TreeParams& p, hipStream_t st) {
-  const TreePlan pl = tree_plan(p.B, p.Hq, p.Hkv, p.D, p.T, p.C);
+hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_t st) {
+  const TreePlan pl = tree_plan(p.B, p.Hq, p.Hkv, p.D, p.T, p.capacity);
   TreeArgs a{};
   a.q = p.q;
-  a.q_sb = p.q_sb;
-  a.q_sh = p.q_sh;
-  a.q_st = p.q_st;
+  a.q_sb = p.q_s[0];
+  a.q_sh = p.q_s[1];
+  a.q_st = p.q_s[2];
   a.kn = p.k_new;
   a.vn = p.v_new;
-  a.kn_sb = p.kn_sb;
-  a.kn_sh = p.kn_sh;
-  a.kn_st = p.kn_st;
-  a.vn_sb = p.vn_sb;
-  a.vn_sh = p.vn_sh;
-  a.vn_st = p.vn_st;
+  a.kn_sb = p.kn_s[0];
+  a.kn_sh = p.kn_s[1];
+  a.kn_st = p.kn_s[2];
+  a.vn_sb = p.vn_s[0];
+  a.vn_sh = p.vn_s[1];
+  a.vn_st = p.vn_s[2];
   a.kbuf = p.k_cache;
   a.vbuf = p.v_cache;
   a.n_rows = p.n_rows;
-  a.n_sb = p.n_sb;
-  a.mask = p.mask;
-  a.m_sb = p.m_sb;
-  a.m_st = p.m_st;
-  a.m_sj = p.m_sj;
-  a.B = p.B;
-  a.Hq = p.Hq;
-  a.Hkv = p.Hkv;
-  a.D = p.D;
-  a.T = p.T;
-  a.C = p.C;
+  a.n_sb = (int)p.n_sb;
+  a.mask = static_cast<const uint8_t*>(p.mask);
+  a.m_sb = p.m_s[0];
+  a.m_st = p.m_s[1];
+  a.m_sj = p.m_s[2];
+  a.B = (int)p.B;
+  a.Hq = (int)p.Hq;
+  a.Hkv = (int)p.Hkv;
+  a.D = (int)p.D;
+  a.T = (int)p.T;
+  a.C = (int)p.capacity;
   a.M = pl.M;
   a.MC = pl.MC;
   a.S = pl.S;
@@ -733,21 +743,21 @@ hipError_t launch_tree_attention(const TreeParams& p, hipStream_t st) {
   a.apart = pl.apart;
   a.ragged = p.n_sb != 0 && p.B > 1 && p.B <= kTreeRaggedB && pl.S > 1;
   a.direct = pl.S == 1 && !pl.apart;
-  a.div_t = Div::of(p.T);
-  a.scale_log2 = p.scale * 1.4426950408889634f;
-  auto vec = [](const void* x, int64_t s0, int64_t s1, int64_t s2) {
-    return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
+  a.div_t = Div::of(a.T);
+  a.scale_log2 = (float)p.scale * 1.4426950408889634f;
+  auto vec = [](const void* x, const int64_t* s) {
+    return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
   };
-  a.qvec = vec(p.q, p.q_sb, p.q_sh, p.q_st);
-  a.nvec = vec(p.k_new, p.kn_sb, p.kn_sh, p.kn_st) && vec(p.v_new, p.vn_sb, p.vn_sh, p.vn_st);
+  a.qvec = vec(p.q, p.q_s);
+  a.nvec = vec(p.k_new, p.kn_s) && vec(p.v_new, p.vn_s);
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
-  a.part_m = reinterpret_cast<float*>(ws);
+  a.part_m = reinterpret_cast<float*>(ws + kSyncBytes);
   a.part_l = a.part_m + pl.rows;
   a.part_o = a.part_m + ((2 * pl.rows + 3) & ~(size_t)3);
   a.out = p.out;
-  a.o_sb = p.o_sb;
-  a.o_st = p.o_st;
-  a.o_sh = p.o_sh;
+  a.o_sb = p.o_s[0];
+  a.o_st = p.o_s[1];
+  a.o_sh = p.o_s[2];
   if (p.dtype == kDtypeBf16) {
     if (p.D == 64) return launch_tree_t<__bf16, 64>(a, pl.rows_wg, st);
     return launch_tree_t<__bf16, 128>(a, pl.rows_wg, st);
@@ -764,7 +774,7 @@ struct CommitArgs {
   const int64_t* tokens;  // [B, T]
   const int64_t* choice;
   const int* parents;
-  int p_sb;  // 0: one tree for every sequence
+  int64_t p_sb;  // 0: one tree for every sequence
   int T;
   int* path;  // [B, T]
   int* accepted;
@@ -774,7 +784,7 @@ struct CommitArgs {
   uint8_t* kbuf;  // [N, B, H, C, row] contiguous
   uint8_t* vbuf;
   const int* n_rows;
-  int n_sn, n_sb;
+  int64_t n_sn, n_sb;
   int B, H, C, units;  // units per row
 };
 
@@ -783,7 +793,7 @@ __global__ void __launch_bounds__(64) tree_walk_kernel(CommitArgs a) {
   const int b = blockIdx.x, lane = threadIdx.x;
   const int64_t* tok = a.tokens + (int64_t)b * a.T;
   const int64_t* cho = a.choice + (int64_t)b * a.T;
-  const int* par = a.parents + (int64_t)b * a.p_sb;
+  const int* par = a.parents + b * a.p_sb;
   int parent[NL];  // of nodes whose token is their parent's choice; -1 otherwise
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
@@ -815,7 +825,7 @@ __global__ void __launch_bounds__(64) tree_walk_kernel(CommitArgs a) {
 template <typename U>
 __global__ void __launch_bounds__(256) tree_commit_kernel(CommitArgs a) {
   const int h = blockIdx.x % a.H, b = (blockIdx.x / a.H) % a.B, l = blockIdx.x / (a.H * a.B);
-  const int n = a.n_rows[(int64_t)l * a.n_sn + (int64_t)b * a.n_sb];
+  const int n = a.n_rows[l * a.n_sn + b * a.n_sb];
   const int len = a.accepted[b];
   if (n < 0) return;
   const int fit = min(len, a.C - n);  // (rows past the capacity are not stored)
@@ -830,35 +840,35 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(CommitArgs a) {
   }
 }
 
-hipError_t launch_tree_commit(const CommitParams& p, hipStream_t st) {
+hipError_t launch_tree_commit(const dropkv_tree_commit_args& p, hipStream_t st) {
   CommitArgs a{};
   a.tokens = p.tokens;
   a.choice = p.choice;
   a.parents = p.parents;
   a.p_sb = p.p_sb;
-  a.T = p.T;
+  a.T = (int)p.T;
   a.path = p.path;
   a.accepted = p.accepted;
   const int64_t eb = p.elem_bytes;
   a.kn = static_cast<const uint8_t*>(p.k_new);
   a.vn = static_cast<const uint8_t*>(p.v_new);
-  a.kn_sn = p.kn_sn * eb;
-  a.kn_sb = p.kn_sb * eb;
-  a.kn_sh = p.kn_sh * eb;
-  a.kn_st = p.kn_st * eb;
-  a.vn_sn = p.vn_sn * eb;
-  a.vn_sb = p.vn_sb * eb;
-  a.vn_sh = p.vn_sh * eb;
-  a.vn_st = p.vn_st * eb;
+  a.kn_sn = p.kn_s[0] * eb;
+  a.kn_sb = p.kn_s[1] * eb;
+  a.kn_sh = p.kn_s[2] * eb;
+  a.kn_st = p.kn_s[3] * eb;
+  a.vn_sn = p.vn_s[0] * eb;
+  a.vn_sb = p.vn_s[1] * eb;
+  a.vn_sh = p.vn_s[2] * eb;
+  a.vn_st = p.vn_s[3] * eb;
   a.kbuf = static_cast<uint8_t*>(p.k_cache);
   a.vbuf = static_cast<uint8_t*>(p.v_cache);
   a.n_rows = p.n_rows;
-  a.n_sn = p.n_sn;
-  a.n_sb = p.n_sb;
-  a.B = p.B;
-  a.H = p.H;
-  a.C = p.C;
-  launch(tree_walk_kernel, dim3(p.B), dim3(64), 0, st, a);
+  a.n_sn = p.n_s[0];
+  a.n_sb = p.n_s[1];
+  a.B = (int)p.B;
+  a.H = (int)p.H;
+  a.C = (int)p.capacity;
+  launch(tree_walk_kernel, dim3(a.B), dim3(64), 0, st, a);
   const int64_t all = (int64_t)reinterpret_cast<uintptr_t>(a.kn) | (int64_t)reinterpret_cast<uintptr_t>(a.vn) |
                       (int64_t)reinterpret_cast<uintptr_t>(a.kbuf) | (int64_t)reinterpret_cast<uintptr_t>(a.vbuf) |
                       a.kn_sn | a.kn_sb | a.kn_sh | a.kn_st | a.vn_sn | a.vn_sb | a.vn_sh | a.vn_st | (p.D * eb);
@@ -867,10 +877,10 @@ hipError_t launch_tree_commit(const CommitParams& p, hipStream_t st) {
     a.units = (int)(p.D * eb / 16);
     launch(tree_commit_kernel<u32x4>, grid, dim3(256), 0, st, a);
   } else if (eb == 4) {
-    a.units = p.D;
+    a.units = (int)p.D;
     launch(tree_commit_kernel<uint32_t>, grid, dim3(256), 0, st, a);
   } else {
-    a.units = p.D;
+    a.units = (int)p.D;
     launch(tree_commit_kernel<uint16_t>, grid, dim3(256), 0, st, a);
   }
   return hipGetLastError();

@@ -9,7 +9,6 @@ alignment) and raise ``RuntimeError`` otherwise; the reference-compatible
 
 from __future__ import annotations
 
-import ctypes
 import threading
 from typing import NamedTuple, Optional
 
@@ -403,25 +402,47 @@ def decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, 
     return out
 
 
-def _call(dev: torch.device, name: str, *args) -> None:
-    """Entry point ``name`` on the current stream of ``dev``, with ``dev`` current."""
+# The wrappers below check by attribute reads of ~0.1 us each and hand the entry
+# point one packed structure: for a call of a few rows their host time is the
+# larger part of it.
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call(name: str, index: int, args: bytes) -> None:
+    """Entry point ``name`` on the current stream of device ``index``, with that
+    device current."""
     fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _stream(dev))
+    if _current_device() == index:
+        rc = fn(args, _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream)
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _stream(dev))
-    _lib.check(rc, name)
+        with torch.cuda.device(index):
+            rc = fn(args, torch.cuda.current_stream(index).cuda_stream)
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _device_index(name: str, *ts) -> int:
+    """The device that all of ``ts`` (None left out) are on."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            index = -1
+            break
+    if index < 0:
+        raise RuntimeError(f"{name}: all tensors must be on one ROCm (cuda) device")
+    return index
 
 
 def _no_grad(name: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+    for t in ts:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with its last axis contiguous."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 else t.contiguous()
 
 
 def tree_workspace(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int, device) -> torch.Tensor:
@@ -430,7 +451,10 @@ def tree_workspace(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int, dev
     nbytes = _lib.load().dropkv_tree_workspace_bytes(B, Hq, Hkv, D, T, capacity)
     if nbytes == 0:
         raise RuntimeError("unsupported tree geometry")
-    return _workspace(nbytes, torch.device(device))
+    return _evict_workspace(nbytes, torch.device(device))
+
+
+_TREE_ARGS = _lib.ARGS["dropkv_tree_attention"].pack
 
 
 def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor,
@@ -444,49 +468,66 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     (second to last axis) sees which; without it they are a chain.  Returns
     ``out`` [B, T, Hq, D]; a row that sees no key is zeros.  The buffers are not
     written: ``tree_commit`` stores the rows of the tokens that stand."""
-    dev = _check_device(q, k_new, v_new, k_cache, v_cache, n_rows)
-    _no_grad("tree_attention", q, k_new, v_new, k_cache, v_cache)
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    index = _device_index("tree_attention", q, k_new, v_new, k_cache, v_cache, n_rows, out, workspace, mask)
+    if torch.is_grad_enabled():
+        _no_grad("tree_attention", q, k_new, v_new, k_cache, v_cache, out)
+    dtype = q.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise RuntimeError("tree_attention: the dtype must be bf16 or fp16")
-    for t in (k_new, v_new, k_cache, v_cache):
-        if t.dtype != q.dtype:
-            raise RuntimeError("tree_attention: all tensors must share a dtype")
-    if q.dim() != 4 or k_new.dim() != 4:
-        raise RuntimeError("tree_attention: q, k_new and v_new must be [B, H, T, D]")
-    B, Hq, T, D = q.shape
-    _check_buffer(k_cache, "k_cache")
-    _check_buffer(v_cache, "v_cache")
-    Hkv, C = k_cache.shape[1], k_cache.shape[2]
-    if k_new.shape != (B, Hkv, T, D) or v_new.shape != k_new.shape:
-        raise RuntimeError("tree_attention: k_new and v_new must be [B, Hkv, T, D]")
-    if k_cache.shape != (B, Hkv, C, D) or v_cache.shape != k_cache.shape:
+    if not dtype is k_new.dtype is v_new.dtype is k_cache.dtype is v_cache.dtype:
+        raise RuntimeError("tree_attention: all tensors must share a dtype")
+    shape, kshape, cshape = q.shape, k_new.shape, k_cache.shape
+    if len(shape) != 4 or len(kshape) != 4 or v_new.shape != kshape:
+        raise RuntimeError("tree_attention: q must be [B, Hq, T, D], k_new and v_new [B, Hkv, T, D]")
+    B, Hq, T, D = shape
+    if len(cshape) != 4 or v_cache.shape != cshape:
         raise RuntimeError("tree_attention: the cache buffers must be [B, Hkv, capacity, D]")
-    if n_rows.dtype != torch.int32 or n_rows.numel() not in (1, B) or not n_rows.is_contiguous():
+    cB, Hkv, C, cD = cshape
+    if cB != B or cD != D or kshape != (B, Hkv, T, D):
+        raise RuntimeError("tree_attention: q, k_new, v_new and the cache buffers do not fit one another")
+    k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or (k_ptr | v_ptr) & 15:
+        raise RuntimeError("tree_attention: the cache buffers must be contiguous and 16-byte aligned")
+    counts = n_rows.numel()
+    if n_rows.dtype is not torch.int32 or (counts != 1 and counts != B) or not n_rows.is_contiguous():
         raise RuntimeError("tree_attention: n_rows must hold one int32 count, or one per sequence")
-    m_ptr, m_strides = None, (0, 0, 0)
+    m_ptr = m_b = m_t = m_j = 0
     if mask is not None:
-        _check_device(q, mask)
-        if mask.dtype != torch.bool or mask.shape not in ((T, T), (B, T, T)):
+        mshape = mask.shape
+        if mask.dtype is not torch.bool or (mshape != (T, T) and mshape != (B, T, T)):
             raise RuntimeError("tree_attention: mask must be bool, [T, T] or [B, T, T]")
         m_ptr = mask.data_ptr()
-        m_strides = (0, *mask.stride()) if mask.dim() == 2 else mask.stride()
+        if len(mshape) == 2:
+            m_t, m_j = mask.stride()
+        else:
+            m_b, m_t, m_j = mask.stride()
     if out is None:
-        out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=dev)
-    else:
-        _check_device(q, out)
-        if out.shape != (B, T, Hq, D) or out.dtype != q.dtype or (out.stride(3) != 1 and D > 1):
-            raise RuntimeError("tree_attention: out must be [B, T, Hq, D] of q's dtype, D contiguous")
+        out = torch.empty((B, T, Hq, D), dtype=dtype, device=q.device)
+    elif out.shape != (B, T, Hq, D) or out.dtype is not dtype or out.stride(3) != 1:
+        raise RuntimeError("tree_attention: out must be [B, T, Hq, D] of q's dtype, D contiguous")
     if workspace is None:
-        workspace = tree_workspace(B, Hq, Hkv, D, T, C, dev)
-    else:
-        _check_device(q, workspace)
-    q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)
-    qs, ks, vs, os = q.stride(), k_new.stride(), v_new.stride(), out.stride()
-    _call(dev, "dropkv_tree_attention", q.data_ptr(), qs[0], qs[1], qs[2], k_new.data_ptr(), ks[0], ks[1], ks[2],
-          v_new.data_ptr(), vs[0], vs[1], vs[2], k_cache.data_ptr(), v_cache.data_ptr(), n_rows.data_ptr(),
-          int(n_rows.numel() > 1), m_ptr, *m_strides, _DTYPE_CODE[q.dtype], B, Hq, Hkv, T, D, C, float(scale),
-          out.data_ptr(), os[0], os[1], os[2], workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        nbytes = _lib.load().dropkv_tree_workspace_bytes(B, Hq, Hkv, D, T, C)
+        if nbytes == 0:
+            raise RuntimeError("tree_attention: unsupported geometry")
+        workspace = _stream_workspace(nbytes, q.device)
+    q_b, q_h, q_t, q_d = q.stride()
+    if q_d != 1:
+        q_b, q_h, q_t, _ = (q := q.contiguous()).stride()
+    kn_b, kn_h, kn_t, kn_d = k_new.stride()
+    if kn_d != 1:
+        kn_b, kn_h, kn_t, _ = (k_new := k_new.contiguous()).stride()
+    vn_b, vn_h, vn_t, vn_d = v_new.stride()
+    if vn_d != 1:
+        vn_b, vn_h, vn_t, _ = (v_new := v_new.contiguous()).stride()
+    o_b, o_t, o_h, _ = out.stride()
+    _call("dropkv_tree_attention", index, _TREE_ARGS(
+        q.data_ptr(), q_b, q_h, q_t, k_new.data_ptr(), kn_b, kn_h, kn_t, v_new.data_ptr(), vn_b, vn_h, vn_t, k_ptr,
+        v_ptr, n_rows.data_ptr(), counts > 1, m_ptr, m_b, m_t, m_j, _DTYPE_CODE[dtype], B, Hq, Hkv, T, D, C, scale,
+        out.data_ptr(), o_b, o_t, o_h, workspace.data_ptr(), workspace.nbytes))
     return out
+
+
+_COMMIT_ARGS = _lib.ARGS["dropkv_tree_commit"].pack
 
 
 def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tensor, k_new: torch.Tensor,
@@ -500,39 +541,61 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tenso
     an axis N in front; ``n_rows`` int32, [1] or [B], or [N, 1] or [N, B].
     Returns ``(path [B, T] int32, the nodes that stand, then -1; accepted [B]
     int32)``.  ``n_rows`` is not advanced."""
-    dev = _check_device(tokens, parents, choice, k_new, v_new, k_cache, v_cache, n_rows)
-    _no_grad("tree_commit", k_new, v_new, k_cache, v_cache)
-    if tokens.dim() != 2 or choice.shape != tokens.shape or tokens.dtype != torch.int64 or choice.dtype != torch.int64:
+    index = _device_index("tree_commit", tokens, parents, choice, k_new, v_new, k_cache, v_cache, n_rows)
+    if torch.is_grad_enabled():
+        _no_grad("tree_commit", k_new, v_new, k_cache, v_cache)
+    tshape = tokens.shape
+    if len(tshape) != 2 or choice.shape != tshape or not tokens.dtype is choice.dtype is torch.int64:
         raise RuntimeError("tree_commit: tokens and choice must be int64 [B, T]")
-    B, T = tokens.shape
-    if parents.dtype != torch.int32 or parents.shape not in ((T,), (1, T), (B, T)):
+    B, T = tshape
+    pshape, cshape = parents.shape, k_cache.shape
+    if parents.dtype is not torch.int32 or (pshape != (B, T) and pshape != (T,) and pshape != (1, T)):
         raise RuntimeError("tree_commit: parents must be int32 [T] or [B, T]")
-    if k_cache.dim() not in (4, 5) or k_new.dim() != k_cache.dim():
-        raise RuntimeError("tree_commit: rows and buffers must be [B, H, ., D] or [N, B, H, ., D]")
+    layers = len(cshape) == 5
+    if not (layers or len(cshape) == 4) or v_cache.shape != cshape:
+        raise RuntimeError("tree_commit: the buffers must be [B, H, capacity, D] or [N, B, H, capacity, D]")
+    *lead, H, C, D = cshape
+    if lead[-1] != B or k_new.shape != (*lead, H, T, D) or v_new.shape != k_new.shape:
+        raise RuntimeError("tree_commit: tokens, rows and buffers do not fit one another")
+    dtype = k_cache.dtype
+    if dtype not in _DTYPE_CODE or not dtype is v_cache.dtype is k_new.dtype is v_new.dtype:
+        raise RuntimeError("tree_commit: rows and buffers must share a bf16, fp16 or fp32 dtype")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise RuntimeError("tree_commit: the cache buffers must be contiguous")
-    *lead, H, C, D = k_cache.shape
-    if lead[-1] != B or k_new.shape != (*lead, H, T, D) or v_new.shape != k_new.shape or v_cache.shape != k_cache.shape:
-        raise RuntimeError("tree_commit: shape mismatch")
-    if not k_cache.dtype == v_cache.dtype == k_new.dtype == v_new.dtype or k_cache.dtype not in _DTYPE_CODE:
-        raise RuntimeError("tree_commit: rows and buffers must share a bf16, fp16 or fp32 dtype")
-    if n_rows.dtype != torch.int32 or n_rows.dim() != len(lead) or any(
-            a not in (1, b) for a, b in zip(n_rows.shape, lead)) or (len(lead) == 2 and n_rows.shape[0] != lead[0]):
+    N = lead[0] if layers else 1
+    nshape = n_rows.shape
+    if n_rows.dtype is not torch.int32 or len(nshape) != len(lead) or nshape[-1] not in (1, B) or nshape[0] not in (
+            (N,) if layers else (1, B)):
         raise RuntimeError("tree_commit: n_rows must be int32, [1] or [B], or [N, 1] or [N, B]")
-    N = lead[0] if len(lead) == 2 else 1
-    path = torch.empty(B, T, dtype=torch.int32, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    if path.numel() == 0:
+    path = torch.empty((B, T), dtype=torch.int32, device=tokens.device)
+    accepted = torch.empty((B,), dtype=torch.int32, device=tokens.device)
+    if B == 0 or N == 0:
         return path, accepted
     tokens, choice, parents = tokens.contiguous(), choice.contiguous(), parents.contiguous()
     k_new, v_new = _rows(k_new), _rows(v_new)
-    ks, vs, ns = k_new.stride()[:-1], v_new.stride()[:-1], n_rows.expand(lead).stride()
-    if N == 1 and len(lead) == 1:
+    ks, vs, ns = k_new.stride(), v_new.stride(), n_rows.stride()
+    if not layers:
         ks, vs, ns = (0, *ks), (0, *vs), (0, *ns)
-    _call(dev, "dropkv_tree_commit", tokens.data_ptr(), parents.data_ptr(), T if parents.numel() > T else 0,
-          choice.data_ptr(), path.data_ptr(), accepted.data_ptr(), k_new.data_ptr(), *ks, v_new.data_ptr(), *vs,
-          k_cache.data_ptr(), v_cache.data_ptr(), n_rows.data_ptr(), *ns, k_cache.element_size(), N, B, H, T, D, C)
+    _call("dropkv_tree_commit", index, _COMMIT_ARGS(
+        tokens.data_ptr(), parents.data_ptr(), T if parents.numel() != T else 0, choice.data_ptr(), path.data_ptr(),
+        accepted.data_ptr(), k_new.data_ptr(), *ks[:4], v_new.data_ptr(), *vs[:4], k_cache.data_ptr(),
+        v_cache.data_ptr(), n_rows.data_ptr(), ns[0], ns[1] if nshape[-1] > 1 else 0, k_cache.element_size(), N, B, H,
+        T, D, C))
     return path, accepted
+
+
+_ROPE_ARGS = _lib.ARGS["dropkv_norm_rope"].pack
+
+
+def _rope_out(t, like, name):
+    if t is None:
+        t = torch.empty_like(like)  # (its layout too, where it is dense)
+        if t.stride(3) == 1:
+            return t
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if t.shape != like.shape or t.dtype is not like.dtype or t.stride(3) != 1:
+        raise RuntimeError(f"norm_rope: {name} must have its input's shape and dtype, D contiguous")
+    return t
 
 
 def norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -549,71 +612,75 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     ``v`` its rows are copied too.  The outputs may be views of cache buffers
     (``k_buf[:, :, n:n + L]``), or the inputs themselves, and are new tensors
     otherwise.  Returns ``(q_out, k_out)``, or ``(q_out, k_out, v_out)``."""
-    dev = _check_device(q, k, cos, sin)
-    _no_grad("norm_rope", q, k, v, cos, sin, q_weight, k_weight)
-    if q.dtype not in _DTYPE_CODE or k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
+    index = _device_index("norm_rope", q, k, cos, sin, positions, q_weight, k_weight, v, q_out, k_out, v_out)
+    if torch.is_grad_enabled():
+        _no_grad("norm_rope", q, k, v, cos, sin, q_weight, k_weight, q_out, k_out, v_out)
+    dtype, cdtype = q.dtype, cos.dtype
+    if dtype not in _DTYPE_CODE or k.dtype is not dtype or (v is not None and v.dtype is not dtype):
         raise RuntimeError("norm_rope: q, k and v must share a bf16, fp16 or fp32 dtype")
-    if q.dim() != 4 or k.dim() != 4:
+    shape, kshape = q.shape, k.shape
+    if len(shape) != 4 or len(kshape) != 4:
         raise RuntimeError("norm_rope: q and k must be [B, H, L, D]")
-    B, Hq, L, D = q.shape
-    Hkv = k.shape[1]
-    if k.shape != (B, Hkv, L, D) or (v is not None and v.shape != k.shape):
+    B, Hq, L, D = shape
+    Hkv = kshape[1]
+    if kshape != (B, Hkv, L, D) or (v is not None and v.shape != kshape):
         raise RuntimeError("norm_rope: k and v must be [B, Hkv, L, D]")
-    R = cos.shape[-1]
-    if sin.shape != cos.shape or sin.dtype != cos.dtype or cos.dtype not in (torch.float32, q.dtype):
+    ashape = cos.shape
+    if sin.shape != ashape or sin.dtype is not cdtype or (cdtype is not torch.float32 and cdtype is not dtype):
         raise RuntimeError("norm_rope: cos and sin must be alike, fp32 or of q's dtype")
-    p_ptr, p_sb = None, 0
+    R = ashape[-1] if ashape else 0
+    c_stride = cos.stride()
+    if ashape and (c_stride[-1] != 1 or sin.stride() != c_stride):
+        cos, sin = cos.contiguous(), sin.contiguous()
+        c_stride = cos.stride()
+    p_ptr = p_b = c_b = 0
     if positions is not None:
-        _check_device(q, positions)
-        if cos.dim() != 2 or positions.dtype != torch.int64 or positions.shape not in ((L,), (1, L), (B, L)):
+        pshape = positions.shape
+        if len(ashape) != 2 or positions.dtype is not torch.int64 or (
+                pshape != (B, L) and pshape != (L,) and pshape != (1, L)):
             raise RuntimeError("norm_rope: positions must be int64 [L] or [B, L], with cos and sin [rows, R]")
         positions = positions.contiguous()
-        p_ptr, p_sb = positions.data_ptr(), L if positions.numel() > L else 0
-    elif cos.shape not in ((L, R), (1, L, R), (B, L, R)):
+        p_ptr, p_b = positions.data_ptr(), L if len(pshape) == 2 and pshape[0] > 1 else 0
+    elif ashape == (B, L, R):
+        c_b = c_stride[0] if B > 1 else 0
+    elif ashape != (L, R) and ashape != (1, L, R):
         raise RuntimeError("norm_rope: cos and sin must be [L, R], [1, L, R] or [B, L, R]")
-    if cos.stride(-1) != 1 or sin.stride() != cos.stride():
-        cos, sin = cos.contiguous(), sin.contiguous()
-    c_sb = cos.stride(0) if positions is None and cos.dim() == 3 and cos.shape[0] > 1 else 0
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        _check_device(q, w)
-        if w.shape != (D,) or w.dtype not in (torch.float32, q.dtype) or w.dtype != weights[0].dtype:
-            raise RuntimeError("norm_rope: norm weights must be [D], fp32 or of q's dtype, and alike")
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    qw = kw = w_code = 0
+    if q_weight is not None or k_weight is not None:
+        weights = [w for w in (q_weight, k_weight) if w is not None]
+        wdtype = weights[0].dtype
+        for w in weights:
+            if w.shape != (D,) or w.dtype is not wdtype or (wdtype is not torch.float32 and wdtype is not dtype):
+                raise RuntimeError("norm_rope: norm weights must be [D], fp32 or of q's dtype, and alike")
+        w_code = _DTYPE_CODE[wdtype]
+        if q_weight is not None:
+            q_weight = q_weight.contiguous()
+            qw = q_weight.data_ptr()
+        if k_weight is not None:
+            k_weight = k_weight.contiguous()
+            kw = k_weight.data_ptr()
     if v is None and v_out is not None:
         raise RuntimeError("norm_rope: v_out without v")
-
-    def target(t, like, name):
-        if t is None:
-            return torch.empty(like.shape, dtype=q.dtype, device=dev)
-        _check_device(q, t)
-        if t.shape != like.shape or t.dtype != q.dtype or t.stride(3) != 1:
-            raise RuntimeError(f"norm_rope: {name} must have its input's shape and dtype, D contiguous")
-        return t
-
-    q_out, k_out = target(q_out, q, "q_out"), target(k_out, k, "k_out")
-    outs = (q_out, k_out)
     q, k = _rows(q), _rows(k)
-    pairs = [(q, q_out), (k, k_out)]
+    q_out, k_out = _rope_out(q_out, q, "q_out"), _rope_out(k_out, k, "k_out")
+    v_ptr = v_b = v_h = v_l = vo_ptr = vo_b = vo_h = vo_l = 0
     if v is not None:
-        v_out = target(v_out, v, "v_out")
         v = _rows(v)
-        outs += (v_out,)
-        pairs.append((v, v_out))
-    if q.numel() == 0:
-        return outs
-    strides = (ctypes.c_int64 * 18)(*[s for pair in pairs for t in pair for s in t.stride()[:3]])
-    args = []
-    for i, pair in enumerate(pairs):
-        for j, t in enumerate(pair):
-            args += [t.data_ptr(), ctypes.addressof(strides) + 24 * (2 * i + j)]
-    if v is None:
-        args += [None] * 4
-    _call(dev, "dropkv_norm_rope", *args, None if q_weight is None else q_weight.data_ptr(),
-          None if k_weight is None else k_weight.data_ptr(), _DTYPE_CODE[weights[0].dtype] if weights else 0,
-          cos.data_ptr(), sin.data_ptr(), _DTYPE_CODE[cos.dtype], c_sb, cos.stride(-2), p_ptr, p_sb, cos.shape[0],
-          _DTYPE_CODE[q.dtype], B, Hq, Hkv, L, D, R, float(eps))
-    return outs
+        v_out = _rope_out(v_out, v, "v_out")
+        v_ptr, vo_ptr = v.data_ptr(), v_out.data_ptr()
+        v_b, v_h, v_l, _ = v.stride()
+        vo_b, vo_h, vo_l, _ = v_out.stride()
+    if B and L:
+        q_b, q_h, q_l, _ = q.stride()
+        qo_b, qo_h, qo_l, _ = q_out.stride()
+        k_b, k_h, k_l, _ = k.stride()
+        ko_b, ko_h, ko_l, _ = k_out.stride()
+        _call("dropkv_norm_rope", index, _ROPE_ARGS(
+            q.data_ptr(), q_b, q_h, q_l, q_out.data_ptr(), qo_b, qo_h, qo_l, k.data_ptr(), k_b, k_h, k_l,
+            k_out.data_ptr(), ko_b, ko_h, ko_l, v_ptr, v_b, v_h, v_l, vo_ptr, vo_b, vo_h, vo_l, qw, kw, w_code,
+            cos.data_ptr(), sin.data_ptr(), _DTYPE_CODE[cdtype], c_b, c_stride[-2], p_ptr, p_b, ashape[0],
+            _DTYPE_CODE[dtype], B, Hq, Hkv, L, D, R, eps))
+    return (q_out, k_out) if v is None else (q_out, k_out, v_out)
 
 
 class TokenLogprobs(NamedTuple):
@@ -625,41 +692,46 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor            # [..., top] int64
 
 
+_LOGPROB_ARGS = _lib.ARGS["dropkv_token_logprobs"].pack
+
+
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
     """Log probability of a given token, entropy, and the ``top`` (at most 32)
     most probable tokens of every row of ``logits`` [..., V] (bf16, fp16 or
     fp32), in one pass over them (``dropkv_token_logprobs``).  ``tokens`` [...]
     int64: 0 comes out where it is negative, NaN where it is V or more.  The top
     tokens come largest first, the lowest id first among equals."""
-    dev = _check_device(logits)
-    _no_grad("token_logprobs", logits)
-    if logits.dtype not in _DTYPE_CODE:
+    index = _device_index("token_logprobs", logits, tokens)
+    if torch.is_grad_enabled():
+        _no_grad("token_logprobs", logits)
+    dtype, shape, device = logits.dtype, logits.shape, logits.device
+    if dtype not in _DTYPE_CODE:
         raise RuntimeError("token_logprobs: logits must be bf16, fp16 or fp32")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
+    if len(shape) < 1 or shape[-1] < 1:
         raise RuntimeError("token_logprobs: logits must be [..., V]")
-    *lead, V = logits.shape
+    lead, V = shape[:-1], shape[-1]
     if not 0 <= top <= V:
         raise RuntimeError("token_logprobs: top must be in [0, V]")
     if tokens is not None:
-        _check_device(logits, tokens)
-        if tokens.dtype != torch.int64 or list(tokens.shape) != lead:
+        if tokens.dtype is not torch.int64 or tokens.shape != lead:
             raise RuntimeError("token_logprobs: tokens must be int64, of the logits' leading shape")
         tokens = tokens.contiguous()
-    x = _rows(logits.reshape(-1, V))
+    x = _rows(logits if len(shape) == 2 else logits.reshape(-1, V))
     N = x.shape[0]
-    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    top_lp = torch.empty(*lead, top, dtype=torch.float32, device=dev)
-    top_id = torch.empty(*lead, top, dtype=torch.int64, device=dev)
-    res = TokenLogprobs(logprob, entropy, top_lp, top_id)
-    if N == 0:
-        return res
-    nbytes = _lib.load().dropkv_token_logprobs_workspace_bytes(N, V, top)
-    ws = _workspace(nbytes, dev) if nbytes else None
-    _call(dev, "dropkv_token_logprobs", x.data_ptr(), x.stride(0), _DTYPE_CODE[x.dtype], N, V,
-          None if tokens is None else tokens.data_ptr(), int(top), None if logprob is None else logprob.data_ptr(),
-          entropy.data_ptr(), top_lp.data_ptr(), top_id.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
-    return res
+    if tokens is None:
+        logprob, entropy = None, torch.empty(lead, dtype=torch.float32, device=device)
+    else:
+        logprob, entropy = torch.empty((2, *lead), dtype=torch.float32, device=device).unbind()
+    top_lp = torch.empty((*lead, top), dtype=torch.float32, device=device)
+    top_id = torch.empty((*lead, top), dtype=torch.int64, device=device)
+    if N:
+        nbytes = _lib.load().dropkv_token_logprobs_workspace_bytes(N, V, top)
+        ws = _stream_workspace(nbytes, device) if nbytes else None
+        _call("dropkv_token_logprobs", index, _LOGPROB_ARGS(
+            x.data_ptr(), x.stride(0), _DTYPE_CODE[dtype], N, V, 0 if tokens is None else tokens.data_ptr(), top,
+            0 if logprob is None else logprob.data_ptr(), entropy.data_ptr(), top_lp.data_ptr(), top_id.data_ptr(),
+            0 if ws is None else ws.data_ptr(), nbytes))
+    return TokenLogprobs(logprob, entropy, top_lp, top_id)
 
 
 def mfma_selftest(device="cuda") -> torch.Tensor:

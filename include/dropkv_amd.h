@@ -314,34 +314,54 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  * counterpart in the reference, whose decode takes one token per step
  * (dropkv_cache.py:609-617).
  *
+ * These entry points take their arguments in a structure of 8-byte fields,
+ * read before the call returns (binding three dozen arguments one by one costs
+ * a Python caller more than the launch).  Strides are in elements.
+ *
  * dropkv_tree_attention: the attention of the drafted tokens over the rows that
  * the cache holds and over one another.  Nothing but `out` and the workspace is
  * written; the drafted rows go to the cache with dropkv_tree_commit.
- *   q        [B, Hq, T, D], k_new / v_new [B, Hkv, T, D]: element strides, D
- *            contiguous, any alignment; rotated already
+ *   q        [B, Hq, T, D], k_new / v_new [B, Hkv, T, D]: strides {batch, head,
+ *            token}, D contiguous, any alignment; rotated already
  *   k_cache, v_cache  [B, Hkv, capacity, D] contiguous, 16-byte aligned
  *   n_rows   device int32, rows stored of sequence b at n_rows[b * n_sb]
- *            (n_sb 0: one count for all), 0 <= n <= capacity (clamped)
+ *            (n_sb 0: one count for all; else 1), 0 <= n <= capacity (clamped)
  *   mask     device bytes, nonzero where drafted token t sees drafted token j,
- *            at mask[b * m_sb + t * m_st + j * m_sj]; NULL: j <= t (a chain).
- *            Every token sees all stored rows.
- *   out      [B, T, Hq, D], element strides, D contiguous
+ *            at mask[b * m_s[0] + t * m_s[1] + j * m_s[2]]; NULL: j <= t (a
+ *            chain).  Every token sees all stored rows.
+ *   out      [B, T, Hq, D], strides {batch, token, head}, D contiguous
  * out = softmax(scale q K^T) V over the keys seen; a row that sees none, or none
  * whose logit is above -inf, comes out as zeros.  Values and keys that a row
  * does not see do not reach it, also where they are not finite.
  * 1 <= T <= 256, bf16 / fp16, D 64 or 128, capacity * D * 2 <= 2^31,
  * B * Hq * T <= 2^24.
- * The workspace holds the partial results of the splits; calls that share one
- * must be serialised.
+ * The workspace (dropkv_tree_workspace_bytes for the same geometry; other
+ * geometries can need more, fewer tokens too) holds the partial results of the
+ * splits.  Its first DROPKV_SYNC_BYTES must be zero when it is first used, and
+ * every call leaves them zero; calls that share one must be serialised.
  * ------------------------------------------------------------------------ */
+typedef struct {
+  const void* q;
+  int64_t q_s[3];
+  const void* k_new;
+  int64_t kn_s[3];
+  const void* v_new;
+  int64_t vn_s[3];
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* n_rows;
+  int64_t n_sb;
+  const void* mask;
+  int64_t m_s[3];
+  int64_t dtype, B, Hq, Hkv, T, D, capacity;
+  double scale;
+  void* out;
+  int64_t o_s[3];
+  void* workspace;
+  int64_t workspace_bytes;
+} dropkv_tree_attention_args;
 size_t dropkv_tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t capacity);
-int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k_new, int64_t kn_sb,
-                          int64_t kn_sh, int64_t kn_st, const void* v_new, int64_t vn_sb, int64_t vn_sh,
-                          int64_t vn_st, const void* k_cache, const void* v_cache, const int32_t* n_rows,
-                          int64_t n_sb, const void* mask, int64_t m_sb, int64_t m_st, int64_t m_sj, int dtype,
-                          int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int64_t capacity, float scale,
-                          void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, void* workspace,
-                          size_t workspace_bytes, void* stream);
+int dropkv_tree_attention(const dropkv_tree_attention_args* args, void* stream);
 
 /* dropkv_tree_commit: which drafted tokens stand, and their rows appended.
  * Node 0 stands (the step was fed it); from a node c that stands, the walk goes
@@ -351,18 +371,30 @@ int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_s
  *   tokens, choice [B, T] int64; parents int32, sequence b's T at b * p_sb (0:
  *   one tree for all);  path [B, T] int32 (output): the nodes that stand, in
  *   order, then -1;  accepted [B] int32 (output): how many
- *   k_new, v_new [N, B, H, T, D]: the drafted rows of N layers, element strides,
- *   D contiguous;  k_cache, v_cache [N, B, H, capacity, D] contiguous;  n_rows
- *   int32 at l * n_sn + b * n_sb
+ *   k_new, v_new [N, B, H, T, D]: the drafted rows of N layers, strides {layer,
+ *   batch, head, token}, D contiguous;  k_cache, v_cache [N, B, H, capacity, D]
+ *   contiguous;  n_rows int32 at l * n_s[0] + b * n_s[1]
  * Row path[i] of k_new / v_new goes to row n + i of its cache, bit for bit; rows
  * that would lie beyond the capacity (and all of a negative n) are left out.
  * n_rows is not advanced.  1 <= T <= 256; elem_bytes 2 or 4. */
-int dropkv_tree_commit(const int64_t* tokens, const int32_t* parents, int64_t p_sb, const int64_t* choice,
-                       int32_t* path, int32_t* accepted, const void* k_new, int64_t kn_sn, int64_t kn_sb,
-                       int64_t kn_sh, int64_t kn_st, const void* v_new, int64_t vn_sn, int64_t vn_sb, int64_t vn_sh,
-                       int64_t vn_st, void* k_cache, void* v_cache, const int32_t* n_rows, int64_t n_sn,
-                       int64_t n_sb, int64_t elem_bytes, int64_t N, int64_t B, int64_t H, int64_t T, int64_t D,
-                       int64_t capacity, void* stream);
+typedef struct {
+  const int64_t* tokens;
+  const int32_t* parents;
+  int64_t p_sb;
+  const int64_t* choice;
+  int32_t* path;
+  int32_t* accepted;
+  const void* k_new;
+  int64_t kn_s[4];
+  const void* v_new;
+  int64_t vn_s[4];
+  void* k_cache;
+  void* v_cache;
+  const int32_t* n_rows;
+  int64_t n_s[2];
+  int64_t elem_bytes, N, B, H, T, D, capacity;
+} dropkv_tree_commit_args;
+int dropkv_tree_commit(const dropkv_tree_commit_args* args, void* stream);
 
 /* dropkv_norm_rope: queries and keys made ready for the attention and the cache
  * in one pass: an RMS norm over each head where its weight is not NULL
@@ -371,37 +403,67 @@ int dropkv_tree_commit(const int64_t* tokens, const int32_t* parents, int64_t p_
  *   z_i       = y_i cos_i - y_{i+R/2} sin_i
  *   z_{i+R/2} = y_{i+R/2} cos_{i+R/2} + y_i sin_{i+R/2}
  * in fp32 with one rounding at the store; v (may be NULL) is copied.
- *   q [B, Hq, L, D], k, v [B, Hkv, L, D] and their outputs: element strides
- *   {batch, head, token}, D contiguous.  An output may be its input itself; no
- *   other overlap is allowed.
+ *   q [B, Hq, L, D], k, v [B, Hkv, L, D] and their outputs: strides {batch,
+ *   head, token}, D contiguous.  An output may be its input itself; no other
+ *   overlap is allowed.
  *   q_w, k_w [D] of w_dtype (fp32 or the inputs' type)
  *   cos, sin of c_dtype (fp32 or the inputs' type): with positions NULL, token
  *   (b, l)'s R values at b * c_sb + l * c_sl; with positions (int64, b * p_sb +
  *   l), row `position` of a table of c_rows rows c_sl apart.  A position outside
  *   the table makes its token's rotated values NaN.
  * D <= 4096, R even, 2 <= R <= D. */
-int dropkv_norm_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* qo_strides, const void* k,
-                     const int64_t* k_strides, void* k_out, const int64_t* ko_strides, const void* v,
-                     const int64_t* v_strides, void* v_out, const int64_t* vo_strides, const void* q_w,
-                     const void* k_w, int w_dtype, const void* cos, const void* sin, int c_dtype, int64_t c_sb,
-                     int64_t c_sl, const int64_t* positions, int64_t p_sb, int64_t c_rows, int dtype, int64_t B,
-                     int64_t Hq, int64_t Hkv, int64_t L, int64_t D, int64_t R, float eps, void* stream);
+typedef struct {
+  const void* q;
+  int64_t q_s[3];
+  void* q_out;
+  int64_t qo_s[3];
+  const void* k;
+  int64_t k_s[3];
+  void* k_out;
+  int64_t ko_s[3];
+  const void* v;
+  int64_t v_s[3];
+  void* v_out;
+  int64_t vo_s[3];
+  const void* q_w;
+  const void* k_w;
+  int64_t w_dtype;
+  const void* cos;
+  const void* sin;
+  int64_t c_dtype, c_sb, c_sl;
+  const int64_t* positions;
+  int64_t p_sb, c_rows;
+  int64_t dtype, B, Hq, Hkv, L, D, R;
+  double eps;
+} dropkv_norm_rope_args;
+int dropkv_norm_rope(const dropkv_norm_rope_args* args, void* stream);
 
-/* dropkv_token_logprobs: for each row x of logits [N, V] (element stride
- * row_stride between rows, V contiguous; bf16, fp16 or fp32)
+/* dropkv_token_logprobs: for each row x of logits [N, V] (row_stride between
+ * rows, V contiguous; bf16, fp16 or fp32)
  *   logprob[n]  = x[t] - lse  for t = tokens[n] (tokens and logprob may be NULL
  *                 together); 0 where t < 0 (no token), NaN where t >= V
  *   entropy[n]  = -sum p ln p  (natural logarithm)
- *   top_ids     the `top` largest logits' places [N, top], largest first, the
- *               lowest place first among equals, NaN above all
+ *   top_ids     the `top` largest logits' places [N, top] int64, largest first,
+ *               the lowest place first among equals, NaN above all
  *   top_logprobs their log probabilities [N, top] fp32
  * Logits of -inf have no weight; a row that holds +inf or NaN, or only -inf,
- * gives NaN.  0 <= top <= min(32, V), V <= 2^30.  The workspace may be NULL
- * where dropkv_token_logprobs_workspace_bytes is 0. */
+ * gives NaN.  0 <= top <= min(32, V), V <= 2^30.  The workspace (may be NULL
+ * where dropkv_token_logprobs_workspace_bytes is 0): its first DROPKV_SYNC_BYTES
+ * must be zero when it is first used, and every call leaves them zero. */
+typedef struct {
+  const void* logits;
+  int64_t row_stride, dtype, N, V;
+  const int64_t* tokens;
+  int64_t top;
+  float* logprob;
+  float* entropy;
+  float* top_logprobs;
+  int64_t* top_ids;
+  void* workspace;
+  int64_t workspace_bytes;
+} dropkv_token_logprobs_args;
 size_t dropkv_token_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top);
-int dropkv_token_logprobs(const void* logits, int64_t row_stride, int dtype, int64_t N, int64_t V,
-                          const int64_t* tokens, int64_t top, float* logprob, float* entropy, float* top_logprobs,
-                          int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
+int dropkv_token_logprobs(const dropkv_token_logprobs_args* args, void* stream);
 
 #ifdef __cplusplus
 }

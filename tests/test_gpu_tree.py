@@ -355,3 +355,24 @@ def test_refusals(gpu):
                    dict(n_rows=torch.zeros(1, B, dtype=torch.int32, device=gpu))]:
         with pytest.raises(RuntimeError):
             ops.tree_commit(**{**ok, **change})
+
+
+def test_shared_workspace(gpu):
+    """Calls that bring no workspace share the stream's with the layer-calls of
+    the eviction, whose counters at its start every call leaves zero."""
+    from dropkv_amd import ops
+    ops.release_workspaces()
+    g = torch.Generator().manual_seed(0)
+    Q, K, V = (torch.randn(1, h, 4096, 64, generator=g).bfloat16().to(gpu) for h in (14, 2, 2))
+    x = torch.randn(3, 50000, generator=g).to(gpu)
+    q, kn, vn, kc, vc = (t.to(gpu) for t in case(1, 14, 2, 64, 8, 700, torch.bfloat16, 1))
+    n = torch.tensor([600], dtype=torch.int32, device=gpu)
+    calls = [lambda: ops.evict(Q, K, V, 8, 11, 400), lambda: (ops.tree_attention(q, kn, vn, kc, vc, n, 0.1),),
+             lambda: ops.token_logprobs(x, top=9)[1:]]
+    first = [tuple(t.clone() for t in c()) for c in calls]
+    for _ in range(3):
+        for c, want in zip(calls, first):
+            for a, b in zip(c(), want):
+                assert torch.equal(a, b)
+            for ws in ops._shared_ws.values():
+                assert not ws[:4096].any()

@@ -2,15 +2,16 @@
 (drafted-token attention, accepted rows, norms and rotation, log
 probabilities): every refusal comes before anything is enqueued.  CPU only."""
 
-import ctypes
 import os
+import re
 
 import pytest
 import torch
 
 from dropkv_amd import _lib, ops
 
-FAKE = ctypes.c_void_p(1 << 20)   # never dereferenced: the checks fail first
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "dropkv_amd.h")
+FAKE = 1 << 20   # a pointer that is never dereferenced: the checks fail first
 
 
 @pytest.fixture(scope="module")
@@ -19,6 +20,33 @@ def lib():
         from dropkv_amd import _build
         _build.build()
     return _lib.load()
+
+
+def args(name, **values):
+    """The argument structure of ``name``: the values given, else 0."""
+    fields = [f.removesuffix(":d") for f in _lib.ARG_FIELDS[name].split()]
+    assert not set(values) - set(fields), set(values) - set(fields)
+    return _lib.ARGS[name].pack(*[values.get(f, 0) for f in fields])
+
+
+def test_structures_match_the_header():
+    """Fields of the header's structures, in order (arrays spelled out)."""
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    for name, fields in _lib.ARG_FIELDS.items():
+        body = re.search(r"typedef struct \{([^}]*)\} " + name + "_args;", text).group(1)
+        want = []
+        for decl in filter(None, (d.strip() for d in body.split(";"))):
+            kind, names = re.match(r"((?:const )?\w+\s*\*?)\s*(.*)", decl, re.S).groups()
+            for n in (x.strip() for x in names.split(",")):
+                m = re.match(r"(\w+)\[(\d)\]", n)
+                want += [(m.group(1), "q")] * int(m.group(2)) if m else [(n, "d" if kind.strip() == "double" else "q")]
+        got = [f.removesuffix(":d") for f in fields.split()]
+        assert len(got) == len(want), name
+        for g, (w, kind) in zip(got, want):
+            # (an element of x_s[] is spelled x_ and the axis)
+            assert g == w or (w.endswith("_s") and g.startswith(w)) , (name, g, w)
+        assert _lib.ARGS[name].format == "@" + "".join(k for _, k in want)
+        assert _lib.ARGS[name].size == 8 * len(want)
 
 
 def refused(lib, rc, code, msg):
@@ -36,33 +64,31 @@ def test_tree_workspace(lib):
 
 
 @pytest.mark.parametrize("change,code,msg", [
-    (dict(q=None), 1, "null pointer"),
-    (dict(ws=None), 1, "null pointer"),
+    (dict(q=0), 1, "null pointer"),
+    (dict(workspace=0), 1, "null pointer"),
     (dict(dtype=3), 1, "bf16 or fp16"),
     (dict(Hq=30), 1, "Hkv | Hq"),
     (dict(B=0), 1, "must be positive"),
     (dict(T=0), 2, "T must be in"),
     (dict(T=257), 2, "T must be in"),
     (dict(D=80), 2, "head dim 80"),
-    (dict(C=0), 1, "capacity"),
-    (dict(C=(1 << 23) + 1), 1, "capacity"),
+    (dict(capacity=0), 1, "capacity"),
+    (dict(capacity=(1 << 23) + 1), 1, "capacity"),
     (dict(B=1 << 17), 2, "B*Hq*T"),
     (dict(n_sb=2), 1, "n_sb"),
-    (dict(k=ctypes.c_void_p((1 << 20) + 8)), 1, "16-byte aligned"),
-    (dict(ws_bytes=1000), 3, "workspace too small"),
+    (dict(k_cache=FAKE + 8), 1, "16-byte aligned"),
+    (dict(workspace_bytes=1000), 3, "workspace too small"),
+    (dict(workspace_bytes=-1), 3, "workspace too small"),
 ])
 def test_tree_attention(lib, change, code, msg):
-    a = dict(q=FAKE, k=FAKE, ws=FAKE, dtype=1, B=1, Hq=32, Hkv=8, T=8, D=128, C=300, n_sb=0, ws_bytes=1 << 40)
-    a.update(change)
-    rc = lib.dropkv_tree_attention(a["q"], 0, 0, 0, FAKE, 0, 0, 0, FAKE, 0, 0, 0, a["k"], FAKE, FAKE, a["n_sb"], None,
-                                   0, 0, 0, a["dtype"], a["B"], a["Hq"], a["Hkv"], a["T"], a["D"], a["C"], 0.1, FAKE,
-                                   0, 0, 0, a["ws"], a["ws_bytes"], None)
-    refused(lib, rc, code, msg)
+    good = dict(q=FAKE, k_new=FAKE, v_new=FAKE, k_cache=FAKE, v_cache=FAKE, n_rows=FAKE, out=FAKE, workspace=FAKE,
+                dtype=1, B=1, Hq=32, Hkv=8, T=8, D=128, capacity=300, scale=0.1, workspace_bytes=1 << 40)
+    refused(lib, lib.dropkv_tree_attention(args("dropkv_tree_attention", **{**good, **change}), None), code, msg)
 
 
 @pytest.mark.parametrize("change,code,msg", [
-    (dict(tok=None), 1, "null pointer"),
-    (dict(eb=8), 1, "elem_bytes"),
+    (dict(tokens=0), 1, "null pointer"),
+    (dict(elem_bytes=8), 1, "elem_bytes"),
     (dict(N=0), 1, "must be positive"),
     (dict(T=0), 2, "T must be in"),
     (dict(T=300), 2, "T must be in"),
@@ -72,66 +98,57 @@ def test_tree_attention(lib, change, code, msg):
     (dict(n_sb=-1), 1, "strides"),
 ])
 def test_tree_commit(lib, change, code, msg):
-    a = dict(tok=FAKE, eb=2, N=1, B=1, T=8, D=128, p_sb=0, n_sb=0)
-    a.update(change)
-    rc = lib.dropkv_tree_commit(a["tok"], FAKE, a["p_sb"], FAKE, FAKE, FAKE, FAKE, 0, 0, 0, 0, FAKE, 0, 0, 0, 0, FAKE,
-                                FAKE, FAKE, 0, a["n_sb"], a["eb"], a["N"], a["B"], 8, a["T"], a["D"], 100, None)
-    refused(lib, rc, code, msg)
+    good = dict(tokens=FAKE, parents=FAKE, choice=FAKE, path=FAKE, accepted=FAKE, k_new=FAKE, v_new=FAKE, k_cache=FAKE,
+                v_cache=FAKE, n_rows=FAKE, elem_bytes=2, N=1, B=1, H=8, T=8, D=128, capacity=100)
+    refused(lib, lib.dropkv_tree_commit(args("dropkv_tree_commit", **{**good, **change}), None), code, msg)
+
+
+ROPE = dict(q=FAKE, q_out=FAKE, k=FAKE, k_out=FAKE, cos=FAKE, sin=FAKE, c_dtype=3, c_sl=64, c_rows=10, dtype=1, B=1,
+            Hq=8, Hkv=2, L=4, D=64, R=64, eps=1e-6)
 
 
 @pytest.mark.parametrize("change,code,msg", [
-    (dict(q=None), 1, "null pointer"),
-    (dict(v=FAKE), 1, "v without"),
+    (dict(q=0), 1, "null pointer"),
+    (dict(v=FAKE), 1, "null pointer"),
     (dict(dtype=4), 1, "bf16, fp16 or fp32"),
     (dict(c_dtype=2), 1, "c_dtype"),
-    (dict(w=FAKE, w_dtype=2), 1, "w_dtype"),
+    (dict(q_w=FAKE, w_dtype=2), 1, "w_dtype"),
     (dict(D=1), 2, "head dim"),
     (dict(D=4098), 2, "head dim"),
     (dict(R=63), 1, "R must be"),
     (dict(R=0), 1, "R must be"),
     (dict(R=66), 1, "R must be"),
-    (dict(pos=FAKE, rows=0), 1, "c_rows"),
+    (dict(positions=FAKE, c_rows=0), 1, "c_rows"),
     (dict(eps=-1.0), 1, "eps"),
     (dict(eps=float("nan")), 1, "eps"),
     (dict(B=1 << 20, L=1 << 10), 2, "above"),
     (dict(Hkv=0), 1, "invalid shape"),
 ])
 def test_norm_rope(lib, change, code, msg):
-    a = dict(q=FAKE, v=None, dtype=1, c_dtype=3, w=None, w_dtype=0, pos=None, rows=10, B=1, Hkv=2, L=4, D=64, R=64,
-             eps=1e-6)
-    a.update(change)
-    s = (ctypes.c_int64 * 3)()
-    rc = lib.dropkv_norm_rope(a["q"], s, FAKE, s, FAKE, s, FAKE, s, a["v"], None, None, None, a["w"], None,
-                              a["w_dtype"], FAKE, FAKE, a["c_dtype"], 0, 64, a["pos"], 0, a["rows"], a["dtype"],
-                              a["B"], 8, a["Hkv"], a["L"], a["D"], a["R"], a["eps"], None)
-    refused(lib, rc, code, msg)
+    refused(lib, lib.dropkv_norm_rope(args("dropkv_norm_rope", **{**ROPE, **change}), None), code, msg)
 
 
 def test_norm_rope_of_nothing(lib):
-    s = (ctypes.c_int64 * 3)()
-    assert lib.dropkv_norm_rope(FAKE, s, FAKE, s, FAKE, s, FAKE, s, None, None, None, None, None, None, 0, FAKE, FAKE,
-                                3, 0, 64, None, 0, 0, 1, 2, 8, 2, 0, 64, 64, 1e-6, None) == 0
+    assert lib.dropkv_norm_rope(args("dropkv_norm_rope", **{**ROPE, "L": 0}), None) == 0
 
 
 @pytest.mark.parametrize("change,code,msg", [
-    (dict(x=None), 1, "null pointer"),
-    (dict(tok=FAKE, lp=None), 1, "go together"),
+    (dict(logits=0), 1, "null pointer"),
+    (dict(tokens=FAKE), 1, "go together"),
     (dict(dtype=0), 1, "bf16, fp16 or fp32"),
     (dict(V=0), 1, "V must be positive"),
     (dict(V=(1 << 30) + 1), 2, "too large"),
     (dict(top=-1), 1, "top must be"),
     (dict(V=5, top=6), 1, "top must be"),
     (dict(top=33), 2, "above 32"),
-    (dict(top=4, ids=None), 1, "null top"),
-    (dict(ws=None), 3, "workspace too small"),
-    (dict(ws_bytes=64), 3, "workspace too small"),
+    (dict(top=4, top_ids=0), 1, "null top"),
+    (dict(workspace=0), 3, "workspace too small"),
+    (dict(workspace_bytes=64), 3, "workspace too small"),
 ])
 def test_token_logprobs(lib, change, code, msg):
-    a = dict(x=FAKE, tok=None, lp=None, dtype=1, N=2, V=100000, top=4, ids=FAKE, ws=FAKE, ws_bytes=1 << 40)
-    a.update(change)
-    rc = lib.dropkv_token_logprobs(a["x"], a["V"], a["dtype"], a["N"], a["V"], a["tok"], a["top"], a["lp"], FAKE, FAKE,
-                                   a["ids"], a["ws"], a["ws_bytes"], None)
-    refused(lib, rc, code, msg)
+    good = dict(logits=FAKE, row_stride=100000, dtype=1, N=2, V=100000, top=4, entropy=FAKE, top_logprobs=FAKE,
+                top_ids=FAKE, workspace=FAKE, workspace_bytes=1 << 40)
+    refused(lib, lib.dropkv_token_logprobs(args("dropkv_token_logprobs", **{**good, **change}), None), code, msg)
 
 
 def test_token_logprobs_workspace(lib):
@@ -139,7 +156,7 @@ def test_token_logprobs_workspace(lib):
     assert size(1, 151936, 5) > 0 and size(100000, 1000, 5) == 0
     for bad in [(0, 10, 1), (1, 0, 0), (1, 10, 11), (1, 100, 33), (1, 100, -1), (1, (1 << 30) + 1, 1)]:
         assert size(*bad) == 0, bad
-    assert lib.dropkv_token_logprobs(None, 0, 1, 0, 5, None, 0, None, None, None, None, None, 0, None) == 0
+    assert lib.dropkv_token_logprobs(args("dropkv_token_logprobs", V=5, dtype=1), None) == 0
 
 
 def test_host_tensors_are_refused():
@@ -150,5 +167,5 @@ def test_host_tensors_are_refused():
     for call in (lambda: ops.token_logprobs(x), lambda: ops.norm_rope(q, k, c, c),
                  lambda: ops.tree_attention(q, k, k, k, k, n, 0.1),
                  lambda: ops.tree_commit(t, t[0].int(), t, k, k, k, k, n)):
-        with pytest.raises(RuntimeError, match="cuda"):
+        with pytest.raises(RuntimeError, match="device"):
             call()
