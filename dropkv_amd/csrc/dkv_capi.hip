@@ -547,6 +547,8 @@ int dropkv_tree_attention(const dropkv_tree_attention_args* a, void* stream) {
   const int rc = check_tree_shape(a->B, a->Hq, a->Hkv, a->T, a->D, a->capacity);
   if (rc) return rc;
   if (a->n_sb != 0 && a->n_sb != 1) return fail(DROPKV_E_ARG, "n_sb must be 0 or 1");
+  if (!((float)a->scale > 0.f) || !((float)a->scale < 1e37f))
+    return fail(DROPKV_E_ARG, "scale must be positive and finite");
   if (!aligned16(a->k_cache) || !aligned16(a->v_cache))
     return fail(DROPKV_E_ARG, "cache buffers must be 16-byte aligned");
   const size_t need = dkv::tree_workspace_bytes(a->B, a->Hq, a->Hkv, a->D, a->T, a->capacity);

@@ -24,24 +24,6 @@
 
 namespace dkv {
 
-#ifndef W16
-#define W16 2048
-#endif
-#ifndef W64
-#define W64 512
-#endif
-#ifndef W128
-#define W128 512
-#endif
-#ifndef W256
-#define W256 256
-#endif
-#ifndef LO128
-#define LO128 true
-#endif
-#ifndef LO256
-#define LO256 true
-#endif
 constexpr int kTreeTile = 32;       // keys per tile
 constexpr int kTreeMaxSplits = 63;  // of the cache: one lane of the merge each, with the drafted keys'
 
@@ -60,6 +42,7 @@ struct TreeArgs {
   int B, Hq, Hkv, D, T, C, M, S, MC;
   int P;       // parts of a KV head: S per sequence, and one more each where the drafted keys are a part of their own
   int apart;   // they are
+  int tail_tiles;
   int ragged;  // the B * S parts are dealt out by the sequences' lengths
   int direct;  // one part: the output is written by it
   int qvec, nvec;
@@ -109,9 +92,11 @@ __device__ __forceinline__ int tree_rows(const TreeArgs& a, int b) {
 // each.  With one count for all, or one sequence, S parts each.  Otherwise the
 // B * S parts go by length, so that no workgroup has much more than the mean (8
 // sequences of 940 to 8003 rows at equal parts: the longest took twice the
-// mean's time): ceil(tiles / per) parts each, at least one, `per` the mean where
-// that fits, else what always does: sum ceil(t_b / per) <= sum t_b / per + B.
-// Every lane of the wave calls this; lane i looks at sequence i.
+// mean's time): ceil(tiles / per) parts each, at least one, with about the least
+// `per` whose parts fit; sum ceil(t_b / per) <= sum t_b / per + B always does at
+// sum / (B (S - 1)).  Every lane of the wave calls this; lane i looks at
+// sequence i.  Drafted keys that go with a sequence's last part count as
+// `tail_tiles` tiles of it.
 constexpr int kTreeRaggedB = 64;
 struct TreeParts {
   int first, count, per;
@@ -126,21 +111,19 @@ __device__ __forceinline__ int wave_sum_int(int x) {
   return x;
 }
 __device__ __forceinline__ TreeParts tree_parts_ragged(const TreeArgs& a, int lane) {
-  const int t = lane < a.B ? tree_tiles(a, lane) : 0;
+  const int t = lane < a.B ? tree_tiles(a, lane) + a.tail_tiles : 0;
   int sum = t, most = t;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     sum += __shfl_xor(sum, o);
     most = max(most, __shfl_xor(most, o));
   }
-  const int floor_per = max(1, ceil_div(most, kTreeMaxSplits));
   TreeParts p;
-  p.per = max(floor_per, ceil_div(sum, a.B * a.S));
-  auto parts = [&]() { return lane < a.B ? max(1, ceil_div(t, p.per)) : 0; };
-  p.count = parts();
-  if (wave_sum_int(p.count) > a.B * a.S) {
-    p.per = max(floor_per, ceil_div(sum, a.B * (a.S - 1)));
-    p.count = parts();
+  p.per = max(max(1, ceil_div(most, kTreeMaxSplits)), ceil_div(sum, a.B * a.S));
+  for (;;) {
+    p.count = lane < a.B ? max(1, ceil_div(t, p.per)) : 0;
+    if (wave_sum_int(p.count) <= a.B * a.S) break;
+    p.per += max(1, p.per / 32);  // (ends where per >= sum / (B (S - 1)) at the latest)
   }
   int off = p.count;
 #pragma unroll
@@ -152,7 +135,7 @@ __device__ __forceinline__ TreeParts tree_parts_ragged(const TreeArgs& a, int la
   return p;
 }
 __device__ __forceinline__ TreeParts tree_parts(const TreeArgs& a, int b, int lane) {
-  if (!a.ragged) return TreeParts{b * a.S, a.S, ceil_div(tree_tiles(a, b), a.S)};
+  if (!a.ragged) return TreeParts{b * a.S, a.S, ceil_div(tree_tiles(a, b) + a.tail_tiles, a.S)};
   TreeParts p = tree_parts_ragged(a, lane);
   return TreeParts{__builtin_amdgcn_readlane(p.first, b), __builtin_amdgcn_readlane(p.count, b),
                    __builtin_amdgcn_readfirstlane(p.per)};
@@ -182,7 +165,7 @@ __device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int slot, int l
     p.n = tree_rows(a, p.b);
     first = p.b * a.S;
     count = a.S;
-    per = ceil_div((p.n + kTreeTile - 1) / kTreeTile, a.S);
+    per = ceil_div((p.n + kTreeTile - 1) / kTreeTile + a.tail_tiles, a.S);
   }
   const int tiles = (p.n + kTreeTile - 1) / kTreeTile;
   p.t_lo = min((slot - first) * per, tiles);
@@ -191,6 +174,16 @@ __device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int slot, int l
   return p;
 }
 
+// What a tile's keys are to the rows: all seen, the first ones, or by the mask.
+template <int k>
+struct Kind {
+  static constexpr int value = k;
+};
+
+// Up to 16 rows per KV head: one wave per part, its own tiles.  K comes in
+// registers as the matrix operand, V through LDS for the transposing reads; the
+// next tile's loads are issued as soon as a tile's registers are consumed.
+// Bound by memory: 4 x 16 heads of 6553 rows, D = 64 (107 MB).
 template <typename T, int D>
 __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   typedef typename Elem<T>::v8 v8;
@@ -202,9 +195,35 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   __shared__ __attribute__((aligned(16))) T vt[kTreeTile * kVPitch];
 
   const TreePart part = tree_part(a, slot, lane);
-  const int b = part.b;
+  const int b = part.b, n = part.n;
   if (b < 0) return;
   const int bh = b * a.Hkv + hkv;
+  // Rows past n read as zeros.
+  const rsrc_t krs = make_rsrc(static_cast<const T*>(a.kbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
+  const rsrc_t vrs = make_rsrc(static_cast<const T*>(a.vbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
+  const int v_row = lane / CPR, v_col = 8 * (lane % CPR);
+  const int tr_row = 4 * lg + li / 4, tr_col = 4 * (li % 4);
+  v8 kop[2][KK], vch[NVC];
+  auto load_k = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        kop[hf][kk] = bitcast_u4<v8>(buf_load16(krs, (uint32_t)(j0 + 16 * hf + li) * kRowBytes + 64u * kk + 16u * lg));
+  };
+  auto load_v = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NVC; ++i)
+      vch[i] = bitcast_u4<v8>(
+          buf_load16(vrs, (uint32_t)(j0 + v_row + i * GRP) * kRowBytes + v_col * (uint32_t)sizeof(T)));
+  };
+  int j0 = part.t_lo * kTreeTile;
+  const int j_hi = min(n, part.t_hi * kTreeTile);
+  if (j0 < j_hi) {
+    load_k(j0);
+    load_v(j0);
+  }
+
   // Row li of the KV head: query head hkv g + h, token t.
   const int row = li;
   const bool valid = row < a.M;
@@ -214,56 +233,13 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) qop[kk] = tree_load8(qr + 32 * kk + 8 * lg, a.qvec);
 
-  const bool drafted = part.tail;
-  const int n = drafted ? a.T : part.n;
-  const int j_lo = drafted ? 0 : part.t_lo * kTreeTile, j_hi = drafted ? n : min(n, part.t_hi * kTreeTile);
-  // Rows past n read as zeros.
-  const rsrc_t krs = make_rsrc(static_cast<const T*>(a.kbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
-  const rsrc_t vrs = make_rsrc(static_cast<const T*>(a.vbuf) + (int64_t)bh * a.C * D, (uint32_t)n * kRowBytes);
-  const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
-  const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
-  const uint8_t* mrow = a.mask ? a.mask + (int64_t)b * a.m_sb + (int64_t)t * a.m_st : nullptr;
-
-  const int v_row = lane / CPR, v_col = 8 * (lane % CPR);
-  const int tr_row = 4 * lg + li / 4, tr_col = 4 * (li % 4);
   float m = -__FLT_MAX__, lsum = 0.f;  // (finite, so that logits of -inf get no weight)
-  f32x4 o[DT];
+  float pf[8];
+  f32x4 s[2], o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int j0 = j_lo; j0 < j_hi; j0 += kTreeTile) {
-    v8 kop[2][KK];
-    bool odd = false;  // drafted values that are not finite
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int j = j0 + 16 * hf + li;
-        if (!drafted)
-          kop[hf][kk] = bitcast_u4<v8>(buf_load16(krs, (uint32_t)j * kRowBytes + 64u * kk + 16u * lg));
-        else if (j < n)
-          kop[hf][kk] = tree_load8(kn + (int64_t)j * a.kn_st + 32 * kk + 8 * lg, a.nvec);
-        else
-          kop[hf][kk] = v8{};
-      }
-#pragma unroll
-    for (int i = 0; i < NVC; ++i) {
-      const int j = j0 + v_row + i * GRP;
-      v8 x = v8{};
-      if (!drafted) {
-        x = bitcast_u4<v8>(buf_load16(vrs, (uint32_t)j * kRowBytes + v_col * (uint32_t)sizeof(T)));
-      } else if (j < n) {
-        x = tree_load8(vn + (int64_t)j * a.vn_st + v_col, a.nvec);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (not_finite<T>(x[e])) {
-            odd = true;
-            x[e] = static_cast<T>(0.f);
-          }
-      }
-      *reinterpret_cast<v8*>(vt + (v_row + i * GRP) * kVPitch + v_col) = x;
-    }
-    f32x4 s[2];
+  auto logits = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -271,38 +247,38 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
       for (int kk = 0; kk < KK; ++kk) acc = Elem<T>::mfma(kop[hf][kk], qop[kk], acc);
       s[hf] = acc;
     }
-    uint32_t seen = 0;  // bit e: the lane's key e is visible
+  };
+  auto put_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = j0 + 16 * (e / 4) + 4 * lg + e % 4;
-      bool see = j < j_hi;
-      if (drafted && see) see = mrow ? mrow[(int64_t)j * a.m_sj] != 0 : j <= t;
-      seen |= (uint32_t)see << e;
-    }
+    for (int i = 0; i < NVC; ++i) *reinterpret_cast<v8*>(vt + (v_row + i * GRP) * kVPitch + v_col) = vch[i];
+  };
+  // Softmax step and O^T += V^T P^T; bit e of `seen`: the lane's key e counts.
+  auto attend = [&](uint32_t seen) __attribute__((always_inline)) {
     float tmax = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = (seen >> e) & 1 ? s[e / 4][e % 4] * a.scale_log2 : -INFINITY;
+      const float x = (seen >> e) & 1 ? s[e / 4][e % 4] : -INFINITY;
       s[e / 4][e % 4] = x;
       tmax = __builtin_elementwise_maximum(tmax, x);
     }
-    const float mnew = fmaxf(m, max_xor32(max_xor16(tmax)));
-    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-    float psum = 0.f, pf[8];
+    const float mnew = fmaxf(m, max_xor32(max_xor16(tmax)) * a.scale_log2);
+    const float alpha = __builtin_amdgcn_exp2f(m - mnew), ref = mnew - kPBias<T>;
+    float psum = 0.f;
     v8 phi, plo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = __builtin_amdgcn_exp2f(s[e / 4][e % 4] - (mnew - kPBias<T>));
+      const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], a.scale_log2, -ref));
       pf[e] = x;
       psum += x;
       phi[e] = static_cast<T>(x);
       plo[e] = static_cast<T>(x - static_cast<float>(phi[e]));
     }
-    lsum = lsum * alpha + psum;
+    lsum = fmaf(lsum, alpha, psum);
+    const bool turn = mnew != m;
     m = mnew;
+    if (wave_any(turn))
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-    __syncthreads();
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       typedef short s4 __attribute__((ext_vector_type(4)));
@@ -314,26 +290,82 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
       o[dt] = Elem<T>::mfma(aop, phi, o[dt]);
       o[dt] = Elem<T>::mfma(aop, plo, o[dt]);
     }
-    __syncthreads();
-    if (wave_any(odd)) {
-      // A drafted value that is not finite reaches only the rows that see its
-      // key: the product above took it as zero (0 * inf is NaN), and here it
-      // is added where it is seen.
+  };
+
+  // (One wave: its own LDS operations stay in order.)
+  for (; j0 + kTreeTile <= j_hi; j0 += kTreeTile) {
+    logits();
+    load_k(j0 + kTreeTile);
+    put_v();
+    load_v(j0 + kTreeTile);
+    attend(0xff);
+  }
+  if (j0 < j_hi) {
+    logits();
+    put_v();
+    uint32_t seen = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 8; ++e) seen |= (j0 + 16 * (e / 4) + 4 * lg + e % 4 < j_hi ? 1u : 0u) << e;
+    attend(seen);
+  }
+
+  if (part.tail) {
+    const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
+    const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
+    const uint8_t* mrow = a.mask + (int64_t)b * a.m_sb + (int64_t)t * a.m_st;
 #pragma unroll 1
-        for (int lgp = 0; lgp < 4; ++lgp) {
-          const int j = j0 + 16 * (e / 4) + 4 * lgp + e % 4;
-          const float p = __shfl((seen >> e) & 1 ? pf[e] : -1.f, li + 16 * lgp);
-          if (j < n && !(p < 0.f))
+    for (j0 = 0; j0 < a.T; j0 += kTreeTile) {
+      // Rows, and the mask's bytes, on their way together.
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+      for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const T x = vn[(int64_t)j * a.vn_st + 16 * dt + 4 * lg + r];
-                if (not_finite<T>(x)) o[dt][r] = fmaf(p, static_cast<float>(x), o[dt][r]);
-              }
+        for (int kk = 0; kk < KK; ++kk) {
+          const int j = j0 + 16 * hf + li;
+          kop[hf][kk] = j < a.T ? tree_load8(kn + (int64_t)j * a.kn_st + 32 * kk + 8 * lg, a.nvec) : v8{};
         }
+#pragma unroll
+      for (int i = 0; i < NVC; ++i) {
+        const int j = j0 + v_row + i * GRP;
+        vch[i] = j < a.T ? tree_load8(vn + (int64_t)j * a.vn_st + v_col, a.nvec) : v8{};
+      }
+      uint32_t seen = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + 16 * (e / 4) + 4 * lg + e % 4;
+        seen |= ((j >= a.T ? 0 : a.mask ? mrow[(int64_t)j * a.m_sj] : j <= t) != 0 ? 1u : 0u) << e;
+      }
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < NVC; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (not_finite<T>(vch[i][e])) {
+            odd = true;
+            vch[i][e] = static_cast<T>(0.f);
+          }
+      logits();
+      put_v();
+      attend(seen);
+      if (wave_any(odd)) {
+        // A drafted value that is not finite reaches only the rows that see its
+        // key: the product above took it as zero (0 * inf is NaN), and here it
+        // is added where it is seen.
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll 1
+          for (int lgp = 0; lgp < 4; ++lgp) {
+            const int j = j0 + 16 * (e / 4) + 4 * lgp + e % 4;
+            const float p = __shfl((seen >> e) & 1 ? pf[e] : -1.f, li + 16 * lgp);
+            if (j < a.T && !(p < 0.f))
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const T x = vn[(int64_t)j * a.vn_st + 16 * dt + 4 * lg + r];
+                  if (not_finite<T>(x)) o[dt][r] = fmaf(p, static_cast<float>(x), o[dt][r]);
+                }
+          }
+      }
     }
   }
 
@@ -350,12 +382,12 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   }
 }
 
-// What a tile's keys are to the rows: all seen, the first ones, or by the mask.
-template <int k>
-struct Kind {
-  static constexpr int value = k;
-};
-
+// With LO, P goes into the product in two parts, rounded and remainder (about 16
+// significant bits).  Beyond 64 rows a call is bound by the matrix cores and the
+// ALUs and not by memory, and P is rounded once: each weight is off by at most
+// half a step of the element type, as the output is by its own rounding (4 x 64
+// heads of 26214 rows, 64 tokens: 339 us in two parts, 265 in one).
+//
 // More than 16 rows: NW waves of QB blocks of 16 rows take the same keys, so
 // that a tile of K and V is read once for all of them, into LDS.  The next tile
 // is on its way in registers while the waves compute on this one, and goes to
@@ -438,6 +470,7 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
   }
   const int tr_row = 4 * lg + li / 4, tr_col = 4 * (li % 4);
 
+  uint32_t see_bits[QB];  // of the stage's drafted keys: bit 8 sub + e is the lane's key e of tile sub
   // Tile `sub` of the stage in buffer `buf`.  Kind 0: every key seen; 1: the
   // first `keys`; 2: drafted keys j0 ..., seen by the mask.
   auto compute = [&](int buf, int sub, auto kind, int keys, int j0) __attribute__((always_inline)) {
@@ -463,15 +496,10 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
     for (int x = 0; x < QB; ++x) {
       uint32_t seen = 0xff;
       if (kKind != 0) {
-        const uint8_t* mrow =
-            kKind == 2 && a.mask ? a.mask + (int64_t)b * a.m_sb + (int64_t)tq[x] * a.m_st : nullptr;
-        seen = 0;
+        seen = kKind == 2 ? see_bits[x] >> (8 * sub) : 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int j = 16 * (e / 4) + 4 * lg + e % 4;
-          bool see = j < keys;
-          if (kKind == 2 && see) see = mrow ? mrow[(int64_t)(j0 + j) * a.m_sj] != 0 : j0 + j <= tq[x];
-          seen |= (uint32_t)see << e;
+          const bool see = kKind == 2 ? ((seen >> e) & 1) != 0 : 16 * (e / 4) + 4 * lg + e % 4 < keys;
           s[x][e / 4][e % 4] = see ? s[x][e / 4][e % 4] : -INFINITY;
         }
       }
@@ -559,24 +587,47 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
   if (part.tail)
     for (j0 = 0; j0 < a.T; j0 += kStage) {
       if (tid == 0) odd_flag = 0;
-      __syncthreads();  // (also: nobody reads the buffer any more)
-      bool odd = false;
+      // Rows, and the mask's bytes, on their way together.
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         int r, col;
         const bool v = place(i, &r, &col);
         v8 x = v8{};
-        if (j0 + r < a.T) {
+        if (j0 + r < a.T)
           x = tree_load8((v ? vn + (int64_t)(j0 + r) * a.vn_st : kn + (int64_t)(j0 + r) * a.kn_st) + col, a.nvec);
-          if (v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (not_finite<T>(x[e])) {
-                odd = true;
-                x[e] = static_cast<T>(0.f);
-              }
-        }
         piece[i] = __builtin_bit_cast(u32x4, x);
+      }
+      uint8_t mb[QB][8 * kSub];
+#pragma unroll
+      for (int x = 0; x < QB; ++x) {
+        const uint8_t* mrow = a.mask + (int64_t)b * a.m_sb + (int64_t)tq[x] * a.m_st;
+#pragma unroll
+        for (int e = 0; e < 8 * kSub; ++e) {
+          const int j = j0 + 16 * (e / 4) + 4 * lg + e % 4;
+          mb[x][e] = j >= a.T ? 0 : a.mask ? mrow[(int64_t)j * a.m_sj] : j <= tq[x];
+        }
+      }
+      __syncthreads();  // (nobody reads the buffer any more)
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        int r, col;
+        if (place(i, &r, &col)) {
+          v8 x = bitcast_u4<v8>(piece[i]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (not_finite<T>(x[e])) {
+              odd = true;
+              x[e] = static_cast<T>(0.f);
+            }
+          piece[i] = __builtin_bit_cast(u32x4, x);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < QB; ++x) {
+        see_bits[x] = 0;
+#pragma unroll
+        for (int e = 0; e < 8 * kSub; ++e) see_bits[x] |= (mb[x][e] != 0 ? 1u : 0u) << e;
       }
       put(buf);
       if (odd) odd_flag = 1;
@@ -603,12 +654,12 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
       continue;
     }
     const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + row;
-    float* po = a.part_o + base * D + 4 * lg;
+    const rsrc_t prs = make_rsrc(a.part_o + (base - 16 * x - li) * D, (16 * x + 16) * D * 4u);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[x][dt];
+    for (int dt = 0; dt < DT; ++dt) st_dev16(prs, ((16 * x + li) * D + 16 * dt + 4 * lg) * 4u, o[x][dt]);
     if (lg == 0) {
-      a.part_m[base] = m[x] - kPBias<T>;
-      a.part_l[base] = l;
+      st_dev(a.part_m + base, m[x] - kPBias<T>);
+      st_dev(a.part_l + base, l);
     }
   }
 }
@@ -668,6 +719,15 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
 
 // How a call is cut: rows per workgroup, parts of the cache per sequence, and
 // whether the drafted keys are parts of their own.
+//
+// More parts shorten the longest workgroup, but each costs a prologue and an
+// epilogue (about four tiles' time) and rows x D floats written and read again.
+// In tiles: rounds x (tiles / S + 4) + S x `join`, where a round is as many
+// workgroups as run at once (one of 8 waves, two of 4 or 2, or eight single
+// waves per CU) and `join` the partial rows' traffic at 4 TB/s over a tile's
+// time (0.5 us for up to 64 rows, 1.5 us beyond, half of it at D = 64).  32
+// heads over 8 KV heads of 3276 rows, 16 tokens: 24 parts 13.7 us, 16 parts
+// 14.7, 32 parts 15.5, 53 parts 17.7.
 struct TreePlan {
   int M, rows_wg, MC, S, P, apart;
   size_t rows, bytes;
@@ -678,9 +738,20 @@ static TreePlan tree_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t
   p.rows_wg = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256;
   p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
   const int64_t chunks = B * Hkv * p.MC, tiles = (C + kTreeTile - 1) / kTreeTile;
-  const int64_t want = (p.rows_wg == 16 ? W16 : p.rows_wg <= 64 ? W64 : p.rows_wg == 128 ? W128 : W256) / chunks;
-  p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, kTreeMaxSplits, (tiles + 1) / 2}));
-  p.apart = p.rows_wg == 16 || chunks * p.S < 192;
+  const int64_t round = p.rows_wg == 16 ? 2048 : p.rows_wg <= 128 ? 512 : 256;
+  const double tile_us = p.rows_wg <= 64 ? 0.5 : 1.5;
+  const double join = (double)chunks * std::min(p.M, p.rows_wg) * 128 * 4 * 2 / 4e6 / tile_us;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>({kTreeMaxSplits, (tiles + 1) / 2}));
+  double best = 0;
+  p.S = 0;
+  for (int64_t S = 1; S <= most; ++S) {
+    const double cost = (double)((chunks * S + round - 1) / round) * ((double)tiles / S + 4) + S * join;
+    if (p.S == 0 || cost < best) {
+      best = cost;
+      p.S = (int)S;
+    }
+  }
+  p.apart = p.rows_wg <= 64 || chunks * p.S < 192;
   p.P = (int)(B * (p.S + p.apart));
   p.rows = (size_t)Hkv * p.P * p.M;
   p.bytes = kSyncBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
@@ -700,9 +771,9 @@ static hipError_t launch_tree_t(const TreeArgs& a, int rows_wg, hipStream_t st) 
   else if (rows_wg == 64)
     launch((tree_wide_kernel<T, D, 1, 4, true>), grid, dim3(256), 0, st, a);
   else if (rows_wg == 128)
-    launch((tree_wide_kernel<T, D, 2, 4, LO128>), grid, dim3(256), 0, st, a);
+    launch((tree_wide_kernel<T, D, 2, 4, false>), grid, dim3(256), 0, st, a);
   else
-    launch((tree_wide_kernel<T, D, 2, 8, LO256>), grid, dim3(512), 0, st, a);
+    launch((tree_wide_kernel<T, D, 2, 8, false>), grid, dim3(512), 0, st, a);
   if (!a.direct) launch((tree_merge_kernel<T, D>), dim3((a.B * a.Hkv * a.M + 3) / 4), dim3(256), 0, st, a);
   return hipGetLastError();
 }
@@ -741,6 +812,7 @@ hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_
   a.S = pl.S;
   a.P = pl.P;
   a.apart = pl.apart;
+  a.tail_tiles = pl.apart ? 0 : 3 + 2 * ((a.T + kTreeTile - 1) / kTreeTile);
   a.ragged = p.n_sb != 0 && p.B > 1 && p.B <= kTreeRaggedB && pl.S > 1;
   a.direct = pl.S == 1 && !pl.apart;
   a.div_t = Div::of(a.T);

@@ -334,7 +334,7 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  * whose logit is above -inf, comes out as zeros.  Values and keys that a row
  * does not see do not reach it, also where they are not finite.
  * 1 <= T <= 256, bf16 / fp16, D 64 or 128, capacity * D * 2 <= 2^31,
- * B * Hq * T <= 2^24.
+ * B * Hq * T <= 2^24, 0 < scale < 1e37.
  * The workspace (dropkv_tree_workspace_bytes for the same geometry; other
  * geometries can need more, fewer tokens too) holds the partial results of the
  * splits.  Its first DROPKV_SYNC_BYTES must be zero when it is first used, and

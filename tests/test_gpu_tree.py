@@ -5,7 +5,11 @@ Tolerance of the attention.  Products of bf16 / fp16 values are exact in fp32,
 so a logit is off by at most D 2^-24 |scale| |q| |k| =: d, a weight relative by
 2 d (its own and the sum's) and by 2^-16 for P held in two parts and the
 exponential; each addition of the sums over n keys adds 2^-24, one for 16 keys
-at the most and one for a split.  The store adds half a step."""
+at the most and one for a split.  The store adds half a step.
+
+With more than 64 rows (g T) to a KV head P is rounded once to the element type:
+each weight is off by half a step, 2^-8 (bf16) or 2^-11 (fp16) of itself, and the
+output by at most that of sum p |v|."""
 
 import math
 
@@ -33,7 +37,7 @@ def reference(q, kn, vn, kc, vc, lens, mask, scale):
     B, Hq, T, D = q.shape
     g = Hq // kc.shape[1]
     out = torch.zeros(B, T, Hq, D, dtype=torch.float64)
-    tol = torch.zeros(B, T, Hq, 1, dtype=torch.float64)
+    tol = torch.zeros(B, T, Hq, D, dtype=torch.float64)
     for b, n in enumerate(lens):
         for h in range(Hq):
             k = torch.cat([kc[b, h // g, :n], kn[b, h // g]]).double()
@@ -46,7 +50,10 @@ def reference(q, kn, vn, kc, vc, lens, mask, scale):
                 s = ks @ q[b, h, t].double() * scale
                 out[b, t, h] = torch.softmax(s, 0) @ vs
                 d = D * 2.0 ** -24 * abs(scale) * q[b, h, t].double().norm() * ks.norm(dim=1).max()
+                p = torch.softmax(s, 0)
                 tol[b, t, h] = vs.abs().max() * (2 * d + 2.0 ** -16 + (n / 16 + T / 16 + 80) * 2.0 ** -24)
+                if g * T > 64:
+                    tol[b, t, h] = tol[b, t, h] + torch.finfo(q.dtype).eps / 2 * (p @ vs.abs())
     half = torch.finfo(q.dtype).eps / 2
     return out, tol * (1 + half) + half * out.abs()
 

@@ -76,6 +76,10 @@ def test_tree_workspace(lib):
     (dict(capacity=(1 << 23) + 1), 1, "capacity"),
     (dict(B=1 << 17), 2, "B*Hq*T"),
     (dict(n_sb=2), 1, "n_sb"),
+    (dict(scale=0.0), 1, "scale"),
+    (dict(scale=-0.1), 1, "scale"),
+    (dict(scale=float("nan")), 1, "scale"),
+    (dict(scale=float("inf")), 1, "scale"),
     (dict(k_cache=FAKE + 8), 1, "16-byte aligned"),
     (dict(workspace_bytes=1000), 3, "workspace too small"),
     (dict(workspace_bytes=-1), 3, "workspace too small"),
