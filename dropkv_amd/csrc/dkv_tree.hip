@@ -18,9 +18,11 @@
 // every layer's cache.
 #include "dkv_common.h"
 #include "dkv_internal.h"
+#include "dkv_select_dev.h"
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace dkv {
 
@@ -45,7 +47,6 @@ struct TreeArgs {
   int tail_tiles;
   int ragged;  // the B * S parts are dealt out by the sequences' lengths
   int direct;  // one part: the output is written by it
-  int qvec, nvec;
   Div div_t;
   float scale_log2;
   float* part_m;  // [Hkv, P, M]
@@ -70,16 +71,24 @@ __device__ __forceinline__ bool not_finite(T x) {
   return (__builtin_bit_cast(uint16_t, x) & kExp) == kExp;
 }
 
+// Eight elements of a row that may start anywhere (the hardware's 16-byte loads
+// take any address).
 template <typename T>
-__device__ __forceinline__ typename Elem<T>::v8 tree_load8(const T* p, bool vec) {
-  typename Elem<T>::v8 x;
-  if (vec) {
-    x = *reinterpret_cast<const typename Elem<T>::v8*>(p);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = p[e];
-  }
-  return x;
+__device__ __forceinline__ typename Elem<T>::v8 tree_load8(const T* p) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw {
+    T e[8];
+  };
+  return __builtin_bit_cast(typename Elem<T>::v8, *reinterpret_cast<const Raw*>(p));
+}
+
+// Lane i's value and lane i ^ 16's (32's), the larger; NaN where either is.
+__device__ __forceinline__ float maximum_xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float maximum_xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Sequence b's stored rows.  The host keeps 0 <= n <= C; the clamp keeps every
@@ -105,19 +114,10 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 __device__ __forceinline__ int tree_tiles(const TreeArgs& a, int b) {
   return (tree_rows(a, b) + kTreeTile - 1) / kTreeTile;
 }
-__device__ __forceinline__ int wave_sum_int(int x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
-  return x;
-}
+__device__ __forceinline__ int wave_sum_int(int x) { return (int)wave_reduce_add((uint32_t)x); }
 __device__ __forceinline__ TreeParts tree_parts_ragged(const TreeArgs& a, int lane) {
   const int t = lane < a.B ? tree_tiles(a, lane) + a.tail_tiles : 0;
-  int sum = t, most = t;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    sum += __shfl_xor(sum, o);
-    most = max(most, __shfl_xor(most, o));
-  }
+  const int sum = wave_sum_int(t), most = (int)wave_reduce_max((uint32_t)t);
   TreeParts p;
   p.per = max(max(1, ceil_div(most, kTreeMaxSplits)), ceil_div(sum, a.B * a.S));
   for (;;) {
@@ -125,13 +125,7 @@ __device__ __forceinline__ TreeParts tree_parts_ragged(const TreeArgs& a, int la
     if (wave_sum_int(p.count) <= a.B * a.S) break;
     p.per += max(1, p.per / 32);  // (ends where per >= sum / (B (S - 1)) at the latest)
   }
-  int off = p.count;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(off, o);
-    if (lane >= o) off += x;
-  }
-  p.first = off - p.count;
+  p.first = (int)wave_incl_scan((uint32_t)p.count) - p.count;
   return p;
 }
 __device__ __forceinline__ TreeParts tree_parts(const TreeArgs& a, int b, int lane) {
@@ -174,11 +168,66 @@ __device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int slot, int l
   return p;
 }
 
-// What a tile's keys are to the rows: all seen, the first ones, or by the mask.
-template <int k>
-struct Kind {
-  static constexpr int value = k;
-};
+// The mask of drafted keys j0 .. j0 + 63, a word per token: a wave takes every
+// NW-th token, a lane a key (a lane's own bytes one by one, a row each, took
+// longer than the tile's products).
+// The loads are unconditional (the last token's row and key again past the
+// ends): behind branches they went out one after the other.
+template <int NW>
+__device__ __forceinline__ void tree_mask_words(const TreeArgs& a, int b, int j0, int wave, int lane, uint64_t* words) {
+  const int j = j0 + lane;
+  if (!a.mask) {  // a chain
+    for (int t = 64 * wave + lane; t < a.T; t += 64 * NW)
+      words[t] = t < j0 ? 0 : t - j0 >= 63 ? ~uint64_t(0) : (uint64_t(2) << (t - j0)) - 1;
+    return;
+  }
+  const uint8_t* m = a.mask + (int64_t)b * a.m_sb + (int64_t)min(j, a.T - 1) * a.m_sj;
+  for (int t0 = wave; t0 < a.T; t0 += 8 * NW) {
+    uint8_t x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = m[(int64_t)min(t0 + i * NW, a.T - 1) * a.m_st];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t w = __builtin_amdgcn_ballot_w64(j < a.T && x[i] != 0);
+      if (lane == 0 && t0 + i * NW < a.T) words[t0 + i * NW] = w;
+    }
+  }
+}
+// Bits 0 .. 3 and 16 .. 19 of a tile's word (shifted by 4 lg): the lane's keys.
+__device__ __forceinline__ uint32_t tree_key_bits(uint32_t w) { return (w & 0xf) | ((w >> 12) & 0xf0); }
+// The same of a word whose first `keys` bits are set.
+__device__ __forceinline__ uint32_t tree_first_bits(int keys, int lg) {
+  return tree_key_bits(keys >= 32 ? 0xffffffffu : ((1u << max(keys, 0)) - 1u) >> (4 * lg));
+}
+
+// A drafted value that is not finite reaches only the rows that see its key: the
+// products take it as zero (0 * inf is NaN), and here, once the part's rows are
+// stored, it is added where it is seen.  Rare: one element at a time.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void tree_add_odd(const TreeArgs& a, int b, int hkv, int slot, int row0, int rows) {
+  const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
+  for (int i = threadIdx.x; i < rows * D; i += NT) {
+    const int row = row0 + i / D, d = i % D;
+    if (row >= a.M) break;
+    const int h = a.div_t.div(row), t = row - h * a.T;
+    float sum = 0.f;
+    for (int j = 0; j < a.T; ++j) {
+      const bool see =
+          a.mask ? a.mask[(int64_t)b * a.m_sb + (int64_t)t * a.m_st + (int64_t)j * a.m_sj] != 0 : j <= t;
+      const T x = vn[(int64_t)j * a.vn_st + d];
+      if (see && not_finite<T>(x)) sum += static_cast<float>(x);
+    }
+    if (sum == 0.f) continue;
+    if (a.direct) {
+      T* o = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)t * a.o_st +
+             (int64_t)(hkv * (a.Hq / a.Hkv) + h) * a.o_sh + d;
+      *o = static_cast<T>(static_cast<float>(*o) + sum);
+    } else {
+      float* o = a.part_o + (((int64_t)hkv * a.P + slot) * a.M + row) * D + d;
+      st_dev(o, *o + sum);
+    }
+  }
+}
 
 // Up to 16 rows per KV head: one wave per part, its own tiles.  K comes in
 // registers as the matrix operand, V through LDS for the transposing reads; the
@@ -193,6 +242,7 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   const int slot = blockIdx.x % a.P, hkv = blockIdx.x / a.P, g = a.Hq / a.Hkv;
   const int lane = threadIdx.x, li = lane & 15, lg = lane >> 4;
   __shared__ __attribute__((aligned(16))) T vt[kTreeTile * kVPitch];
+  __shared__ uint64_t mask_words[16];  // (T <= 16 rows)
 
   const TreePart part = tree_part(a, slot, lane);
   const int b = part.b, n = part.n;
@@ -231,10 +281,9 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   v8 qop[KK];
   const T* qr = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hkv * g + h) * a.q_sh + (int64_t)t * a.q_st;
 #pragma unroll
-  for (int kk = 0; kk < KK; ++kk) qop[kk] = tree_load8(qr + 32 * kk + 8 * lg, a.qvec);
+  for (int kk = 0; kk < KK; ++kk) qop[kk] = tree_load8(qr + 32 * kk + 8 * lg);
 
   float m = -__FLT_MAX__, lsum = 0.f;  // (finite, so that logits of -inf get no weight)
-  float pf[8];
   f32x4 s[2], o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -262,13 +311,13 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
       tmax = __builtin_elementwise_maximum(tmax, x);
     }
     const float mnew = fmaxf(m, max_xor32(max_xor16(tmax)) * a.scale_log2);
-    const float alpha = __builtin_amdgcn_exp2f(m - mnew), ref = mnew - kPBias<T>;
+    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+    const float ref = mnew - kPBias<T>;
     float psum = 0.f;
     v8 phi, plo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], a.scale_log2, -ref));
-      pf[e] = x;
       psum += x;
       phi[e] = static_cast<T>(x);
       plo[e] = static_cast<T>(x - static_cast<float>(phi[e]));
@@ -276,9 +325,10 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
     lsum = fmaf(lsum, alpha, psum);
     const bool turn = mnew != m;
     m = mnew;
-    if (wave_any(turn))
+    if (wave_any(turn)) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       typedef short s4 __attribute__((ext_vector_type(4)));
@@ -300,73 +350,44 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
     load_v(j0 + kTreeTile);
     attend(0xff);
   }
-  if (j0 < j_hi) {
-    logits();
-    put_v();
-    uint32_t seen = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) seen |= (j0 + 16 * (e / 4) + 4 * lg + e % 4 < j_hi ? 1u : 0u) << e;
-    attend(seen);
-  }
-
-  if (part.tail) {
-    const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
-    const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
-    const uint8_t* mrow = a.mask + (int64_t)b * a.m_sb + (int64_t)t * a.m_st;
+  // A last tile of the cache, and the drafted keys (T <= 16: one tile), through
+  // the same code: what a short call fetches of it counts.
+  bool stored = j0 < j_hi, drafted = part.tail, odd = false;
 #pragma unroll 1
-    for (j0 = 0; j0 < a.T; j0 += kTreeTile) {
-      // Rows, and the mask's bytes, on their way together.
+  while (stored || drafted) {
+    uint32_t seen;
+    if (stored) {
+      seen = tree_first_bits(j_hi - j0, lg);
+    } else {
+      const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
+      const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const int j = j0 + 16 * hf + li;
-          kop[hf][kk] = j < a.T ? tree_load8(kn + (int64_t)j * a.kn_st + 32 * kk + 8 * lg, a.nvec) : v8{};
-        }
+      for (int kk = 0; kk < KK; ++kk) {
+        kop[0][kk] = tree_load8(kn + (int64_t)min(li, a.T - 1) * a.kn_st + 32 * kk + 8 * lg);
+        kop[1][kk] = v8{};
+      }
 #pragma unroll
       for (int i = 0; i < NVC; ++i) {
-        const int j = j0 + v_row + i * GRP;
-        vch[i] = j < a.T ? tree_load8(vn + (int64_t)j * a.vn_st + v_col, a.nvec) : v8{};
+        vch[i] = tree_load8(vn + (int64_t)min(v_row + i * GRP, a.T - 1) * a.vn_st + v_col);
       }
-      uint32_t seen = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = j0 + 16 * (e / 4) + 4 * lg + e % 4;
-        seen |= ((j >= a.T ? 0 : a.mask ? mrow[(int64_t)j * a.m_sj] : j <= t) != 0 ? 1u : 0u) << e;
-      }
-      bool odd = false;
+      tree_mask_words<1>(a, b, 0, 0, lane, mask_words);
 #pragma unroll
       for (int i = 0; i < NVC; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (not_finite<T>(vch[i][e])) {
+          if (v_row + i * GRP >= a.T) {
+            vch[i][e] = static_cast<T>(0.f);
+          } else if (not_finite<T>(vch[i][e])) {
             odd = true;
             vch[i][e] = static_cast<T>(0.f);
           }
-      logits();
-      put_v();
-      attend(seen);
-      if (wave_any(odd)) {
-        // A drafted value that is not finite reaches only the rows that see its
-        // key: the product above took it as zero (0 * inf is NaN), and here it
-        // is added where it is seen.
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll 1
-          for (int lgp = 0; lgp < 4; ++lgp) {
-            const int j = j0 + 16 * (e / 4) + 4 * lgp + e % 4;
-            const float p = __shfl((seen >> e) & 1 ? pf[e] : -1.f, li + 16 * lgp);
-            if (j < a.T && !(p < 0.f))
-#pragma unroll
-              for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const T x = vn[(int64_t)j * a.vn_st + 16 * dt + 4 * lg + r];
-                  if (not_finite<T>(x)) o[dt][r] = fmaf(p, static_cast<float>(x), o[dt][r]);
-                }
-          }
-      }
+      seen = tree_key_bits((uint32_t)(mask_words[t] >> (4 * lg)));
+      drafted = false;
     }
+    stored = false;
+    logits();
+    put_v();
+    attend(seen);
   }
 
   lsum = add_xor32(add_xor16(lsum));
@@ -379,6 +400,10 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
       a.part_m[base] = m - kPBias<T>;
       a.part_l[base] = lsum;
     }
+  }
+  if (__builtin_expect(wave_any(odd), 0)) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    tree_add_odd<T, D, 64>(a, b, hkv, slot, 0, 16);
   }
 }
 
@@ -395,7 +420,7 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 // read from LDS serves QB products.  LDS pitches leave every 16 lanes of a
 // K read, and every 32 of a transposing V read, on banks of their own.
 template <typename T, int D, int QB, int NW, bool LO>
-__global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
+__global__ void __launch_bounds__(64 * NW, NW == 2 ? 1 : 2) tree_wide_kernel(TreeArgs a) {
   typedef typename Elem<T>::v8 v8;
   constexpr int KK = D / 32, DT = D / 16, CPR = D / 8, NT = 64 * NW;
   constexpr int kSub = 2, kStage = kSub * kTreeTile;
@@ -426,7 +451,7 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
     const T* qr =
         static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hkv * g + h) * a.q_sh + (int64_t)t * a.q_st;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qop[x][kk] = tree_load8(qr + 32 * kk + 8 * lg, a.qvec);
+    for (int kk = 0; kk < KK; ++kk) qop[x][kk] = tree_load8(qr + 32 * kk + 8 * lg);
   }
 
   // Rows past n read as zeros.
@@ -459,160 +484,144 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
     }
   };
 
-  float m[QB], lsum[QB];
-  f32x4 o[QB][DT];
+  v8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = static_cast<T>(1.f);
+  float m[QB];
+  f32x4 lsum[QB], o[QB][DT];  // (each of lsum's values is the whole sum of row li)
 #pragma unroll
   for (int x = 0; x < QB; ++x) {
     m[x] = -__FLT_MAX__;  // (finite, so that logits of -inf get no weight)
-    lsum[x] = 0.f;
+    lsum[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const int tr_row = 4 * lg + li / 4, tr_col = 4 * (li % 4);
 
-  uint32_t see_bits[QB];  // of the stage's drafted keys: bit 8 sub + e is the lane's key e of tile sub
-  // Tile `sub` of the stage in buffer `buf`.  Kind 0: every key seen; 1: the
-  // first `keys`; 2: drafted keys j0 ..., seen by the mask.
-  auto compute = [&](int buf, int sub, auto kind, int keys, int j0) __attribute__((always_inline)) {
-    constexpr int kKind = decltype(kind)::value;
-    const T* kt = lds + buf * kBuf + sub * kTreeTile * kKP;
-    const T* vt = lds + buf * kBuf + kStage * kKP + sub * kTreeTile * kVP;
-    f32x4 s[QB][2];
+  uint32_t see_bits[QB];  // bit 8 sub + e: the lane's key e of the stage's tile sub counts
+  __shared__ uint64_t mask_words[kTreeMaxT];
+  // The stage in buffer `buf`; with `masked` the keys of see_bits.
+  auto compute = [&](int buf, auto masked) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked)::value;
+    const T* kt = lds + buf * kBuf;
+    const T* vt = kt + kStage * kKP;
+    f32x4 s[QB][2 * kSub];  // keys 16 i + 4 lg + r
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int i = 0; i < 2 * kSub; ++i) {
 #pragma unroll
-      for (int x = 0; x < QB; ++x) s[x][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < QB; ++x) s[x][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        const v8 kop = *reinterpret_cast<const v8*>(kt + (16 * hf + li) * kKP + 32 * kk + 8 * lg);
+        const v8 kop = *reinterpret_cast<const v8*>(kt + (16 * i + li) * kKP + 32 * kk + 8 * lg);
 #pragma unroll
-        for (int x = 0; x < QB; ++x) s[x][hf] = Elem<T>::mfma(kop, qop[x][kk], s[x][hf]);
+        for (int x = 0; x < QB; ++x) s[x][i] = Elem<T>::mfma(kop, qop[x][kk], s[x][i]);
       }
     }
-    v8 phi[QB], plo[LO ? QB : 1];
-    float alpha[QB], pf[kKind == 2 ? QB : 1][8];
+    float alpha[QB], ref[QB];
     bool turn = false;
 #pragma unroll
     for (int x = 0; x < QB; ++x) {
-      uint32_t seen = 0xff;
-      if (kKind != 0) {
-        seen = kKind == 2 ? see_bits[x] >> (8 * sub) : 0;
+      if (kMasked) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool see = kKind == 2 ? ((seen >> e) & 1) != 0 : 16 * (e / 4) + 4 * lg + e % 4 < keys;
-          s[x][e / 4][e % 4] = see ? s[x][e / 4][e % 4] : -INFINITY;
-        }
+        for (int e = 0; e < 8 * kSub; ++e)
+          s[x][e / 4][e % 4] = (see_bits[x] >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
       }
       float tmax = s[x][0][0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
-      tmax = max_xor32(max_xor16(tmax)) * a.scale_log2;
+      for (int e = 1; e < 8 * kSub; ++e) tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
+      tmax = maximum_xor32(maximum_xor16(tmax)) * a.scale_log2;
       const float mnew = fmaxf(m[x], tmax);
       alpha[x] = __builtin_amdgcn_exp2f(m[x] - mnew);
       turn |= mnew != m[x];
       m[x] = mnew;
-      const float ref = mnew - kPBias<T>;
-      float psum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[x][e / 4][e % 4], a.scale_log2, -ref));
-        psum += p;
-        phi[x][e] = static_cast<T>(p);
-        if (LO) plo[x][e] = static_cast<T>(p - static_cast<float>(phi[x][e]));
-        if (kKind == 2) pf[x][e] = (seen >> e) & 1 ? p : -1.f;
-      }
-      lsum[x] = fmaf(lsum[x], alpha[x], psum);
+      ref[x] = mnew - kPBias<T>;
     }
     if (wave_any(turn)) {
 #pragma unroll
-      for (int x = 0; x < QB; ++x)
+      for (int x = 0; x < QB; ++x) {
+        lsum[x] *= alpha[x];
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha[x];
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      typedef short s4 __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) s4 lds_s4;
-      const s4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vt + tr_row * kVP + 16 * dt + tr_col));
-      const s4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vt + (16 + tr_row) * kVP + 16 * dt + tr_col));
-      const v8 aop = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int x = 0; x < QB; ++x) {
-        o[x][dt] = Elem<T>::mfma(aop, phi[x], o[x][dt]);
-        if (LO) o[x][dt] = Elem<T>::mfma(aop, plo[x], o[x][dt]);
       }
     }
-    if (kKind == 2 && odd_flag) {
-      // A drafted value that is not finite reaches only the rows that see its
-      // key: the product above took it as zero (0 * inf is NaN), and here it
-      // is added where it is seen.
+#pragma unroll
+    for (int sub = 0; sub < kSub; ++sub) {
+      v8 phi[QB], plo[LO ? QB : 1];
 #pragma unroll
       for (int x = 0; x < QB; ++x)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll 1
-          for (int lgp = 0; lgp < 4; ++lgp) {
-            const int j = 16 * (e / 4) + 4 * lgp + e % 4;
-            const float p = __shfl(pf[x][e], li + 16 * lgp);
-            if (j < keys && !(p < 0.f))
+        for (int e = 0; e < 8; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[x][2 * sub + e / 4][e % 4], a.scale_log2, -ref[x]));
+          phi[x][e] = static_cast<T>(p);
+          if (LO) plo[x][e] = static_cast<T>(p - static_cast<float>(phi[x][e]));
+        }
+      // The weights' sum as one more product, with ones.
 #pragma unroll
-              for (int dt = 0; dt < DT; ++dt)
+      for (int x = 0; x < QB; ++x) {
+        lsum[x] = Elem<T>::mfma(ones, phi[x], lsum[x]);
+        if (LO) lsum[x] = Elem<T>::mfma(ones, plo[x], lsum[x]);
+      }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const T val = vn[(int64_t)(j0 + j) * a.vn_st + 16 * dt + 4 * lg + r];
-                  if (not_finite<T>(val)) o[x][dt][r] = fmaf(p, static_cast<float>(val), o[x][dt][r]);
-                }
-          }
+      for (int dt = 0; dt < DT; ++dt) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        const T* vs = vt + (kTreeTile * sub + tr_row) * kVP + 16 * dt + tr_col;
+        const s4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)vs);
+        const s4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vs + 16 * kVP));
+        const v8 aop = __builtin_bit_cast(v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int x = 0; x < QB; ++x) {
+          o[x][dt] = Elem<T>::mfma(aop, phi[x], o[x][dt]);
+          if (LO) o[x][dt] = Elem<T>::mfma(aop, plo[x], o[x][dt]);
+        }
+      }
     }
   };
 
+  if (tid == 0) odd_flag = 0;
   int buf = 0;
   const int j_hi = min(n, part.t_hi * kTreeTile);
   int j0 = part.t_lo * kTreeTile;
-  if (j0 < j_hi) {
+  bool stored = j0 < j_hi;
+  if (stored) {
     fetch(j0);
     put(0);
     for (; j0 + kStage < j_hi; j0 += kStage) {
       fetch(j0 + kStage);
       __syncthreads();
-#pragma unroll
-      for (int sub = 0; sub < kSub; ++sub) compute(buf, sub, Kind<0>{}, kTreeTile, 0);
+      compute(buf, std::false_type{});
       buf ^= 1;
       put(buf);
     }
-    __syncthreads();
-    for (int sub = 0; j0 < j_hi; ++sub, j0 += kTreeTile) compute(buf, sub, Kind<1>{}, j_hi - j0, 0);
-    buf ^= 1;
   }
-  if (part.tail)
-    for (j0 = 0; j0 < a.T; j0 += kStage) {
-      if (tid == 0) odd_flag = 0;
-      // Rows, and the mask's bytes, on their way together.
+  // The cache's last stage, and the drafted keys, through the same code: what a
+  // short call fetches of it counts (with three copies of the stage and the
+  // drafted keys' rare cases in line a part of one stage took 9 us, not 6).
+#pragma unroll 1
+  for (int jd = part.tail ? 0 : a.T; stored || jd < a.T;) {
+    if (stored) {
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+        see_bits[x] = tree_first_bits(j_hi - j0, lg) | tree_first_bits(j_hi - j0 - kTreeTile, lg) << 8;
+      stored = false;
+    } else {
+      __syncthreads();  // (the words' and the buffer's last readers are done)
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         int r, col;
         const bool v = place(i, &r, &col);
-        v8 x = v8{};
-        if (j0 + r < a.T)
-          x = tree_load8((v ? vn + (int64_t)(j0 + r) * a.vn_st : kn + (int64_t)(j0 + r) * a.kn_st) + col, a.nvec);
-        piece[i] = __builtin_bit_cast(u32x4, x);
+        const int j = min(jd + r, a.T - 1);
+        piece[i] = __builtin_bit_cast(u32x4, tree_load8((v ? vn + (int64_t)j * a.vn_st : kn + (int64_t)j * a.kn_st) + col));
       }
-      uint8_t mb[QB][8 * kSub];
-#pragma unroll
-      for (int x = 0; x < QB; ++x) {
-        const uint8_t* mrow = a.mask + (int64_t)b * a.m_sb + (int64_t)tq[x] * a.m_st;
-#pragma unroll
-        for (int e = 0; e < 8 * kSub; ++e) {
-          const int j = j0 + 16 * (e / 4) + 4 * lg + e % 4;
-          mb[x][e] = j >= a.T ? 0 : a.mask ? mrow[(int64_t)j * a.m_sj] : j <= tq[x];
-        }
-      }
-      __syncthreads();  // (nobody reads the buffer any more)
+      tree_mask_words<NW>(a, b, jd, wave, lane, mask_words);
       bool odd = false;
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         int r, col;
-        if (place(i, &r, &col)) {
+        const bool v = place(i, &r, &col);
+        if (jd + r >= a.T) piece[i] = u32x4{0u, 0u, 0u, 0u};
+        if (v) {
           v8 x = bitcast_u4<v8>(piece[i]);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -623,24 +632,24 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
           piece[i] = __builtin_bit_cast(u32x4, x);
         }
       }
-#pragma unroll
-      for (int x = 0; x < QB; ++x) {
-        see_bits[x] = 0;
-#pragma unroll
-        for (int e = 0; e < 8 * kSub; ++e) see_bits[x] |= (mb[x][e] != 0 ? 1u : 0u) << e;
-      }
       put(buf);
       if (odd) odd_flag = 1;
       __syncthreads();
-      for (int sub = 0; sub < kSub && j0 + sub * kTreeTile < a.T; ++sub)
-        compute(buf, sub, Kind<2>{}, a.T - j0 - sub * kTreeTile, j0 + sub * kTreeTile);
-      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < QB; ++x) {
+        const uint64_t w = mask_words[tq[x]] >> (4 * lg);
+        see_bits[x] = tree_key_bits((uint32_t)w) | tree_key_bits((uint32_t)(w >> 32)) << 8;
+      }
+      jd += kStage;
     }
+    compute(buf, std::true_type{});
+    buf ^= 1;
+  }
 
 #pragma unroll
   for (int x = 0; x < QB; ++x) {
     const int row = row0 + 16 * x;
-    const float l = add_xor32(add_xor16(lsum[x]));
+    const float l = lsum[x][0];
     if (row >= a.M) continue;
     if (a.direct) {
       const int h = a.div_t.div(row), t = row - h * a.T;
@@ -661,6 +670,11 @@ __global__ void __launch_bounds__(64 * NW) tree_wide_kernel(TreeArgs a) {
       st_dev(a.part_m + base, m[x] - kPBias<T>);
       st_dev(a.part_l + base, l);
     }
+  }
+  if (part.tail && __builtin_expect(odd_flag != 0, 0)) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    tree_add_odd<T, D, NT>(a, b, hkv, slot, mc * NW * 16 * QB, NW * 16 * QB);
   }
 }
 
@@ -817,11 +831,6 @@ hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_
   a.direct = pl.S == 1 && !pl.apart;
   a.div_t = Div::of(a.T);
   a.scale_log2 = (float)p.scale * 1.4426950408889634f;
-  auto vec = [](const void* x, const int64_t* s) {
-    return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
-  };
-  a.qvec = vec(p.q, p.q_s);
-  a.nvec = vec(p.k_new, p.kn_s) && vec(p.v_new, p.vn_s);
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
   a.part_m = reinterpret_cast<float*>(ws + kSyncBytes);
   a.part_l = a.part_m + pl.rows;
