@@ -5,17 +5,23 @@
 // in one pass over the row, with the running maximum; u is taken against the
 // maximum and not against zero, so that H does not come from the difference of
 // two large numbers.  Rows are cut into segments where there are few of them,
-// and a second kernel joins the segments.
+// and a second kernel joins the segments.  Bound by memory: 2047 rows of 151936
+// (622 MB).
 //
-// The `top` largest come from the same pass.  A value and its place make one
-// 64-bit key (value above, the complement of the place below): keys are all
-// different, larger means more probable, ties go to the lowest place.  A
-// workgroup keeps a threshold that at least `top` keys of its segment reach;
-// only keys above it are appended to a list in LDS, whose `top` largest are
-// kept, and their last one made the threshold, whenever it has grown long.  The
-// threshold of the first tile is the top-th largest of 64 groups' maxima.
+// The `top` largest.  A value and its place make one 64-bit key (value above,
+// the complement of the place below): keys are all different, larger means more
+// probable, ties go to the lowest place.  The pass leaves the maximum of each
+// block of 16 vectors (128 elements, or 64 of fp32).  The `top` best elements
+// lie in the `top` best blocks by (maximum, lowest place): for any element of
+// another block, each of those holds one that comes before it.  The second
+// kernel picks the blocks, reads them again (1 to 2 in a hundred of the row)
+// and picks the elements.  (Keeping a list of candidates within the pass took
+// 263 us for 20 of 2047 x 151936, where the pass alone takes 118.)  For the one
+// largest the pass itself keeps each thread's maximum and its tile, and the
+// threads that hold the workgroup's look into that tile again.
 #include "dkv_common.h"
 #include "dkv_internal.h"
+#include "dkv_select_dev.h"
 
 #include <algorithm>
 
@@ -25,11 +31,15 @@ constexpr int kLpThreads = 256;
 constexpr int kLpElems = 16;                        // elements per thread and tile
 constexpr int kLpTile = kLpThreads * kLpElems;
 constexpr int kLpMaxTop = 32;
-constexpr int kLpMaxSegs = 64;                      // a lane of the merge each
-// List: what is kept, and what one tile adds at most once its own threshold
-// holds: (top - 1) whole groups of 64 elements, and one key.
-constexpr int kLpCap = kLpMaxTop + (kLpMaxTop - 1) * (kLpTile / 64) + 1;
-constexpr int kLpTrim = 96;                         // a longer list is cut back
+constexpr int kLpMaxSegs = 64;  // a lane of the second kernel each
+template <typename T>
+constexpr int kLpBlock = 16 * 16 / (int)sizeof(T);  // elements: a row of 16 lanes' vectors
+// The second kernel's selection takes kLpItems items a thread at a time, and
+// those kept so far.
+constexpr int kLpItems = 8;
+// Its list: what a threshold that `top` of 64 groups (of four threads) reach
+// leaves at most, (top - 1) whole groups and one item.
+constexpr int kLpCap = (kLpMaxTop - 1) * 4 * (kLpItems + 1) + 1;
 constexpr int kLpPer = (kLpCap + kLpThreads - 1) / kLpThreads;
 
 struct LogprobArgs {
@@ -39,7 +49,9 @@ struct LogprobArgs {
   int64_t N;
   int V, top, S, seg;  // segments per row, elements per segment (whole tiles)
   float* part;         // [N, S, 3]: m, s, u
-  uint64_t* keys;      // [N, S, top]
+  uint32_t* blocks;    // [N, nb]: block maxima as ordered keys (top > 1)
+  int nb;
+  uint64_t* best;      // [N, S]: the segments' best keys (top 1)
   float* logprob;
   float* entropy;
   float* top_lp;
@@ -57,9 +69,9 @@ __device__ __forceinline__ void stat_to(Stat& a, float M) {
   a.m = M;
 }
 
-__device__ __forceinline__ uint64_t lp_key(float x, int i) {
-  const uint32_t k = x != x ? 0xffffffffu : float_key(x);  // NaN above all, as in torch's topk
-  return ((uint64_t)k << 32) | (0xffffffffu - (uint32_t)i);
+__device__ __forceinline__ uint32_t lp_order(float x) { return x != x ? 0xffffffffu : float_key(x); }
+__device__ __forceinline__ uint64_t lp_key(uint32_t order, int i) {  // NaN above all, as in torch's topk
+  return ((uint64_t)order << 32) | (0xffffffffu - (uint32_t)i);
 }
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int o) {
@@ -84,42 +96,17 @@ __device__ __forceinline__ void lp_write(const LogprobArgs& a, int64_t row, Stat
   }
 }
 
-// Keys of the list in order of rank: those of rank < top stay, at their rank.
-__device__ __forceinline__ void lp_trim(uint64_t* list, int c, int top) {
-  uint64_t key[kLpPer];
-  int rank[kLpPer];
-#pragma unroll
-  for (int q = 0; q < kLpPer; ++q) {
-    const int i = threadIdx.x + q * kLpThreads;
-    rank[q] = top;
-    if (i < c) {
-      key[q] = list[i];
-      int r = 0;
-      for (int j = 0; j < c; ++j) r += list[j] > key[q];
-      rank[q] = r;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < kLpPer; ++q)
-    if (rank[q] < top) list[rank[q]] = key[q];
-  __syncthreads();
-}
-
-// kTop 0: none; 1: the largest; 2: more.
-template <typename T, int kTop>
+// The pass: statistics of a segment; kMode 1: and its best key; 2: and its blocks'
+// maxima.
+template <typename T, int kMode>
 __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
   constexpr int EPV = 16 / (int)sizeof(T), NV = kLpElems / EPV;
   struct __attribute__((packed, aligned(sizeof(T)))) Raw {
     T e[EPV];
   };
   __shared__ Stat wstat[kLpThreads / 64];
-  __shared__ uint64_t wkey[kLpThreads / 64];
-  __shared__ uint64_t list[kTop == 2 ? kLpCap : 1];
-  __shared__ uint64_t group[kTop == 2 ? 64 : 1];
-  // Keys listed by a tile.  Tile i counts in word i mod 3 and clears the next
-  // one: its last readers (tile i - 2) have passed tile i - 1's barrier.
-  __shared__ int added[3];
+  __shared__ uint32_t worder[kLpThreads / 64];
+  __shared__ int place;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / a.S;
   const int sg = (int)(blockIdx.x - row * a.S);
@@ -127,19 +114,10 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
   const int lo = sg * a.seg, hi = min(a.V, lo + a.seg);
 
   Stat st{-__FLT_MAX__, 0.f, 0.f};
-  float best = -INFINITY;  // kTop 1: the thread's largest value and its place
-  int best_i = -1;
-  uint64_t T0 = 0;         // kTop 2: keys above it are listed
-  float T0f = -INFINITY;
-  int listed = 0;
-  int turn = 0;
-  if (kTop == 2) {
-    if (tid == 0) added[0] = 0;
-    __syncthreads();
-  }
-
+  uint32_t order = 0;  // kMode 1: the thread's largest value, and the first tile that holds it
+  int tile = lo;
   for (int j0 = lo; j0 < hi; j0 += kLpTile) {
-    float v[kLpElems];
+    float v[kLpElems], vmax[NV];
     // Element q EPV + e of the thread is at place j0 + (q 256 + tid) EPV + e.
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
@@ -153,9 +131,15 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
         for (int e = 0; e < EPV; ++e) v[q * EPV + e] = j + e < hi ? static_cast<float>(x[j + e]) : -INFINITY;
       }
     }
-    float tmax = v[0];
 #pragma unroll
-    for (int e = 1; e < kLpElems; ++e) tmax = __builtin_elementwise_maximum(tmax, v[e]);
+    for (int q = 0; q < NV; ++q) {
+      vmax[q] = v[q * EPV];
+#pragma unroll
+      for (int e = 1; e < EPV; ++e) vmax[q] = __builtin_elementwise_maximum(vmax[q], v[q * EPV + e]);
+    }
+    float tmax = vmax[0];
+#pragma unroll
+    for (int q = 1; q < NV; ++q) tmax = __builtin_elementwise_maximum(tmax, vmax[q]);
     if (tmax > st.m) stat_to(st, tmax);
 #pragma unroll
     for (int e = 0; e < kLpElems; ++e) {
@@ -164,96 +148,55 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
       st.s += f;
       st.u = fmaf(f, fmaxf(d, -__FLT_MAX__), st.u);  // (0 * -inf is no NaN of ours; a NaN has made f NaN)
     }
-    auto place = [&](int e) { return j0 + ((e / EPV) * kLpThreads + tid) * EPV + e % EPV; };
-    if (kTop == 1) {
-      if (best_i < 0 ? place(0) < hi : (tmax > best || (tmax != tmax && best == best))) {
-        best = tmax;
-        best_i = 0x7fffffff;
-#pragma unroll
-        for (int e = kLpElems - 1; e >= 0; --e)
-          if (place(e) < hi && (v[e] == tmax || v[e] != v[e])) best_i = place(e);
-      }
+    if (kMode == 1) {
+      const uint32_t k = lp_order(tmax);
+      tile = k > order ? j0 : tile;
+      order = max(order, k);
     }
-    if (kTop == 2) {
-      auto threshold = [&]() {  // the top-th largest of the tile's 64 group maxima, and every key above
-        uint64_t k = 0;
+    if (kMode == 2) {
 #pragma unroll
-        for (int e = 0; e < kLpElems; ++e)
-          if (place(e) < hi) k = max(k, lp_key(v[e], place(e)));
-        k = max(k, shfl_xor64(k, 1));
-        k = max(k, shfl_xor64(k, 2));
-        if ((lane & 3) == 0) group[tid >> 2] = k;
-        __syncthreads();
-        const uint64_t mine = group[lane];
-        int r = 0;
-        for (int j = 0; j < 64; ++j) r += group[j] > mine;
-        const uint64_t at = __builtin_amdgcn_ballot_w64(r == a.top - 1 && mine != 0);
-        // (Fewer groups than `top` hold anything: all keys pass.)
-        const uint64_t t = at ? group[__builtin_ctzll(at)] - 1 : 0;
-        __syncthreads();
-        return t;
-      };
-      auto append = [&]() {
-        if (!wave_any(!(tmax < T0f))) return;
-#pragma unroll
-        for (int e = 0; e < kLpElems; ++e) {
-          const uint64_t k = place(e) < hi ? lp_key(v[e], place(e)) : 0;
-          if (k > T0) {
-            const int at = listed + atomicAdd(&added[turn], 1);
-            if (at < kLpCap) list[at] = k;
-          }
-        }
-      };
-      auto set = [&](uint64_t t) {
-        if (t <= T0) return;
-        T0 = t;
-        const uint32_t hk = (uint32_t)(t >> 32);
-        T0f = hk == 0xffffffffu ? INFINITY : key_float(hk);
-      };
-      const int next = turn == 2 ? 0 : turn + 1;
-      if (tid == 0) added[next] = 0;
-      if (j0 == lo) set(threshold());
-      append();
-      __syncthreads();
-      int c = listed + added[turn];
-      if (c > kLpCap) {
-        // More than fits: the list as it was before this tile is cut back, and
-        // the tile goes in again above a threshold of its own.
-        lp_trim(list, listed, a.top);
-        if (listed >= a.top) set(list[a.top - 1]);
-        listed = min(listed, a.top);
-        if (tid == 0) added[turn] = 0;
-        set(threshold());
-        append();
-        __syncthreads();
-        c = listed + added[turn];
+      for (int q = 0; q < NV; ++q) {
+        uint32_t k = lp_order(vmax[q]);
+        k = max(k, (uint32_t)dpp_i<kDppQuadSwap1>((int)k));
+        k = max(k, (uint32_t)dpp_i<kDppQuadSwap2>((int)k));
+        k = max(k, (uint32_t)dpp_i<kDppHalfMirror>((int)k));
+        k = max(k, (uint32_t)dpp_i<kDppMirror>((int)k));
+        const int j = j0 + (q * kLpThreads + tid) * EPV;
+        if ((lane & 15) == 0 && j < hi) a.blocks[row * a.nb + j / kLpBlock<T>] = k;
       }
-      if (c > kLpTrim) {
-        lp_trim(list, c, a.top);
-        set(list[a.top - 1]);
-        c = a.top;
-      }
-      listed = c;
-      turn = next;
     }
   }
 
   // The workgroup's statistics.
-  const float wm = wave_max(st.m);
-  float M = wm;
-  stat_to(st, wm);
-  st.s = wave_sum(st.s);
-  st.u = wave_sum(st.u);
+  float M = wave_max_dpp(st.m);
+  stat_to(st, M);
+  st.s = wave_sum_dpp(st.s);
+  st.u = wave_sum_dpp(st.u);
   if (lane == 0) wstat[wave] = st;
-  if (kTop == 1) {
-    uint64_t k = best_i < 0 ? 0 : lp_key(best, best_i);
+  uint64_t key = 0;
+  if (kMode == 1) {
+    const uint32_t wo = wave_reduce_max(order);
+    if (lane == 0) worder[wave] = wo;
+    if (tid == 0) place = 0x7fffffff;
+    __syncthreads();
+    uint32_t most = worder[0];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) k = max(k, shfl_xor64(k, o));
-    if (lane == 0) wkey[wave] = k;
+    for (int w = 1; w < kLpThreads / 64; ++w) most = max(most, worder[w]);
+    if (order == most) {
+#pragma unroll 1
+      for (int e = 0; e < kLpElems; ++e) {
+        const int j = tile + ((e / EPV) * kLpThreads + tid) * EPV + e % EPV;
+        if (j < hi && lp_order(static_cast<float>(x[j])) == most) {
+          atomicMin(&place, j);
+          break;
+        }
+      }
+    }
+    key = most;  // (with the place below, once every thread has looked)
   }
   __syncthreads();
-  if (kTop == 2) lp_trim(list, listed, a.top);
   if (wave != 0) return;
+  if (kMode == 1) key = lp_key((uint32_t)key, place);
 #pragma unroll
   for (int w = 0; w < kLpThreads / 64; ++w) M = fmaxf(M, wstat[w].m);
   Stat all{M, 0.f, 0.f};
@@ -264,13 +207,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
     all.s += p.s;
     all.u += p.u;
   }
-  uint64_t key = 0;
-  if (kTop == 1) {
-#pragma unroll
-    for (int w = 0; w < kLpThreads / 64; ++w) key = max(key, wkey[w]);
-  }
-  if (kTop == 2 && lane < min(listed, a.top)) key = list[lane];
-  if (a.S == 1) {
+  if (kMode != 2 && a.S == 1) {
     lp_write<T>(a, row, all, lane, key);
     return;
   }
@@ -279,34 +216,116 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
     a.part[3 * p] = all.m;
     a.part[3 * p + 1] = all.s;
     a.part[3 * p + 2] = all.u;
+    if (kMode == 1) a.best[p] = key;
   }
-  if (lane < a.top) a.keys[p * a.top + lane] = key;
 }
 
-// One wave per row: a lane per segment, whose keys are in falling order.
-template <typename T>
-__global__ void __launch_bounds__(64) logprob_merge_kernel(LogprobArgs a) {
-  const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
-  const bool on = lane < a.S;
-  const int64_t p = row * a.S + lane;
-  Stat st{-__FLT_MAX__, 0.f, 0.f};
-  if (on) st = Stat{a.part[3 * p], a.part[3 * p + 1], a.part[3 * p + 2]};
-  stat_to(st, wave_max(st.m));
-  st.s = wave_sum(st.s);
-  st.u = wave_sum(st.u);
-  const uint64_t* mine = a.keys + p * a.top;
-  uint64_t head = on && a.top > 0 ? mine[0] : 0, key = 0;
-  int at = 0;
-  for (int i = 0; i < a.top; ++i) {
-    uint64_t k = head;
+struct LpList {
+  uint64_t list[kLpCap];
+  uint64_t group[64];
+  int count;
+};
+// The k largest of item(0) .. item(n - 1) (distinct, or 0: none), in falling
+// order in list[0 .. k); the whole workgroup.  kLpItems items a thread at a time:
+// a threshold that k of them reach (the k-th largest of 64 groups' maxima), the
+// few above it into the list, and the list in order by each item's rank in it.
+template <typename F>
+__device__ __forceinline__ void lp_select(F&& item, int n, int k, LpList* s) {
+  const int tid = threadIdx.x, lane = tid & 63;
+#pragma unroll 1
+  for (int base = 0; base < n; base += kLpItems * kLpThreads) {
+    uint64_t key[kLpItems + 1], most = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) k = max(k, shfl_xor64(k, o));
-    if (lane == i) key = k;
-    if (head == k && k != 0) {
-      ++at;
-      head = at < a.top ? mine[at] : 0;
+    for (int q = 0; q < kLpItems; ++q) key[q] = item(base + q * kLpThreads + tid);
+    key[kLpItems] = base > 0 && tid < k ? s->list[tid] : 0;
+#pragma unroll
+    for (int q = 0; q <= kLpItems; ++q) most = max(most, key[q]);
+    most = max(most, shfl_xor64(most, 1));
+    most = max(most, shfl_xor64(most, 2));
+    if ((lane & 3) == 0) s->group[tid >> 2] = most;
+    if (tid == 0) s->count = 0;
+    __syncthreads();
+    const uint64_t mine = s->group[lane];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) rank += s->group[j] > mine;
+    const uint64_t at = __builtin_amdgcn_ballot_w64(rank == k - 1 && mine != 0);
+    // (Where fewer than k groups hold anything, everything passes.)
+    const uint64_t t = at ? s->group[__builtin_ctzll(at)] - 1 : 0;
+#pragma unroll
+    for (int q = 0; q <= kLpItems; ++q)
+      if (key[q] > t) s->list[atomicAdd(&s->count, 1)] = key[q];
+    __syncthreads();
+    const int c = s->count;
+    uint64_t mykey[kLpPer];
+    int place[kLpPer];
+#pragma unroll
+    for (int q = 0; q < kLpPer; ++q) {
+      const int i = tid + q * kLpThreads;
+      place[q] = k;
+      mykey[q] = 0;
+      if (q * kLpThreads < c && i < c) {
+        mykey[q] = s->list[i];
+        int r = 0;
+        for (int j = 0; j < c; ++j) r += s->list[j] > mykey[q];
+        place[q] = r;
+      }
     }
+    __syncthreads();
+    if (tid >= c && tid < k) s->list[tid] = 0;
+#pragma unroll
+    for (int q = 0; q < kLpPer; ++q)
+      if (place[q] < k) s->list[place[q]] = mykey[q];
+    __syncthreads();
+  }
+}
+
+// A row's results: its segments joined, its best blocks and their best elements.
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads) logprob_finish_kernel(LogprobArgs a) {
+  constexpr int kBlock = kLpBlock<T>;
+  __shared__ LpList s;
+  __shared__ int chosen[kLpMaxTop];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  Stat st{-__FLT_MAX__, 0.f, 0.f};
+  if (lane < a.S) {
+    const int64_t p = row * a.S + lane;
+    st = Stat{a.part[3 * p], a.part[3 * p + 1], a.part[3 * p + 2]};
+  }
+  uint64_t key = 0;
+  if (a.top == 1 && lane < a.S) key = a.best[row * a.S + lane];
+  if (a.top > 1) {
+    const int nb = a.nb, kb = min(a.top, nb);
+    const uint32_t* blocks = a.blocks + row * nb;
+    lp_select(
+        [&](int i) {
+          const uint64_t k = lp_key(blocks[min(i, nb - 1)], i);
+          return i < nb ? k : 0;
+        },
+        nb, kb, &s);
+    if (tid < kb) chosen[tid] = (int)(0xffffffffu - (uint32_t)s.list[tid]);
+    __syncthreads();
+    const T* x = static_cast<const T*>(a.x) + row * a.sx;
+    const int n = kb * kBlock;
+    lp_select(
+        [&](int i) {
+          const int j = chosen[min(i, n - 1) / kBlock] * kBlock + i % kBlock;
+          const uint64_t k = lp_key(lp_order(static_cast<float>(x[min(j, a.V - 1)])), j);
+          return i < n && j < a.V ? k : 0;
+        },
+        n, a.top, &s);
+  }
+  if (tid >= 64) return;
+  stat_to(st, wave_max_dpp(st.m));
+  st.s = wave_sum_dpp(st.s);
+  st.u = wave_sum_dpp(st.u);
+  if (a.top == 1) {
+    const uint32_t order = wave_reduce_max((uint32_t)(key >> 32));
+    const uint32_t low = wave_reduce_max((uint32_t)(key >> 32) == order ? (uint32_t)key : 0u);
+    key = ((uint64_t)order << 32) | low;
+  } else if (lane < a.top) {
+    key = s.list[lane];
   }
   lp_write<T>(a, row, st, lane, key);
 }
@@ -325,14 +344,18 @@ static LogprobPlan logprob_plan(int64_t N, int64_t V, int64_t top) {
   LogprobPlan p;
   p.S = (int)((tiles + per - 1) / per);
   p.seg = (int)std::min<int64_t>(per * kLpTile, INT32_MAX - kLpTile);
-  p.bytes = p.S == 1 ? 0 : kSyncBytes + (size_t)N * p.S * (3 * sizeof(float) + (size_t)top * sizeof(uint64_t)) + 256;
+  // (Bytes of a part and its best key; 64 elements to the smaller block.)
+  p.bytes = p.S == 1 && top <= 1
+                ? 0
+                : kSyncBytes + 256 + (size_t)N * p.S * 24 + (top > 1 ? (size_t)N * ((V + 63) / 64) * 4 : 0);
   return p;
 }
 size_t logprob_workspace_bytes(int64_t N, int64_t V, int64_t top) { return logprob_plan(N, V, top).bytes; }
 int64_t logprob_max_top() { return kLpMaxTop; }
 
 template <typename T>
-static hipError_t launch_logprob_t(const LogprobArgs& a, hipStream_t st) {
+static hipError_t launch_logprob_t(LogprobArgs a, hipStream_t st) {
+  a.nb = (a.V + kLpBlock<T> - 1) / kLpBlock<T>;
   const dim3 grid((unsigned)(a.N * a.S));
   if (a.top == 0)
     launch((logprob_kernel<T, 0>), grid, dim3(kLpThreads), 0, st, a);
@@ -340,7 +363,7 @@ static hipError_t launch_logprob_t(const LogprobArgs& a, hipStream_t st) {
     launch((logprob_kernel<T, 1>), grid, dim3(kLpThreads), 0, st, a);
   else
     launch((logprob_kernel<T, 2>), grid, dim3(kLpThreads), 0, st, a);
-  if (a.S > 1) launch((logprob_merge_kernel<T>), dim3((unsigned)a.N), dim3(64), 0, st, a);
+  if (a.S > 1 || a.top > 1) launch((logprob_finish_kernel<T>), dim3((unsigned)a.N), dim3(kLpThreads), 0, st, a);
   return hipGetLastError();
 }
 
@@ -356,8 +379,9 @@ hipError_t launch_token_logprobs(const dropkv_token_logprobs_args& p, hipStream_
   a.S = pl.S;
   a.seg = pl.seg;
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
-  a.keys = reinterpret_cast<uint64_t*>(ws + kSyncBytes);
-  a.part = reinterpret_cast<float*>(a.keys + (size_t)p.N * pl.S * p.top);
+  a.best = reinterpret_cast<uint64_t*>(ws + kSyncBytes);
+  a.part = reinterpret_cast<float*>(a.best + (size_t)p.N * pl.S);
+  a.blocks = reinterpret_cast<uint32_t*>(a.part + (size_t)p.N * pl.S * 3);
   a.logprob = p.logprob;
   a.entropy = p.entropy;
   a.top_lp = p.top_logprobs;
