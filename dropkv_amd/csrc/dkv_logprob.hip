@@ -4,18 +4,18 @@
 //   log p_i = x_i - m - ln s,  H = -sum p_i ln p_i = ln s - u / s
 // in one pass over the row, with the running maximum; u is taken against the
 // maximum and not against zero, so that H does not come from the difference of
-// two large numbers.  Rows are cut into segments where there are few of them,
-// and a second kernel joins the segments.  Bound by memory: 2047 rows of 151936
-// (622 MB).
+// two large numbers.  Rows are cut into segments where there are few of them;
+// they are joined by the workgroup that finishes a row last, or by a second
+// kernel.  Bound by memory: 2047 rows of 151936 (622 MB).
 //
 // The `top` largest.  A value and its place make one 64-bit key (value above,
 // the complement of the place below): keys are all different, larger means more
 // probable, ties go to the lowest place.  The pass leaves the maximum of each
 // block of 16 vectors (128 elements, or 64 of fp32).  The `top` best elements
 // lie in the `top` best blocks by (maximum, lowest place): for any element of
-// another block, each of those holds one that comes before it.  The second
-// kernel picks the blocks, reads them again (1 to 2 in a hundred of the row)
-// and picks the elements.  (Keeping a list of candidates within the pass took
+// another block, each of those holds one that comes before it.  Then the
+// blocks are picked, read again (1 to 2 in a hundred of the row), and the elements
+// picked.  (Keeping a list of candidates within the pass took
 // 263 us for 20 of 2047 x 151936, where the pass alone takes 118.)  For the one
 // largest the pass itself keeps each thread's maximum and its tile, and the
 // threads that hold the workgroup's look into that tile again.
@@ -31,11 +31,10 @@ constexpr int kLpThreads = 256;
 constexpr int kLpElems = 16;                        // elements per thread and tile
 constexpr int kLpTile = kLpThreads * kLpElems;
 constexpr int kLpMaxTop = 32;
-constexpr int kLpMaxSegs = 64;  // a lane of the second kernel each
+constexpr int kLpMaxSegs = 64;  // a lane each where they are joined
 template <typename T>
 constexpr int kLpBlock = 16 * 16 / (int)sizeof(T);  // elements: a row of 16 lanes' vectors
-// The second kernel's selection takes kLpItems items a thread at a time, and
-// those kept so far.
+// The selection takes kLpItems items a thread at a time, and those kept so far.
 constexpr int kLpItems = 8;
 // Its list: what a threshold that `top` of 64 groups (of four threads) reach
 // leaves at most, (top - 1) whole groups and one item.
@@ -48,10 +47,12 @@ struct LogprobArgs {
   const int64_t* tokens;
   int64_t N;
   int V, top, S, seg;  // segments per row, elements per segment (whole tiles)
+  int one;             // the row's last workgroup joins its segments (else a second kernel)
   float* part;         // [N, S, 3]: m, s, u
   uint32_t* blocks;    // [N, nb]: block maxima as ordered keys (top > 1)
   int nb;
   uint64_t* best;      // [N, S]: the segments' best keys (top 1)
+  uint32_t* arrived;   // [N]: segments done (S > 1)
   float* logprob;
   float* entropy;
   float* top_lp;
@@ -93,130 +94,6 @@ __device__ __forceinline__ void lp_write(const LogprobArgs& a, int64_t row, Stat
   if (lane < a.top) {
     a.top_lp[row * a.top + lane] = (key_float((uint32_t)(key >> 32)) - st.m) - ln_s;
     a.top_id[row * a.top + lane] = 0xffffffffu - (uint32_t)key;
-  }
-}
-
-// The pass: statistics of a segment; kMode 1: and its best key; 2: and its blocks'
-// maxima.
-template <typename T, int kMode>
-__global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
-  constexpr int EPV = 16 / (int)sizeof(T), NV = kLpElems / EPV;
-  struct __attribute__((packed, aligned(sizeof(T)))) Raw {
-    T e[EPV];
-  };
-  __shared__ Stat wstat[kLpThreads / 64];
-  __shared__ uint32_t worder[kLpThreads / 64];
-  __shared__ int place;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x / a.S;
-  const int sg = (int)(blockIdx.x - row * a.S);
-  const T* x = static_cast<const T*>(a.x) + row * a.sx;
-  const int lo = sg * a.seg, hi = min(a.V, lo + a.seg);
-
-  Stat st{-__FLT_MAX__, 0.f, 0.f};
-  uint32_t order = 0;  // kMode 1: the thread's largest value, and the first tile that holds it
-  int tile = lo;
-  for (int j0 = lo; j0 < hi; j0 += kLpTile) {
-    float v[kLpElems], vmax[NV];
-    // Element q EPV + e of the thread is at place j0 + (q 256 + tid) EPV + e.
-#pragma unroll
-    for (int q = 0; q < NV; ++q) {
-      const int j = j0 + (q * kLpThreads + tid) * EPV;
-      if (j + EPV <= hi) {
-        const Raw r = *reinterpret_cast<const Raw*>(x + j);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) v[q * EPV + e] = static_cast<float>(r.e[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) v[q * EPV + e] = j + e < hi ? static_cast<float>(x[j + e]) : -INFINITY;
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < NV; ++q) {
-      vmax[q] = v[q * EPV];
-#pragma unroll
-      for (int e = 1; e < EPV; ++e) vmax[q] = __builtin_elementwise_maximum(vmax[q], v[q * EPV + e]);
-    }
-    float tmax = vmax[0];
-#pragma unroll
-    for (int q = 1; q < NV; ++q) tmax = __builtin_elementwise_maximum(tmax, vmax[q]);
-    if (tmax > st.m) stat_to(st, tmax);
-#pragma unroll
-    for (int e = 0; e < kLpElems; ++e) {
-      const float d = v[e] - st.m;
-      const float f = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
-      st.s += f;
-      st.u = fmaf(f, fmaxf(d, -__FLT_MAX__), st.u);  // (0 * -inf is no NaN of ours; a NaN has made f NaN)
-    }
-    if (kMode == 1) {
-      const uint32_t k = lp_order(tmax);
-      tile = k > order ? j0 : tile;
-      order = max(order, k);
-    }
-    if (kMode == 2) {
-#pragma unroll
-      for (int q = 0; q < NV; ++q) {
-        uint32_t k = lp_order(vmax[q]);
-        k = max(k, (uint32_t)dpp_i<kDppQuadSwap1>((int)k));
-        k = max(k, (uint32_t)dpp_i<kDppQuadSwap2>((int)k));
-        k = max(k, (uint32_t)dpp_i<kDppHalfMirror>((int)k));
-        k = max(k, (uint32_t)dpp_i<kDppMirror>((int)k));
-        const int j = j0 + (q * kLpThreads + tid) * EPV;
-        if ((lane & 15) == 0 && j < hi) a.blocks[row * a.nb + j / kLpBlock<T>] = k;
-      }
-    }
-  }
-
-  // The workgroup's statistics.
-  float M = wave_max_dpp(st.m);
-  stat_to(st, M);
-  st.s = wave_sum_dpp(st.s);
-  st.u = wave_sum_dpp(st.u);
-  if (lane == 0) wstat[wave] = st;
-  uint64_t key = 0;
-  if (kMode == 1) {
-    const uint32_t wo = wave_reduce_max(order);
-    if (lane == 0) worder[wave] = wo;
-    if (tid == 0) place = 0x7fffffff;
-    __syncthreads();
-    uint32_t most = worder[0];
-#pragma unroll
-    for (int w = 1; w < kLpThreads / 64; ++w) most = max(most, worder[w]);
-    if (order == most) {
-#pragma unroll 1
-      for (int e = 0; e < kLpElems; ++e) {
-        const int j = tile + ((e / EPV) * kLpThreads + tid) * EPV + e % EPV;
-        if (j < hi && lp_order(static_cast<float>(x[j])) == most) {
-          atomicMin(&place, j);
-          break;
-        }
-      }
-    }
-    key = most;  // (with the place below, once every thread has looked)
-  }
-  __syncthreads();
-  if (wave != 0) return;
-  if (kMode == 1) key = lp_key((uint32_t)key, place);
-#pragma unroll
-  for (int w = 0; w < kLpThreads / 64; ++w) M = fmaxf(M, wstat[w].m);
-  Stat all{M, 0.f, 0.f};
-#pragma unroll
-  for (int w = 0; w < kLpThreads / 64; ++w) {
-    Stat p = wstat[w];
-    stat_to(p, M);
-    all.s += p.s;
-    all.u += p.u;
-  }
-  if (kMode != 2 && a.S == 1) {
-    lp_write<T>(a, row, all, lane, key);
-    return;
-  }
-  const int64_t p = row * a.S + sg;
-  if (lane == 0) {
-    a.part[3 * p] = all.m;
-    a.part[3 * p + 1] = all.s;
-    a.part[3 * p + 2] = all.u;
-    if (kMode == 1) a.best[p] = key;
   }
 }
 
@@ -281,21 +158,18 @@ __device__ __forceinline__ void lp_select(F&& item, int n, int k, LpList* s) {
 }
 
 // A row's results: its segments joined, its best blocks and their best elements.
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprob_finish_kernel(LogprobArgs a) {
+template <typename T, int kMode>
+__device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t row, LpList* s, int* chosen) {
   constexpr int kBlock = kLpBlock<T>;
-  __shared__ LpList s;
-  __shared__ int chosen[kLpMaxTop];
-  const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63;
   Stat st{-__FLT_MAX__, 0.f, 0.f};
+  uint64_t key = 0;
   if (lane < a.S) {
     const int64_t p = row * a.S + lane;
     st = Stat{a.part[3 * p], a.part[3 * p + 1], a.part[3 * p + 2]};
+    if (kMode == 1) key = a.best[p];
   }
-  uint64_t key = 0;
-  if (a.top == 1 && lane < a.S) key = a.best[row * a.S + lane];
-  if (a.top > 1) {
+  if (kMode == 2) {
     const int nb = a.nb, kb = min(a.top, nb);
     const uint32_t* blocks = a.blocks + row * nb;
     lp_select(
@@ -303,8 +177,8 @@ __global__ void __launch_bounds__(kLpThreads) logprob_finish_kernel(LogprobArgs 
           const uint64_t k = lp_key(blocks[min(i, nb - 1)], i);
           return i < nb ? k : 0;
         },
-        nb, kb, &s);
-    if (tid < kb) chosen[tid] = (int)(0xffffffffu - (uint32_t)s.list[tid]);
+        nb, kb, s);
+    if (tid < kb) chosen[tid] = (int)(0xffffffffu - (uint32_t)s->list[tid]);
     __syncthreads();
     const T* x = static_cast<const T*>(a.x) + row * a.sx;
     const int n = kb * kBlock;
@@ -314,24 +188,178 @@ __global__ void __launch_bounds__(kLpThreads) logprob_finish_kernel(LogprobArgs 
           const uint64_t k = lp_key(lp_order(static_cast<float>(x[min(j, a.V - 1)])), j);
           return i < n && j < a.V ? k : 0;
         },
-        n, a.top, &s);
+        n, a.top, s);
   }
   if (tid >= 64) return;
   stat_to(st, wave_max_dpp(st.m));
   st.s = wave_sum_dpp(st.s);
   st.u = wave_sum_dpp(st.u);
-  if (a.top == 1) {
+  if (kMode == 1) {
     const uint32_t order = wave_reduce_max((uint32_t)(key >> 32));
     const uint32_t low = wave_reduce_max((uint32_t)(key >> 32) == order ? (uint32_t)key : 0u);
     key = ((uint64_t)order << 32) | low;
-  } else if (lane < a.top) {
-    key = s.list[lane];
+  } else if (kMode == 2 && lane < a.top) {
+    key = s->list[lane];
   }
   lp_write<T>(a, row, st, lane, key);
 }
 
+// The pass: statistics of a segment; kMode 1: and its best key; 2: and its blocks'
+// maxima.
+template <typename T, int kMode>
+__global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
+  constexpr int EPV = 16 / (int)sizeof(T), NV = kLpElems / EPV;
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw {
+    T e[EPV];
+  };
+  __shared__ Stat wstat[kLpThreads / 64];
+  __shared__ uint32_t worder[kLpThreads / 64];
+  __shared__ int place, last;
+  __shared__ char select_lds[kMode == 2 ? sizeof(LpList) : 1] __attribute__((aligned(8)));
+  __shared__ int chosen[kMode == 2 ? kLpMaxTop : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x / a.S;
+  const int sg = (int)(blockIdx.x - row * a.S);
+  const T* x = static_cast<const T*>(a.x) + row * a.sx;
+  const int lo = sg * a.seg, hi = min(a.V, lo + a.seg);
+
+  Stat st{-__FLT_MAX__, 0.f, 0.f};
+  uint32_t order = 0;  // kMode 1: the thread's largest value, and the first tile that holds it
+  int tile = lo;
+  for (int j0 = lo; j0 < hi; j0 += kLpTile) {
+    float v[kLpElems], vmax[NV];
+    // Element q EPV + e of the thread is at place j0 + (q 256 + tid) EPV + e.
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const int j = j0 + (q * kLpThreads + tid) * EPV;
+      if (j + EPV <= hi) {
+        const Raw r = *reinterpret_cast<const Raw*>(x + j);
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) v[q * EPV + e] = static_cast<float>(r.e[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) v[q * EPV + e] = j + e < hi ? static_cast<float>(x[j + e]) : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      vmax[q] = v[q * EPV];
+#pragma unroll
+      for (int e = 1; e < EPV; ++e) vmax[q] = __builtin_elementwise_maximum(vmax[q], v[q * EPV + e]);
+    }
+    float tmax = vmax[0];
+#pragma unroll
+    for (int q = 1; q < NV; ++q) tmax = __builtin_elementwise_maximum(tmax, vmax[q]);
+    if (tmax > st.m) stat_to(st, tmax);
+#pragma unroll
+    for (int e = 0; e < kLpElems; ++e) {
+      const float d = v[e] - st.m;
+      const float f = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+      st.s += f;
+      st.u = fmaf(f, fmaxf(d, -__FLT_MAX__), st.u);  // (0 * -inf is no NaN of ours; a NaN has made f NaN)
+    }
+    if (kMode == 1) {
+      const uint32_t k = lp_order(tmax);
+      tile = k > order ? j0 : tile;
+      order = max(order, k);
+    }
+    if (kMode == 2) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        uint32_t k = lp_order(vmax[q]);
+        k = max(k, (uint32_t)dpp_i<kDppQuadSwap1>((int)k));
+        k = max(k, (uint32_t)dpp_i<kDppQuadSwap2>((int)k));
+        k = max(k, (uint32_t)dpp_i<kDppHalfMirror>((int)k));
+        k = max(k, (uint32_t)dpp_i<kDppMirror>((int)k));
+        const int j = j0 + (q * kLpThreads + tid) * EPV;
+        if ((lane & 15) == 0 && j < hi) st_dev(a.blocks + row * a.nb + j / kLpBlock<T>, k);
+      }
+    }
+  }
+
+  // The workgroup's statistics.
+  float M = wave_max_dpp(st.m);
+  stat_to(st, M);
+  st.s = wave_sum_dpp(st.s);
+  st.u = wave_sum_dpp(st.u);
+  if (lane == 0) wstat[wave] = st;
+  uint64_t key = 0;
+  if (kMode == 1) {
+    const uint32_t wo = wave_reduce_max(order);
+    if (lane == 0) worder[wave] = wo;
+    if (tid == 0) place = 0x7fffffff;
+    __syncthreads();
+    uint32_t most = worder[0];
+#pragma unroll
+    for (int w = 1; w < kLpThreads / 64; ++w) most = max(most, worder[w]);
+    if (order == most) {
+#pragma unroll 1
+      for (int e = 0; e < kLpElems; ++e) {
+        const int j = tile + ((e / EPV) * kLpThreads + tid) * EPV + e % EPV;
+        if (j < hi && lp_order(static_cast<float>(x[j])) == most) {
+          atomicMin(&place, j);
+          break;
+        }
+      }
+    }
+    key = most;  // (with the place below, once every thread has looked)
+  }
+  __syncthreads();
+  if (wave == 0) {
+    if (kMode == 1) key = lp_key((uint32_t)key, place);
+#pragma unroll
+    for (int w = 0; w < kLpThreads / 64; ++w) M = fmaxf(M, wstat[w].m);
+    Stat all{M, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kLpThreads / 64; ++w) {
+      Stat p = wstat[w];
+      stat_to(p, M);
+      all.s += p.s;
+      all.u += p.u;
+    }
+    if (kMode != 2 && a.S == 1) lp_write<T>(a, row, all, lane, key);
+    if (lane == 0) {
+      const int64_t p = row * a.S + sg;
+      if (kMode == 2 || a.S > 1) {
+        st_dev(a.part + 3 * p, all.m);
+        st_dev(a.part + 3 * p + 1, all.s);
+        st_dev(a.part + 3 * p + 2, all.u);
+        if (kMode == 1) st_dev(a.best + p, key);
+      }
+    }
+  }
+  if (a.S == 1 ? kMode != 2 : !a.one) return;
+  // The row's last workgroup goes on (a row's counter is zero before the call,
+  // counts its segments and wraps to zero).  Every wave's stores are out first.
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (a.S > 1) {
+    if (tid == 0) {
+      last = atomicInc(a.arrived + row, (uint32_t)a.S - 1u) == (uint32_t)a.S - 1u;
+      if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    }
+    __syncthreads();
+    if (!last) return;
+  }
+  lp_finish<T, kMode>(a, row, reinterpret_cast<LpList*>(select_lds), chosen);
+}
+
+template <typename T, int kMode>
+__global__ void __launch_bounds__(kLpThreads) logprob_finish_kernel(LogprobArgs a) {
+  __shared__ LpList sel;
+  __shared__ int chosen[kLpMaxTop];
+  lp_finish<T, kMode>(a, blockIdx.x, &sel, chosen);
+}
+
 // Workgroups of a call: enough to fill the GPU where a row can be cut.
 constexpr int64_t kLpGroups = 2048;
+// Up to so many, the row's last workgroup joins its segments: one launch (one row
+// of 151936, 5 alternatives: 12.9 us in a graph either way, 11.3 us of host time
+// against 14.3).  With more, its wait for the stores and the counter comes on top
+// of every segment, and a second kernel is faster (8 rows 13.5 against 15.5 us,
+// 216 rows 27.9 against 33.4).
+constexpr int64_t kLpOneLaunch = 128;
+static_assert(kLpOneLaunch * sizeof(uint32_t) <= kSyncBytes, "a counter per row");
 
 struct LogprobPlan {
   int S, seg;
@@ -356,14 +384,18 @@ int64_t logprob_max_top() { return kLpMaxTop; }
 template <typename T>
 static hipError_t launch_logprob_t(LogprobArgs a, hipStream_t st) {
   a.nb = (a.V + kLpBlock<T> - 1) / kLpBlock<T>;
-  const dim3 grid((unsigned)(a.N * a.S));
-  if (a.top == 0)
-    launch((logprob_kernel<T, 0>), grid, dim3(kLpThreads), 0, st, a);
-  else if (a.top == 1)
-    launch((logprob_kernel<T, 1>), grid, dim3(kLpThreads), 0, st, a);
-  else
-    launch((logprob_kernel<T, 2>), grid, dim3(kLpThreads), 0, st, a);
-  if (a.S > 1 || a.top > 1) launch((logprob_finish_kernel<T>), dim3((unsigned)a.N), dim3(kLpThreads), 0, st, a);
+  const dim3 grid((unsigned)(a.N * a.S)), rows((unsigned)a.N), block(kLpThreads);
+  const bool two = a.S > 1 && !a.one;
+  if (a.top == 0) {
+    launch((logprob_kernel<T, 0>), grid, block, 0, st, a);
+    if (two) launch((logprob_finish_kernel<T, 0>), rows, block, 0, st, a);
+  } else if (a.top == 1) {
+    launch((logprob_kernel<T, 1>), grid, block, 0, st, a);
+    if (two) launch((logprob_finish_kernel<T, 1>), rows, block, 0, st, a);
+  } else {
+    launch((logprob_kernel<T, 2>), grid, block, 0, st, a);
+    if (two) launch((logprob_finish_kernel<T, 2>), rows, block, 0, st, a);
+  }
   return hipGetLastError();
 }
 
@@ -377,8 +409,10 @@ hipError_t launch_token_logprobs(const dropkv_token_logprobs_args& p, hipStream_
   a.V = (int)p.V;
   a.top = (int)p.top;
   a.S = pl.S;
+  a.one = p.N * pl.S <= kLpOneLaunch;
   a.seg = pl.seg;
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
+  a.arrived = reinterpret_cast<uint32_t*>(ws);
   a.best = reinterpret_cast<uint64_t*>(ws + kSyncBytes);
   a.part = reinterpret_cast<float*>(a.best + (size_t)p.N * pl.S);
   a.blocks = reinterpret_cast<uint32_t*>(a.part + (size_t)p.N * pl.S * 3);
