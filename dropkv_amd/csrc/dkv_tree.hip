@@ -49,6 +49,7 @@ struct TreeArgs {
   int direct;  // one part: the output is written by it
   Div div_t;
   float scale_log2;
+  int* deal;      // [B, 2]: first part and number of parts (ragged), for the joining kernel
   float* part_m;  // [Hkv, P, M]
   float* part_l;
   float* part_o;  // [Hkv, P, M, D]
@@ -107,6 +108,7 @@ __device__ __forceinline__ int tree_rows(const TreeArgs& a, int b) {
 // sequence i.  Drafted keys that go with a sequence's last part count as
 // `tail_tiles` tiles of it.
 constexpr int kTreeRaggedB = 64;
+constexpr size_t kTreeDealBytes = kTreeRaggedB * 2 * sizeof(int);
 struct TreeParts {
   int first, count, per;
 };
@@ -128,25 +130,22 @@ __device__ __forceinline__ TreeParts tree_parts_ragged(const TreeArgs& a, int la
   p.first = (int)wave_incl_scan((uint32_t)p.count) - p.count;
   return p;
 }
-__device__ __forceinline__ TreeParts tree_parts(const TreeArgs& a, int b, int lane) {
-  if (!a.ragged) return TreeParts{b * a.S, a.S, ceil_div(tree_tiles(a, b) + a.tail_tiles, a.S)};
-  TreeParts p = tree_parts_ragged(a, lane);
-  return TreeParts{__builtin_amdgcn_readlane(p.first, b), __builtin_amdgcn_readlane(p.count, b),
-                   __builtin_amdgcn_readfirstlane(p.per)};
-}
-
 // Part `slot` of a KV head: tiles t_lo .. t_hi of sequence b, whose stored rows
 // are n, and with `tail` the drafted keys; b < 0: none.
 struct TreePart {
   int b, n, t_lo, t_hi;
   bool tail;
 };
-__device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int slot, int lane) {
+__device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int hkv, int slot, int lane) {
   TreePart p;
   if (slot >= a.B * a.S) return TreePart{slot - a.B * a.S, 0, 0, 0, true};
   int first, count, per;
   if (a.ragged) {
     const TreeParts all = tree_parts_ragged(a, lane);
+    if (slot == 0 && hkv == 0 && lane < a.B) {  // (by each workgroup of the slot's rows alike)
+      a.deal[2 * lane] = all.first;
+      a.deal[2 * lane + 1] = all.count;
+    }
     const uint64_t hit = __builtin_amdgcn_ballot_w64(all.first <= slot && slot < all.first + all.count);
     if (!hit) return TreePart{-1, 0, 0, 0, false};
     p.b = __builtin_ctzll(hit);
@@ -244,7 +243,7 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   __shared__ __attribute__((aligned(16))) T vt[kTreeTile * kVPitch];
   __shared__ uint64_t mask_words[16];  // (T <= 16 rows)
 
-  const TreePart part = tree_part(a, slot, lane);
+  const TreePart part = tree_part(a, hkv, slot, lane);
   const int b = part.b, n = part.n;
   if (b < 0) return;
   const int bh = b * a.Hkv + hkv;
@@ -435,7 +434,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 2 ? 1 : 2) tree_wide_kernel(Tre
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int mc = id % a.MC, slot = (id / a.MC) % a.P, hkv = id / (a.MC * a.P), g = a.Hq / a.Hkv;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
-  const TreePart part = tree_part(a, slot, lane);
+  const TreePart part = tree_part(a, hkv, slot, lane);
   const int b = part.b, n = part.n;
   if (b < 0) return;
   const int bh = b * a.Hkv + hkv;
@@ -691,10 +690,10 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
   const int b = bh / a.Hkv, hkv = bh % a.Hkv;
   const int h = a.div_t.div(row), t = row - h * a.T;
   const int sub = lane / LPR, d0 = 4 * (lane % LPR);
-  const TreeParts parts = tree_parts(a, b, lane);
-  const int S1 = parts.count + a.apart;
+  const int first = a.ragged ? a.deal[2 * b] : b * a.S, count = a.ragged ? a.deal[2 * b + 1] : a.S;
+  const int S1 = count + a.apart;
   // Row of part s: those of the cache, then the drafted keys'.
-  auto at = [&](int s) { return ((int64_t)hkv * a.P + (s < parts.count ? parts.first + s : a.B * a.S + b)) * a.M + row; };
+  auto at = [&](int s) { return ((int64_t)hkv * a.P + (s < count ? first + s : a.B * a.S + b)) * a.M + row; };
   const float ml = lane < S1 ? a.part_m[at(lane)] : -__FLT_MAX__;
   const float ll = lane < S1 ? a.part_l[at(lane)] : 0.f;
   f32x4 x[NL];
@@ -768,7 +767,7 @@ static TreePlan tree_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t
   p.apart = p.rows_wg <= 64 || chunks * p.S < 192;
   p.P = (int)(B * (p.S + p.apart));
   p.rows = (size_t)Hkv * p.P * p.M;
-  p.bytes = kSyncBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
+  p.bytes = kSyncBytes + kTreeDealBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
   return p;
 }
 size_t tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C) {
@@ -832,7 +831,8 @@ hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_
   a.div_t = Div::of(a.T);
   a.scale_log2 = (float)p.scale * 1.4426950408889634f;
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
-  a.part_m = reinterpret_cast<float*>(ws + kSyncBytes);
+  a.deal = reinterpret_cast<int*>(ws + kSyncBytes);
+  a.part_m = reinterpret_cast<float*>(ws + kSyncBytes + kTreeDealBytes);
   a.part_l = a.part_m + pl.rows;
   a.part_o = a.part_m + ((2 * pl.rows + 3) & ~(size_t)3);
   a.out = p.out;

@@ -457,7 +457,7 @@ def tree_workspace(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int, dev
     nbytes = _tree_bytes(B, Hq, Hkv, D, T, capacity)
     if nbytes == 0:
         raise RuntimeError("unsupported tree geometry")
-    return _evict_workspace(nbytes, torch.device(device))
+    return _workspace(nbytes, torch.device(device))
 
 
 _TREE_ARGS = _lib.ARGS["dropkv_tree_attention"].pack

@@ -337,8 +337,9 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  * B * Hq * T <= 2^24, 0 < scale < 1e37.
  * The workspace (dropkv_tree_workspace_bytes for the same geometry; other
  * geometries can need more, fewer tokens too) holds the partial results of the
- * splits.  Its first DROPKV_SYNC_BYTES must be zero when it is first used, and
- * every call leaves them zero; calls that share one must be serialised.
+ * splits; it needs no initialisation, and its first DROPKV_SYNC_BYTES are left
+ * alone, so that it may be one that layer-calls use too.  Calls that share one
+ * must be serialised.
  * ------------------------------------------------------------------------ */
 typedef struct {
   const void* q;
