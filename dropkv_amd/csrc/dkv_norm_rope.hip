@@ -23,11 +23,14 @@
 
 namespace dkv {
 
+struct RopeSide {  // of q, k or v: row (b, h, l) at element b sb + h sh + l sl
+  const void* src;
+  void* dst;
+  int64_t s_sb, s_sh, s_sl, d_sb, d_sh, d_sl;
+  const void* w;  // norm weight, or null
+};
 struct RopeArgs {
-  const void* src[3];  // q, k, v: row (b, h, l) at element b sb + h sh + l sl
-  void* dst[3];
-  int64_t s_sb[3], s_sh[3], s_sl[3], d_sb[3], d_sh[3], d_sl[3];
-  const void* w[2];  // norm weights of q and of k, or null
+  RopeSide q, k, v;
   int w_f32;
   const void* cos;  // row l of sequence b at element b c_sb + l c_sl; with positions, row `position` at position * c_sl
   const void* sin;
@@ -39,23 +42,49 @@ struct RopeArgs {
   float eps;
 };
 
-template <typename T>
-struct Vec8 {
-  T x[8];
-};
-
+// Eight values from or to a 16-byte aligned place.
 template <typename T>
 __device__ __forceinline__ void load_vec8(const T* p, float* f) {
-  const Vec8<T> v = *reinterpret_cast<const Vec8<T>*>(__builtin_assume_aligned(p, 16));
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 x0 = reinterpret_cast<const f32x4*>(p)[0], x1 = reinterpret_cast<const f32x4*>(p)[1];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(v.x[e]);
+    for (int e = 0; e < 8; ++e) f[e] = e < 4 ? x0[e % 4] : x1[e % 4];
+  } else {
+    const typename Elem<T>::v8 x = *reinterpret_cast<const typename Elem<T>::v8*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(x[e]);
+  }
 }
 template <typename T>
 __device__ __forceinline__ void store_vec8(T* p, const float* f) {
-  Vec8<T> v;
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{f[0], f[1], f[2], f[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{f[4], f[5], f[6], f[7]};
+  } else {
+    typename Elem<T>::v8 x;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v.x[e] = static_cast<T>(f[e]);
-  *reinterpret_cast<Vec8<T>*>(__builtin_assume_aligned(p, 16)) = v;
+    for (int e = 0; e < 8; ++e) x[e] = static_cast<T>(f[e]);
+    *reinterpret_cast<typename Elem<T>::v8*>(p) = x;
+  }
+}
+
+// The side that head hh of the list (q's, k's, v's heads) belongs to, and its head
+// there.  (Member by member: an array indexed by the lane is kept in LDS.)
+__device__ __forceinline__ RopeSide rope_side(const RopeArgs& a, int hh, int* h, bool* copy) {
+  const bool q = hh < a.Hq, k = hh < a.Hq + a.Hk;
+  *h = hh - (q ? 0 : k ? a.Hq : a.Hq + a.Hk);
+  *copy = !k;
+  RopeSide s;
+  s.src = q ? a.q.src : k ? a.k.src : a.v.src;
+  s.dst = q ? a.q.dst : k ? a.k.dst : a.v.dst;
+  s.s_sb = q ? a.q.s_sb : k ? a.k.s_sb : a.v.s_sb;
+  s.s_sh = q ? a.q.s_sh : k ? a.k.s_sh : a.v.s_sh;
+  s.s_sl = q ? a.q.s_sl : k ? a.k.s_sl : a.v.s_sl;
+  s.d_sb = q ? a.q.d_sb : k ? a.k.d_sb : a.v.d_sb;
+  s.d_sh = q ? a.q.d_sh : k ? a.k.d_sh : a.v.d_sh;
+  s.d_sl = q ? a.q.d_sl : k ? a.k.d_sl : a.v.d_sl;
+  s.w = q ? a.q.w : a.k.w;
+  return s;
 }
 
 // The token's row of the tables; false where its position is not in them.
@@ -105,21 +134,24 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
   }
   const int heads = a.Hq + a.Hk + a.Hv, h_end = min(heads, h0 + a.per);
   for (int hh = h0 + lane / LPR; hh < h_end; hh += HPW) {
-    const int kind = hh < a.Hq ? 0 : hh < a.Hq + a.Hk ? 1 : 2;
-    const int h = hh - (kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hk);
-    const T* src = static_cast<const T*>(a.src[kind]) + b * a.s_sb[kind] + h * a.s_sh[kind] + l * a.s_sl[kind];
-    T* dst = static_cast<T*>(a.dst[kind]) + b * a.d_sb[kind] + h * a.d_sh[kind] + l * a.d_sl[kind];
-    if (kind == 2) {
-      const Vec8<T> x0 = *reinterpret_cast<const Vec8<T>*>(__builtin_assume_aligned(src + i0, 16));
-      const Vec8<T> x1 = *reinterpret_cast<const Vec8<T>*>(__builtin_assume_aligned(src + i1, 16));
-      *reinterpret_cast<Vec8<T>*>(__builtin_assume_aligned(dst + i0, 16)) = x0;
-      *reinterpret_cast<Vec8<T>*>(__builtin_assume_aligned(dst + i1, 16)) = x1;
+    int h;
+    bool copy;
+    const RopeSide side = rope_side(a, hh, &h, &copy);
+    const T* src = static_cast<const T*>(side.src) + b * side.s_sb + h * side.s_sh + l * side.s_sl;
+    T* dst = static_cast<T*>(side.dst) + b * side.d_sb + h * side.d_sh + l * side.d_sl;
+    if (copy) {
+#pragma unroll
+      for (int u = 0; u < (int)sizeof(T) / 2; ++u) {  // 16 bytes each
+        const u32x4 x0 = reinterpret_cast<const u32x4*>(src + i0)[u], x1 = reinterpret_cast<const u32x4*>(src + i1)[u];
+        reinterpret_cast<u32x4*>(dst + i0)[u] = x0;
+        reinterpret_cast<u32x4*>(dst + i1)[u] = x1;
+      }
       continue;
     }
     float x0[8], x1[8];
     load_vec8(src + i0, x0);
     load_vec8(src + i1, x1);
-    const void* w = a.w[kind];
+    const void* w = side.w;
     if (w) {
       float ss = 0.f, w0[8], w1[8];
       if (a.w_f32) {
@@ -163,15 +195,16 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(RopeArgs a) {
   if (wid >= (int64_t)a.tokens * heads) return;
   const int token = (int)(wid / heads), hh = (int)(wid - (int64_t)token * heads);
   const int b = token / a.L, l = token - b * a.L;
-  const int kind = hh < a.Hq ? 0 : hh < a.Hq + a.Hk ? 1 : 2;
-  const int h = hh - (kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hk);
-  const T* src = static_cast<const T*>(a.src[kind]) + b * a.s_sb[kind] + h * a.s_sh[kind] + l * a.s_sl[kind];
-  T* dst = static_cast<T*>(a.dst[kind]) + b * a.d_sb[kind] + h * a.d_sh[kind] + l * a.d_sl[kind];
-  if (kind == 2) {
+  int h;
+  bool copy;
+  const RopeSide side = rope_side(a, hh, &h, &copy);
+  const T* src = static_cast<const T*>(side.src) + b * side.s_sb + h * side.s_sh + l * side.s_sl;
+  T* dst = static_cast<T*>(side.dst) + b * side.d_sb + h * side.d_sh + l * side.d_sl;
+  if (copy) {
     for (int i = lane; i < a.D; i += 64) dst[i] = src[i];
     return;
   }
-  const void* w = a.w[kind];
+  const void* w = side.w;
   float inv = 1.f;
   if (w) {
     float ss = 0.f;
@@ -230,23 +263,14 @@ hipError_t launch_norm_rope(const dropkv_norm_rope_args& p, hipStream_t st) {
   RopeArgs a{};
   const int64_t eb = p.dtype == kDtypeFp32 ? 4 : 2, cb = p.c_dtype == kDtypeFp32 ? 4 : eb;
   uint64_t all = 0;
-  auto tensor = [&](int i, const void* src, const int64_t* s, void* dst, const int64_t* d) {
-    a.src[i] = src;
-    a.dst[i] = dst;
-    a.s_sb[i] = s[0];
-    a.s_sh[i] = s[1];
-    a.s_sl[i] = s[2];
-    a.d_sb[i] = d[0];
-    a.d_sh[i] = d[1];
-    a.d_sl[i] = d[2];
-    all |= reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) |
+  auto tensor = [&](const void* src, const int64_t* s, void* dst, const int64_t* d, const void* w) {
+    all |= reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(w) |
            (uint64_t)((s[0] | s[1] | s[2] | d[0] | d[1] | d[2]) * eb);
+    return RopeSide{src, dst, s[0], s[1], s[2], d[0], d[1], d[2], w};
   };
-  tensor(0, p.q, p.q_s, p.q_out, p.qo_s);
-  tensor(1, p.k, p.k_s, p.k_out, p.ko_s);
-  if (p.v) tensor(2, p.v, p.v_s, p.v_out, p.vo_s);
-  a.w[0] = p.q_w;
-  a.w[1] = p.k_w;
+  a.q = tensor(p.q, p.q_s, p.q_out, p.qo_s, p.q_w);
+  a.k = tensor(p.k, p.k_s, p.k_out, p.ko_s, p.k_w);
+  if (p.v) a.v = tensor(p.v, p.v_s, p.v_out, p.vo_s, nullptr);
   a.w_f32 = p.w_dtype == kDtypeFp32;
   a.cos = p.cos;
   a.sin = p.sin;
@@ -263,8 +287,7 @@ hipError_t launch_norm_rope(const dropkv_norm_rope_args& p, hipStream_t st) {
   a.D = (int)p.D;
   a.R = (int)p.R;
   a.eps = (float)p.eps;
-  all |= reinterpret_cast<uintptr_t>(p.q_w) | reinterpret_cast<uintptr_t>(p.k_w) | reinterpret_cast<uintptr_t>(p.cos) |
-         reinterpret_cast<uintptr_t>(p.sin) | (uint64_t)((a.c_sb | a.c_sl) * cb);
+  all |= reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin) | (uint64_t)((a.c_sb | a.c_sl) * cb);
   const bool vec = all % 16 == 0 && p.R % 16 == 0;
   if (p.dtype == kDtypeFp32) return launch_rope_t<float, float>(a, vec, st);
   if (p.dtype == kDtypeBf16)
