@@ -85,7 +85,7 @@ int check_tree_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, i
   if (B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv) return fail(DROPKV_E_ARG, "B, Hq, Hkv must be positive, Hkv | Hq");
   if (T < 1 || T > dkv::kTreeMaxT) return fail(DROPKV_E_UNSUPPORTED, "T must be in [1, %d]", (int)dkv::kTreeMaxT);
   if (!decode_head_dim_supported(D)) return fail(DROPKV_E_UNSUPPORTED, "head dim %lld not supported", (long long)D);
-  if (capacity < 1 || capacity > ((int64_t)1 << 30) / D) return fail(DROPKV_E_ARG, "capacity out of range");
+  if (capacity < 0 || capacity > ((int64_t)1 << 30) / D) return fail(DROPKV_E_ARG, "capacity out of range");
   if ((double)B * (double)Hq * (double)T > (double)(1 << 24))
     return fail(DROPKV_E_UNSUPPORTED, "B*Hq*T above %d", 1 << 24);
   return DROPKV_OK;
@@ -120,7 +120,7 @@ bool timing_pair(hipEvent_t* start, hipEvent_t* stop) {
 
 extern "C" {
 
-int dropkv_version(void) { return 100; }
+int dropkv_version(void) { return 200; }
 
 const char* dropkv_last_error(void) { return g_err.c_str(); }
 
@@ -541,7 +541,8 @@ size_t dropkv_tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D
 
 int dropkv_tree_attention(const dropkv_tree_attention_args* a, void* stream) {
   (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
-  if (!a || !a->q || !a->k_new || !a->v_new || !a->k_cache || !a->v_cache || !a->n_rows || !a->out || !a->workspace)
+  if (!a || !a->q || !a->k_new || !a->v_new || !a->n_rows || !a->out || !a->workspace ||
+      (a->capacity != 0 && (!a->k_cache || !a->v_cache)))
     return fail(DROPKV_E_ARG, "null pointer argument");
   if (a->dtype != DROPKV_BF16 && a->dtype != DROPKV_FP16) return fail(DROPKV_E_ARG, "dtype must be bf16 or fp16");
   const int rc = check_tree_shape(a->B, a->Hq, a->Hkv, a->T, a->D, a->capacity);

@@ -154,6 +154,8 @@ class CompressedDecoder:
         _register()
         self.model = model
         self.tree_size = int(tree_size)
+        if not 0 <= self.tree_size <= 256:
+            raise ValueError(f"tree_size must be in [0, 256], got {tree_size}")
         self._angles = None  # of the forward that runs
         kv = _stored_kv(cache)
         if not kv:

@@ -511,6 +511,8 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
         out = torch.empty((B, T, Hq, D), dtype=dtype, device=q.device)
     elif out.shape != (B, T, Hq, D) or out.dtype is not dtype or out.stride(3) != 1:
         raise RuntimeError("tree_attention: out must be [B, T, Hq, D] of q's dtype, D contiguous")
+    if not (B and T and Hq):
+        return out
     if workspace is None:
         nbytes = _tree_bytes(B, Hq, Hkv, D, T, C)
         if nbytes == 0:
@@ -546,7 +548,8 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tenso
     [B, H, T, D] and the buffers [B, H, capacity, D], or those of N layers with
     an axis N in front; ``n_rows`` int32, [1] or [B], or [N, 1] or [N, B].
     Returns ``(path [B, T] int32, the nodes that stand, then -1; accepted [B]
-    int32)``.  ``n_rows`` is not advanced."""
+    int32)``.  ``n_rows`` is not advanced.  The drafted rows must not lie in the
+    buffers themselves."""
     index = _device_index("tree_commit", tokens, parents, choice, k_new, v_new, k_cache, v_cache, n_rows)
     if torch.is_grad_enabled():
         _no_grad("tree_commit", k_new, v_new, k_cache, v_cache)
@@ -575,7 +578,7 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tenso
         raise RuntimeError("tree_commit: n_rows must be int32, [1] or [B], or [N, 1] or [N, B]")
     path = torch.empty((B, T), dtype=torch.int32, device=tokens.device)
     accepted = torch.empty((B,), dtype=torch.int32, device=tokens.device)
-    if B == 0 or N == 0:
+    if B == 0:
         return path, accepted
     tokens, choice, parents = tokens.contiguous(), choice.contiguous(), parents.contiguous()
     k_new, v_new = _rows(k_new), _rows(v_new)

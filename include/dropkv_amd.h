@@ -323,7 +323,8 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  * written; the drafted rows go to the cache with dropkv_tree_commit.
  *   q        [B, Hq, T, D], k_new / v_new [B, Hkv, T, D]: strides {batch, head,
  *            token}, D contiguous, any alignment; rotated already
- *   k_cache, v_cache  [B, Hkv, capacity, D] contiguous, 16-byte aligned
+ *   k_cache, v_cache  [B, Hkv, capacity, D] contiguous, 16-byte aligned (capacity
+ *            0: may be NULL)
  *   n_rows   device int32, rows stored of sequence b at n_rows[b * n_sb]
  *            (n_sb 0: one count for all; else 1), 0 <= n <= capacity (clamped)
  *   mask     device bytes, nonzero where drafted token t sees drafted token j,
@@ -377,7 +378,8 @@ int dropkv_tree_attention(const dropkv_tree_attention_args* args, void* stream);
  *   contiguous;  n_rows int32 at l * n_s[0] + b * n_s[1]
  * Row path[i] of k_new / v_new goes to row n + i of its cache, bit for bit; rows
  * that would lie beyond the capacity (and all of a negative n) are left out.
- * n_rows is not advanced.  1 <= T <= 256; elem_bytes 2 or 4. */
+ * n_rows is not advanced.  The drafted rows must not lie in the buffers.
+ * 1 <= T <= 256; elem_bytes 2 or 4. */
 typedef struct {
   const int64_t* tokens;
   const int32_t* parents;

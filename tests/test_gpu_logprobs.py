@@ -56,6 +56,11 @@ def check(gpu, x, top, tokens=None):
     (5, 32001, 20, torch.bfloat16),       # rows at odd addresses
     (2, 4096, 8, torch.float32),
     (2, 4097, 8, torch.float32),
+    (2, 300001, 32, torch.float32),       # blocks of several selection rounds
+    (1, 600000, 20, torch.bfloat16),
+    (20, 151936, 7, torch.bfloat16),      # segments joined by a second kernel
+    (20, 151936, 1, torch.float16),
+    (20, 50000, 0, torch.bfloat16),
     (7, 1, 1, torch.float32),
     (4, 31, 31, torch.bfloat16),
     (4, 8, 0, torch.float16),
@@ -157,6 +162,25 @@ def test_tokens_outside_and_shapes(gpu):
     assert one.logprob.shape == () and one.top_ids.shape == (2,)
     none = ops.token_logprobs(part[:0], top=3)
     assert none.logprob is None and none.top_ids.shape == (0, 3)
+
+
+def test_two_streams(gpu):
+    """Calls on two streams at once keep their workspaces apart."""
+    from dropkv_amd import ops
+    xs = [torch.randn(3, 100000 + 7 * i, generator=torch.Generator().manual_seed(i)).to(gpu) for i in range(2)]
+    want = [ops.token_logprobs(x, top=9) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.token_logprobs(xs[i], top=9))
+    torch.cuda.synchronize()
+    for w, rs in zip(want, got):
+        for r in rs:
+            assert all(torch.equal(a, b) for a, b in zip(r[1:], w[1:]))
 
 
 def test_in_a_graph(gpu):

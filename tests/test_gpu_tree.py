@@ -106,6 +106,33 @@ def test_attention_of_projections(gpu, T):
     check(gpu, 2, 14, 2, 64, T, 333, [300, 17], torch.bfloat16, strided=True, seed=T)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,T,C,top", [
+    (64, 4, 2, 64, 3, 3000, 3000),     # up to 16 rows: lengths 0 .. 3000, the most sequences dealt by length
+    (65, 2, 1, 64, 2, 900, 900),       # one more: equal parts
+    (12, 8, 2, 64, 9, 2500, 2500),     # up to 64 rows
+    (9, 8, 1, 128, 13, 1900, 1900),    # up to 128
+    (7, 16, 2, 64, 33, 1500, 1500),    # beyond: two chunks of rows
+    (3, 16, 2, 64, 33, 4200, 70),      # short sequences in long buffers
+])
+def test_lengths_of_their_own(gpu, B, Hq, Hkv, D, T, C, top):
+    """Sequences from empty to full, dealt out to the workgroups by length."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, top + 1, (B,), generator=g).tolist()
+    lens[0], lens[-1] = 0, top
+    if B > 10:      # a sample is compared; the reference walks row by row
+        from dropkv_amd import ops
+        q, kn, vn, kc, vc = case(B, Hq, Hkv, D, T, C, torch.bfloat16, 5)
+        m = make_tree(B, T, 5)[1]
+        got = ops.tree_attention(q.to(gpu), kn.to(gpu), vn.to(gpu), kc.to(gpu), vc.to(gpu),
+                                 torch.tensor(lens, dtype=torch.int32, device=gpu), D ** -0.5, mask=m.to(gpu)).cpu()
+        for b in (0, 1, B // 2, B - 2, B - 1):
+            s = slice(b, b + 1)
+            ref, tol = reference(q[s], kn[s], vn[s], kc[s], vc[s], lens[s], m[s], D ** -0.5)
+            assert ((got[s].double() - ref).abs() <= tol).all(), b
+    else:
+        check(gpu, B, Hq, Hkv, D, T, C, lens, torch.bfloat16, seed=5)
+
+
 def test_attention_unaligned(gpu):
     """Rows of q, k_new and v_new that start at no whole 16 bytes, a mask of
     other strides, one mask and one count for all sequences, out by strides."""
@@ -248,6 +275,25 @@ def test_attention_in_a_graph(gpu):
             assert torch.equal(o, want), step
 
 
+def test_two_streams(gpu):
+    """Calls on two streams at once, with the streams' own workspaces."""
+    from dropkv_amd import ops
+    cases = [tuple(x.to(gpu) for x in case(1, 16, 2, 64, T, 2000, torch.bfloat16, T)) for T in (2, 40)]
+    n = torch.tensor([1900], dtype=torch.int32, device=gpu)
+    want = [ops.tree_attention(*c, n, 0.125) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.tree_attention(*cases[i], n, 0.125))
+    torch.cuda.synchronize()
+    for w, rs in zip(want, got):
+        assert all(torch.equal(r, w) for r in rs)
+
+
 def test_one_token_is_a_decode_step(gpu):
     """T = 1 agrees with the decode step on the same rows to a rounding."""
     from dropkv_amd import ops
@@ -335,6 +381,26 @@ def test_commit_chain_and_capacity(gpu):
         if fit:
             want[:, :, n:n + fit] = kn[:, :, :fit]
         assert torch.equal(kc.cpu(), want)
+
+
+def test_nothing_drafted_and_no_capacity(gpu):
+    """T = 0 and B = 0 give empty tensors; buffers without a row leave the
+    drafted tokens to one another; the walk needs a root and a layer."""
+    from dropkv_amd import ops
+    q, kn, vn, kc, vc = (x.to(gpu) for x in case(2, 4, 2, 64, 5, 70, torch.bfloat16, 8))
+    n = torch.zeros(2, dtype=torch.int32, device=gpu)
+    assert ops.tree_attention(q[:, :, :0], kn[:, :, :0], vn[:, :, :0], kc, vc, n, 0.1).shape == (2, 0, 4, 64)
+    assert ops.tree_attention(q[:0], kn[:0], vn[:0], kc[:0], vc[:0], n[:1], 0.1).shape == (0, 5, 4, 64)
+    got = ops.tree_attention(q, kn, vn, kc[:, :, :0].contiguous(), vc[:, :, :0].contiguous(), n, 0.1)
+    assert torch.equal(got, ops.tree_attention(q, kn, vn, kc, vc, n, 0.1))
+    tok = torch.zeros(2, 5, dtype=torch.int64, device=gpu)
+    par = torch.zeros(5, dtype=torch.int32, device=gpu)
+    path, acc = ops.tree_commit(tok[:0], par, tok[:0], kn[:0], vn[:0], kc[:0], vc[:0], n[:0])
+    assert path.shape == (0, 5) and acc.shape == (0,)
+    with pytest.raises(RuntimeError):
+        ops.tree_commit(tok[:, :0], par[:0], tok[:, :0], kn[:, :, :0], vn[:, :, :0], kc, vc, n)
+    with pytest.raises(RuntimeError):
+        ops.tree_commit(tok, par, tok, kn[None][:0], vn[None][:0], kc[None][:0], vc[None][:0], n[None][:0])
 
 
 def test_refusals(gpu):

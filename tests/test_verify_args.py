@@ -58,7 +58,7 @@ def test_tree_workspace(lib):
     size = lib.dropkv_tree_workspace_bytes
     assert size(1, 32, 8, 128, 16, 3392) > 0
     for bad in [(0, 32, 8, 128, 16, 100), (1, 30, 8, 128, 16, 100), (1, 32, 8, 96, 16, 100), (1, 32, 8, 128, 0, 100),
-                (1, 32, 8, 128, 257, 100), (1, 32, 8, 128, 16, 0), (1, 32, 8, 128, 16, 1 << 24),
+                (1, 32, 8, 128, 257, 100), (1, 32, 8, 128, 16, -1), (1, 32, 8, 128, 16, 1 << 24),
                 (1 << 13, 32, 8, 128, 256, 100)]:
         assert size(*bad) == 0, bad
 
@@ -72,7 +72,8 @@ def test_tree_workspace(lib):
     (dict(T=0), 2, "T must be in"),
     (dict(T=257), 2, "T must be in"),
     (dict(D=80), 2, "head dim 80"),
-    (dict(capacity=0), 1, "capacity"),
+    (dict(capacity=-1), 1, "capacity"),
+    (dict(k_cache=0), 1, "null pointer"),
     (dict(capacity=(1 << 23) + 1), 1, "capacity"),
     (dict(B=1 << 17), 2, "B*Hq*T"),
     (dict(n_sb=2), 1, "n_sb"),
@@ -157,7 +158,7 @@ def test_token_logprobs(lib, change, code, msg):
 
 def test_token_logprobs_workspace(lib):
     size = lib.dropkv_token_logprobs_workspace_bytes
-    assert size(1, 151936, 5) > 0 and size(100000, 1000, 5) == 0
+    assert size(1, 151936, 5) > 0 and size(100000, 1000, 5) > 0 and size(100000, 1000, 1) == 0
     for bad in [(0, 10, 1), (1, 0, 0), (1, 10, 11), (1, 100, 33), (1, 100, -1), (1, (1 << 30) + 1, 1)]:
         assert size(*bad) == 0, bad
     assert lib.dropkv_token_logprobs(args("dropkv_token_logprobs", V=5, dtype=1), None) == 0
