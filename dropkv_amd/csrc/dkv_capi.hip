@@ -552,12 +552,13 @@ int dropkv_tree_attention(const dropkv_tree_attention_args* a, void* stream) {
     return fail(DROPKV_E_ARG, "scale must be positive and finite");
   if (!aligned16(a->k_cache) || !aligned16(a->v_cache))
     return fail(DROPKV_E_ARG, "cache buffers must be 16-byte aligned");
-  const size_t need = dkv::tree_workspace_bytes(a->B, a->Hq, a->Hkv, a->D, a->T, a->capacity);
+  size_t need = 0;
+  timing_start(static_cast<hipStream_t>(stream));
+  const hipError_t e = dkv::launch_tree_attention(*a, &need, static_cast<hipStream_t>(stream));
   if (a->workspace_bytes < 0 || (size_t)a->workspace_bytes < need)
     return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %lld", need,
                 (long long)a->workspace_bytes);
-  timing_start(static_cast<hipStream_t>(stream));
-  return hip_status(dkv::launch_tree_attention(*a, static_cast<hipStream_t>(stream)), "dropkv_tree_attention launch");
+  return hip_status(e, "dropkv_tree_attention launch");
 }
 
 int dropkv_tree_commit(const dropkv_tree_commit_args* a, void* stream) {

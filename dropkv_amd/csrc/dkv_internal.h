@@ -140,7 +140,8 @@ hipError_t launch_decode_attention(const DecodeParams& p, hipStream_t st);
 // probabilities (dkv_logprob.hip).  The arguments are the C ABI's, checked.
 constexpr int64_t kTreeMaxT = 256;
 size_t tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C);
-hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_t st);
+// (A workspace below *need: nothing is launched.)
+hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, size_t* need, hipStream_t st);
 hipError_t launch_tree_commit(const dropkv_tree_commit_args& p, hipStream_t st);
 hipError_t launch_norm_rope(const dropkv_norm_rope_args& p, hipStream_t st);
 int64_t logprob_max_top();

@@ -407,19 +407,21 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 }
 
 // With LO, P goes into the product in two parts, rounded and remainder (about 16
-// significant bits).  Beyond 64 rows a call is bound by the matrix cores and the
-// ALUs and not by memory, and P is rounded once: each weight is off by at most
-// half a step of the element type, as the output is by its own rounding (4 x 64
-// heads of 26214 rows, 64 tokens: 339 us in two parts, 265 in one).
+// significant bits).  In workgroups of 128 rows and more a call is bound by the
+// matrix cores and the ALUs and not by memory, and P is rounded once: each weight
+// is off by at most half a step of the element type, as the output is by its own
+// rounding (4 x 64 heads of 26214 rows, 64 tokens: 336 us in two parts, 255 in
+// one; 8 x 32 heads of up to 8003 rows, 27 tokens: 53 and 45).
 //
-// More than 16 rows: NW waves of QB blocks of 16 rows take the same keys, so
+// More than 16 rows: NW waves of QB blocks of 16 rows (4 of one or two, 8 of two)
+// take the same keys, so
 // that a tile of K and V is read once for all of them, into LDS.  The next tile
 // is on its way in registers while the waves compute on this one, and goes to
 // the other of two buffers: one barrier per tile.  A K operand (a V operand)
 // read from LDS serves QB products.  LDS pitches leave every 16 lanes of a
 // K read, and every 32 of a transposing V read, on banks of their own.
 template <typename T, int D, int QB, int NW, bool LO>
-__global__ void __launch_bounds__(64 * NW, NW == 2 ? 1 : 2) tree_wide_kernel(TreeArgs a) {
+__global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
   typedef typename Elem<T>::v8 v8;
   constexpr int KK = D / 32, DT = D / 16, CPR = D / 8, NT = 64 * NW;
   constexpr int kSub = 2, kStage = kSub * kTreeTile;
@@ -595,7 +597,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 2 ? 1 : 2) tree_wide_kernel(Tre
   }
   // The cache's last stage, and the drafted keys, through the same code: what a
   // short call fetches of it counts (with three copies of the stage and the
-  // drafted keys' rare cases in line a part of one stage took 9 us, not 6).
+  // drafted keys' rare cases in line the drafted keys of 8 tokens took 6.0 us, not
+  // 4.5).
 #pragma unroll 1
   for (int jd = part.tail ? 0 : a.T; stored || jd < a.T;) {
     if (stored) {
@@ -730,41 +733,69 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
   }
 }
 
-// How a call is cut: rows per workgroup, parts of the cache per sequence, and
-// whether the drafted keys are parts of their own.
-//
-// More parts shorten the longest workgroup, but each costs a prologue and an
-// epilogue (about four tiles' time) and rows x D floats written and read again.
-// In tiles: rounds x (tiles / S + 4) + S x `join`, where a round is as many
-// workgroups as run at once (one of 8 waves, two of 4 or 2, or eight single
-// waves per CU) and `join` the partial rows' traffic at 4 TB/s over a tile's
-// time (0.5 us for up to 64 rows, 1.5 us beyond, half of it at D = 64).  32
-// heads over 8 KV heads of 3276 rows, 16 tokens: 24 parts 13.7 us, 16 parts
-// 14.7, 32 parts 15.5, 53 parts 17.7.
+// How a call is cut: rows per workgroup (16: one wave), parts of the cache per
+// sequence, and whether the drafted keys are parts of their own.
 struct TreePlan {
   int M, rows_wg, MC, S, P, apart;
   size_t rows, bytes;
 };
+
+// An estimate of a call's time in us, from sweeps of both over calls of 1 to 1024
+// rows per KV head, 900 to 100,000 keys and 2 to 256 heads (the plan chosen by it
+// took up to a tenth longer than the best one there).  The sum of
+// - the longest workgroup's tiles, a tile's time by the rows, 0.65 of it at D =
+//   64, and longer where two workgroups share a CU or take turns;
+//   or, if longer, K and V at 5.2 TB/s, where 8 MB or a quarter of them are in
+//   flight;
+// - the partial rows, written and read at 4 TB/s, and a round trip of the joining
+//   kernel for every 16 (D = 128) or 32 parts;
+// - the two kernels' fixed part.
+struct TreeShape {
+  int rows;
+  double tile_us, fixed_us, shared;  // shared: two workgroups on a CU, against one
+  int per_cu;
+};
+constexpr TreeShape kTreeShapes[] = {
+    {16, 0.50, 6.5, 1.0, 8}, {64, 0.60, 7.0, 1.45, 2}, {128, 0.72, 7.2, 1.7, 2}, {256, 1.10, 8.5, 1.0, 1}};
+
+static double tree_cost(const TreeShape& w, double heads, double M, double D, double tiles, int64_t S) {
+  const double wgs = heads * std::ceil(M / w.rows) * S, wide = D / 128;
+  const double per = std::ceil(tiles / S), load = wgs / (256.0 * w.per_cu);
+  double tile = w.tile_us * (wide < 1 ? 0.65 : 1);
+  if (load > 1)
+    tile *= std::ceil(load) * w.shared;
+  else if (w.per_cu == 2 && load > 0.5)
+    tile *= w.shared;
+  const double flight = std::min(wgs, 256.0 * w.per_cu) * (w.rows == 16 ? 16384 : 32768) * wide;
+  const double bytes = heads * tiles * kTreeTile * D * 4;
+  const double stream = bytes / 5.2e6 / std::min(1.0, flight / std::max(1.0, std::min(8e6, bytes / 4)));
+  return std::max(per * tile, stream) + S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16) + w.fixed_us;
+}
+
 static TreePlan tree_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C) {
   TreePlan p;
   p.M = (int)(Hq / Hkv * T);
-  p.rows_wg = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256;
-  p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
-  const int64_t chunks = B * Hkv * p.MC, tiles = (C + kTreeTile - 1) / kTreeTile;
-  const int64_t round = p.rows_wg == 16 ? 2048 : p.rows_wg <= 128 ? 512 : 256;
-  const double tile_us = p.rows_wg <= 64 ? 0.5 : 1.5;
-  const double join = (double)chunks * std::min(p.M, p.rows_wg) * 128 * 4 * 2 / 4e6 / tile_us;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>({kTreeMaxSplits, (tiles + 1) / 2}));
+  const int64_t heads = B * Hkv, tiles = (C + kTreeTile - 1) / kTreeTile;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kTreeMaxSplits, (tiles + 1) / 2));
   double best = 0;
   p.S = 0;
-  for (int64_t S = 1; S <= most; ++S) {
-    const double cost = (double)((chunks * S + round - 1) / round) * ((double)tiles / S + 4) + S * join;
-    if (p.S == 0 || cost < best) {
-      best = cost;
-      p.S = (int)S;
+  for (const TreeShape& w : kTreeShapes) {
+    // One wave for up to 16 rows; no shape that the rows would leave half empty.
+    if ((w.rows == 16) != (p.M <= 16) || (w.rows > 64 && p.M <= w.rows / 2)) continue;
+    const int64_t chunks = heads * ((p.M + w.rows - 1) / w.rows);
+    const int64_t tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kTreeMaxSplits, 256 / chunks, 512 / chunks};
+    for (int64_t S : tries) {
+      S = std::max<int64_t>(1, std::min(S, most));
+      const double cost = tree_cost(w, (double)heads, p.M, (double)D, (double)tiles, S);
+      if (p.S == 0 || cost < best) {
+        best = cost;
+        p.S = (int)S;
+        p.rows_wg = w.rows;
+      }
     }
   }
-  p.apart = p.rows_wg <= 64 || chunks * p.S < 192;
+  p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
+  p.apart = p.rows_wg <= 64 || heads * p.MC * p.S < 192;
   p.P = (int)(B * (p.S + p.apart));
   p.rows = (size_t)Hkv * p.P * p.M;
   p.bytes = kSyncBytes + kTreeDealBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
@@ -779,8 +810,6 @@ static hipError_t launch_tree_t(const TreeArgs& a, int rows_wg, hipStream_t st) 
   const dim3 grid(a.Hkv * a.P * a.MC);
   if (rows_wg == 16)
     launch((tree_partial_kernel<T, D>), grid, dim3(64), 0, st, a);
-  else if (rows_wg == 32)
-    launch((tree_wide_kernel<T, D, 1, 2, true>), grid, dim3(128), 0, st, a);
   else if (rows_wg == 64)
     launch((tree_wide_kernel<T, D, 1, 4, true>), grid, dim3(256), 0, st, a);
   else if (rows_wg == 128)
@@ -791,8 +820,10 @@ static hipError_t launch_tree_t(const TreeArgs& a, int rows_wg, hipStream_t st) 
   return hipGetLastError();
 }
 
-hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, hipStream_t st) {
+hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, size_t* need, hipStream_t st) {
   const TreePlan pl = tree_plan(p.B, p.Hq, p.Hkv, p.D, p.T, p.capacity);
+  *need = pl.bytes;
+  if (p.workspace_bytes < 0 || (size_t)p.workspace_bytes < pl.bytes) return hipSuccess;  // (the caller says so)
   TreeArgs a{};
   a.q = p.q;
   a.q_sb = p.q_s[0];

@@ -7,7 +7,7 @@ so a logit is off by at most D 2^-24 |scale| |q| |k| =: d, a weight relative by
 exponential; each addition of the sums over n keys adds 2^-24, one for 16 keys
 at the most and one for a split.  The store adds half a step.
 
-With more than 64 rows (g T) to a KV head P is rounded once to the element type:
+With more than 64 rows (g T) to a KV head P may be rounded once to the element type:
 each weight is off by half a step, 2^-8 (bf16) or 2^-11 (fp16) of itself, and the
 output by at most that of sum p |v|."""
 
