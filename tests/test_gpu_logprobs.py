@@ -127,6 +127,20 @@ def test_masked_logits(gpu, dtype, top):
     assert float(got.logprob[6]) == 0 and float(got.entropy[6]) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("top", [1, 6])
+@pytest.mark.parametrize("N", [1, 2100])
+def test_zeros_of_either_sign(gpu, dtype, top, N):
+    """-0 and 0 are equals: the lowest places come first."""
+    V = 5000
+    x = torch.full((1, V), -2.0, dtype=dtype)
+    x[0, 3:4000:5] = 0.0
+    x[0, 3:4000:10] = -0.0
+    from dropkv_amd import ops
+    got = ops.token_logprobs(x.to(gpu).expand(N, V), top=top)
+    assert torch.equal(got.top_ids.cpu(), torch.arange(3, 3 + 5 * top, 5).expand(N, top))
+
+
 @pytest.mark.parametrize("top", [1, 6])
 def test_nan_and_inf(gpu, top):
     """NaN or +inf anywhere: the row is NaN; NaN ranks above all, ties and NaN
