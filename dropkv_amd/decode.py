@@ -254,7 +254,8 @@ class CompressedDecoder:
         """A forward over the drafted tokens, and the path of them that stands.
         The counts are not advanced."""
         with self._active():
-            logits = self.model(self._tree_tok, position_ids=self.pos + self._tree_depth,
+            # (A negative token has no embedding, and equals no best token.)
+            logits = self.model(self._tree_tok.clamp(min=0), position_ids=self.pos + self._tree_depth,
                                 past_key_values=_StepCache(self.logical), use_cache=True).logits
         best = ops.token_logprobs(logits, top=1)
         choice = best.top_ids[..., 0]
@@ -354,10 +355,11 @@ class CompressedDecoder:
     @torch.no_grad()
     def verify(self, tokens: torch.Tensor) -> Verified:
         """One forward over the tree: ``tokens`` [B, t], the last token of each
-        sequence at node 0 and drafted ones at the others.  From the root on the
-        path follows the children that the model's best token agrees with; the
-        rows of its nodes are appended and the positions advanced, by
-        ``accepted`` tokens a sequence, of which the last is the model's own."""
+        sequence at node 0 and drafted ones at the others (a negative one never
+        stands: it may fill a node that is left out).  From the root on the path
+        follows the children that the model's best token agrees with; the rows of
+        its nodes are appended and the positions advanced, by ``accepted`` tokens
+        a sequence, of which the last is the model's own."""
         if not self.tree_size:
             raise RuntimeError("the decoder was made without tree_size")
         if tuple(tokens.shape) != (self._tree_tok.shape[0], self.tree_nodes):

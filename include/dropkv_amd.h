@@ -333,7 +333,8 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  *   out      [B, T, Hq, D], strides {batch, token, head}, D contiguous
  * out = softmax(scale q K^T) V over the keys seen; a row that sees none, or none
  * whose logit is above -inf, comes out as zeros.  Values and keys that a row
- * does not see do not reach it, also where they are not finite.
+ * does not see do not reach it, also where they are not finite; a value that it
+ * sees and that is not finite makes that element of it inf or NaN.
  * 1 <= T <= 256, bf16 / fp16, D 64 or 128, capacity * D * 2 <= 2^31,
  * B * Hq * T <= 2^24, 0 < scale < 1e37.
  * The workspace (dropkv_tree_workspace_bytes for the same geometry; other

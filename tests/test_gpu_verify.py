@@ -133,6 +133,23 @@ def test_accepted_tree_path_continues_like_steps(gpu, tiny):
     assert int(out[:, -1].argmax(-1)) == right[4]
 
 
+def test_negative_tokens_never_stand(gpu, tiny):
+    """Nodes left out filled with -1, and a node of the tree that holds it: the
+    others come out as without them."""
+    a, tok = decoder(tiny, gpu, tree_size=6)
+    b, _ = decoder(tiny, gpu, tree_size=6, use_graph=False)
+    c, _ = decoder(tiny, gpu, tree_size=6, use_graph=False)
+    right = int(a.step(tok)[:, -1].argmax(-1))
+    b.set_tree([-1, 0, 0, 2, -1, -1])
+    c.set_tree([-1, 0, 0, 2, -1, -1])
+    row = [int(tok), -1, right, (right + 1) % 1000, -1, -7]
+    v = b.verify(torch.tensor([row], device=gpu))
+    w = c.verify(torch.tensor([[max(x, 0) for x in row]], device=gpu))
+    assert v.path[0].tolist()[:2] == [0, 2] and torch.equal(v.path, w.path)
+    assert torch.equal(v.tokens, w.tokens) and torch.equal(v.logits, w.logits)
+    assert int(v.path.max()) < 4
+
+
 def test_capacity_and_refusals(gpu, tiny):
     d, tok = decoder(tiny, gpu, tokens=5, tree_size=4, use_graph=False)
     plain, _ = decoder(tiny, gpu, tokens=5, use_graph=False)
