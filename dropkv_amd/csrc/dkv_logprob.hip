@@ -37,8 +37,8 @@ constexpr int kLpBlock = 16 * 16 / (int)sizeof(T);  // elements: a row of 16 lan
 // The selection takes kLpItems items a thread at a time, and those kept so far.
 constexpr int kLpItems = 8;
 // Its list: what a threshold that `top` of 64 groups (of four threads) reach
-// leaves at most, (top - 1) whole groups and one item.
-constexpr int kLpCap = (kLpMaxTop - 1) * 4 * (kLpItems + 1) + 1;
+// leaves at most, `top` whole groups.
+constexpr int kLpCap = kLpMaxTop * 4 * (kLpItems + 1);
 constexpr int kLpPer = (kLpCap + kLpThreads - 1) / kLpThreads;
 
 struct LogprobArgs {
@@ -103,11 +103,63 @@ struct LpList {
   uint64_t group[64];
   int count;
 };
-// The k largest of item(0) .. item(n - 1) (distinct, or 0: none), in falling
-// order in list[0 .. k); the whole workgroup.  kLpItems items a thread at a time:
-// a threshold that k of them reach (the k-th largest of 64 groups' maxima), the
-// few above it into the list, and the list in order by each item's rank in it.
-template <typename F>
+
+// One less than the k-th largest of a wave's keys (all different, or 0: none), 0
+// where there are fewer: its order two bits at a time, by counts of the lanes
+// above, then among equals its place, unless all of them are among the k.  (The
+// last 12 bits of a 2-byte type's order follow from the others.)
+template <typename T>
+__device__ __forceinline__ uint64_t lp_below_kth(uint64_t key, int k) {
+  constexpr int kLow = sizeof(T) == 2 ? 12 : 0;
+  const uint32_t hi = (uint32_t)(key >> 32);
+  auto reach = [&](uint32_t x, uint32_t t) { return __builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= t)) >= k; };
+  uint32_t t = 0, u = 0;
+#pragma unroll
+  for (int b = 30; b >= kLow; b -= 2)
+    t += (uint32_t)(reach(hi, t + (1u << b)) + reach(hi, t + (2u << b)) + reach(hi, t + (3u << b))) << b;
+  if (t == 0) return 0;
+  if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(hi >= t)) > k) {
+    const bool above = (hi >> kLow) > (t >> kLow), tie = (hi >> kLow) == (t >> kLow);
+    t = (uint32_t)__builtin_amdgcn_readlane((int)hi, __builtin_ctzll(__builtin_amdgcn_ballot_w64(tie)));
+    const uint32_t lo = above ? 0xffffffffu : tie ? (uint32_t)key : 0;
+#pragma unroll 1
+    for (int b = 30; b >= 0; b -= 2)
+      u += (uint32_t)(reach(lo, u + (1u << b)) + reach(lo, u + (2u << b)) + reach(lo, u + (3u << b))) << b;
+  }
+  return (((uint64_t)t << 32) | u) - 1;
+}
+
+// The list's k largest of its `count` keys to list[0 .. k), falling (0: none);
+// the whole workgroup, from a barrier to a barrier.
+__device__ __forceinline__ void lp_rank(int k, LpList* s) {
+  const int tid = threadIdx.x, c = s->count;
+  uint64_t mykey[kLpPer];
+  int place[kLpPer];
+#pragma unroll
+  for (int q = 0; q < kLpPer; ++q) {
+    const int i = tid + q * kLpThreads;
+    place[q] = k;
+    mykey[q] = 0;
+    if (q * kLpThreads < c && i < c) {
+      mykey[q] = s->list[i];
+      int r = 0;
+      for (int j = 0; j < c; ++j) r += s->list[j] > mykey[q];
+      place[q] = r;
+    }
+  }
+  __syncthreads();
+  if (tid >= c && tid < k) s->list[tid] = 0;
+#pragma unroll
+  for (int q = 0; q < kLpPer; ++q)
+    if (place[q] < k) s->list[place[q]] = mykey[q];
+  __syncthreads();
+}
+
+// The k largest of item(0) .. item(n - 1) (keys, or 0: none), in falling order in
+// list[0 .. k); the whole workgroup.  kLpItems items a thread at a time: a
+// threshold that k of them reach (the k-th largest of 64 groups' maxima), the few
+// above it into the list, and the list in order by each item's rank in it.
+template <typename T, typename F>
 __device__ __forceinline__ void lp_select(F&& item, int n, int k, LpList* s) {
   const int tid = threadIdx.x, lane = tid & 63;
 #pragma unroll 1
@@ -123,45 +175,37 @@ __device__ __forceinline__ void lp_select(F&& item, int n, int k, LpList* s) {
     if ((lane & 3) == 0) s->group[tid >> 2] = most;
     if (tid == 0) s->count = 0;
     __syncthreads();
-    const uint64_t mine = s->group[lane];
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) rank += s->group[j] > mine;
-    const uint64_t at = __builtin_amdgcn_ballot_w64(rank == k - 1 && mine != 0);
     // (Where fewer than k groups hold anything, everything passes.)
-    const uint64_t t = at ? s->group[__builtin_ctzll(at)] - 1 : 0;
+    const uint64_t t = lp_below_kth<T>(s->group[lane], k);
 #pragma unroll
     for (int q = 0; q <= kLpItems; ++q)
       if (key[q] > t) s->list[atomicAdd(&s->count, 1)] = key[q];
     __syncthreads();
-    const int c = s->count;
-    uint64_t mykey[kLpPer];
-    int place[kLpPer];
+    lp_rank(k, s);
+  }
+}
+
+// Elements j .. j + 15 / sizeof(T) of x, -inf from `hi` on.
+template <typename T>
+__device__ __forceinline__ void lp_load(const T* x, int j, int hi, float* v) {
+  constexpr int EPV = 16 / (int)sizeof(T);
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw {
+    T e[EPV];
+  };
+  if (j + EPV <= hi) {
+    const Raw r = *reinterpret_cast<const Raw*>(x + j);
 #pragma unroll
-    for (int q = 0; q < kLpPer; ++q) {
-      const int i = tid + q * kLpThreads;
-      place[q] = k;
-      mykey[q] = 0;
-      if (q * kLpThreads < c && i < c) {
-        mykey[q] = s->list[i];
-        int r = 0;
-        for (int j = 0; j < c; ++j) r += s->list[j] > mykey[q];
-        place[q] = r;
-      }
-    }
-    __syncthreads();
-    if (tid >= c && tid < k) s->list[tid] = 0;
+    for (int e = 0; e < EPV; ++e) v[e] = static_cast<float>(r.e[e]);
+  } else {
 #pragma unroll
-    for (int q = 0; q < kLpPer; ++q)
-      if (place[q] < k) s->list[place[q]] = mykey[q];
-    __syncthreads();
+    for (int e = 0; e < EPV; ++e) v[e] = j + e < hi ? static_cast<float>(x[j + e]) : -INFINITY;
   }
 }
 
 // A row's results: its segments joined, its best blocks and their best elements.
 template <typename T, int kMode>
 __device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t row, LpList* s, int* chosen) {
-  constexpr int kBlock = kLpBlock<T>;
+  constexpr int kBlock = kLpBlock<T>, EPV = 16 / (int)sizeof(T);
   const int tid = threadIdx.x, lane = tid & 63;
   Stat st{-__FLT_MAX__, 0.f, 0.f};
   uint64_t key = 0;
@@ -173,23 +217,52 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t row, LpL
   if (kMode == 2) {
     const int nb = a.nb, kb = min(a.top, nb);
     const uint32_t* blocks = a.blocks + row * nb;
-    lp_select(
+    lp_select<T>(
         [&](int i) {
           const uint64_t k = lp_key(blocks[min(i, nb - 1)], i);
           return i < nb ? k : 0;
         },
         nb, kb, s);
     if (tid < kb) chosen[tid] = (int)(0xffffffffu - (uint32_t)s->list[tid]);
+    const uint32_t least = kb < a.top ? 0 : (uint32_t)(s->list[kb - 1] >> 32);
+    if (tid == 0) s->count = 0;
     __syncthreads();
+    // Each of the `top` blocks holds a value of at least the last one's maximum: so
+    // do the `top` values.
     const T* x = static_cast<const T*>(a.x) + row * a.sx;
-    const int n = kb * kBlock;
-    lp_select(
-        [&](int i) {
-          const int j = chosen[min(i, n - 1) / kBlock] * kBlock + i % kBlock;
-          const uint64_t k = lp_key(lp_order(static_cast<float>(x[min(j, a.V - 1)])), j);
-          return i < n && j < a.V ? k : 0;
-        },
-        n, a.top, s);
+    constexpr int kVecs = kLpMaxTop * 16 / kLpThreads;
+    float v[kVecs][EPV];
+    int at[kVecs];
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+      const int i = tid + q * kLpThreads;
+      at[q] = chosen[min(i / 16, kb - 1)] * kBlock + i % 16 * EPV;
+      lp_load<T>(x, at[q], i < 16 * kb ? a.V : 0, v[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q)
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) {
+        const uint32_t o = lp_order(v[q][e]);
+        if (o >= least && at[q] + e < a.V && tid + q * kLpThreads < 16 * kb) {
+          const int p = atomicAdd(&s->count, 1);
+          if (p < kLpThreads) s->list[p] = lp_key(o, at[q] + e);
+        }
+      }
+    __syncthreads();
+    if (s->count <= kLpThreads) {
+      lp_rank(a.top, s);
+    } else {  // (many equals, or few blocks)
+      __syncthreads();
+      const int n = kb * kBlock;
+      lp_select<T>(
+          [&](int i) {
+            const int j = chosen[min(i, n - 1) / kBlock] * kBlock + i % kBlock;
+            const uint64_t k = lp_key(lp_order(static_cast<float>(x[min(j, a.V - 1)])), j);
+            return i < n && j < a.V ? k : 0;
+          },
+          n, a.top, s);
+    }
   }
   if (tid >= 64) return;
   stat_to(st, wave_max_dpp(st.m));
@@ -210,9 +283,6 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t row, LpL
 template <typename T, int kMode>
 __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
   constexpr int EPV = 16 / (int)sizeof(T), NV = kLpElems / EPV;
-  struct __attribute__((packed, aligned(sizeof(T)))) Raw {
-    T e[EPV];
-  };
   __shared__ Stat wstat[kLpThreads / 64];
   __shared__ uint32_t worder[kLpThreads / 64];
   __shared__ int place, last;
@@ -231,17 +301,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
     float v[kLpElems], vmax[NV];
     // Element q EPV + e of the thread is at place j0 + (q 256 + tid) EPV + e.
 #pragma unroll
-    for (int q = 0; q < NV; ++q) {
-      const int j = j0 + (q * kLpThreads + tid) * EPV;
-      if (j + EPV <= hi) {
-        const Raw r = *reinterpret_cast<const Raw*>(x + j);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) v[q * EPV + e] = static_cast<float>(r.e[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) v[q * EPV + e] = j + e < hi ? static_cast<float>(x[j + e]) : -INFINITY;
-      }
-    }
+    for (int q = 0; q < NV; ++q) lp_load<T>(x, j0 + (q * kLpThreads + tid) * EPV, hi, v + q * EPV);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       vmax[q] = v[q * EPV];

@@ -128,6 +128,26 @@ def test_masked_logits(gpu, dtype, top):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("value", [-1.7, 0.3, math.nan, -60000.0])
+@pytest.mark.parametrize("V,N,top", [(20000, 3, 32), (150001, 1, 20), (3000, 2500, 7), (90, 4, 32), (700, 2, 31)])
+def test_equal_logits(gpu, dtype, value, V, N, top):
+    """More equals than the list of candidates holds, of either sign, a few
+    larger ones among them: the lowest places come first."""
+    x = torch.full((V,), value, dtype=dtype)
+    more = [V // 2, V // 3, V - 1]
+    if value == value:
+        x[more] = 2.0
+        want = sorted(more)
+    else:
+        x[more] = 2.0        # NaN is above them
+        want = []
+    rest = [i for i in range(top + 6) if i not in more]
+    from dropkv_amd import ops
+    got = ops.token_logprobs(x.to(gpu).expand(N, V), top=top)
+    assert torch.equal(got.top_ids.cpu(), torch.tensor((want + rest)[:top]).expand(N, top))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("top", [1, 6])
 @pytest.mark.parametrize("N", [1, 2100])
 def test_zeros_of_either_sign(gpu, dtype, top, N):
