@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
   Stat st{-__FLT_MAX__, 0.f, 0.f};
   uint32_t order = 0;  // kMode 1: the thread's largest value, and the first tile that holds it
   int tile = lo;
+  const bool across = a.one && a.S > 1;  // (read by a workgroup of another XCD in this launch)
   for (int j0 = lo; j0 < hi; j0 += kLpTile) {
     float v[kLpElems], vmax[NV];
     // Element q EPV + e of the thread is at place j0 + (q 256 + tid) EPV + e.
@@ -333,7 +334,11 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
         k = max(k, (uint32_t)dpp_i<kDppHalfMirror>((int)k));
         k = max(k, (uint32_t)dpp_i<kDppMirror>((int)k));
         const int j = j0 + (q * kLpThreads + tid) * EPV;
-        if ((lane & 15) == 0 && j < hi) st_dev(a.blocks + row * a.nb + j / kLpBlock<T>, k);
+        if ((lane & 15) == 0 && j < hi) {
+          uint32_t* to = a.blocks + row * a.nb + j / kLpBlock<T>;
+          if (across) st_dev(to, k);
+          else *to = k;
+        }
       }
     }
   }
