@@ -6,7 +6,9 @@
 // maximum and not against zero, so that H does not come from the difference of
 // two large numbers.  Rows are cut into segments where there are few of them;
 // they are joined by the workgroup that finishes a row last, or by a second
-// kernel.  Bound by memory: 2047 rows of 151936 (622 MB).
+// kernel.  Bound by memory: 2047 rows of 151936 bf16 (622 MB) take 119 us (5.2
+// TB/s), 122 with the best token and 147 with the 20 best; 216 rows 20, 25 and 29
+// us; one row 7, 9 and 13, which is three dependent round trips or more.
 //
 // The `top` largest.  A value and its place make one 64-bit key (value above,
 // the complement of the place below): keys are all different, larger means more
@@ -15,10 +17,10 @@
 // lie in the `top` best blocks by (maximum, lowest place): for any element of
 // another block, each of those holds one that comes before it.  Then the
 // blocks are picked, read again (1 to 2 in a hundred of the row), and the elements
-// picked.  (Keeping a list of candidates within the pass took
-// 263 us for 20 of 2047 x 151936, where the pass alone takes 118.)  For the one
-// largest the pass itself keeps each thread's maximum and its tile, and the
-// threads that hold the workgroup's look into that tile again.
+// picked.  (Keeping a list of candidates within the pass took 263 us for 20 of
+// 2047 x 151936.)  For the one largest the pass itself keeps each thread's
+// maximum and its tile, and the threads that hold the workgroup's look into that
+// tile again.
 #include "dkv_common.h"
 #include "dkv_internal.h"
 #include "dkv_select_dev.h"
@@ -420,10 +422,10 @@ __global__ void __launch_bounds__(kLpThreads) logprob_finish_kernel(LogprobArgs 
 // Workgroups of a call: enough to fill the GPU where a row can be cut.
 constexpr int64_t kLpGroups = 2048;
 // Up to so many, the row's last workgroup joins its segments: one launch (one row
-// of 151936, 5 alternatives: 12.9 us in a graph either way, 11.3 us of host time
-// against 14.3).  With more, its wait for the stores and the counter comes on top
-// of every segment, and a second kernel is faster (8 rows 13.5 against 15.5 us,
-// 216 rows 27.9 against 33.4).
+// of 151936, 5 alternatives: 12 to 13 us in a graph either way, 11.2 us a call from
+// the host against 14.0).  With more, its wait for the stores and the counter comes
+// on top of every segment, and a second kernel is faster (20 rows 14.3 against 18.7
+// us in a graph, 8 rows 13.7 against 14.1).
 constexpr int64_t kLpOneLaunch = 128;
 static_assert(kLpOneLaunch * sizeof(uint32_t) <= kSyncBytes, "a counter per row");
 

@@ -231,7 +231,10 @@ __device__ __forceinline__ void tree_add_odd(const TreeArgs& a, int b, int hkv, 
 // Up to 16 rows per KV head: one wave per part, its own tiles.  K comes in
 // registers as the matrix operand, V through LDS for the transposing reads; the
 // next tile's loads are issued as soon as a tile's registers are consumed.
-// Bound by memory: 4 x 16 heads of 6553 rows, D = 64 (107 MB).
+// Bound by memory: 4 x 16 heads of 6553 rows, D = 64 (107 MB) take 19 to 20 us (5.4
+// TB/s) and 24.5 with the join.  P goes into the product in two parts, rounded and
+// remainder (the matrix cores have room here), so that the result is off by its
+// own rounding alone.
 template <typename T, int D>
 __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
   typedef typename Elem<T>::v8 v8;
@@ -410,8 +413,11 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 // significant bits).  In workgroups of 128 rows and more a call is bound by the
 // matrix cores and the ALUs and not by memory, and P is rounded once: each weight
 // is off by at most half a step of the element type, as the output is by its own
-// rounding (4 x 64 heads of 26214 rows, 64 tokens: 336 us in two parts, 255 in
-// one; 8 x 32 heads of up to 8003 rows, 27 tokens: 53 and 45).
+// rounding (4 x 64 heads of 26214 rows, 64 tokens: 333 us in two parts, 255 in
+// one, 860 TFLOP/s; 8 x 32 heads of up to 8003 rows, 27 tokens: 58 and 48, of
+// which 41 are this kernel's, 3.7 TB/s).  What bounds the one: matrix cores busy 46%
+// of the time and vector units 50%, hardly ever together, with two waves on a
+// SIMD; wave priorities, and waves of 64 rows (388 us), did not help.
 //
 // More than 16 rows: NW waves of QB blocks of 16 rows (4 of one or two, 8 of two)
 // take the same keys, so
@@ -683,7 +689,8 @@ __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
 // One wave per row: lane s holds part s's maximum and sum, D / 4 lanes a
 // partial output row.  The first eight loads of partial outputs are issued with
 // the statistics, before the reductions: one round trip for up to 16 (D = 128)
-// or 32 parts.
+// or 32 parts.  4 to 5 us for a few hundred rows, all latency; 16384 rows of 4 parts
+// 12 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
   constexpr int LPR = D / 4, SPL = 64 / LPR, NL = 8;
@@ -880,7 +887,8 @@ hipError_t launch_tree_attention(const dropkv_tree_attention_args& p, size_t* ne
 
 // Accepted rows: one workgroup per (layer, sequence, head).  Each walks its tree
 // by itself, a few hundred cycles for usual depths, so that one launch does (two
-// took 13 us of host and GPU time a call, this one 10).
+// took 13 us of host and GPU time a call, this one 10; its kernel takes 3.5 us for
+// 24 layers' 2 heads and 6.3 for 32 x 8 x 8 heads of 64 tokens).
 struct CommitArgs {
   const int64_t* tokens;  // [B, T]
   const int64_t* choice;
