@@ -127,6 +127,46 @@ def test_masked_logits(gpu, dtype, top):
     assert float(got.logprob[6]) == 0 and float(got.entropy[6]) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("top", [0, 1, 4])
+@pytest.mark.parametrize("N", [1, 2100])
+def test_huge_logits(gpu, dtype, top, N):
+    """Logits near and beyond 1e38, of either sign, rising and falling through it
+    within a thread's share: differences that large leave weight to the largest
+    alone, or to its equals."""
+    V, big = 20000, 3e38
+    line = lambda lo, hi: torch.linspace(lo, hi, V, dtype=torch.float64).float()     # (its span is beyond fp32)
+    rows = [line(-big, -9e37), line(-9e37, -big), line(-big, big), line(big, 9e37),
+            torch.full((V,), -2e38), torch.full((V,), 9e37), torch.full((V,), 1e30)]
+    rows[4][[5, 4101, 9000]] = -1.5e38
+    rows[5][[17, 8209]] = 1.1e38
+    rows[6][4096:] = -3.3e38
+    x = torch.stack(rows).to(dtype)
+    tokens = torch.tensor([0, 0, V - 1, 0, 5, 8209, 100])
+    want = reference(x, tokens, top)
+    from dropkv_amd import ops
+    for i in range(len(rows)):
+        got = ops.token_logprobs(x[i:i + 1].to(gpu).expand(N, V), tokens[i:i + 1].to(gpu).expand(N), top=top)
+        for g, w, name in zip(got[:3], want[:3], ("logprob", "entropy", "top_logprobs")):
+            assert close(g.cpu(), w[i:i + 1].expand(N, *w.shape[1:]), V), (i, name)
+        assert torch.equal(got.top_ids.cpu(), want[3][i:i + 1].expand(N, top)), i
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shift", [50.0, 300.0, -4000.0])
+@pytest.mark.parametrize("N", [1, 2100])
+def test_logits_far_from_zero(gpu, dtype, shift, N):
+    """What is said of a row does not lose by where its logits lie."""
+    V = 30000
+    x = (torch.randn(V, generator=torch.Generator().manual_seed(3)) * 4 + shift).to(dtype)[None]
+    tokens = torch.tensor([77])
+    want = reference(x, tokens, 3)
+    from dropkv_amd import ops
+    got = ops.token_logprobs(x.to(gpu).expand(N, V), tokens.to(gpu).expand(N), top=3)
+    for g, w, name in zip(got[:3], want[:3], ("logprob", "entropy", "top_logprobs")):
+        assert close(g.cpu(), w.expand(N, *w.shape[1:]), V), name
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("value", [-1.7, 0.3, math.nan, -60000.0])
 @pytest.mark.parametrize("V,N,top", [(20000, 3, 32), (150001, 1, 20), (3000, 2500, 7), (90, 4, 32), (700, 2, 31)])
