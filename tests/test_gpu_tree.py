@@ -172,6 +172,46 @@ def test_rows_that_see_nothing(gpu, dtype, D):
     assert (got[:, [4, 8]] == 0).all()
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,T,C,dtype", [
+    (48, 4, 4, 64, 70, 130, torch.float16),       # one part: its workgroup writes the output
+    (24, 8, 4, 128, 70, 130, torch.bfloat16),
+    (70, 12, 4, 64, 24, 65, torch.bfloat16),
+    (48, 8, 4, 128, 100, 300, torch.float16),     # 200 rows of one workgroup
+    (64, 8, 4, 128, 40, 1200, torch.bfloat16),
+    (48, 8, 4, 64, 40, 1200, torch.bfloat16),     # two parts, the drafted keys with the last
+    (48, 4, 4, 128, 100, 0, torch.bfloat16),      # no cache
+])
+@pytest.mark.parametrize("own", [True, False])
+def test_many_heads(gpu, B, Hq, Hkv, D, T, C, dtype, own):
+    """Heads enough to fill the GPU: few parts, the drafted keys in the last.  Rows
+    that see nothing of an empty cache, a drafted value that is not finite and
+    that one token sees, outputs in a buffer with room between the tokens."""
+    from dropkv_amd import ops
+    q, kn, vn, kc, vc = case(B, Hq, Hkv, D, T, C, dtype, 9)
+    g = torch.Generator().manual_seed(9)
+    lens = torch.randint(0, C + 1, (B,), generator=g).tolist() if own else [max(0, C - 3)] * B
+    if own:
+        lens[0], lens[1] = 0, C
+    m = make_tree(B, T, 9)[1]
+    m[:, 5] = False
+    m[:, :, 11] = False
+    m[:, 11, 11] = True
+    refs = {b: reference(q[b:b + 1], kn[b:b + 1], vn[b:b + 1], kc[b:b + 1], vc[b:b + 1], lens[b:b + 1], m[b:b + 1], 0.1)
+            for b in (0, 1, B - 1)}
+    vn[:, :, 11, 3] = math.inf
+    out = torch.full((B, T, Hq, D + 8), 7.0, dtype=dtype, device=gpu)
+    ops.tree_attention(q.to(gpu), kn.to(gpu), vn.to(gpu), kc.to(gpu), vc.to(gpu),
+                       torch.tensor(lens if own else lens[:1], dtype=torch.int32, device=gpu), 0.1, mask=m.to(gpu),
+                       out=out[..., :D])
+    got = out.cpu()
+    assert (got[..., D:] == 7).all()
+    for b, (ref, tol) in refs.items():
+        x = got[b:b + 1, ..., :D].double()
+        assert torch.isposinf(x[:, 11, :, 3]).all(), b
+        x[:, 11, :, 3] = ref[:, 11, :, 3]
+        assert ((x - ref).abs() <= tol).all(), b
+
+
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_values_that_are_not_finite(gpu, value, which):
