@@ -7,7 +7,7 @@
 // two large numbers.  Rows are cut into segments where there are few of them;
 // they are joined by the workgroup that finishes a row last, or by a second
 // kernel.  Bound by memory: 2047 rows of 151936 bf16 (622 MB) take 119 us (5.2
-// TB/s), 122 with the best token and 147 with the 20 best; 216 rows 20, 25 and 29
+// TB/s), 122 with the best token and 147 with the 20 best; 216 rows 20, 23 and 29
 // us; one row 7, 9 and 13, which is three dependent round trips or more.
 //
 // The `top` largest.  A value and its place make one 64-bit key (value above,
@@ -361,14 +361,16 @@ __global__ void __launch_bounds__(kLpThreads) logprob_kernel(LogprobArgs a) {
 #pragma unroll
     for (int w = 1; w < kLpThreads / 64; ++w) most = max(most, worder[w]);
     if (order == most) {
-#pragma unroll 1
-      for (int e = 0; e < kLpElems; ++e) {
+      float v[kLpElems];
+#pragma unroll
+      for (int q = 0; q < NV; ++q) lp_load<T>(x, tile + (q * kLpThreads + tid) * EPV, hi, v + q * EPV);
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int e = kLpElems - 1; e >= 0; --e) {
         const int j = tile + ((e / EPV) * kLpThreads + tid) * EPV + e % EPV;
-        if (j < hi && lp_order(static_cast<float>(x[j])) == most) {
-          atomicMin(&place, j);
-          break;
-        }
+        at = j < hi && lp_order(v[e]) == most ? j : at;
       }
+      atomicMin(&place, at);
     }
     key = most;  // (with the place below, once every thread has looked)
   }
