@@ -66,6 +66,17 @@ constexpr float kPBias = 0.f;
 template <>
 constexpr float kPBias<_Float16> = 14.f;
 
+// The wide kernel lets a row's maximum rise so far above the reference that its
+// weights are taken against (powers of two) before it moves the reference and
+// turns what it has summed: P is at most 2^8 in bf16, and 2^15 with the bias in
+// fp16, whose largest number is just below 2^16.  (Moving it at every new maximum
+// turned two stages of three over 26214 keys in 4 parts, one vector
+// instruction in six: 255 and 248 us where this takes 248 and 243.)
+template <typename T>
+constexpr float kPRise = 8.f;
+template <>
+constexpr float kPRise<_Float16> = 1.f;
+
 template <typename T>
 __device__ __forceinline__ bool not_finite(T x) {
   constexpr uint16_t kExp = std::is_same<T, _Float16>::value ? 0x7c00 : 0x7f80;
@@ -413,8 +424,8 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 // significant bits).  In workgroups of 128 rows and more a call is bound by the
 // matrix cores and the ALUs and not by memory, and P is rounded once: each weight
 // is off by at most half a step of the element type, as the output is by its own
-// rounding (4 x 64 heads of 26214 rows, 64 tokens: 333 us in two parts, 255 in
-// one, 860 TFLOP/s; 8 x 32 heads of up to 8003 rows, 27 tokens: 58 and 48, of
+// rounding (4 x 64 heads of 26214 rows, 64 tokens: 333 us in two parts, 246 in
+// one, 890 TFLOP/s; 8 x 32 heads of up to 8003 rows, 27 tokens: 58 and 48, of
 // which 41 are this kernel's, 3.7 TB/s).  What bounds the one: matrix cores busy 46%
 // of the time and vector units 50%, hardly ever together, with two waves on a
 // SIMD; wave priorities, and waves of 64 rows (388 us), did not help.
@@ -537,7 +548,7 @@ __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
 #pragma unroll
       for (int e = 1; e < 8 * kSub; ++e) tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
       tmax = maximum_xor32(maximum_xor16(tmax)) * a.scale_log2;
-      const float mnew = fmaxf(m[x], tmax);
+      const float mnew = tmax > m[x] + kPRise<T> ? tmax : m[x];
       alpha[x] = __builtin_amdgcn_exp2f(m[x] - mnew);
       turn |= mnew != m[x];
       m[x] = mnew;

@@ -275,6 +275,30 @@ def test_many_small_weights_fp16(gpu):
         assert ((got.cpu().double() - ref).abs() <= tol).all(), scale
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Hq,T", [(1, 2, 1), (1, 4, 10), (200, 4, 30), (200, 8, 20)])   # rows of each kernel
+@pytest.mark.parametrize("step", [0.01, 0.05, 0.3, -0.05])
+def test_rising_logits(gpu, dtype, B, Hq, T, step):
+    """Logits that rise (or fall) from key to key, by a little or much per tile:
+    the running maximum is behind or far behind."""
+    from dropkv_amd import ops
+    D, n = 64, 700
+    g = torch.Generator().manual_seed(T)
+    q = (torch.randn(1, Hq, T, D, generator=g) * 0.2)
+    q[..., 0] = 4.0 + torch.rand(1, Hq, T, generator=g)
+    kc = torch.randn(1, 1, n, D, generator=g) * 0.2
+    kc[..., 0] = torch.arange(n) * (step / 4)
+    vc, kn, vn = (torch.randn(1, 1, x, D, generator=g) for x in (n, T, T))
+    q, kc, vc, kn, vn = (x.to(dtype) for x in (q, kc, vc, kn, vn))
+    m = torch.ones(1, T, T, dtype=torch.bool).tril()
+    ref, tol = reference(q, kn, vn, kc, vc, [n], m, 1.0)
+    many = [x.to(gpu).repeat(B, 1, 1, 1) for x in (q, kn, vn, kc, vc)]
+    got = ops.tree_attention(*many, torch.tensor([n], dtype=torch.int32, device=gpu), 1.0)
+    assert (got == got[:1]).all()
+    got = got[:1].cpu().double()
+    assert ((got - ref).abs() <= tol).all(), float(((got - ref).abs() / tol).max())
+
+
 def test_counts_out_of_range_stay_in_bounds(gpu):
     """A count past the capacity reads as the capacity, a negative one as 0."""
     from dropkv_amd import ops
