@@ -15,7 +15,8 @@
 // and 8 KV heads of 128, fp16, norms and V: 688 MB in 147 us, 4.7 TB/s, where a
 // large copy reaches 4.9; 8 tokens 3.7 us, one round trip).  A lane holds 8 values
 // of the first half and their partners of the second, so that a pair never
-// leaves the lane and the norm is a reduction over the row's D / 16 lanes.  A
+// leaves the lane and the norm is a reduction over the row's 4, 8 or 16 lanes, of
+// which D / 16 hold values.  A
 // wave takes several heads of one token, since c and s (as long as a row, and
 // in fp32 twice its bytes) are then loaded once for all of them.
 #include "dkv_common.h"
@@ -103,15 +104,17 @@ __device__ __forceinline__ bool rope_row(const RopeArgs& a, int b, int l, const 
   return true;
 }
 
-template <typename T, typename TC, int D>
+// LPR lanes a row, D / 16 of them at work (D a multiple of 16).
+template <typename T, typename TC, int LPR>
 __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
-  constexpr int LPR = D / 16, HPW = 64 / LPR;
+  constexpr int HPW = 64 / LPR;
   const int wid = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
   const int token = wid / a.chunks, h0 = (wid - token * a.chunks) * a.per;
   if (token >= a.tokens) return;
   const int b = token / a.L, l = token - b * a.L;
   const int c = lane % LPR;
   const int R = a.R, pairs = R / 16;
+  const bool live = 16 * c < a.D;
   // The lane's two runs of 8 values.
   const bool turned = c < pairs;
   const int i0 = turned ? 8 * c : R + 16 * (c - pairs), i1 = turned ? i0 + R / 2 : i0 + 8;
@@ -142,6 +145,7 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
     const T* src = static_cast<const T*>(side.src) + b * side.s_sb + h * side.s_sh + l * side.s_sl;
     T* dst = static_cast<T*>(side.dst) + b * side.d_sb + h * side.d_sh + l * side.d_sl;
     if (copy) {
+      if (!live) continue;
 #pragma unroll
       for (int u = 0; u < (int)sizeof(T) / 2; ++u) {  // 16 bytes each
         const u32x4 x0 = reinterpret_cast<const u32x4*>(src + i0)[u], x1 = reinterpret_cast<const u32x4*>(src + i1)[u];
@@ -150,13 +154,16 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
       }
       continue;
     }
-    float x0[8], x1[8];
-    load_vec8(src + i0, x0);
-    load_vec8(src + i1, x1);
+    float x0[8] = {}, x1[8] = {};
+    if (live) {
+      load_vec8(src + i0, x0);
+      load_vec8(src + i1, x1);
+    }
     const void* w = side.w;
     if (w) {
-      float ss = 0.f, w0[8], w1[8];
-      if (a.w_f32) {
+      float ss = 0.f, w0[8] = {}, w1[8] = {};
+      if (!live) {
+      } else if (a.w_f32) {
         load_vec8(static_cast<const float*>(w) + i0, w0);
         load_vec8(static_cast<const float*>(w) + i1, w1);
       } else {
@@ -167,7 +174,7 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
       for (int e = 0; e < 8; ++e) ss = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], ss));
 #pragma unroll
       for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor(ss, o);
-      const float inv = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+      const float inv = 1.f / sqrtf(ss / (float)a.D + a.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x0[e] = x0[e] * inv * w0[e];
@@ -182,13 +189,16 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
         x0[e] = y0;
       }
     }
-    store_vec8(dst + i0, x0);
-    store_vec8(dst + i1, x1);
+    if (live) {
+      store_vec8(dst + i0, x0);
+      store_vec8(dst + i1, x1);
+    }
   }
 }
 
 // Any head dimension, alignment and rotated width: a wave per head's row, a
-// pair per lane at a time.
+// pair per lane at a time (4096 tokens of 32 + 8 heads of 96: 112 us where the
+// kernel above takes 19).
 template <typename T, typename TC>
 __global__ void __launch_bounds__(256) norm_rope_any_kernel(RopeArgs a) {
   const int heads = a.Hq + a.Hk + a.Hv;
@@ -241,20 +251,20 @@ constexpr int64_t kRopeWaves = 4096;
 template <typename T, typename TC>
 static hipError_t launch_rope_t(RopeArgs a, bool vec, hipStream_t st) {
   const int64_t heads = (int64_t)a.Hq + a.Hk + a.Hv;
-  if (vec && (a.D == 64 || a.D == 128 || a.D == 256)) {
-    const int hpw = 64 / (a.D / 16);
+  if (vec && a.D % 16 == 0 && a.D <= 256) {
+    const int lanes = a.D <= 64 ? 4 : a.D <= 128 ? 8 : 16, hpw = 64 / lanes;
     const int64_t its = (heads + hpw - 1) / hpw;
     const int64_t want = std::min<int64_t>(its, std::max<int64_t>(1, kRopeWaves / a.tokens));  // waves per token
     const int64_t its_w = (its + want - 1) / want;
     a.per = (int)(its_w * hpw);
     a.chunks = (int)((its + its_w - 1) / its_w);
     const dim3 grid((unsigned)(((int64_t)a.tokens * a.chunks + 3) / 4));
-    if (a.D == 64)
-      launch((norm_rope_kernel<T, TC, 64>), grid, dim3(256), 0, st, a);
-    else if (a.D == 128)
-      launch((norm_rope_kernel<T, TC, 128>), grid, dim3(256), 0, st, a);
+    if (lanes == 4)
+      launch((norm_rope_kernel<T, TC, 4>), grid, dim3(256), 0, st, a);
+    else if (lanes == 8)
+      launch((norm_rope_kernel<T, TC, 8>), grid, dim3(256), 0, st, a);
     else
-      launch((norm_rope_kernel<T, TC, 256>), grid, dim3(256), 0, st, a);
+      launch((norm_rope_kernel<T, TC, 16>), grid, dim3(256), 0, st, a);
   } else {
     launch((norm_rope_any_kernel<T, TC>), dim3((unsigned)(((int64_t)a.tokens * heads + 3) / 4)), dim3(256), 0, st, a);
   }

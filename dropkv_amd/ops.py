@@ -472,7 +472,8 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     ``n_rows`` rows (int32 on the device, one count or one per sequence) are
     filled.  ``mask`` (bool, [T, T] or [B, T, T]) says which drafted token
     (second to last axis) sees which; without it they are a chain.  Returns
-    ``out`` [B, T, Hq, D]; a row that sees no key is zeros.  The buffers are not
+    ``out`` [B, T, Hq, D], which must not lie in an input; a row that sees no key
+    is zeros.  The buffers are not
     written: ``tree_commit`` stores the rows of the tokens that stand."""
     index = _device_index("tree_attention", q, k_new, v_new, k_cache, v_cache, n_rows, out, workspace, mask)
     if torch.is_grad_enabled():

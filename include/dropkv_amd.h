@@ -330,7 +330,8 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  *   mask     device bytes, nonzero where drafted token t sees drafted token j,
  *            at mask[b * m_s[0] + t * m_s[1] + j * m_s[2]]; NULL: j <= t (a
  *            chain).  Every token sees all stored rows.
- *   out      [B, T, Hq, D], strides {batch, token, head}, D contiguous
+ *   out      [B, T, Hq, D], strides {batch, token, head}, D contiguous; it and the
+ *            workspace overlap no input
  * out = softmax(scale q K^T) V over the keys seen; a row that sees none, or none
  * whose logit is above -inf, comes out as zeros.  Values and keys that a row
  * does not see do not reach it, also where they are not finite; a value that it

@@ -41,7 +41,14 @@ def angles(L, R, seed, first=0):
     (2, 32, 8, 37, 128, 128),
     (1, 8, 8, 129, 128, 64),       # half of the head rotated
     (1, 4, 1, 5, 256, 256),
-    (2, 3, 1, 11, 96, 96),         # generic kernel
+    (2, 3, 1, 11, 96, 96),         # lanes without values
+    (2, 3, 1, 11, 80, 48),
+    (1, 4, 2, 7, 192, 192),
+    (1, 3, 1, 300, 48, 32),
+    (1, 3, 2, 4, 16, 16),
+    (1, 2, 1, 9, 240, 16),
+    (2, 3, 1, 11, 100, 96),        # generic kernel
+    (1, 2, 1, 3, 272, 272),
     (1, 5, 5, 4, 64, 24),          # a rotated width of no whole 16
     (1, 2, 2, 3, 6, 4),
     (1, 2, 1, 2, 1000, 998),
