@@ -403,9 +403,10 @@ def decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, 
     return out
 
 
-# The wrappers below check by attribute reads of ~0.1 us each and hand the entry
-# point one packed structure: for a call of a few rows their host time is the
-# larger part of it.
+# The wrappers below check by attribute reads of ~0.1 us each, make outputs like a
+# tensor at hand (1.2 us; 1.9 from a shape, 3 for the parts of one) and hand the
+# entry point one packed structure: for a call of a few rows their host time is
+# the larger part of it.
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -509,7 +510,7 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
         else:
             m_b, m_t, m_j = mask.stride()
     if out is None:
-        out = torch.empty((B, T, Hq, D), dtype=dtype, device=q.device)
+        out = q.new_empty((B, T, Hq, D))
     elif out.shape != (B, T, Hq, D) or out.dtype is not dtype or out.stride(3) != 1:
         raise RuntimeError("tree_attention: out must be [B, T, Hq, D] of q's dtype, D contiguous")
     if not (B and T and Hq):
@@ -577,8 +578,8 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tenso
     if n_rows.dtype is not torch.int32 or len(nshape) != len(lead) or nshape[-1] not in (1, B) or nshape[0] not in (
             (N,) if layers else (1, B)):
         raise RuntimeError("tree_commit: n_rows must be int32, [1] or [B], or [N, 1] or [N, B]")
-    path = torch.empty((B, T), dtype=torch.int32, device=tokens.device)
-    accepted = torch.empty((B,), dtype=torch.int32, device=tokens.device)
+    path = torch.empty_like(tokens, dtype=torch.int32, memory_format=torch.contiguous_format)
+    accepted = tokens.new_empty((B,), dtype=torch.int32)
     if B == 0:
         return path, accepted
     tokens, choice, parents = tokens.contiguous(), choice.contiguous(), parents.contiguous()
@@ -734,11 +735,12 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     x = _rows(logits if len(shape) == 2 else logits.reshape(-1, V))
     N = x.shape[0]
     if tokens is None:
-        logprob, entropy = None, torch.empty(lead, dtype=torch.float32, device=device)
+        logprob, entropy = None, logits.new_empty(lead, dtype=torch.float32)
     else:
-        logprob, entropy = torch.empty((2, *lead), dtype=torch.float32, device=device).unbind()
-    top_lp = torch.empty((*lead, top), dtype=torch.float32, device=device)
-    top_id = torch.empty((*lead, top), dtype=torch.int64, device=device)
+        logprob = torch.empty_like(tokens, dtype=torch.float32, memory_format=torch.contiguous_format)
+        entropy = torch.empty_like(logprob)
+    top_lp = logits.new_empty((*lead, top), dtype=torch.float32)
+    top_id = torch.empty_like(top_lp, dtype=torch.int64)
     if N:
         nbytes = _logprob_bytes(N, V, top)
         ws = _stream_workspace(nbytes, device) if nbytes else None
