@@ -43,9 +43,10 @@ def _evict_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     return ws
 
 
-# One workspace per (device, stream), grown on demand and reused by every
-# ``scores`` / ``evict`` call on that stream: calls on one stream run in
-# order, so they never use it at the same time.
+# One workspace per (device, stream, thread), grown on demand and reused by every
+# call of that thread on that stream that brings none: the kernels of one
+# thread's calls run in order, so they never use it at the same time.  (Two
+# threads' calls on one stream may put their kernels between one another's.)
 _shared_ws: dict = {}
 _shared_ws_lock = threading.Lock()
 
@@ -54,7 +55,7 @@ def _stream_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     nbytes = max(int(nbytes), 1)
     if torch.cuda.is_current_stream_capturing():
         return _evict_workspace(nbytes, dev)  # a graph keeps its own (private-pool) workspace
-    key = (dev.index, _stream(dev))
+    key = (dev.index, _stream(dev), threading.get_ident())
     with _shared_ws_lock:
         ws = _shared_ws.get(key)
         if ws is None or ws.numel() < nbytes:
@@ -64,9 +65,9 @@ def _stream_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
 
 
 def release_workspaces() -> None:
-    """Drop the per-(device, stream) workspaces kept for calls that bring
-    none (they only grow, to the largest call seen on that stream, and are
-    otherwise held for the life of the process).  Each goes back to
+    """Drop the per-(device, stream, thread) workspaces kept for calls that bring
+    none (they only grow, to the largest call seen there, and are otherwise
+    held for the life of the process).  Each goes back to
     PyTorch's caching allocator, which orders its reuse after the work
     already enqueued on its stream (``torch.cuda.empty_cache()`` can then
     return it to the device); the next call allocates a fresh workspace."""

@@ -4,6 +4,7 @@ probabilities): every refusal comes before anything is enqueued.  CPU only."""
 
 import os
 import re
+import threading
 
 import pytest
 import torch
@@ -174,3 +175,19 @@ def test_host_tensors_are_refused():
                  lambda: ops.tree_commit(t, t[0].int(), t, k, k, k, k, n)):
         with pytest.raises(RuntimeError, match="device"):
             call()
+
+
+def test_threads_have_their_own_workspace(monkeypatch):
+    """A call is several kernels: another thread's, on the same stream, may come
+    between them."""
+    monkeypatch.setattr(ops, "_shared_ws", {})
+    monkeypatch.setattr(ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(ops, "_evict_workspace", lambda nbytes, dev: torch.zeros(nbytes, dtype=torch.uint8))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    dev = torch.device("cuda", 0)
+    mine, theirs = ops._stream_workspace(100, dev), []
+    thread = threading.Thread(target=lambda: theirs.append(ops._stream_workspace(50, dev)))
+    thread.start()
+    thread.join()
+    assert ops._stream_workspace(60, dev) is mine and theirs[0] is not mine
+    assert ops._stream_workspace(200, dev).numel() == 200
