@@ -426,9 +426,10 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 // is off by at most half a step of the element type, as the output is by its own
 // rounding (4 x 64 heads of 26214 rows, 64 tokens: 333 us in two parts, 246 in
 // one, 890 TFLOP/s; 8 x 32 heads of up to 8003 rows, 27 tokens: 58 and 48, of
-// which 41 are this kernel's, 3.7 TB/s).  What bounds the one: matrix cores busy 46%
-// of the time and vector units 50%, hardly ever together, with two waves on a
-// SIMD; wave priorities, and waves of 64 rows (388 us), did not help.
+// which 41 are this kernel's, 3.7 TB/s).  What bounds the one: matrix cores busy 49%
+// of the time and vector units 46%, hardly ever together, with two waves on a
+// SIMD; wave priorities, waves of 64 rows (388 us), and the next stage's products
+// with K beside a stage's softmax (248) did not help.
 //
 // More than 16 rows: NW waves of QB blocks of 16 rows (4 of one or two, 8 of two)
 // take the same keys, so
