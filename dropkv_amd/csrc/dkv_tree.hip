@@ -71,7 +71,9 @@ constexpr float kPBias<_Float16> = 14.f;
 // turns what it has summed: P is at most 2^8 in bf16, and 2^15 with the bias in
 // fp16, whose largest number is just below 2^16.  (Moving it at every new maximum
 // turned two stages of three over 26214 keys in 4 parts, one vector
-// instruction in six: 255 and 248 us where this takes 248 and 243.)
+// instruction in six: 255 and 248 us where this takes 248 and 243.  The largest
+// weight is then no exact 1 and is rounded like the others, in the sum as in the
+// product: there the error against 64 bits is 0.0023, not 0.0021, of the output.)
 template <typename T>
 constexpr float kPRise = 8.f;
 template <>
