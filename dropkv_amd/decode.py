@@ -62,7 +62,10 @@ _rotary_saved: list = []
 def _deferring(orig):
     def apply_rotary_pos_emb(q, k, cos, sin, *args, **kwargs):
         dec = getattr(_active, "decoder", None)
-        if dec is None or not dec.tree_size or args or kwargs:
+        if dec is None or not dec.tree_size:
+            return orig(q, k, cos, sin, *args, **kwargs)
+        if args or kwargs:
+            dec._angles = None
             return orig(q, k, cos, sin, *args, **kwargs)
         dec._angles = (cos, sin)
         return q, k
@@ -156,7 +159,7 @@ class CompressedDecoder:
         self.tree_size = int(tree_size)
         if not 0 <= self.tree_size <= 256:
             raise ValueError(f"tree_size must be in [0, 256], got {tree_size}")
-        self._angles = None  # of the forward that runs
+        self._angles = None  # of a layer whose rotation was deferred, until its attention takes them
         kv = _stored_kv(cache)
         if not kv:
             raise ValueError("the cache holds no layers: run the prefill first")
@@ -232,9 +235,10 @@ class CompressedDecoder:
         i = module.layer_idx
         T, D = query.shape[2], query.shape[3]
         k_new, v_new = self._k_draft[i, :, :, :T], self._v_draft[i, :, :, :T]
-        if self._angles is not None:
-            query, _, _ = ops.norm_rope(query, key, *self._angles, v=value, k_out=k_new, v_out=v_new)
-        else:  # a model whose rotation is not deferred
+        angles, self._angles = self._angles, None
+        if angles is not None:
+            query, _, _ = ops.norm_rope(query, key, *angles, v=value, k_out=k_new, v_out=v_new)
+        else:  # a layer whose rotation was not deferred
             k_new.copy_(key)
             v_new.copy_(value)
         return ops.tree_attention(query, k_new, v_new, self.k_buf[i], self.v_buf[i], self.n_rows[i],
