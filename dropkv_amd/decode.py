@@ -22,14 +22,13 @@ path that stands to every layer's buffer (``dropkv_tree_commit``).
 from __future__ import annotations
 
 import contextlib
-import importlib
 import threading
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import ops
-from .hf_query import DEFAULT_MODELING_MODULES
+from .hf_query import rotary_deferral
 
 ATTN_NAME = "dropkv_decode"
 _active = threading.local()
@@ -52,51 +51,6 @@ def _decode_attention(module, query, key, value, attention_mask=None, scaling=No
     scale = scaling if scaling is not None else D ** -0.5
     ops.decode_attention(query, key, value, dec.k_buf[i], dec.v_buf[i], dec.n_rows[i:i + 1], scale, out, dec.ws)
     return out, None
-
-
-_rotary_lock = threading.Lock()
-_rotary_users = 0
-_rotary_saved: list = []
-
-
-def _deferring(orig):
-    def apply_rotary_pos_emb(q, k, cos, sin, *args, **kwargs):
-        dec = getattr(_active, "decoder", None)
-        if dec is None or not dec.tree_size:
-            return orig(q, k, cos, sin, *args, **kwargs)
-        if args or kwargs:
-            dec._angles = None
-            return orig(q, k, cos, sin, *args, **kwargs)
-        dec._angles = (cos, sin)
-        return q, k
-
-    return apply_rotary_pos_emb
-
-
-@contextlib.contextmanager
-def _deferred_rotary():
-    """Leave the rotation of queries and keys to the attention function of the
-    thread's active decoder with ``tree_size``; other threads, and other layouts
-    of the angles, rotate as ever.  Threads may overlap: the last one restores."""
-    global _rotary_users
-    with _rotary_lock:
-        _rotary_users += 1
-        if _rotary_users == 1:
-            for name in DEFAULT_MODELING_MODULES:
-                mod = importlib.import_module(name)
-                orig = mod.apply_rotary_pos_emb
-                mod.apply_rotary_pos_emb = _deferring(orig)
-                _rotary_saved.append((mod, mod.apply_rotary_pos_emb, orig))
-    try:
-        yield
-    finally:
-        with _rotary_lock:
-            _rotary_users -= 1
-            if _rotary_users == 0:
-                for mod, ours, orig in _rotary_saved:
-                    if mod.apply_rotary_pos_emb is ours:  # (else another wrapper lies on it, and passes through)
-                        mod.apply_rotary_pos_emb = orig
-                _rotary_saved.clear()
 
 
 def _register():
@@ -220,12 +174,19 @@ class CompressedDecoder:
         cfg._attn_implementation = ATTN_NAME
         _active.decoder = self
         try:
-            with _deferred_rotary() if self.tree_size else contextlib.nullcontext():
+            with rotary_deferral(self._defer) if self.tree_size else contextlib.nullcontext():
                 yield
         finally:
             cfg._attn_implementation = prev_impl
             _active.decoder = prev_dec
             self._angles = None
+
+    def _defer(self, cos, sin, *args, **kwargs) -> bool:
+        """Take a layer's angles, for its attention function to rotate with; not
+        in another layout."""
+        mine = not args and not kwargs and getattr(_active, "decoder", None) is self
+        self._angles = (cos, sin) if mine else None
+        return mine
 
     def _tree_attention(self, module, query, key, value, scaling, sliding_window) -> torch.Tensor:
         """One layer of a forward over T tokens: rows into the drafts' buffers,

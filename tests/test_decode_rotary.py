@@ -1,8 +1,10 @@
 """Who rotates queries and keys in a forward over drafted tokens, on the CPU: a
 tiny Qwen2 model with the operators replaced by PyTorch ones that rotate with
 the model's own function, so that a rotation left out, or done twice, shows in
-the logits' bits."""
+the logits' bits.  Threads that capture queries meanwhile, and layers that
+rotate in a way of their own, change nothing."""
 
+import threading
 from types import SimpleNamespace
 
 import pytest
@@ -15,6 +17,7 @@ from transformers.models.qwen2 import modeling_qwen2  # noqa: E402
 
 from dropkv_amd import decode, ops  # noqa: E402
 from dropkv_amd.e2e_qwen2 import build_model, make_config, random_prompt  # noqa: E402
+from dropkv_amd.hf_query import query_capture, take_captured_query  # noqa: E402
 
 TINY = dict(vocab_size=200, hidden_size=256, intermediate_size=256, num_hidden_layers=3,
             num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512)
@@ -93,8 +96,74 @@ def between_layers(model, layer, do):
     return model.model.layers[layer].register_forward_pre_hook(lambda *a: do())
 
 
+class Capturing:
+    """Another thread's query_capture block, entered and left on request."""
+
+    def __init__(self):
+        self.enter, self.entered, self.leave = (threading.Event() for _ in range(3))
+        self.thread = threading.Thread(target=self._run)
+        self.thread.start()
+
+    def _run(self):
+        self.enter.wait(30)
+        with query_capture():
+            self.entered.set()
+            self.leave.wait(30)
+
+    def go_in(self):
+        self.enter.set()
+        assert self.entered.wait(30)
+
+    def go_out(self):
+        self.leave.set()
+        self.thread.join(30)
+        assert not self.thread.is_alive()
+
+
 def same(a, b):
     assert torch.equal(a.logits, b.logits) and torch.equal(a.tokens, b.tokens)
+
+
+@pytest.mark.parametrize("went_in", ["before", "during"])
+@pytest.mark.parametrize("came_out", ["during", "after"])
+def test_a_capture_of_another_thread_in_between(tiny, decoder, went_in, came_out):
+    want_dec, dec, other = decoder(), decoder(), Capturing()
+    want = want_dec.verify(DRAFTS)
+    if went_in == "before":
+        other.go_in()
+    handles = []
+    if went_in == "during":
+        handles.append(between_layers(tiny[1], 1, other.go_in))
+    if came_out == "during":
+        handles.append(between_layers(tiny[1], 2, other.go_out))
+    try:
+        got = dec.verify(DRAFTS)
+    finally:
+        for h in handles:
+            h.remove()
+        other.enter.set()
+        other.go_out()
+    same(got, want)
+    for a, b in zip(dec.k_buf, want_dec.k_buf):
+        n = int(dec.n_rows[0, 0])
+        assert torch.equal(a[:, :, :n], b[:, :, :n])
+    # Nothing is left behind: neither a wrapper nor a recorded query.
+    assert modeling_qwen2.apply_rotary_pos_emb is ORIG
+    assert take_captured_query() is None
+
+
+def test_nested_captures_and_a_verification_within(tiny, decoder):
+    """A capture around a verification stays in force after it."""
+    want, dec = decoder().verify(DRAFTS), decoder()
+    with query_capture():
+        with query_capture():
+            same(dec.verify(DRAFTS), want)
+        assert modeling_qwen2.apply_rotary_pos_emb is not ORIG
+        q = torch.randn(1, 4, 2, 64)
+        cos, sin = torch.randn(1, 2, 64), torch.randn(1, 2, 64)
+        rotated, _ = modeling_qwen2.apply_rotary_pos_emb(q, q, cos, sin)
+        assert take_captured_query() is rotated and torch.equal(rotated, ORIG(q, q, cos, sin)[0])
+    assert modeling_qwen2.apply_rotary_pos_emb is ORIG
 
 
 @pytest.mark.parametrize("own", ["arguments", "another function"])
