@@ -46,9 +46,28 @@ def _evict_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
 # One workspace per (device, stream, thread), grown on demand and reused by every
 # call of that thread on that stream that brings none: the kernels of one
 # thread's calls run in order, so they never use it at the same time.  (Two
-# threads' calls on one stream may put their kernels between one another's.)
+# threads' calls on one stream may put their kernels between one another's.)  A
+# thread's go back to the allocator when it ends.
 _shared_ws: dict = {}
-_shared_ws_lock = threading.Lock()
+_shared_ws_lock = threading.RLock()  # (an ended thread's mark may go in a collection under the lock)
+
+
+class _ThreadMark:
+    """Lives as long as its thread, whose workspaces go with it."""
+
+    def __init__(self):
+        self.ident = threading.get_ident()
+
+    def __del__(self):
+        if _shared_ws_lock is None:  # (the interpreter is ending)
+            return
+        with _shared_ws_lock:
+            for key in list(_shared_ws or ()):
+                if key[-1] == self.ident:
+                    _shared_ws.pop(key, None)
+
+
+_thread_local = threading.local()
 
 
 def _stream_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
@@ -59,6 +78,8 @@ def _stream_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     with _shared_ws_lock:
         ws = _shared_ws.get(key)
         if ws is None or ws.numel() < nbytes:
+            if not hasattr(_thread_local, "mark"):
+                _thread_local.mark = _ThreadMark()
             ws = _evict_workspace(nbytes, dev)
             _shared_ws[key] = ws
     return ws
@@ -67,7 +88,7 @@ def _stream_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
 def release_workspaces() -> None:
     """Drop the per-(device, stream, thread) workspaces kept for calls that bring
     none (they only grow, to the largest call seen there, and are otherwise
-    held for the life of the process).  Each goes back to
+    held for the life of their thread).  Each goes back to
     PyTorch's caching allocator, which orders its reuse after the work
     already enqueued on its stream (``torch.cuda.empty_cache()`` can then
     return it to the device); the next call allocates a fresh workspace."""
