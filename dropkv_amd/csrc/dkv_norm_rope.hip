@@ -42,6 +42,7 @@ struct RopeArgs {
   int64_t p_sb, P;
   int L, Hq, Hk, Hv, D, R, tokens;
   int per, chunks;  // heads (q, k and v, in that order) per wave; waves per token
+  int64_t first;    // the launch's first wave
   float eps;
 };
 
@@ -108,7 +109,7 @@ __device__ __forceinline__ bool rope_row(const RopeArgs& a, int b, int l, const 
 template <typename T, typename TC, int LPR>
 __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
   constexpr int HPW = 64 / LPR;
-  const int wid = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+  const int wid = (int)a.first + blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
   const int token = wid / a.chunks, h0 = (wid - token * a.chunks) * a.per;
   if (token >= a.tokens) return;
   const int b = token / a.L, l = token - b * a.L;
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(RopeArgs a) {
 template <typename T, typename TC>
 __global__ void __launch_bounds__(256) norm_rope_any_kernel(RopeArgs a) {
   const int heads = a.Hq + a.Hk + a.Hv;
-  const int64_t wid = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const int64_t wid = a.first + (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   const int lane = threadIdx.x & 63;
   if (wid >= (int64_t)a.tokens * heads) return;
   const int token = (int)(wid / heads), hh = (int)(wid - (int64_t)token * heads);
@@ -247,6 +248,14 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(RopeArgs a) {
 
 // Waves that a call is spread over, where its tokens allow.
 constexpr int64_t kRopeWaves = 4096;
+// Waves of one launch: a grid holds fewer than 2^32 work-items.
+constexpr int64_t kRopeLaunch = (int64_t)1 << 25;
+
+template <typename F>
+static void launch_waves(F kernel, RopeArgs& a, int64_t waves, hipStream_t st) {
+  for (a.first = 0; a.first < waves; a.first += kRopeLaunch)
+    launch(kernel, dim3((unsigned)((std::min(waves - a.first, kRopeLaunch) + 3) / 4)), dim3(256), 0, st, a);
+}
 
 template <typename T, typename TC>
 static hipError_t launch_rope_t(RopeArgs a, bool vec, hipStream_t st) {
@@ -258,15 +267,15 @@ static hipError_t launch_rope_t(RopeArgs a, bool vec, hipStream_t st) {
     const int64_t its_w = (its + want - 1) / want;
     a.per = (int)(its_w * hpw);
     a.chunks = (int)((its + its_w - 1) / its_w);
-    const dim3 grid((unsigned)(((int64_t)a.tokens * a.chunks + 3) / 4));
+    const int64_t waves = (int64_t)a.tokens * a.chunks;
     if (lanes == 4)
-      launch((norm_rope_kernel<T, TC, 4>), grid, dim3(256), 0, st, a);
+      launch_waves(norm_rope_kernel<T, TC, 4>, a, waves, st);
     else if (lanes == 8)
-      launch((norm_rope_kernel<T, TC, 8>), grid, dim3(256), 0, st, a);
+      launch_waves(norm_rope_kernel<T, TC, 8>, a, waves, st);
     else
-      launch((norm_rope_kernel<T, TC, 16>), grid, dim3(256), 0, st, a);
+      launch_waves(norm_rope_kernel<T, TC, 16>, a, waves, st);
   } else {
-    launch((norm_rope_any_kernel<T, TC>), dim3((unsigned)(((int64_t)a.tokens * heads + 3) / 4)), dim3(256), 0, st, a);
+    launch_waves(norm_rope_any_kernel<T, TC>, a, (int64_t)a.tokens * heads, st);
   }
   return hipGetLastError();
 }
