@@ -451,20 +451,39 @@ static LogprobPlan logprob_plan(int64_t N, int64_t V, int64_t top) {
 size_t logprob_workspace_bytes(int64_t N, int64_t V, int64_t top) { return logprob_plan(N, V, top).bytes; }
 int64_t logprob_max_top() { return kLpMaxTop; }
 
+// Rows of one launch: a grid holds fewer than 2^32 work-items.  (More than
+// kLpGroups rows are not cut into segments.)
+constexpr int64_t kLpLaunch = (int64_t)1 << 23;
+static_assert(kLpLaunch > kLpGroups, "a workgroup a row");
+
 template <typename T>
 static hipError_t launch_logprob_t(LogprobArgs a, hipStream_t st) {
   a.nb = (a.V + kLpBlock<T> - 1) / kLpBlock<T>;
-  const dim3 grid((unsigned)(a.N * a.S)), rows((unsigned)a.N), block(kLpThreads);
+  const dim3 block(kLpThreads);
   const bool two = a.S > 1 && !a.one;
-  if (a.top == 0) {
-    launch((logprob_kernel<T, 0>), grid, block, 0, st, a);
-    if (two) launch((logprob_finish_kernel<T, 0>), rows, block, 0, st, a);
-  } else if (a.top == 1) {
-    launch((logprob_kernel<T, 1>), grid, block, 0, st, a);
-    if (two) launch((logprob_finish_kernel<T, 1>), rows, block, 0, st, a);
-  } else {
-    launch((logprob_kernel<T, 2>), grid, block, 0, st, a);
-    if (two) launch((logprob_finish_kernel<T, 2>), rows, block, 0, st, a);
+  for (int64_t left = a.N; left > 0; left -= kLpLaunch) {
+    a.N = std::min(left, kLpLaunch);
+    const dim3 grid((unsigned)(a.N * a.S)), rows((unsigned)a.N);
+    if (a.top == 0) {
+      launch((logprob_kernel<T, 0>), grid, block, 0, st, a);
+      if (two) launch((logprob_finish_kernel<T, 0>), rows, block, 0, st, a);
+    } else if (a.top == 1) {
+      launch((logprob_kernel<T, 1>), grid, block, 0, st, a);
+      if (two) launch((logprob_finish_kernel<T, 1>), rows, block, 0, st, a);
+    } else {
+      launch((logprob_kernel<T, 2>), grid, block, 0, st, a);
+      if (two) launch((logprob_finish_kernel<T, 2>), rows, block, 0, st, a);
+    }
+    a.x = static_cast<const T*>(a.x) + kLpLaunch * a.sx;
+    if (a.tokens) {
+      a.tokens += kLpLaunch;
+      a.logprob += kLpLaunch;
+    }
+    a.entropy += kLpLaunch;
+    a.top_lp += kLpLaunch * a.top;
+    a.top_id += kLpLaunch * a.top;
+    a.part += kLpLaunch * 3;
+    a.blocks += kLpLaunch * a.nb;
   }
   return hipGetLastError();
 }

@@ -27,3 +27,22 @@ def test_norm_rope(gpu, L, D, R):
     for t in (qo, ko):
         for rows in t[0, 0].split(1 << 24):
             assert (rows != 0).any(-1).all()
+
+
+@pytest.mark.parametrize("top", [0, 1, 2])
+def test_token_logprobs(gpu, top):
+    """A workgroup a row, 2^24 + 5 rows of three logits: rows all along the call
+    as on their own."""
+    from dropkv_amd import ops
+    N, V = (1 << 24) + 5, 3
+    g = torch.Generator(device=gpu).manual_seed(top)
+    x = torch.randn(N, V, generator=g, device=gpu)
+    tokens = torch.randint(0, V, (N,), generator=g, device=gpu)
+    got = ops.token_logprobs(x, tokens, top=top)
+    lp = torch.log_softmax(x.double(), -1)
+    want = [lp.gather(1, tokens[:, None])[:, 0], -(lp.exp() * lp).sum(-1)]
+    ids = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top]
+    # (Values below 20 in size: a few roundings of fp32 each.)
+    for a, b in zip(got[:3], (*want, lp.gather(1, ids))):
+        assert ((a.double() - b).abs() <= 2.0 ** -24 * 64).all()
+    assert torch.equal(got.top_ids, ids)
