@@ -571,8 +571,10 @@ int dropkv_tree_commit(const dropkv_tree_commit_args* a, void* stream) {
     return fail(DROPKV_E_ARG, "N, B, H, D, capacity must be positive");
   if (a->T < 1 || a->T > dkv::kTreeMaxT)
     return fail(DROPKV_E_UNSUPPORTED, "T must be in [1, %d]", (int)dkv::kTreeMaxT);
-  if (a->D > kMaxRowElems || a->capacity > INT32_MAX || (double)a->N * (double)a->B * (double)a->H > (double)INT32_MAX)
-    return fail(DROPKV_E_UNSUPPORTED, "D, capacity or N*B*H too large");
+  if (a->D > kMaxRowElems || a->capacity > INT32_MAX) return fail(DROPKV_E_UNSUPPORTED, "D or capacity too large");
+  // (A workgroup of 256 each, and a grid holds fewer than 2^32 work-items.)
+  if ((double)a->N * (double)a->B * (double)a->H >= (double)(1 << 24))
+    return fail(DROPKV_E_UNSUPPORTED, "N*B*H too large: it must be below %d", 1 << 24);
   if (a->p_sb != 0 && a->p_sb < a->T) return fail(DROPKV_E_ARG, "p_sb must be 0 or at least T");
   if (a->n_s[0] < 0 || a->n_s[1] < 0) return fail(DROPKV_E_ARG, "strides of n_rows must not be negative");
   timing_start(static_cast<hipStream_t>(stream));

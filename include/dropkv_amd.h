@@ -381,7 +381,7 @@ int dropkv_tree_attention(const dropkv_tree_attention_args* args, void* stream);
  * Row path[i] of k_new / v_new goes to row n + i of its cache, bit for bit; rows
  * that would lie beyond the capacity (and all of a negative n) are left out.
  * n_rows is not advanced.  The drafted rows must not lie in the buffers.
- * 1 <= T <= 256; elem_bytes 2 or 4. */
+ * 1 <= T <= 256; D <= 4096; N * B * H < 2^24; elem_bytes 2 or 4. */
 typedef struct {
   const int64_t* tokens;
   const int32_t* parents;
