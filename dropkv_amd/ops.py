@@ -14,6 +14,7 @@ import threading
 from typing import NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 
@@ -458,10 +459,20 @@ def _device_index(name: str, *ts) -> int:
     return index
 
 
+def _differentiating() -> bool:
+    """Gradients are recorded, or tangents carried (which no_grad leaves on)."""
+    return torch.is_grad_enabled() or _forward_ad._current_level >= 0
+
+
 def _no_grad(name: str, *ts) -> None:
+    backward, forward = torch.is_grad_enabled(), _forward_ad._current_level >= 0
     for t in ts:
-        if t is not None and t.requires_grad:
+        if t is None:
+            continue
+        if backward and t.requires_grad:
             raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+        if forward and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no gradient: it takes no tensors with a tangent")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -499,7 +510,7 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     is zeros.  The buffers are not
     written: ``tree_commit`` stores the rows of the tokens that stand."""
     index = _device_index("tree_attention", q, k_new, v_new, k_cache, v_cache, n_rows, out, workspace, mask)
-    if torch.is_grad_enabled():
+    if _differentiating():
         _no_grad("tree_attention", q, k_new, v_new, k_cache, v_cache, out)
     dtype = q.dtype
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
@@ -575,7 +586,7 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tenso
     int32)``.  ``n_rows`` is not advanced.  The drafted rows must not lie in the
     buffers themselves."""
     index = _device_index("tree_commit", tokens, parents, choice, k_new, v_new, k_cache, v_cache, n_rows)
-    if torch.is_grad_enabled():
+    if _differentiating():
         _no_grad("tree_commit", k_new, v_new, k_cache, v_cache)
     tshape = tokens.shape
     if len(tshape) != 2 or choice.shape != tshape or not tokens.dtype is choice.dtype is torch.int64:
@@ -646,7 +657,7 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     (``k_buf[:, :, n:n + L]``), or the inputs themselves, and are new tensors
     otherwise.  Returns ``(q_out, k_out)``, or ``(q_out, k_out, v_out)``."""
     index = _device_index("norm_rope", q, k, cos, sin, positions, q_weight, k_weight, v, q_out, k_out, v_out)
-    if torch.is_grad_enabled():
+    if _differentiating():
         _no_grad("norm_rope", q, k, v, cos, sin, q_weight, k_weight, q_out, k_out, v_out)
     dtype, cdtype = q.dtype, cos.dtype
     if dtype not in _DTYPE_CODE or k.dtype is not dtype or (v is not None and v.dtype is not dtype):
@@ -740,7 +751,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     int64: 0 comes out where it is negative, NaN where it is V or more.  The top
     tokens come largest first, the lowest id first among equals."""
     index = _device_index("token_logprobs", logits, tokens)
-    if torch.is_grad_enabled():
+    if _differentiating():
         _no_grad("token_logprobs", logits)
     dtype, shape, device = logits.dtype, logits.shape, logits.device
     if dtype not in _DTYPE_CODE:
