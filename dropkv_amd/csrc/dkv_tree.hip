@@ -95,6 +95,12 @@ __device__ __forceinline__ typename Elem<T>::v8 tree_load8(const T* p) {
   return __builtin_bit_cast(typename Elem<T>::v8, *reinterpret_cast<const Raw*>(p));
 }
 
+// Beyond 2^22 (in powers of two) a scaled logit's fraction is lost, and the scaled
+// maximum, rounded, may lie below the logit it stands for by more than P has room
+// for: the weights are then taken from differences of the logits themselves
+// (exact where they are near) and scaled after.  Below, by one fma.
+constexpr float kTreeFar = 4194304.f;
+
 // Lane i's value and lane i ^ 16's (32's), the larger; NaN where either is.
 __device__ __forceinline__ float maximum_xor16(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -298,7 +304,10 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) qop[kk] = tree_load8(qr + 32 * kk + 8 * lg);
 
-  float m = -__FLT_MAX__, lsum = 0.f;  // (finite, so that logits of -inf get no weight)
+  // The running maximum of the logits, and times the scale (that one finite, so
+  // that logits of -inf get no weight).
+  float raw = -INFINITY, m = -__FLT_MAX__, lsum = 0.f;
+  bool far = false;  // (of any of the wave's rows)
   f32x4 s[2], o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -325,9 +334,26 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
       s[e / 4][e % 4] = x;
       tmax = __builtin_elementwise_maximum(tmax, x);
     }
-    const float mnew = fmaxf(m, max_xor32(max_xor16(tmax)) * a.scale_log2);
-    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-    const float ref = mnew - kPBias<T>;
+    tmax = max_xor32(max_xor16(tmax));
+    const bool turn = tmax > raw;
+    float ref = m - kPBias<T>;
+    if (wave_any(turn) || far) {
+      const float mnew = turn ? fmaxf(tmax * a.scale_log2, -__FLT_MAX__) : m;
+      const float by = fabsf(mnew) < kTreeFar ? m - mnew : (raw - tmax) * a.scale_log2;
+      const float alpha = turn ? __builtin_amdgcn_exp2f(by) : 1.f;
+      lsum *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      m = mnew;
+      raw = turn ? tmax : raw;
+      ref = m - kPBias<T>;
+      far = wave_any(fabsf(m) >= kTreeFar);
+      if (far) {
+        ref = -kPBias<T>;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e / 4][e % 4] -= fmaxf(raw, -__FLT_MAX__);
+      }
+    }
     float psum = 0.f;
     v8 phi, plo;
 #pragma unroll
@@ -337,13 +363,7 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
       phi[e] = static_cast<T>(x);
       plo[e] = static_cast<T>(x - static_cast<float>(phi[e]));
     }
-    lsum = fmaf(lsum, alpha, psum);
-    const bool turn = mnew != m;
-    m = mnew;
-    if (wave_any(turn)) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-    }
+    lsum += psum;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       typedef short s4 __attribute__((ext_vector_type(4)));
@@ -508,11 +528,15 @@ __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
   v8 ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = static_cast<T>(1.f);
-  float m[QB];
+  // The reference of the weights, and times the scale (that one finite, so that
+  // logits of -inf get no weight).
+  float raw[QB], m[QB];
+  bool far = false;           // (of any of the wave's rows)
   f32x4 lsum[QB], o[QB][DT];  // (each of lsum's values is the whole sum of row li)
 #pragma unroll
   for (int x = 0; x < QB; ++x) {
-    m[x] = -__FLT_MAX__;  // (finite, so that logits of -inf get no weight)
+    raw[x] = -INFINITY;
+    m[x] = -__FLT_MAX__;
     lsum[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -538,7 +562,7 @@ __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
         for (int x = 0; x < QB; ++x) s[x][i] = Elem<T>::mfma(kop, qop[x][kk], s[x][i]);
       }
     }
-    float alpha[QB], ref[QB];
+    float top[QB], ref[QB];
     bool turn = false;
 #pragma unroll
     for (int x = 0; x < QB; ++x) {
@@ -550,19 +574,34 @@ __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
       float tmax = s[x][0][0];
 #pragma unroll
       for (int e = 1; e < 8 * kSub; ++e) tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
-      tmax = maximum_xor32(maximum_xor16(tmax)) * a.scale_log2;
-      const float mnew = tmax > m[x] + kPRise<T> ? tmax : m[x];
-      alpha[x] = __builtin_amdgcn_exp2f(m[x] - mnew);
-      turn |= mnew != m[x];
-      m[x] = mnew;
-      ref[x] = mnew - kPBias<T>;
+      top[x] = maximum_xor32(maximum_xor16(tmax));
+      turn |= (top[x] - raw[x]) * a.scale_log2 > kPRise<T>;
+      ref[x] = m[x] - kPBias<T>;
     }
-    if (wave_any(turn)) {
+    if (wave_any(turn) || far) {
+      bool beyond = false;
 #pragma unroll
       for (int x = 0; x < QB; ++x) {
-        lsum[x] *= alpha[x];
+        const float rise = (top[x] - raw[x]) * a.scale_log2;
+        const bool up = rise > kPRise<T>;
+        const float mnew = up ? fmaxf(top[x] * a.scale_log2, -__FLT_MAX__) : m[x];
+        const float alpha = up ? __builtin_amdgcn_exp2f(fabsf(mnew) < kTreeFar ? m[x] - mnew : -rise) : 1.f;
+        lsum[x] *= alpha;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha[x];
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
+        m[x] = mnew;
+        raw[x] = up ? top[x] : raw[x];
+        ref[x] = m[x] - kPBias<T>;
+        beyond |= fabsf(m[x]) >= kTreeFar;
+      }
+      far = wave_any(beyond);
+      if (far) {
+#pragma unroll
+        for (int x = 0; x < QB; ++x) {
+          ref[x] = -kPBias<T>;
+#pragma unroll
+          for (int e = 0; e < 8 * kSub; ++e) s[x][e / 4][e % 4] -= fmaxf(raw[x], -__FLT_MAX__);
+        }
       }
     }
 #pragma unroll

@@ -332,7 +332,8 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  *            chain).  Every token sees all stored rows.
  *   out      [B, T, Hq, D], strides {batch, token, head}, D contiguous; it and the
  *            workspace overlap no input
- * out = softmax(scale q K^T) V over the keys seen; a row that sees none, or none
+ * out = softmax(scale q K^T) V over the keys seen (products, and times 1.45 scale,
+ * within fp32's range); a row that sees none, or none
  * whose logit is above -inf, comes out as zeros.  Values and keys that a row
  * does not see do not reach it, also where they are not finite; a value that it
  * sees and that is not finite makes that element of it inf or NaN.
