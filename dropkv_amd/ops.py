@@ -553,6 +553,8 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
         if nbytes == 0:
             raise RuntimeError("tree_attention: unsupported geometry")
         workspace = _stream_workspace(nbytes, q.device)
+    elif not workspace.is_contiguous():
+        raise RuntimeError("tree_attention: the workspace must be contiguous")
     q_b, q_h, q_t, q_d = q.stride()
     if q_d != 1:
         q_b, q_h, q_t, _ = (q := q.contiguous()).stride()
