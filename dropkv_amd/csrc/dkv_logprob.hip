@@ -72,8 +72,8 @@ __device__ __forceinline__ void stat_to(Stat& a, float M) {
   a.m = M;
 }
 
-// (-0 and 0 are equals.)
-__device__ __forceinline__ uint32_t lp_order(float x) { return x != x ? 0xffffffffu : float_key(x + 0.f); }
+// (-0 and 0 are equals: float_key sees to it.)
+__device__ __forceinline__ uint32_t lp_order(float x) { return x != x ? 0xffffffffu : float_key(x); }
 __device__ __forceinline__ uint64_t lp_key(uint32_t order, int i) {  // NaN above all, as in torch's topk
   return ((uint64_t)order << 32) | (0xffffffffu - (uint32_t)i);
 }
