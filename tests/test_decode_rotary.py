@@ -15,55 +15,14 @@ pytest.importorskip("transformers")
 from transformers import DynamicCache  # noqa: E402
 from transformers.models.qwen2 import modeling_qwen2  # noqa: E402
 
-from dropkv_amd import decode, ops  # noqa: E402
+import cpu_ops  # noqa: E402
+from cpu_ops import ROTARY as ORIG  # noqa: E402
+from dropkv_amd import decode  # noqa: E402
 from dropkv_amd.e2e_qwen2 import build_model, make_config, random_prompt  # noqa: E402
 from dropkv_amd.hf_query import query_capture, take_captured_query  # noqa: E402
 
 TINY = dict(vocab_size=200, hidden_size=256, intermediate_size=256, num_hidden_layers=3,
             num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512)
-ORIG = modeling_qwen2.apply_rotary_pos_emb
-
-
-def norm_rope(q, k, cos, sin, v=None, k_out=None, v_out=None):
-    q, k = ORIG(q, k, cos, sin)
-    k_out.copy_(k)
-    v_out.copy_(v)
-    return q, k_out, v_out
-
-
-def tree_attention(q, k_new, v_new, k_cache, v_cache, n_rows, scale, workspace=None, mask=None):
-    B, Hq, T, D = q.shape
-    out = torch.zeros(B, T, Hq, D)
-    for b in range(B):
-        n = int(n_rows[b])
-        seen = torch.ones(T, T, dtype=torch.bool).tril() if mask is None else mask[b]
-        seen = torch.cat([torch.ones(T, n, dtype=torch.bool), seen], dim=-1)
-        for h in range(Hq):
-            g = h * k_cache.shape[1] // Hq
-            k, v = torch.cat([k_cache[b, g, :n], k_new[b, g]]), torch.cat([v_cache[b, g, :n], v_new[b, g]])
-            out[b, :, h] = (q[b, h] @ k.t() * scale).masked_fill(~seen, -torch.inf).softmax(-1) @ v
-    return out
-
-
-def token_logprobs(logits, top=1):
-    lp = logits.log_softmax(-1).max(-1, keepdim=True)
-    return ops.TokenLogprobs(None, None, lp.values, lp.indices)
-
-
-def tree_commit(tokens, parents, choice, k_new, v_new, k_cache, v_cache, n_rows):
-    B, T = tokens.shape
-    path = torch.full((B, T), -1, dtype=torch.int32)
-    for b in range(B):
-        nodes = [0]
-        for i in range(1, T):
-            if int(parents[b, i]) == nodes[-1] and tokens[b, i] == choice[b, nodes[-1]]:
-                nodes.append(i)
-        path[b, :len(nodes)] = torch.tensor(nodes, dtype=torch.int32)
-        for l in range(len(k_cache)):
-            n = int(n_rows[l, b])
-            k_cache[l, b, :, n:n + len(nodes)] = k_new[l, b][:, nodes]
-            v_cache[l, b, :, n:n + len(nodes)] = v_new[l, b][:, nodes]
-    return path, (path >= 0).sum(-1).int()
 
 
 @pytest.fixture(scope="module")
@@ -75,9 +34,7 @@ def tiny():
 @pytest.fixture
 def decoder(tiny, monkeypatch):
     """A decoder of chains of four on a prompt of 20 rows."""
-    for fn in (norm_rope, tree_attention, token_logprobs, tree_commit):
-        monkeypatch.setattr(ops, fn.__name__, fn)
-    monkeypatch.setattr(ops, "tree_workspace", lambda *a: torch.empty(1, dtype=torch.uint8))
+    cpu_ops.install(monkeypatch)
     cfg, model = tiny
     cache = DynamicCache(config=cfg)
     with torch.no_grad():
