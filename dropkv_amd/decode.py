@@ -53,6 +53,30 @@ def _decode_attention(module, query, key, value, attention_mask=None, scaling=No
     return out, None
 
 
+# Configurations whose attention is the decoders' at the moment: by id, how many
+# forwards need it, and what it was.  The last one out puts that back, in whatever
+# order threads come and go.
+_attn_users: dict = {}
+_attn_lock = threading.Lock()
+
+
+@contextlib.contextmanager
+def _own_attention(cfg):
+    with _attn_lock:
+        use = _attn_users.setdefault(id(cfg), [0, cfg._attn_implementation])
+        use[0] += 1
+        if use[0] == 1:
+            cfg._attn_implementation = ATTN_NAME
+    try:
+        yield
+    finally:
+        with _attn_lock:
+            use[0] -= 1
+            if use[0] == 0:
+                cfg._attn_implementation = use[1]
+                del _attn_users[id(cfg)]
+
+
 def _register():
     from transformers import AttentionInterface
     if ATTN_NAME not in AttentionInterface._global_mapping:
@@ -169,16 +193,14 @@ class CompressedDecoder:
 
     @contextlib.contextmanager
     def _active(self):
-        cfg = self.model.config
-        prev_impl, prev_dec = cfg._attn_implementation, getattr(_active, "decoder", None)
-        cfg._attn_implementation = ATTN_NAME
+        prev = getattr(_active, "decoder", None)
         _active.decoder = self
         try:
-            with rotary_deferral(self._defer) if self.tree_size else contextlib.nullcontext():
+            with _own_attention(self.model.config), (
+                    rotary_deferral(self._defer) if self.tree_size else contextlib.nullcontext()):
                 yield
         finally:
-            cfg._attn_implementation = prev_impl
-            _active.decoder = prev_dec
+            _active.decoder = prev
             self._angles = None
 
     def _defer(self, cos, sin, *args, **kwargs) -> bool:

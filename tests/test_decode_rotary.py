@@ -153,3 +153,55 @@ def test_a_layer_that_rotates_by_itself(tiny, decoder, monkeypatch, own):
         for h in handles:
             h.remove()
     assert modeling_qwen2.apply_rotary_pos_emb is ORIG
+
+
+@pytest.mark.parametrize("second", ["verify", "plain step"])
+def test_two_decoders_of_one_model_in_two_threads(tiny, decoder, second):
+    """One thread's forward ends in the middle of the other's, whose layers go on
+    as they began; afterwards the model is as it was."""
+    cfg, model = tiny
+    before = cfg._attn_implementation
+
+    def run(dec):
+        return dec.verify(DRAFTS).logits if dec.tree_size else dec.step(DRAFTS[:, :1])
+
+    def make():
+        dec = decoder()
+        if second == "verify":
+            return dec
+        cache = SimpleNamespace(layers=[SimpleNamespace(keys=k[:, :, :20], values=v[:, :, :20])
+                                        for k, v in zip(dec.k_buf, dec.v_buf)], get_seq_length=lambda: 20)
+        return decode.CompressedDecoder(model, cache, max_new_tokens=16, use_graph=False)
+
+    want = [run(decoder()), run(make())]
+    first, other, got = decoder(), make(), [None, None]
+    inside, go_on = threading.Event(), threading.Event()   # the second's forward has begun; the first's is over
+    ids = {}
+
+    def wait(*a):
+        me = threading.get_ident()
+        if me == ids.get("first"):
+            assert inside.wait(30)
+        elif me == ids.get("second"):
+            inside.set()
+            assert go_on.wait(30)
+
+    handle = model.model.layers[1].register_forward_pre_hook(wait)
+
+    def in_thread(name, i, dec):
+        ids[name] = threading.get_ident()
+        got[i] = run(dec)
+
+    a = threading.Thread(target=in_thread, args=("first", 0, first))
+    b = threading.Thread(target=in_thread, args=("second", 1, other))
+    try:
+        a.start()
+        b.start()
+        a.join(60)
+        go_on.set()
+        b.join(60)
+    finally:
+        handle.remove()
+    for g, w in zip(got, want):
+        assert g is not None and torch.equal(g, w)
+    assert cfg._attn_implementation == before and modeling_qwen2.apply_rotary_pos_emb is ORIG
