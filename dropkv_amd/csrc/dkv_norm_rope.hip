@@ -12,7 +12,7 @@
 // in fp32, rounded once, at the store.
 //
 // Bound by memory: every row is read and written once (4 x 7001 tokens of 32 query
-// and 8 KV heads of 128, fp16, norms and V: 688 MB in 147 us, 4.7 TB/s, where a
+// and 8 KV heads of 128, fp16, norms and V: 688 MB in 148 to 151 us, 4.6 TB/s, where a
 // large copy reaches 4.9; 8 tokens 3.7 us, one round trip).  A lane holds 8 values
 // of the first half and their partners of the second, so that a pair never
 // leaves the lane and the norm is a reduction over the row's 4, 8 or 16 lanes, of

@@ -251,7 +251,7 @@ __device__ __forceinline__ void tree_add_odd(const TreeArgs& a, int b, int hkv, 
 // registers as the matrix operand, V through LDS for the transposing reads; the
 // next tile's loads are issued as soon as a tile's registers are consumed.
 // Bound by memory: 4 x 16 heads of 6553 rows, D = 64 (107 MB) take 19 to 20 us (5.4
-// TB/s) and 24.5 with the join.  P goes into the product in two parts, rounded and
+// TB/s) and 25 with the join.  P goes into the product in two parts, rounded and
 // remainder (the matrix cores have room here), so that the result is off by its
 // own rounding alone.
 template <typename T, int D>
@@ -447,8 +447,8 @@ __global__ void __launch_bounds__(64) tree_partial_kernel(TreeArgs a) {
 // matrix cores and the ALUs and not by memory, and P is rounded once: each weight
 // is off by at most half a step of the element type, as the output is by its own
 // rounding (4 x 64 heads of 26214 rows, 64 tokens: 333 us in two parts, 246 in
-// one, 890 TFLOP/s; 8 x 32 heads of up to 8003 rows, 27 tokens: 58 and 48, of
-// which 41 are this kernel's, 3.7 TB/s).  What bounds the one: matrix cores busy 49%
+// one, 890 TFLOP/s; 8 x 32 heads of up to 8003 rows, 27 tokens: 58 and 48.5, of
+// which 42 are this kernel's, 3.6 TB/s).  What bounds the one: matrix cores busy 49%
 // of the time and vector units 46%, hardly ever together, with two waves on a
 // SIMD; wave priorities, waves of 64 rows (388 us), and the next stage's products
 // with K beside a stage's softmax (248) did not help.

@@ -507,8 +507,10 @@ def tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_
     filled.  ``mask`` (bool, [T, T] or [B, T, T]) says which drafted token
     (second to last axis) sees which; without it they are a chain.  Returns
     ``out`` [B, T, Hq, D], which must not lie in an input; a row that sees no key
-    is zeros.  The buffers are not
-    written: ``tree_commit`` stores the rows of the tokens that stand."""
+    is zeros.  Beyond Hq / Hkv * T = 64 the weights may be rounded once to the
+    dtype before they meet the values (half a step each; below, 16 bits or
+    more).  The buffers are not written: ``tree_commit`` stores the rows of the
+    tokens that stand."""
     index = _device_index("tree_attention", q, k_new, v_new, k_cache, v_cache, n_rows, out, workspace, mask)
     if _differentiating():
         _no_grad("tree_attention", q, k_new, v_new, k_cache, v_cache, out)

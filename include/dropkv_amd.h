@@ -336,7 +336,10 @@ int dropkv_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
  * within fp32's range); a row that sees none, or none
  * whose logit is above -inf, comes out as zeros.  Values and keys that a row
  * does not see do not reach it, also where they are not finite; a value that it
- * sees and that is not finite makes that element of it inf or NaN.
+ * sees and that is not finite makes that element of it inf or NaN.  Logits,
+ * weights and sums are fp32; the weights enter the product with V in two parts of
+ * the element type (16 bits or more) up to Hq / Hkv * T = 64 rows a KV head, and may
+ * enter it rounded once to it beyond.
  * 1 <= T <= 256, bf16 / fp16, D 64 or 128, capacity * D * 2 <= 2^31,
  * B * Hq * T <= 2^24, 0 < scale < 1e37.
  * The workspace (dropkv_tree_workspace_bytes for the same geometry; other
