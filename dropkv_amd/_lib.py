@@ -17,6 +17,8 @@ LIB_PATH = os.path.join(_HERE, "libdropkv_amd.so")
 DROPKV_BF16 = 1
 DROPKV_FP16 = 2
 DROPKV_FP32 = 3
+DROPKV_INT8 = 4
+DROPKV_E4M3 = 5
 
 _c_i64 = ctypes.c_int64
 _c_vp = ctypes.c_void_p
@@ -76,6 +78,10 @@ _SIGNATURES = {
     "dropkv_tree_attention": (_c_int, [_c_char_p, _c_vp]),
     "dropkv_tree_commit": (_c_int, [_c_char_p, _c_vp]),
     "dropkv_norm_rope": (_c_int, [_c_char_p, _c_vp]),
+    "dropkv_quant_append": (_c_int, [_c_char_p, _c_vp]),
+    "dropkv_quant_read": (_c_int, [_c_char_p, _c_vp]),
+    "dropkv_quant_workspace_bytes": (_c_size, [_c_i64] * 6),
+    "dropkv_quant_attention": (_c_int, [_c_char_p, _c_vp]),
     "dropkv_token_logprobs_workspace_bytes": (_c_size, [_c_i64] * 3),
     "dropkv_token_logprobs": (_c_int, [_c_char_p, _c_vp]),
 }
@@ -94,6 +100,13 @@ ARG_FIELDS = {
     "dropkv_norm_rope": "q q_sb q_sh q_sl q_out qo_sb qo_sh qo_sl k k_sb k_sh k_sl k_out ko_sb ko_sh ko_sl v v_sb v_sh "
                         "v_sl v_out vo_sb vo_sh vo_sl q_w k_w w_dtype cos sin c_dtype c_sb c_sl positions p_sb c_rows "
                         "dtype B Hq Hkv L D R eps:d",
+    "dropkv_quant_append": "k_new kn_sn kn_sb kn_sh kn_sl v_new vn_sn vn_sb vn_sh vn_sl k v k_scale v_scale k_tail v_tail "
+                           "n_rows n_sn n_sb counts path dtype store N B H L D capacity",
+    "dropkv_quant_read": "k v k_scale v_scale k_tail v_tail n_rows n_sn n_sb k_out v_out dtype store N B H L D capacity "
+                         "row0",
+    "dropkv_quant_attention": "q q_sb q_sh q_st k_new kn_sb kn_sh kn_st v_new vn_sb vn_sh vn_st k v k_scale v_scale "
+                              "k_tail v_tail n_rows n_sb mask m_sb m_st m_sj dtype store B Hq Hkv T D capacity scale:d "
+                              "out o_sb o_st o_sh workspace workspace_bytes",
     "dropkv_token_logprobs": "logits row_stride dtype N V tokens top logprob entropy top_logprobs top_ids workspace "
                              "workspace_bytes",
 }

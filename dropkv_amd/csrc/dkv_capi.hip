@@ -91,6 +91,21 @@ int check_tree_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, i
   return DROPKV_OK;
 }
 
+int check_quant_cache(const void* k, const void* v, const void* k_scale, const void* v_scale, const void* k_tail,
+                      const void* v_tail, int64_t dtype, int64_t store, int64_t N, int64_t B, int64_t H, int64_t D,
+                      int64_t capacity) {
+  if (!k || !v || !k_scale || !v_scale || !k_tail || !v_tail) return fail(DROPKV_E_ARG, "null pointer argument");
+  if (dtype != DROPKV_BF16 && dtype != DROPKV_FP16) return fail(DROPKV_E_ARG, "dtype must be bf16 or fp16");
+  if (store != DROPKV_INT8 && store != DROPKV_E4M3) return fail(DROPKV_E_ARG, "store must be int8 or e4m3");
+  if (N < 1 || B < 1 || H < 1) return fail(DROPKV_E_ARG, "N, B, H must be positive");
+  if (!decode_head_dim_supported(D)) return fail(DROPKV_E_UNSUPPORTED, "head dim %lld not supported", (long long)D);
+  if (capacity < 64 || capacity % 64 || capacity > ((int64_t)1 << 30) / D)
+    return fail(DROPKV_E_ARG, "capacity must be a multiple of 64, capacity * D at most 2^30");
+  for (const void* p : {k, v, k_scale, v_scale, k_tail, v_tail})
+    if (!aligned16(p)) return fail(DROPKV_E_ARG, "the cache's buffers must be 16-byte aligned");
+  return DROPKV_OK;
+}
+
 // Kernel timing (dropkv_timing_*), per calling thread: the i-th kernel of
 // the most recent timed call gets events ev[2i] (start) and ev[2i+1] (stop),
 // filled by hipExtLaunchKernel with the dispatch's begin and end time stamps.
@@ -629,6 +644,65 @@ int dropkv_token_logprobs(const dropkv_token_logprobs_args* a, void* stream) {
                 (long long)a->workspace_bytes);
   timing_start(static_cast<hipStream_t>(stream));
   return hip_status(dkv::launch_token_logprobs(*a, static_cast<hipStream_t>(stream)), "dropkv_token_logprobs launch");
+}
+
+int dropkv_quant_append(const dropkv_quant_append_args* a, void* stream) {
+  (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
+  if (!a || !a->k_new || !a->v_new || !a->n_rows) return fail(DROPKV_E_ARG, "null pointer argument");
+  const int rc = check_quant_cache(a->k, a->v, a->k_scale, a->v_scale, a->k_tail, a->v_tail, a->dtype, a->store, a->N,
+                                   a->B, a->H, a->D, a->capacity);
+  if (rc) return rc;
+  if (a->n_s[0] < 0 || a->n_s[1] < 0) return fail(DROPKV_E_ARG, "strides of n_rows must not be negative");
+  if (a->L < 0 || a->L > INT32_MAX - 64) return fail(DROPKV_E_ARG, "L out of range");
+  // (A workgroup of 256 for each block, and a grid holds fewer than 2^32 work-items.)
+  if ((double)a->N * (double)a->B * (double)a->H * ((double)(a->L + 63) / 64 + 1) >= (double)(1 << 23))
+    return fail(DROPKV_E_UNSUPPORTED, "N*B*H*L too large");
+  if (a->L == 0) return DROPKV_OK;
+  timing_start(static_cast<hipStream_t>(stream));
+  return hip_status(dkv::launch_quant_append(*a, static_cast<hipStream_t>(stream)), "dropkv_quant_append launch");
+}
+
+int dropkv_quant_read(const dropkv_quant_read_args* a, void* stream) {
+  (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
+  if (!a || !a->n_rows || !a->k_out || !a->v_out) return fail(DROPKV_E_ARG, "null pointer argument");
+  const int rc = check_quant_cache(a->k, a->v, a->k_scale, a->v_scale, a->k_tail, a->v_tail, a->dtype, a->store, a->N,
+                                   a->B, a->H, a->D, a->capacity);
+  if (rc) return rc;
+  if (!aligned16(a->k_out) || !aligned16(a->v_out)) return fail(DROPKV_E_ARG, "outputs must be 16-byte aligned");
+  if (a->n_s[0] < 0 || a->n_s[1] < 0) return fail(DROPKV_E_ARG, "strides of n_rows must not be negative");
+  if (a->L < 0 || a->row0 < 0 || a->row0 > a->capacity || a->L > a->capacity - a->row0)
+    return fail(DROPKV_E_ARG, "rows outside the capacity");
+  if ((double)a->N * (double)a->B * (double)a->H * ((double)(a->L + 63) / 64 + 1) >= (double)(1 << 23))
+    return fail(DROPKV_E_UNSUPPORTED, "N*B*H*L too large");
+  if (a->L == 0) return DROPKV_OK;
+  timing_start(static_cast<hipStream_t>(stream));
+  return hip_status(dkv::launch_quant_read(*a, static_cast<hipStream_t>(stream)), "dropkv_quant_read launch");
+}
+
+size_t dropkv_quant_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t capacity) {
+  if (check_tree_shape(B, Hq, Hkv, T, D, capacity) || capacity % 64) return 0;
+  return dkv::quant_workspace_bytes(B, Hq, Hkv, D, T, capacity);
+}
+
+int dropkv_quant_attention(const dropkv_quant_attention_args* a, void* stream) {
+  (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
+  if (!a || !a->q || !a->k_new || !a->v_new || !a->n_rows || !a->out || !a->workspace)
+    return fail(DROPKV_E_ARG, "null pointer argument");
+  int rc = check_tree_shape(a->B, a->Hq, a->Hkv, a->T, a->D, a->capacity);
+  if (!rc)
+    rc = check_quant_cache(a->k, a->v, a->k_scale, a->v_scale, a->k_tail, a->v_tail, a->dtype, a->store, 1, a->B, a->Hkv,
+                           a->D, a->capacity);
+  if (rc) return rc;
+  if (a->n_sb != 0 && a->n_sb != 1) return fail(DROPKV_E_ARG, "n_sb must be 0 or 1");
+  if (!((float)a->scale > 0.f) || !((float)a->scale < 1e37f))
+    return fail(DROPKV_E_ARG, "scale must be positive and finite");
+  size_t need = 0;
+  timing_start(static_cast<hipStream_t>(stream));
+  const hipError_t e = dkv::launch_quant_attention(*a, &need, static_cast<hipStream_t>(stream));
+  if (a->workspace_bytes < 0 || (size_t)a->workspace_bytes < need)
+    return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %lld", need,
+                (long long)a->workspace_bytes);
+  return hip_status(e, "dropkv_quant_attention launch");
 }
 
 int dropkv_selftest_mfma(float* out, void* stream) {

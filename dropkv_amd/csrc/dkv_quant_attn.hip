@@ -1,0 +1,660 @@
+// Attention over a cache in 8 bits (its layout: dkv_quant_dev.h): T new tokens per
+// sequence over the stored rows and over one another under a mask, one token of a
+// decode step or a tree or chain of drafted ones.  (The reference decodes one
+// token per step over a cache in the model's type, dropkv_cache.py:609-617.)
+//
+// The g query heads of a KV head and the T tokens are its M = g T rows, as in
+// dkv_tree.hip.  A block's scales are numbers of their own, so that the stored
+// values themselves enter the products (exactly: they fit the element type):
+//   x_rj = (scale ks_b log2 e) (q_r . k8_j),  out_r = sum_b vs_b sum_j 2^(x_rj - m_r) v8_j / sum_j 2^(x_rj - m_r)
+// with j in block b, and ks, vs = 1 for the keys in 16 bits: the rows of the block
+// that is not full, and the new tokens' own.  The blocks are cut into parts,
+// dealt by the sequences' lengths; the 16-bit keys are one part more, or the last
+// one's end; a second kernel joins the parts.
+//
+// S = K Q^T and O += V^T P^T with 64 keys a step.  Row rho = 4 lg + r of key block kb
+// is key 16 lg + 4 kb + r, so that lane (li, lg) holds row li's weights of keys 16 lg
+// .. 16 lg + 15, which are those of the 16 bytes it holds of a column of V.  The
+// depth of a product is permuted alike for K and Q (bytes 16 lg + 8 h .. + 7 of 64
+// are step h's).
+#include "dkv_quant_dev.h"
+#include "dkv_tree_dev.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace dkv {
+
+struct QuantAttnArgs : TreeArgs {  // (kbuf, vbuf: the 8-bit blocks)
+  const float* ks;    // [B, Hkv, C / 64]
+  const float* vs;
+  const void* ktail;  // [B, Hkv, 128, D]
+  const void* vtail;
+};
+
+struct QuantCut {
+  static __device__ __forceinline__ int tiles(int n) { return n / kQBlock; }
+};
+
+// The wide kernel lets a row's maximum rise so far (powers of two) above the
+// reference that its weights are taken against before it turns what it has summed.
+constexpr float kQRise = 8.f;
+
+// A step of 16-bit keys: the `held` rows of the tail (rows first ..), then `fresh`
+// new ones from j0 on.
+struct Near {
+  int first, held, j0, fresh;
+};
+// Key e of it.
+template <typename T, int D>
+__device__ __forceinline__ const T* near_row(const Near& s, int e, const T* tail, const T* kn, int64_t st) {
+  const int i = min(e, s.held + s.fresh - 1);  // (past the last: its row again)
+  return i < s.held ? tail + ((s.first + i) % kQTail) * D : kn + (int64_t)(s.j0 + i - s.held) * st;
+}
+// The steps of n % 64 tail rows and T new ones: one step if they fit, else the
+// tail's first.
+__device__ __forceinline__ Near near_begin(int n, int T) {
+  const int held = n % kQBlock;
+  return Near{n - held, held, 0, held + T <= kQBlock ? T : held ? 0 : min(T, kQBlock)};
+}
+__device__ __forceinline__ bool near_next(Near* s, int T) {
+  s->j0 += s->fresh;
+  s->held = 0;
+  s->fresh = min(T - s->j0, kQBlock);
+  return s->fresh > 0;
+}
+// The keys of it that a token sees, whose word of the new ones is w.
+__device__ __forceinline__ uint64_t near_bits(const Near& s, uint64_t w) {
+  return s.held ? ((uint64_t(1) << s.held) - 1) | (s.fresh ? w << s.held : 0) : w;
+}
+
+// The V operand of eight 16-bit keys (k0 .. k0 + 7 for this lane's group) at columns
+// d0 .. d0 + 15, by two transposing reads of four keys each.
+template <typename T, int D>
+__device__ __forceinline__ typename Elem<T>::v8 near_v(const T* vt, int k0, int d0, int li, int pitch) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  const T* p = vt + (k0 + li / 4) * pitch + d0 + 4 * (li % 4);
+  const s4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
+  const s4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * pitch));
+  return __builtin_bit_cast(typename Elem<T>::v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Up to 16 rows per KV head: one wave per part.  K and V come as matrix operands
+// straight into registers, the next block's loads issued as soon as a block's
+// registers are consumed.  P goes into the product in two parts, rounded and
+// remainder.
+template <typename T, typename S, int D>
+__global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
+  typedef typename Elem<T>::v8 v8;
+  typedef Elem<__bf16>::v8 b8;
+  constexpr int KC = D / 64, DT = D / 16, CPR = D / 8, GRP = 64 / CPR;
+  constexpr int kVPitch = D + 16;  // transposing reads without bank conflicts
+  const int slot = blockIdx.x % a.P, hkv = blockIdx.x / a.P, g = a.Hq / a.Hkv;
+  const int lane = threadIdx.x, li = lane & 15, lg = lane >> 4;
+  __shared__ __attribute__((aligned(16))) T vt[kQBlock * kVPitch];
+  __shared__ uint64_t mask_words[16];  // (T <= 16 rows)
+
+  const TreePart part = tree_part<QuantCut>(a, hkv, slot, lane);
+  const int b = part.b;
+  if (b < 0) return;
+  const int64_t bh = (int64_t)b * a.Hkv + hkv;
+  const int blocks = a.C / kQBlock;
+  const uint8_t* kb = static_cast<const uint8_t*>(a.kbuf) + bh * a.C * D;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.vbuf) + bh * a.C * D;
+  // Loads at and past the part's end read zeros.
+  const rsrc_t krs = make_rsrc(kb, (uint32_t)part.t_hi * kQBlock * D), vrs = make_rsrc(vb, (uint32_t)part.t_hi * kQBlock * D);
+  const float *ksc = a.ks + bh * blocks, *vsc = a.vs + bh * blocks;
+  u32x4 kx[4][KC], vx[DT];
+  float ks, vs;
+  auto load_k = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+        kx[i][c] = buf_load16(krs, (uint32_t)(j * kQBlock + 16 * (li / 4) + 4 * i + li % 4) * D + 64u * c + 16u * lg);
+    ks = ksc[min(j, blocks - 1)];
+  };
+  auto load_v = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) vx[dt] = buf_load16(vrs, (uint32_t)j * kQBlock * D + (16 * dt + li) * kQBlock + 16u * lg);
+    vs = vsc[min(j, blocks - 1)];
+  };
+  int j = part.t_lo;
+  if (j < part.t_hi) {
+    load_k(j);
+    load_v(j);
+  }
+
+  // Row li of the KV head: query head hkv g + h, token t.
+  const bool valid = li < a.M;
+  const int h = valid ? a.div_t.div(li) : 0, t = valid ? li - h * a.T : 0;
+  v8 qop[KC][2];
+  const T* qr = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hkv * g + h) * a.q_sh + (int64_t)t * a.q_st;
+#pragma unroll
+  for (int c = 0; c < KC; ++c)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) qop[c][hf] = tree_load8(qr + 64 * c + 16 * lg + 8 * hf);
+
+  float m = -__FLT_MAX__, lsum = 0.f;  // (finite, so that logits of -inf get no weight)
+  f32x4 s[4], o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // From products to weights; `seen`: a bit for each of the lane's keys.
+  auto weigh = [&](float mul, uint32_t seen) __attribute__((always_inline)) {
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = (seen >> e) & 1 ? s[e / 4][e % 4] * mul : -INFINITY;
+      s[e / 4][e % 4] = x;
+      tmax = fmaxf(tmax, x);
+    }
+    tmax = max_xor32(max_xor16(tmax));
+    if (wave_any(tmax > m)) {
+      const float mnew = fmaxf(m, tmax), alpha = __builtin_amdgcn_exp2f(m - mnew);
+      lsum *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      m = mnew;
+    }
+    // (The difference of two rounded logits, the larger one itself among them: no
+    // weight is above 1 however large they are.)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p = __builtin_amdgcn_exp2f(s[e / 4][e % 4] - m);
+      s[e / 4][e % 4] = p;
+      lsum += p;
+    }
+  };
+
+  for (; j < part.t_hi; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) s[i] = Elem<T>::mfma(unpack8<S, T>(kx[i][c], hf), qop[c][hf], s[i]);
+    }
+    const float mul = ks * a.scale_log2, vscale = vs;
+    load_k(j + 1);
+    weigh(mul, 0xffffu);
+    b8 phi[2], plo[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = s[2 * hf + e / 4][e % 4] * vscale;
+        phi[hf][e] = static_cast<__bf16>(p);
+        plo[hf][e] = static_cast<__bf16>(p - static_cast<float>(phi[hf][e]));
+      }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const b8 vop = unpack8<S, __bf16>(vx[dt], hf);
+        o[dt] = Elem<__bf16>::mfma(vop, phi[hf], o[dt]);
+        o[dt] = Elem<__bf16>::mfma(vop, plo[hf], o[dt]);
+      }
+    load_v(j + 1);
+  }
+
+  bool odd = false;
+  if (part.tail) {
+    const int n = tree_rows(a, b);
+    const T* kt = static_cast<const T*>(a.ktail) + bh * kQTail * D;
+    const T* vtl = static_cast<const T*>(a.vtail) + bh * kQTail * D;
+    const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
+    const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
+    const int v_row = lane / CPR, v_col = 8 * (lane % CPR);
+    Near step = near_begin(n, a.T);
+#pragma unroll 1
+    do {  // (one wave: its own LDS operations stay in order)
+      v8 kop[4][KC][2], vch[kQBlock / GRP];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T* row = near_row<T, D>(step, 16 * (li / 4) + 4 * i + li % 4, kt, kn, a.kn_st);
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) kop[i][c][hf] = tree_load8(row + 64 * c + 16 * lg + 8 * hf);
+      }
+#pragma unroll
+      for (int i = 0; i < kQBlock / GRP; ++i)
+        vch[i] = tree_load8(near_row<T, D>(step, v_row + i * GRP, vtl, vn, a.vn_st) + v_col);
+      tree_mask_words<1>(a, b, step.j0, 0, lane, mask_words);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) s[i] = Elem<T>::mfma(kop[i][c][hf], qop[c][hf], s[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kQBlock / GRP; ++i) {
+        const int e = v_row + i * GRP;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (e >= step.held + step.fresh) {
+            vch[i][k] = static_cast<T>(0.f);
+          } else if (e >= step.held && not_finite<T>(vch[i][k])) {
+            odd = true;
+            vch[i][k] = static_cast<T>(0.f);
+          }
+        *reinterpret_cast<v8*>(vt + e * kVPitch + v_col) = vch[i];
+      }
+      const uint64_t bits = near_bits(step, mask_words[t]);
+      weigh(a.scale_log2, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
+      v8 phi[2], plo[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = s[2 * hf + e / 4][e % 4];
+          phi[hf][e] = static_cast<T>(p);
+          plo[hf][e] = static_cast<T>(p - static_cast<float>(phi[hf][e]));
+        }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const v8 vop = near_v<T, D>(vt, 16 * lg + 8 * hf, 16 * dt, li, kVPitch);
+          o[dt] = Elem<T>::mfma(vop, phi[hf], o[dt]);
+          o[dt] = Elem<T>::mfma(vop, plo[hf], o[dt]);
+        }
+    } while (near_next(&step, a.T));
+  }
+
+  lsum = add_xor32(add_xor16(lsum));
+  const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + li;
+  if (valid) {
+    float* po = a.part_o + base * D + 4 * lg;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[dt];
+    if (lg == 0) {
+      a.part_m[base] = m;
+      a.part_l[base] = lsum;
+    }
+  }
+  if (__builtin_expect(wave_any(odd), 0)) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    tree_add_odd<T, D, 64>(a, b, hkv, slot, 0, 16);
+  }
+}
+
+// More than 16 rows: NW waves of QB blocks of 16 rows take the same keys, so that a
+// block of K and V is read, and turned into operands, once for all of them.  LDS holds
+// the operands of a stage of 64 keys as the lanes read them, 16 bytes a lane, 1 KB a
+// product; the next stage's bytes are on their way in registers while the waves
+// compute, and go to the other of two buffers: one barrier a stage.  V's scale goes
+// into the reference of the exponent (P is 2^(x - m + log2 vs)), and is taken out of
+// the weights' sum.
+template <typename T, typename S, int D, int QB, int NW, bool LO>
+__global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a) {
+  typedef typename Elem<T>::v8 v8;
+  constexpr int KC = D / 64, DT = D / 16, NT = 64 * NW;
+  constexpr int kPieces = 64 * (4 * KC), NC = 2 * kPieces / NT;  // 16-byte pieces of a block's K (or V); per thread
+  constexpr int kOps = 4 * KC * 2;                               // operands of a stage's K (or V)
+  constexpr int kBuf = 2 * kOps * 64;                            // 16-byte places per buffer
+  static_assert(DT == 4 * KC && NC * NT == 2 * kPieces, "whole pieces per thread");
+  __shared__ u32x4 lds[2 * kBuf];
+  __shared__ uint64_t mask_words[kTreeMaxT];
+  __shared__ int odd_flag;
+
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int mc = id % a.MC, slot = (id / a.MC) % a.P, hkv = id / (a.MC * a.P), g = a.Hq / a.Hkv;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const TreePart part = tree_part<QuantCut>(a, hkv, slot, lane);
+  const int b = part.b;
+  if (b < 0) return;
+  const int64_t bh = (int64_t)b * a.Hkv + hkv;
+  const int row0 = (mc * NW + wave) * (16 * QB) + li;  // the lane's row of block 0
+
+  v8 qop[QB][KC][2];
+  int tq[QB];
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    const int row = min(row0 + 16 * x, a.M - 1);  // (rows past the last repeat it and are not stored)
+    const int h = a.div_t.div(row), t = row - h * a.T;
+    tq[x] = t;
+    const T* qr =
+        static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hkv * g + h) * a.q_sh + (int64_t)t * a.q_st;
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) qop[x][c][hf] = tree_load8(qr + 64 * c + 16 * lg + 8 * hf);
+  }
+
+  const uint8_t* kb = static_cast<const uint8_t*>(a.kbuf) + bh * a.C * D;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.vbuf) + bh * a.C * D;
+  const rsrc_t krs = make_rsrc(kb, (uint32_t)part.t_hi * kQBlock * D), vrs = make_rsrc(vb, (uint32_t)part.t_hi * kQBlock * D);
+  const int blocks = a.C / kQBlock;
+  const float *ksc = a.ks + bh * blocks, *vsc = a.vs + bh * blocks;
+
+  // Piece i of the thread: operand pair `op` of K (key block op / KC, 64 columns op %
+  // KC) or V (16 columns), for lane `lane`.
+  u32x4 piece[NC];
+  float ks, vs;
+  auto place = [&](int i, int* op) __attribute__((always_inline)) {
+    const int f = (tid + i * NT) / 64;
+    *op = f % (4 * KC);
+    return f >= 4 * KC;
+  };
+  auto fetch = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      int op;
+      if (place(i, &op))
+        piece[i] = buf_load16(vrs, (uint32_t)j * kQBlock * D + (16 * op + li) * kQBlock + 16u * lg);
+      else
+        piece[i] = buf_load16(krs, (uint32_t)(j * kQBlock + 16 * (li / 4) + 4 * (op / KC) + li % 4) * D + 64u * (op % KC) + 16u * lg);
+    }
+    ks = ksc[min(j, blocks - 1)];
+    vs = vsc[min(j, blocks - 1)];
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      int op;
+      const bool v = place(i, &op);
+      u32x4* to = lds + buf * kBuf + ((v ? kOps : 0) + 2 * op) * 64 + lane;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        to[64 * hf] = v ? __builtin_bit_cast(u32x4, unpack8<S, __bf16>(piece[i], hf))
+                        : __builtin_bit_cast(u32x4, unpack8<S, T>(piece[i], hf));
+    }
+  };
+
+  // The reference of the weights (finite, so that logits of -inf get no weight), and
+  // the whole sum of row li.
+  float m[QB], lsum[QB];
+  f32x4 o[QB][DT];
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    m[x] = -__FLT_MAX__;
+    lsum[x] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // The stage in buffer `buf`: V's operands of type VT, the logits times `mul`, the
+  // weights times vscale; with `masked` only keys of see_bits.
+  uint32_t see_bits[QB];
+  auto compute = [&](int buf, float mul, float vscale, auto masked, auto vzero) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked)::value;
+    typedef decltype(vzero) VT;
+    typedef typename Elem<VT>::v8 vv8;
+    const u32x4* kt = lds + buf * kBuf + lane;
+    const u32x4* vt = kt + kOps * 64;
+    f32x4 s[QB][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int x = 0; x < QB; ++x) s[x][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2 * KC; ++c) {
+        const v8 kop = bitcast_u4<v8>(kt[(2 * KC * i + c) * 64]);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) s[x][i] = Elem<T>::mfma(kop, qop[x][c / 2][c % 2], s[x][i]);
+      }
+    }
+    float top[QB];
+    bool turn = false;
+#pragma unroll
+    for (int x = 0; x < QB; ++x) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[x][e / 4][e % 4] *= mul;
+        if (kMasked) s[x][e / 4][e % 4] = (see_bits[x] >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
+      }
+      float tmax = s[x][0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, s[x][e / 4][e % 4]);
+      top[x] = max_xor32(max_xor16(tmax));
+      turn |= top[x] - m[x] > kQRise;
+    }
+    if (wave_any(turn)) {
+#pragma unroll
+      for (int x = 0; x < QB; ++x) {
+        const float mnew = top[x] - m[x] > kQRise ? top[x] : m[x], alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
+        lsum[x] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
+        m[x] = mnew;
+      }
+    }
+    // (A block of zeros has no scale: any will do.)
+    const float fold = vscale == 0.f ? 1.f : vscale, up = __builtin_amdgcn_logf(fold), down = 1.f / fold;
+    f32x4 sum[QB];
+#pragma unroll
+    for (int x = 0; x < QB; ++x) sum[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    vv8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = static_cast<VT>(1.f);
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      vv8 phi[QB], plo[LO ? QB : 1];
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = __builtin_amdgcn_exp2f((s[x][2 * hf + e / 4][e % 4] - m[x]) + up);
+          phi[x][e] = static_cast<VT>(p);
+          if (LO) plo[x][e] = static_cast<VT>(p - static_cast<float>(phi[x][e]));
+        }
+#pragma unroll
+      for (int x = 0; x < QB; ++x) {
+        sum[x] = Elem<VT>::mfma(ones, phi[x], sum[x]);
+        if (LO) sum[x] = Elem<VT>::mfma(ones, plo[x], sum[x]);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const vv8 vop = bitcast_u4<vv8>(vt[(2 * dt + hf) * 64]);
+#pragma unroll
+        for (int x = 0; x < QB; ++x) {
+          o[x][dt] = Elem<VT>::mfma(vop, phi[x], o[x][dt]);
+          if (LO) o[x][dt] = Elem<VT>::mfma(vop, plo[x], o[x][dt]);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < QB; ++x) lsum[x] = fmaf(sum[x][0], down, lsum[x]);
+  };
+
+  if (tid == 0) odd_flag = 0;
+  int buf = 0, j = part.t_lo;
+  if (j < part.t_hi) {
+    fetch(j);
+    float mul = ks * a.scale_log2, vscale = vs;
+    put(0);
+    for (; j < part.t_hi; ++j) {
+      fetch(j + 1);
+      __syncthreads();
+      compute(buf, mul, vscale, std::false_type{}, __bf16{});
+      buf ^= 1;
+      mul = ks * a.scale_log2;
+      vscale = vs;
+      put(buf);
+    }
+  }
+  if (part.tail) {
+    const T* kt = static_cast<const T*>(a.ktail) + bh * kQTail * D;
+    const T* vtl = static_cast<const T*>(a.vtail) + bh * kQTail * D;
+    const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
+    const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
+    Near step = near_begin(tree_rows(a, b), a.T);
+#pragma unroll 1
+    do {
+      __syncthreads();  // (the words' and the buffer's last readers are done)
+      tree_mask_words<NW>(a, b, step.j0, wave, lane, mask_words);
+      // K's operands as they lie in the rows; V's eight keys of a column one by one.
+      bool odd = false;
+#pragma unroll 1
+      for (int i = 0; i < NC; ++i) {
+        int op;
+        const bool v = place(i, &op);
+        u32x4* to = lds + buf * kBuf + ((v ? kOps : 0) + 2 * op) * 64 + lane;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          v8 x;
+          if (v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int key = 16 * lg + 8 * hf + e;
+              const T y = near_row<T, D>(step, key, vtl, vn, a.vn_st)[16 * op + li];
+              const bool own = key >= step.held, past = key >= step.held + step.fresh;
+              const bool bad = own && !past && not_finite<T>(y);
+              odd |= bad;
+              x[e] = past || bad ? static_cast<T>(0.f) : y;
+            }
+          } else {
+            x = tree_load8(near_row<T, D>(step, 16 * (li / 4) + 4 * (op / KC) + li % 4, kt, kn, a.kn_st) +
+                           64 * (op % KC) + 16 * lg + 8 * hf);
+          }
+          to[64 * hf] = __builtin_bit_cast(u32x4, x);
+        }
+      }
+      if (odd) odd_flag = 1;
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+        see_bits[x] = (uint32_t)(near_bits(step, mask_words[tq[x]]) >> (16 * lg)) & 0xffffu;
+      compute(buf, a.scale_log2, 1.f, std::true_type{}, T{});
+    } while (near_next(&step, a.T));
+  }
+
+#pragma unroll
+  for (int x = 0; x < QB; ++x) {
+    const int row = row0 + 16 * x;
+    if (row >= a.M) continue;
+    if (a.direct) {
+      const int h = a.div_t.div(row), t = row - h * a.T;
+      T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(hkv * g + h) * a.o_sh;
+      const float l = lsum[x], inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          out[16 * dt + 4 * lg + r] = static_cast<T>(l == 0.f ? 0.f : o[x][dt][r] * inv);
+      continue;
+    }
+    const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + row;
+    const rsrc_t prs = make_rsrc(a.part_o + (base - 16 * x - li) * D, (16 * x + 16) * D * 4u);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) st_dev16(prs, ((16 * x + li) * D + 16 * dt + 4 * lg) * 4u, o[x][dt]);
+    if (lg == 0) {
+      st_dev(a.part_m + base, m[x]);
+      st_dev(a.part_l + base, lsum[x]);
+    }
+  }
+  if (part.tail && __builtin_expect(odd_flag != 0, 0)) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    tree_add_odd<T, D, NT>(a, b, hkv, slot, mc * NW * 16 * QB, NW * 16 * QB);
+  }
+}
+
+// How a call is cut: rows per workgroup (16: one wave), parts of the cache per
+// sequence, and whether the 16-bit keys are parts of their own.
+struct QuantPlan {
+  int M, rows_wg, MC, S, P, apart;
+  size_t rows, bytes;
+};
+
+static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C) {
+  QuantPlan p;
+  p.M = (int)(Hq / Hkv * T);
+  const int64_t heads = B * Hkv, blocks = C / kQBlock;
+  p.rows_wg = p.M <= 16 ? 16 : p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256;
+  p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
+  const int64_t want = (p.rows_wg == 16 ? 1024 : 512) / (heads * p.MC);
+  p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, kTreeMaxSplits, blocks}));
+  p.apart = p.rows_wg <= 64 || heads * p.MC * p.S < 192;
+  p.P = (int)(B * (p.S + p.apart));
+  p.rows = (size_t)Hkv * p.P * p.M;
+  p.bytes = kSyncBytes + kTreeDealBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
+  return p;
+}
+size_t quant_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C) {
+  return quant_plan(B, Hq, Hkv, D, T, C).bytes;
+}
+
+template <typename T, typename S, int D>
+static hipError_t launch_quant_t(const QuantAttnArgs& a, int rows_wg, hipStream_t st) {
+  // fp16 output asks for more than P rounded to bf16.
+  constexpr bool kLo = std::is_same<T, _Float16>::value;
+  const dim3 grid(a.Hkv * a.P * a.MC);
+  if (rows_wg == 16)
+    launch((quant_narrow_kernel<T, S, D>), grid, dim3(64), 0, st, a);
+  else if (rows_wg == 64)
+    launch((quant_wide_kernel<T, S, D, 1, 4, true>), grid, dim3(256), 0, st, a);
+  else if (rows_wg == 128)
+    launch((quant_wide_kernel<T, S, D, 2, 4, kLo>), grid, dim3(256), 0, st, a);
+  else
+    launch((quant_wide_kernel<T, S, D, 2, 8, kLo>), grid, dim3(512), 0, st, a);
+  if (!a.direct)
+    launch((tree_merge_kernel<T, D>), dim3((a.B * a.Hkv * a.M + 3) / 4), dim3(256), 0, st, static_cast<const TreeArgs&>(a));
+  return hipGetLastError();
+}
+
+hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* need, hipStream_t st) {
+  const QuantPlan pl = quant_plan(p.B, p.Hq, p.Hkv, p.D, p.T, p.capacity);
+  *need = pl.bytes;
+  if (p.workspace_bytes < 0 || (size_t)p.workspace_bytes < pl.bytes) return hipSuccess;  // (the caller says so)
+  QuantAttnArgs a{};
+  a.q = p.q;
+  a.q_sb = p.q_s[0];
+  a.q_sh = p.q_s[1];
+  a.q_st = p.q_s[2];
+  a.kn = p.k_new;
+  a.vn = p.v_new;
+  a.kn_sb = p.kn_s[0];
+  a.kn_sh = p.kn_s[1];
+  a.kn_st = p.kn_s[2];
+  a.vn_sb = p.vn_s[0];
+  a.vn_sh = p.vn_s[1];
+  a.vn_st = p.vn_s[2];
+  a.kbuf = p.k;
+  a.vbuf = p.v;
+  a.ks = p.k_scale;
+  a.vs = p.v_scale;
+  a.ktail = p.k_tail;
+  a.vtail = p.v_tail;
+  a.n_rows = p.n_rows;
+  a.n_sb = (int)p.n_sb;
+  a.mask = static_cast<const uint8_t*>(p.mask);
+  a.m_sb = p.m_s[0];
+  a.m_st = p.m_s[1];
+  a.m_sj = p.m_s[2];
+  a.B = (int)p.B;
+  a.Hq = (int)p.Hq;
+  a.Hkv = (int)p.Hkv;
+  a.D = (int)p.D;
+  a.T = (int)p.T;
+  a.C = (int)p.capacity;
+  a.M = pl.M;
+  a.MC = pl.MC;
+  a.S = pl.S;
+  a.P = pl.P;
+  a.apart = pl.apart;
+  a.tail_tiles = pl.apart ? 0 : 3 + (a.T + kQBlock - 1) / kQBlock;
+  a.ragged = p.n_sb != 0 && p.B > 1 && p.B <= kTreeRaggedB && pl.S > 1;
+  a.direct = pl.S == 1 && !pl.apart;
+  a.div_t = Div::of(a.T);
+  a.scale_log2 = (float)p.scale * 1.4426950408889634f;
+  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
+  a.deal = reinterpret_cast<int*>(ws + kSyncBytes);
+  a.part_m = reinterpret_cast<float*>(ws + kSyncBytes + kTreeDealBytes);
+  a.part_l = a.part_m + pl.rows;
+  a.part_o = a.part_m + ((2 * pl.rows + 3) & ~(size_t)3);
+  a.out = p.out;
+  a.o_sb = p.o_s[0];
+  a.o_st = p.o_s[1];
+  a.o_sh = p.o_s[2];
+  return quant_types(p.dtype, p.store, p.D, [&](auto t, auto s, auto d) {
+    return launch_quant_t<decltype(t), decltype(s), decltype(d)::value>(a, pl.rows_wg, st);
+  });
+}
+
+}  // namespace dkv

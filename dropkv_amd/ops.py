@@ -632,6 +632,237 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tenso
     return path, accepted
 
 
+# --- a cache in 8 bits ----------------------------------------------------------
+
+QUANT_BLOCK = 64  # rows of a block, which has one scale for K and one for V
+
+_STORE_CODE = {torch.int8: _lib.DROPKV_INT8, torch.float8_e4m3fn: _lib.DROPKV_E4M3}
+
+
+class QuantCache(NamedTuple):
+    """Buffers of a cache in 8 bits (``quant_cache``).  A full block of 64 rows holds
+    ``q`` in ``k`` (row-major) and ``v`` (transposed within the block) standing for
+    ``scale * q``; the rows of the last block, while it is not full, are in the
+    tails, row r at ``r % 128``.  With ``layers`` there is an axis N in front."""
+
+    k: torch.Tensor        # [B, H, capacity, D] int8 or float8_e4m3fn
+    v: torch.Tensor        # [B, H, capacity / 64, D, 64]
+    k_scale: torch.Tensor  # [B, H, capacity / 64] fp32
+    v_scale: torch.Tensor
+    k_tail: torch.Tensor   # [B, H, 128, D] bf16 or fp16
+    v_tail: torch.Tensor
+
+    def layer(self, i: int) -> "QuantCache":
+        """Layer ``i`` of a cache of several (views)."""
+        if self.k.dim() != 5:
+            raise RuntimeError("the cache has no axis of layers")
+        return QuantCache(*(t[i] for t in self))
+
+
+def quant_cache(B: int, H: int, capacity: int, D: int, dtype: torch.dtype = torch.bfloat16,
+                store: torch.dtype = torch.int8, layers: Optional[int] = None, device="cuda") -> QuantCache:
+    """An empty cache for rows of ``dtype`` (bf16 or fp16), held as ``store`` (int8 or
+    float8_e4m3fn); the capacity is rounded up to whole blocks of 64 rows."""
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError("quant_cache: dtype must be bf16 or fp16")
+    if store not in _STORE_CODE:
+        raise RuntimeError("quant_cache: store must be int8 or float8_e4m3fn")
+    if D not in (64, 128):
+        raise RuntimeError("quant_cache: the head dim must be 64 or 128")
+    if B < 1 or H < 1 or capacity < 1 or (layers is not None and layers < 1):
+        raise RuntimeError("quant_cache: B, H, capacity and layers must be positive")
+    n = (capacity + QUANT_BLOCK - 1) // QUANT_BLOCK
+    if n * QUANT_BLOCK * D > 1 << 30:
+        raise RuntimeError("quant_cache: capacity * D must be at most 2^30")
+    lead = (B, H) if layers is None else (layers, B, H)
+
+    def zeros(dt, *shape):
+        if dt in _STORE_CODE:
+            return torch.zeros(*lead, *shape, dtype=torch.uint8, device=device).view(dt)
+        return torch.zeros(*lead, *shape, dtype=dt, device=device)
+
+    return QuantCache(zeros(store, n * QUANT_BLOCK, D), zeros(store, n, D, QUANT_BLOCK), zeros(torch.float32, n),
+                      zeros(torch.float32, n), zeros(dtype, 2 * QUANT_BLOCK, D), zeros(dtype, 2 * QUANT_BLOCK, D))
+
+
+def _quant_shape(name: str, c: QuantCache):
+    """(leading axes, H, capacity, D, layers or not) of a cache whose buffers fit one
+    another."""
+    kshape = c.k.shape
+    if len(kshape) != 4 and len(kshape) != 5:
+        raise RuntimeError(f"{name}: the cache's buffers must be those of quant_cache")
+    *lead, H, C, D = kshape
+    n, store, dtype = C // QUANT_BLOCK, c.k.dtype, c.k_tail.dtype
+    if (c.v.shape != (*lead, H, n, D, QUANT_BLOCK) or c.k_scale.shape != (*lead, H, n)
+            or c.v_scale.shape != c.k_scale.shape or c.k_tail.shape != (*lead, H, 2 * QUANT_BLOCK, D)
+            or c.v_tail.shape != c.k_tail.shape or C % QUANT_BLOCK or store not in _STORE_CODE
+            or c.v.dtype is not store or not c.k_scale.dtype is c.v_scale.dtype is torch.float32
+            or (dtype is not torch.bfloat16 and dtype is not torch.float16) or c.v_tail.dtype is not dtype):
+        raise RuntimeError(f"{name}: the cache's buffers must be those of quant_cache")
+    for t in c:
+        if not t.is_contiguous():
+            raise RuntimeError(f"{name}: the cache's buffers must be contiguous")
+    return lead, H, C, D, len(kshape) == 5
+
+
+def _layer_counts(name: str, n_rows: torch.Tensor, lead, layers: bool):
+    """Strides {layer, batch} of the stored rows' counts."""
+    nshape, B = n_rows.shape, lead[-1]
+    if n_rows.dtype is not torch.int32 or len(nshape) != len(lead) or nshape[-1] not in (1, B) or (
+            layers and nshape[0] != lead[0]):
+        raise RuntimeError(f"{name}: n_rows must be int32, [1] or [B], or [N, 1] or [N, B]")
+    ns = n_rows.stride()
+    return (ns[0] if layers else 0), (ns[-1] if nshape[-1] > 1 else 0)
+
+
+_QAPPEND_ARGS = _lib.ARGS["dropkv_quant_append"].pack
+
+
+def quant_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor, n_rows: torch.Tensor,
+                 path: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None) -> None:
+    """Rows k / v [B, H, L, D] (any strides; [N, B, H, L, D] for a cache of layers)
+    behind the ``n_rows`` that are stored (int32 on the device, [1] or [B], or [N,
+    1] or [N, B]; not advanced), quantised block by block as blocks fill up
+    (``dropkv_quant_append``).  ``counts`` [B] int32: so many rows of each sequence
+    (else all L); ``path`` [B, L] int32: row i is row ``path[b, i]`` (what
+    ``tree_commit`` returns).  Rows beyond the capacity are dropped.  k and v must
+    not lie in the cache's own buffers."""
+    index = _device_index("quant_append", k, v, n_rows, path, counts, *cache)
+    if _differentiating():
+        _no_grad("quant_append", k, v, *cache)
+    lead, H, C, D, layers = _quant_shape("quant_append", cache)
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != len(lead) + 3 or shape[:-2] != (*lead, H) or shape[-1] != D or v.shape != shape:
+        raise RuntimeError("quant_append: k and v must be [B, H, L, D] or [N, B, H, L, D], as the cache")
+    if dtype is not cache.k_tail.dtype or v.dtype is not dtype:
+        raise RuntimeError("quant_append: k and v must have the cache's dtype")
+    L, B = shape[-2], lead[-1]
+    n_sn, n_sb = _layer_counts("quant_append", n_rows, lead, layers)
+    if counts is not None:
+        if counts.dtype is not torch.int32 or counts.shape != (B,):
+            raise RuntimeError("quant_append: counts must be int32 [B]")
+        counts = counts.contiguous()
+    if path is not None:
+        if path.dtype is not torch.int32 or path.shape != (B, L):
+            raise RuntimeError("quant_append: path must be int32 [B, L]")
+        path = path.contiguous()
+    if not (L and B and H):
+        return
+    k, v = _rows(k), _rows(v)
+    ks, vs = k.stride(), v.stride()
+    if not layers:
+        ks, vs = (0, *ks), (0, *vs)
+    _call("dropkv_quant_append", index, _QAPPEND_ARGS(
+        k.data_ptr(), *ks[:4], v.data_ptr(), *vs[:4], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+        cache.v_scale.data_ptr(), cache.k_tail.data_ptr(), cache.v_tail.data_ptr(), n_rows.data_ptr(), n_sn, n_sb,
+        0 if counts is None else counts.data_ptr(), 0 if path is None else path.data_ptr(), _DTYPE_CODE[dtype],
+        _STORE_CODE[cache.k.dtype], lead[0] if layers else 1, B, H, L, D, C))
+
+
+_QREAD_ARGS = _lib.ARGS["dropkv_quant_read"].pack
+
+
+def quant_read(cache: QuantCache, n_rows: torch.Tensor, rows: int, first: int = 0):
+    """Rows ``first .. first + rows - 1`` of every head as new tensors ``(k, v)``
+    [B, H, rows, D] (or [N, B, H, rows, D]) of the cache's 16-bit dtype
+    (``dropkv_quant_read``); zeros behind the ``n_rows`` that are stored."""
+    index = _device_index("quant_read", n_rows, *cache)
+    if _differentiating():
+        _no_grad("quant_read", *cache)
+    lead, H, C, D, layers = _quant_shape("quant_read", cache)
+    if rows < 0 or first < 0 or first + rows > C:
+        raise RuntimeError(f"quant_read: rows must lie within the capacity of {C}")
+    n_sn, n_sb = _layer_counts("quant_read", n_rows, lead, layers)
+    k = cache.k_tail.new_empty((*lead, H, rows, D))
+    v = torch.empty_like(k)
+    if k.numel():
+        _call("dropkv_quant_read", index, _QREAD_ARGS(
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+            cache.k_tail.data_ptr(), cache.v_tail.data_ptr(), n_rows.data_ptr(), n_sn, n_sb, k.data_ptr(), v.data_ptr(),
+            _DTYPE_CODE[k.dtype], _STORE_CODE[cache.k.dtype], lead[0] if layers else 1, lead[-1], H, rows, D, C, first))
+    return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def _quant_bytes(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int) -> int:
+    return _lib.load().dropkv_quant_workspace_bytes(B, Hq, Hkv, D, T, capacity)
+
+
+def quant_workspace(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int, device) -> torch.Tensor:
+    """Workspace of ``quant_attention`` for one geometry (reusable across steps and
+    layers of that geometry, one call at a time); the capacity as in
+    ``quant_cache``."""
+    nbytes = _quant_bytes(B, Hq, Hkv, D, T, (capacity + QUANT_BLOCK - 1) // QUANT_BLOCK * QUANT_BLOCK)
+    if nbytes == 0:
+        raise RuntimeError("unsupported geometry of a cache in 8 bits")
+    return _workspace(nbytes, torch.device(device))
+
+
+_QATTN_ARGS = _lib.ARGS["dropkv_quant_attention"].pack
+
+
+def quant_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: QuantCache, n_rows: torch.Tensor,
+                    scale: float, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                    mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of T tokens per sequence (one, or drafted ones) over a cache in 8 bits
+    and over one another (``dropkv_quant_attention``): ``tree_attention`` with the
+    one layer's ``cache`` in the place of the buffers.  Returns ``out`` [B, T, Hq, D],
+    which must not lie in an input.  The cache is not written: ``quant_append``
+    stores the rows."""
+    index = _device_index("quant_attention", q, k_new, v_new, n_rows, out, workspace, mask, *cache)
+    if _differentiating():
+        _no_grad("quant_attention", q, k_new, v_new, out, *cache)
+    lead, Hkv, C, D, layers = _quant_shape("quant_attention", cache)
+    dtype, shape, kshape = q.dtype, q.shape, k_new.shape
+    if layers:
+        raise RuntimeError("quant_attention: takes one layer of the cache (cache.layer(i))")
+    if not dtype is k_new.dtype is v_new.dtype is cache.k_tail.dtype:
+        raise RuntimeError("quant_attention: q, k_new and v_new must have the cache's dtype")
+    if len(shape) != 4:
+        raise RuntimeError("quant_attention: q must be [B, Hq, T, D]")
+    B, Hq, T, qD = shape
+    if lead[0] != B or qD != D or kshape != (B, Hkv, T, D) or v_new.shape != kshape:
+        raise RuntimeError("quant_attention: q, k_new, v_new and the cache do not fit one another")
+    counts = n_rows.numel()
+    if n_rows.dtype is not torch.int32 or (counts != 1 and counts != B) or not n_rows.is_contiguous():
+        raise RuntimeError("quant_attention: n_rows must hold one int32 count, or one per sequence")
+    m_ptr = m_b = m_t = m_j = 0
+    if mask is not None:
+        mshape = mask.shape
+        if mask.dtype is not torch.bool or (mshape != (T, T) and mshape != (B, T, T)):
+            raise RuntimeError("quant_attention: mask must be bool, [T, T] or [B, T, T]")
+        m_ptr = mask.data_ptr()
+        if len(mshape) == 2:
+            m_t, m_j = mask.stride()
+        else:
+            m_b, m_t, m_j = mask.stride()
+    if out is None:
+        out = q.new_empty((B, T, Hq, D))
+    elif out.shape != (B, T, Hq, D) or out.dtype is not dtype or out.stride(3) != 1:
+        raise RuntimeError("quant_attention: out must be [B, T, Hq, D] of q's dtype, D contiguous")
+    if not (B and T and Hq):
+        return out
+    if workspace is None:
+        nbytes = _quant_bytes(B, Hq, Hkv, D, T, C)
+        if nbytes == 0:
+            raise RuntimeError("quant_attention: unsupported geometry")
+        workspace = _stream_workspace(nbytes, q.device)
+    elif not workspace.is_contiguous():
+        raise RuntimeError("quant_attention: the workspace must be contiguous")
+    q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)
+    q_b, q_h, q_t, _ = q.stride()
+    kn_b, kn_h, kn_t, _ = k_new.stride()
+    vn_b, vn_h, vn_t, _ = v_new.stride()
+    o_b, o_t, o_h, _ = out.stride()
+    _call("dropkv_quant_attention", index, _QATTN_ARGS(
+        q.data_ptr(), q_b, q_h, q_t, k_new.data_ptr(), kn_b, kn_h, kn_t, v_new.data_ptr(), vn_b, vn_h, vn_t,
+        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+        cache.k_tail.data_ptr(), cache.v_tail.data_ptr(), n_rows.data_ptr(), counts > 1, m_ptr, m_b, m_t, m_j,
+        _DTYPE_CODE[dtype], _STORE_CODE[cache.k.dtype], B, Hq, Hkv, T, D, C, scale, out.data_ptr(), o_b, o_t, o_h,
+        workspace.data_ptr(), workspace.nbytes))
+    return out
+
+
 _ROPE_ARGS = _lib.ARGS["dropkv_norm_rope"].pack
 
 

@@ -26,6 +26,8 @@ extern "C" {
 #define DROPKV_BF16 1
 #define DROPKV_FP16 2
 #define DROPKV_FP32 3  /* scoring and eviction only (not decode) */
+#define DROPKV_INT8 4  /* stored values of a cache in 8 bits */
+#define DROPKV_E4M3 5  /* likewise: 8-bit floats of 4 exponent bits, largest 448 */
 
 /* status codes */
 #define DROPKV_OK 0
@@ -473,6 +475,108 @@ typedef struct {
 } dropkv_token_logprobs_args;
 size_t dropkv_token_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top);
 int dropkv_token_logprobs(const dropkv_token_logprobs_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A cache in 8 bits.  No counterpart in the reference, whose cache keeps the
+ * model's type (dropkv_cache.py:609-620).
+ *
+ * Rows lie in blocks of 64 per (layer, batch, KV head).  A full block holds q with
+ *   a = max |x| over the block's 64 x D values,  s = a / top,  q = round(x top / a)
+ * (nearest, ties to even; top 127 for DROPKV_INT8, 448 for DROPKV_E4M3), standing
+ * for s q.  A block whose a is below 2^-100 is zeros; one that holds a value that is
+ * not finite reads as NaN.  The rows of the last block, while it is not full, are
+ * kept as they are.  Buffers (N layers, 1 where there is no such axis; capacity a
+ * multiple of 64), all contiguous and 16-byte aligned, zeros at first:
+ *   k        [N, B, H, capacity, D] bytes
+ *   v        [N, B, H, capacity / 64, D, 64] bytes: transposed within the block
+ *   k_scale, v_scale  [N, B, H, capacity / 64] fp32: s
+ *   k_tail, v_tail    [N, B, H, 128, D] of dtype: row r of the block that is not
+ *            full at r % 128
+ * dtype bf16 or fp16, D 64 or 128, capacity * D <= 2^30.
+ *
+ * dropkv_quant_append: rows behind the n that are stored.
+ *   k_new, v_new [N, B, H, L, D] of dtype: strides {layer, batch, head, row}, D
+ *            contiguous, any alignment; not in the cache's own buffers
+ *   n_rows   int32 at l * n_s[0] + b * n_s[1]; not advanced
+ *   counts   [B] int32: rows of each sequence to append (clamped to 0 .. L); NULL: L
+ *   path     [B, L] int32: row i of the append is row path[b][i] of k_new / v_new
+ *            (clamped to 0 .. L - 1; entries from counts on are not read); NULL: i
+ * Rows that would lie beyond the capacity (and all where n is negative) are left
+ * out.  Blocks that are filled up are written once, from the tail and the new
+ * rows.  The same call again, at the same n, gives the same cache as long as no
+ * more than 64 rows are appended.  N * B * H * ceil((63 + L) / 64) < 2^23. */
+typedef struct {
+  const void* k_new;
+  int64_t kn_s[4];
+  const void* v_new;
+  int64_t vn_s[4];
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  void* k_tail;
+  void* v_tail;
+  const int32_t* n_rows;
+  int64_t n_s[2];
+  const int32_t* counts;
+  const int32_t* path;
+  int64_t dtype, store, N, B, H, L, D, capacity;
+} dropkv_quant_append_args;
+int dropkv_quant_append(const dropkv_quant_append_args* args, void* stream);
+
+/* dropkv_quant_read: rows row0 .. row0 + L - 1 of every head to k_out / v_out
+ * [N, B, H, L, D] contiguous (16-byte aligned), of dtype: s q rounded once where the
+ * row's block is full, the row as it was appended where it is not, zeros from row
+ * n on.  row0 + L <= capacity. */
+typedef struct {
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  const void* k_tail;
+  const void* v_tail;
+  const int32_t* n_rows;
+  int64_t n_s[2];
+  void* k_out;
+  void* v_out;
+  int64_t dtype, store, N, B, H, L, D, capacity, row0;
+} dropkv_quant_read_args;
+int dropkv_quant_read(const dropkv_quant_read_args* args, void* stream);
+
+/* dropkv_quant_attention: dropkv_tree_attention over such a cache (one layer's):
+ * T tokens over its n rows and over one another under a mask; T = 1 is a decode
+ * step.  Arguments, masks, rows that see nothing and values that are not finite as
+ * there; the new rows are not stored (dropkv_quant_append does).  Logits, weights
+ * and sums are fp32; the stored values enter the products as they are.  The weights
+ * enter the product with V in two parts (16 bits or more) up to Hq / Hkv * T = 64
+ * rows a KV head, and for fp16; for bf16 they may enter it rounded once beyond.
+ * Values of V below 2^118.  The workspace as for dropkv_tree_attention. */
+typedef struct {
+  const void* q;
+  int64_t q_s[3];
+  const void* k_new;
+  int64_t kn_s[3];
+  const void* v_new;
+  int64_t vn_s[3];
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  const void* k_tail;
+  const void* v_tail;
+  const int32_t* n_rows;
+  int64_t n_sb;
+  const void* mask;
+  int64_t m_s[3];
+  int64_t dtype, store, B, Hq, Hkv, T, D, capacity;
+  double scale;
+  void* out;
+  int64_t o_s[3];
+  void* workspace;
+  int64_t workspace_bytes;
+} dropkv_quant_attention_args;
+size_t dropkv_quant_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t capacity);
+int dropkv_quant_attention(const dropkv_quant_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }
