@@ -18,7 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJDIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libdropkv_amd.so")
 SOURCES = ["dkv_score.hip", "dkv_generic.hip", "dkv_generic_mfma.hip", "dkv_select.hip", "dkv_compact.hip", "dkv_decode.hip",
-           "dkv_tree.hip", "dkv_quant.hip", "dkv_quant_attn.hip", "dkv_norm_rope.hip", "dkv_logprob.hip", "dkv_capi.hip"]
+           "dkv_tree.hip", "dkv_quant.hip", "dkv_quant_attn.hip", "dkv_verify.hip", "dkv_norm_rope.hip",
+           "dkv_logprob.hip", "dkv_capi.hip"]
 ARCH = os.environ.get("DROPKV_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

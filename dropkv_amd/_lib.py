@@ -82,6 +82,8 @@ _SIGNATURES = {
     "dropkv_quant_read": (_c_int, [_c_char_p, _c_vp]),
     "dropkv_quant_workspace_bytes": (_c_size, [_c_i64] * 6),
     "dropkv_quant_attention": (_c_int, [_c_char_p, _c_vp]),
+    "dropkv_verify_drafts_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int]),
+    "dropkv_verify_drafts": (_c_int, [_c_char_p, _c_vp]),
     "dropkv_token_logprobs_workspace_bytes": (_c_size, [_c_i64] * 3),
     "dropkv_token_logprobs": (_c_int, [_c_char_p, _c_vp]),
 }
@@ -107,6 +109,8 @@ ARG_FIELDS = {
     "dropkv_quant_attention": "q q_sb q_sh q_st k_new kn_sb kn_sh kn_st v_new vn_sb vn_sh vn_st k v k_scale v_scale "
                               "k_tail v_tail n_rows n_sb mask m_sb m_st m_sj dtype store B Hq Hkv T D capacity scale:d "
                               "out o_sb o_st o_sh workspace workspace_bytes",
+    "dropkv_verify_drafts": "logits x_sb x_st draft_logits y_sb y_st tokens uniforms dtype B T V temperature:d choice "
+                            "accepted logprobs workspace workspace_bytes",
     "dropkv_token_logprobs": "logits row_stride dtype N V tokens top logprob entropy top_logprobs top_ids workspace "
                              "workspace_bytes",
 }

@@ -106,6 +106,15 @@ int check_quant_cache(const void* k, const void* v, const void* k_scale, const v
   return DROPKV_OK;
 }
 
+int check_verify_shape(int64_t B, int64_t T, int64_t V) {
+  if (B < 1 || T < 1 || V < 1) return fail(DROPKV_E_ARG, "B, T, V must be positive");
+  if (T > dkv::kTreeMaxT) return fail(DROPKV_E_UNSUPPORTED, "T must be in [1, %d]", (int)dkv::kTreeMaxT);
+  if (V > kMaxLk) return fail(DROPKV_E_UNSUPPORTED, "V too large");
+  // (Up to 64 workgroups of 256 a row, and a grid holds fewer than 2^32 work-items.)
+  if (B >= (1 << 17) || B * (2 * T - 1) >= (1 << 17)) return fail(DROPKV_E_UNSUPPORTED, "B*(2*T-1) too large");
+  return DROPKV_OK;
+}
+
 // Kernel timing (dropkv_timing_*), per calling thread: the i-th kernel of
 // the most recent timed call gets events ev[2i] (start) and ev[2i+1] (stop),
 // filled by hipExtLaunchKernel with the dispatch's begin and end time stamps.
@@ -703,6 +712,29 @@ int dropkv_quant_attention(const dropkv_quant_attention_args* a, void* stream) {
     return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %lld", need,
                 (long long)a->workspace_bytes);
   return hip_status(e, "dropkv_quant_attention launch");
+}
+
+size_t dropkv_verify_drafts_workspace_bytes(int64_t B, int64_t T, int64_t V, int draft) {
+  if (check_verify_shape(B, T, V)) return 0;
+  return dkv::verify_workspace_bytes(B, T, V, draft != 0);
+}
+
+int dropkv_verify_drafts(const dropkv_verify_drafts_args* a, void* stream) {
+  (void)hipGetLastError();  // a failure left by an unrelated earlier call is not ours
+  if (!a || !a->logits || !a->tokens || !a->uniforms || !a->choice || !a->accepted || !a->logprobs || !a->workspace)
+    return fail(DROPKV_E_ARG, "null pointer argument");
+  if (a->dtype != DROPKV_BF16 && a->dtype != DROPKV_FP16 && a->dtype != DROPKV_FP32)
+    return fail(DROPKV_E_ARG, "dtype must be bf16, fp16 or fp32");
+  const int rc = check_verify_shape(a->B, a->T, a->V);
+  if (rc) return rc;
+  if (!(a->temperature > 0.) || !(1. / a->temperature < 1e30) || !(a->temperature < 1e30))
+    return fail(DROPKV_E_ARG, "temperature must be positive and finite");
+  const size_t need = dkv::verify_workspace_bytes(a->B, a->T, a->V, a->draft_logits != nullptr);
+  if (a->workspace_bytes < 0 || (size_t)a->workspace_bytes < need)
+    return fail(DROPKV_E_WORKSPACE, "workspace too small: need %zu bytes, got %lld", need,
+                (long long)a->workspace_bytes);
+  timing_start(static_cast<hipStream_t>(stream));
+  return hip_status(dkv::launch_verify_drafts(*a, static_cast<hipStream_t>(stream)), "dropkv_verify_drafts launch");
 }
 
 int dropkv_selftest_mfma(float* out, void* stream) {

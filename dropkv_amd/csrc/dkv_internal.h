@@ -157,6 +157,10 @@ hipError_t launch_quant_read(const dropkv_quant_read_args& p, hipStream_t st);
 size_t quant_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C);
 hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* need, hipStream_t st);
 
+// Drafted chains verified by sampling (dkv_verify.hip).
+size_t verify_workspace_bytes(int64_t B, int64_t T, int64_t V, bool draft);
+hipError_t launch_verify_drafts(const dropkv_verify_drafts_args& p, hipStream_t st);
+
 size_t select_workspace_bytes(int64_t rows, int64_t Lk);
 // Workspace of a layer-call: the plan's, the scores and the selection's.
 inline size_t evict_bytes(const ScorePlan& p, int64_t Lk) {

@@ -1019,6 +1019,71 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     return TokenLogprobs(logprob, entropy, top_lp, top_id)
 
 
+class DraftsVerified(NamedTuple):
+    """What ``verify_drafts`` returns."""
+
+    choice: torch.Tensor    # [B, T] int64: the token after each node that stands, then -1
+    accepted: torch.Tensor  # [B] int32: nodes that stand (1 or more), so many new tokens
+    logprobs: torch.Tensor  # [B, T] fp32: their log probabilities, then 0
+
+
+_VERIFY_ARGS = _lib.ARGS["dropkv_verify_drafts"].pack
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_bytes(B: int, T: int, V: int, draft: bool) -> int:
+    return _lib.load().dropkv_verify_drafts_workspace_bytes(B, T, V, draft)
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor,
+                  draft_logits: Optional[torch.Tensor] = None, temperature: float = 1.0) -> DraftsVerified:
+    """Which tokens of drafted chains stand, and the token after them, from given random
+    numbers, distributed as samples of the model (``dropkv_verify_drafts``).
+    ``logits`` [B, T, V] (bf16, fp16 or fp32) after each node, ``tokens`` [B, T] int64
+    the nodes' (the last token at node 0, drafted ones after it; a negative one ends
+    its chain), ``uniforms`` [B, T] fp32 in [0, 1): entry i judges node i, entry 0
+    draws the last token.  ``draft_logits`` [B, T - 1, V], of the logits' dtype: row i
+    - 1 is what node i was drawn from; without it the drafts are taken as given (a
+    lookup's).  Both are divided by ``temperature``.  ``choice`` is what
+    ``tree_commit`` takes."""
+    index = _device_index("verify_drafts", logits, tokens, uniforms, draft_logits)
+    if _differentiating():
+        _no_grad("verify_drafts", logits, uniforms, draft_logits)
+    dtype, shape = logits.dtype, logits.shape
+    if dtype not in _DTYPE_CODE:
+        raise RuntimeError("verify_drafts: logits must be bf16, fp16 or fp32")
+    if len(shape) != 3 or not (shape[1] and shape[2]):
+        raise RuntimeError("verify_drafts: logits must be [B, T, V]")
+    B, T, V = shape
+    if tokens.dtype is not torch.int64 or tokens.shape != (B, T):
+        raise RuntimeError("verify_drafts: tokens must be int64 [B, T]")
+    if uniforms.dtype is not torch.float32 or uniforms.shape != (B, T):
+        raise RuntimeError("verify_drafts: uniforms must be fp32 [B, T]")
+    if draft_logits is not None and (draft_logits.dtype is not dtype or draft_logits.shape != (B, T - 1, V)):
+        raise RuntimeError("verify_drafts: draft_logits must be [B, T - 1, V] of the logits' dtype")
+    if not 1e-30 < temperature < 1e30:
+        raise RuntimeError("verify_drafts: temperature must be positive and finite")
+    choice = torch.empty_like(tokens, memory_format=torch.contiguous_format)
+    accepted = tokens.new_empty((B,), dtype=torch.int32)
+    logprobs = torch.empty_like(uniforms, memory_format=torch.contiguous_format)
+    if B == 0:
+        return DraftsVerified(choice, accepted, logprobs)
+    tokens, uniforms, logits = tokens.contiguous(), uniforms.contiguous(), _rows(logits)
+    d_ptr = d_b = d_t = 0
+    if draft_logits is not None and T > 1:
+        draft_logits = _rows(draft_logits)
+        d_ptr, (d_b, d_t, _) = draft_logits.data_ptr(), draft_logits.stride()
+    nbytes = _verify_bytes(B, T, V, d_ptr != 0)
+    if nbytes == 0:
+        raise RuntimeError("verify_drafts: T must be at most 256, V at most 2^30, B * (2 T - 1) below 2^17")
+    ws = _stream_workspace(nbytes, logits.device)
+    x_b, x_t, _ = logits.stride()
+    _call("dropkv_verify_drafts", index, _VERIFY_ARGS(
+        logits.data_ptr(), x_b, x_t, d_ptr, d_b, d_t, tokens.data_ptr(), uniforms.data_ptr(), _DTYPE_CODE[dtype], B, T, V,
+        temperature, choice.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), ws.nbytes))
+    return DraftsVerified(choice, accepted, logprobs)
+
+
 def mfma_selftest(device="cuda") -> torch.Tensor:
     out = torch.empty(16, 16, dtype=torch.float32, device=device)
     rc = _lib.load().dropkv_selftest_mfma(out.data_ptr(), _stream(out.device))

@@ -578,6 +578,48 @@ typedef struct {
 size_t dropkv_quant_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t capacity);
 int dropkv_quant_attention(const dropkv_quant_attention_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * dropkv_verify_drafts: which tokens of a drafted chain stand, and the token after
+ * them, from given random numbers, so that the tokens are distributed as samples of
+ * the model's own.  No counterpart in the reference (one token per step,
+ * dropkv_cache.py:609-617).
+ *   logits       [B, T, V] (bf16, fp16 or fp32; strides {batch, node}, V contiguous):
+ *                after each node, node 0 being the last token
+ *   draft_logits [B, T - 1, V] of the same type (strides y_s), or NULL: row i - 1 is
+ *                what node i was drawn from; NULL: the drafts were not drawn
+ *   tokens       [B, T] int64: node i's token (that of node 0 is not read); one that
+ *                is negative, or V or more, ends its chain before it
+ *   uniforms     [B, T] fp32 in [0, 1): u_i judges node i, u_0 draws the last token
+ * With p = softmax(logits / temperature) after the node before, and q = softmax(
+ * draft_logits / temperature) (1 at the token and 0 elsewhere without), node i stands
+ * while u_i q(x_i) < p(x_i).  After the last node that stands a token is drawn from
+ * max(p - q, 0) where a node failed there (from p where that is 0 everywhere or NaN),
+ * else from p: the lowest whose running sum, in order, exceeds u_0 times the whole.
+ * Weights and sums are in 64 bits.
+ *   choice   [B, T] int64: the token after each node that stands (the next node's, and
+ *            last the one drawn), then -1: what dropkv_tree_commit takes
+ *   accepted [B] int32: how many; logprobs [B, T] fp32: ln p of each, then 0
+ * A sampled row that holds +inf or NaN, or only -inf, gives -1 and NaN.
+ * 1 <= T <= 256, V <= 2^30, 0 < temperature < inf, B * (2 T - 1) < 2^17.  The
+ * workspace needs no initialisation; its first DROPKV_SYNC_BYTES are left alone. */
+typedef struct {
+  const void* logits;
+  int64_t x_s[2];
+  const void* draft_logits;
+  int64_t y_s[2];
+  const int64_t* tokens;
+  const float* uniforms;
+  int64_t dtype, B, T, V;
+  double temperature;
+  int64_t* choice;
+  int32_t* accepted;
+  float* logprobs;
+  void* workspace;
+  int64_t workspace_bytes;
+} dropkv_verify_drafts_args;
+size_t dropkv_verify_drafts_workspace_bytes(int64_t B, int64_t T, int64_t V, int draft);
+int dropkv_verify_drafts(const dropkv_verify_drafts_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
