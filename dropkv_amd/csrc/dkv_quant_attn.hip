@@ -45,10 +45,12 @@ constexpr float kQRise = 8.f;
 struct Near {
   int first, held, j0, fresh;
 };
-// Key e of it.
+// Key e of it.  (Past the last: its row again, whose weight there is 0; 0 times a value
+// that is not finite is NaN, which only a tail row leaves there, and it reaches every
+// token anyway.)
 template <typename T, int D>
 __device__ __forceinline__ const T* near_row(const Near& s, int e, const T* tail, const T* kn, int64_t st) {
-  const int i = min(e, s.held + s.fresh - 1);  // (past the last: its row again)
+  const int i = min(e, s.held + s.fresh - 1);
   return i < s.held ? tail + ((s.first + i) % kQTail) * D : kn + (int64_t)(s.j0 + i - s.held) * st;
 }
 // The steps of n % 64 tail rows and T new ones: one step if they fit, else the
@@ -80,20 +82,59 @@ __device__ __forceinline__ typename Elem<T>::v8 near_v(const T* vt, int k0, int 
   return __builtin_bit_cast(typename Elem<T>::v8, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// Up to 16 rows per KV head: one wave per part.  K and V come as matrix operands
-// straight into registers, the next block's loads issued as soon as a block's
-// registers are consumed.  P goes into the product in two parts, rounded and
-// remainder.
+// Whether an element of `n` 16-byte pieces is not finite, by the largest magnitude as
+// a whole number; and, where some lane has one, those of new rows taken out of the
+// rows in LDS (`at(i)`: piece i's row and column).  (One by one in line they were
+// 20 KB of code, fetched by every call: the 16-bit step took 7 us, 2 without.)
+template <typename T, int N>
+__device__ __forceinline__ bool near_any_odd(const typename Elem<T>::v8 (&x)[N]) {
+  typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+  us2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const u32x4 w = __builtin_bit_cast(u32x4, x[i]) & 0x7fff7fffu;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, (uint32_t)w[e]));
+  }
+  return wave_any(max(m[0], m[1]) >= (std::is_same<T, _Float16>::value ? 0x7c00 : 0x7f80));
+}
+template <typename T, typename F>
+__device__ __forceinline__ bool near_take_out(T* rows, int pitch, const Near& s, int n, F&& at) {
+  bool odd = false;
+#pragma unroll 1
+  for (int i = 0; i < 8 * n; ++i) {
+    int e, col;
+    at(i / 8, &e, &col);
+    T* x = rows + e * pitch + col + i % 8;
+    if (e >= s.held && not_finite<T>(*x)) {
+      odd = true;
+      *x = static_cast<T>(0.f);
+    }
+  }
+  return odd;
+}
+
+// Up to 16 rows per KV head: workgroups of four waves, which take the blocks of a
+// part in turn, and the step of 16-bit keys as one block more.  K and V come as
+// matrix operands straight into registers, the next block's loads issued as soon as
+// a block's registers are consumed.  P goes into the product in two parts, rounded
+// and remainder.  The waves' results are joined in LDS; the only part's workgroup
+// writes the output.
+constexpr int kNarrowWaves = 4;
 template <typename T, typename S, int D>
-__global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
+__global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(QuantAttnArgs a) {
   typedef typename Elem<T>::v8 v8;
   typedef Elem<__bf16>::v8 b8;
-  constexpr int KC = D / 64, DT = D / 16, CPR = D / 8, GRP = 64 / CPR;
+  constexpr int KC = D / 64, DT = D / 16, CPR = D / 8, GRP = 64 / CPR, NW = kNarrowWaves;
   constexpr int kVPitch = D + 16;  // transposing reads without bank conflicts
+  constexpr int kOPitch = D + 4;   // floats
+  constexpr int kLds = std::max(kQBlock * kVPitch * (int)sizeof(T), NW * 16 * kOPitch * 4);
   const int slot = blockIdx.x % a.P, hkv = blockIdx.x / a.P, g = a.Hq / a.Hkv;
-  const int lane = threadIdx.x, li = lane & 15, lg = lane >> 4;
-  __shared__ __attribute__((aligned(16))) T vt[kQBlock * kVPitch];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
   __shared__ uint64_t mask_words[16];  // (T <= 16 rows)
+  __shared__ float part_m[NW][16], part_l[NW][16];
+  __shared__ int odd_flag;
 
   const TreePart part = tree_part<QuantCut>(a, hkv, slot, lane);
   const int b = part.b;
@@ -120,7 +161,7 @@ __global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
     for (int dt = 0; dt < DT; ++dt) vx[dt] = buf_load16(vrs, (uint32_t)j * kQBlock * D + (16 * dt + li) * kQBlock + 16u * lg);
     vs = vsc[min(j, blocks - 1)];
   };
-  int j = part.t_lo;
+  int j = part.t_lo + wave;
   if (j < part.t_hi) {
     load_k(j);
     load_v(j);
@@ -167,7 +208,7 @@ __global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
     }
   };
 
-  for (; j < part.t_hi; ++j) {
+  for (; j < part.t_hi; j += NW) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -177,7 +218,7 @@ __global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
         for (int hf = 0; hf < 2; ++hf) s[i] = Elem<T>::mfma(unpack8<S, T>(kx[i][c], hf), qop[c][hf], s[i]);
     }
     const float mul = ks * a.scale_log2, vscale = vs;
-    load_k(j + 1);
+    load_k(j + NW);
     weigh(mul, 0xffffu);
     b8 phi[2], plo[2];
 #pragma unroll
@@ -196,18 +237,19 @@ __global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
         o[dt] = Elem<__bf16>::mfma(vop, phi[hf], o[dt]);
         o[dt] = Elem<__bf16>::mfma(vop, plo[hf], o[dt]);
       }
-    load_v(j + 1);
+    load_v(j + NW);
   }
 
+  // The 16-bit keys: by the wave whose turn it is.
   bool odd = false;
-  if (part.tail) {
-    const int n = tree_rows(a, b);
+  if (part.tail && (part.t_hi - part.t_lo) % NW == wave) {
     const T* kt = static_cast<const T*>(a.ktail) + bh * kQTail * D;
     const T* vtl = static_cast<const T*>(a.vtail) + bh * kQTail * D;
     const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
     const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
     const int v_row = lane / CPR, v_col = 8 * (lane % CPR);
-    Near step = near_begin(n, a.T);
+    T* vt = reinterpret_cast<T*>(lds);
+    Near step = near_begin(part.n, a.T);
 #pragma unroll 1
     do {  // (one wave: its own LDS operations stay in order)
       v8 kop[4][KC][2], vch[kQBlock / GRP];
@@ -232,18 +274,12 @@ __global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
           for (int hf = 0; hf < 2; ++hf) s[i] = Elem<T>::mfma(kop[i][c][hf], qop[c][hf], s[i]);
       }
 #pragma unroll
-      for (int i = 0; i < kQBlock / GRP; ++i) {
-        const int e = v_row + i * GRP;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (e >= step.held + step.fresh) {
-            vch[i][k] = static_cast<T>(0.f);
-          } else if (e >= step.held && not_finite<T>(vch[i][k])) {
-            odd = true;
-            vch[i][k] = static_cast<T>(0.f);
-          }
-        *reinterpret_cast<v8*>(vt + e * kVPitch + v_col) = vch[i];
-      }
+      for (int i = 0; i < kQBlock / GRP; ++i) *reinterpret_cast<v8*>(vt + (v_row + i * GRP) * kVPitch + v_col) = vch[i];
+      if (__builtin_expect(near_any_odd<T>(vch), 0))
+        odd |= near_take_out(vt, kVPitch, step, kQBlock / GRP, [&](int i, int* e, int* col) {
+          *e = v_row + i * GRP;
+          *col = v_col;
+        });
       const uint64_t bits = near_bits(step, mask_words[t]);
       weigh(a.scale_log2, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
       v8 phi[2], plo[2];
@@ -266,20 +302,61 @@ __global__ void __launch_bounds__(64) quant_narrow_kernel(QuantAttnArgs a) {
     } while (near_next(&step, a.T));
   }
 
+  // The waves' results joined: 16 threads a row.
   lsum = add_xor32(add_xor16(lsum));
-  const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + li;
+  if (threadIdx.x == 0) odd_flag = 0;
+  __syncthreads();  // (V's rows have been read)
+  float* ol = reinterpret_cast<float*>(lds) + (wave * 16 + li) * kOPitch + 4 * lg;
   if (valid) {
-    float* po = a.part_o + base * D + 4 * lg;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[dt];
-    if (lg == 0) {
-      a.part_m[base] = m;
-      a.part_l[base] = lsum;
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(ol + 16 * dt) = o[dt];
+  }
+  if (lg == 0) {
+    part_m[wave][li] = m;
+    part_l[wave][li] = lsum;
+  }
+  if (wave_any(odd) && lane == 0) odd_flag = 1;
+  __syncthreads();
+  const int row = threadIdx.x >> 4;
+  if (row < a.M) {
+    float mx = part_m[0][row], l = 0.f, f[NW];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, part_m[w][row]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(part_m[w][row] - mx);
+      l += part_l[w][row] * f[w];
+    }
+    const int hr = a.div_t.div(row), tr = row - hr * a.T;
+    T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)tr * a.o_st + (int64_t)(hkv * g + hr) * a.o_sh;
+    const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + row;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const int d0 = 4 * (threadIdx.x & 15) + 64 * i;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + (w * 16 + row) * kOPitch + d0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(f[w], x[e], acc[e]);
+      }
+      if (a.direct) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[d0 + e] = static_cast<T>(l == 0.f ? 0.f : acc[e] * inv);
+      } else {
+        *reinterpret_cast<f32x4*>(a.part_o + base * D + d0) = acc;
+      }
+    }
+    if (!a.direct && (threadIdx.x & 15) == 0) {
+      a.part_m[base] = mx;
+      a.part_l[base] = l;
     }
   }
-  if (__builtin_expect(wave_any(odd), 0)) {
+  if (__builtin_expect(odd_flag, 0)) {
     __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    tree_add_odd<T, D, 64>(a, b, hkv, slot, 0, 16);
+    __syncthreads();
+    tree_add_odd<T, D, 64 * NW>(a, b, hkv, slot, 0, 16);
   }
 }
 
@@ -378,12 +455,14 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // The stage in buffer `buf`: V's operands of type VT, the logits times `mul`, the
-  // weights times vscale; with `masked` only keys of see_bits.
+  // The stage in buffer `buf`, the logits times `mul`, the weights times vscale; or,
+  // `near`, 16-bit keys of see_bits, their V in rows behind K's operands.
   uint32_t see_bits[QB];
-  auto compute = [&](int buf, float mul, float vscale, auto masked, auto vzero) __attribute__((always_inline)) {
-    constexpr bool kMasked = decltype(masked)::value;
-    typedef decltype(vzero) VT;
+  constexpr int kVPitch = D + 16;  // transposing reads without bank conflicts
+  static_assert(kOps * 64 * 16 + kQBlock * kVPitch * 2 <= (int)sizeof(lds), "a step of 16-bit keys fits");
+  auto compute = [&](int buf, float mul, float vscale, auto near) __attribute__((always_inline)) {
+    constexpr bool kNear = decltype(near)::value;
+    typedef std::conditional_t<kNear, T, __bf16> VT;
     typedef typename Elem<VT>::v8 vv8;
     const u32x4* kt = lds + buf * kBuf + lane;
     const u32x4* vt = kt + kOps * 64;
@@ -406,7 +485,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[x][e / 4][e % 4] *= mul;
-        if (kMasked) s[x][e / 4][e % 4] = (see_bits[x] >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
+        if (kNear) s[x][e / 4][e % 4] = (see_bits[x] >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
       }
       float tmax = s[x][0][0];
 #pragma unroll
@@ -450,7 +529,11 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const vv8 vop = bitcast_u4<vv8>(vt[(2 * dt + hf) * 64]);
+        vv8 vop;
+        if constexpr (kNear)
+          vop = near_v<T, D>(reinterpret_cast<const T*>(lds + kOps * 64), 16 * lg + 8 * hf, 16 * dt, li, kVPitch);
+        else
+          vop = bitcast_u4<vv8>(vt[(2 * dt + hf) * 64]);
 #pragma unroll
         for (int x = 0; x < QB; ++x) {
           o[x][dt] = Elem<VT>::mfma(vop, phi[x], o[x][dt]);
@@ -471,7 +554,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     for (; j < part.t_hi; ++j) {
       fetch(j + 1);
       __syncthreads();
-      compute(buf, mul, vscale, std::false_type{}, __bf16{});
+      compute(buf, mul, vscale, std::false_type{});
       buf ^= 1;
       mul = ks * a.scale_log2;
       vscale = vs;
@@ -484,43 +567,40 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
     const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
     Near step = near_begin(tree_rows(a, b), a.T);
+    constexpr int NK = kOps * 64 / NT, CPR = D / 8, NV = kQBlock * CPR / NT;
 #pragma unroll 1
     do {
-      __syncthreads();  // (the words' and the buffer's last readers are done)
-      tree_mask_words<NW>(a, b, step.j0, wave, lane, mask_words);
-      // K's operands as they lie in the rows; V's eight keys of a column one by one.
-      bool odd = false;
-#pragma unroll 1
-      for (int i = 0; i < NC; ++i) {
-        int op;
-        const bool v = place(i, &op);
-        u32x4* to = lds + buf * kBuf + ((v ? kOps : 0) + 2 * op) * 64 + lane;
+      u32x4 kpc[NK];
+      v8 vch[NV];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          v8 x;
-          if (v) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int key = 16 * lg + 8 * hf + e;
-              const T y = near_row<T, D>(step, key, vtl, vn, a.vn_st)[16 * op + li];
-              const bool own = key >= step.held, past = key >= step.held + step.fresh;
-              const bool bad = own && !past && not_finite<T>(y);
-              odd |= bad;
-              x[e] = past || bad ? static_cast<T>(0.f) : y;
-            }
-          } else {
-            x = tree_load8(near_row<T, D>(step, 16 * (li / 4) + 4 * (op / KC) + li % 4, kt, kn, a.kn_st) +
-                           64 * (op % KC) + 16 * lg + 8 * hf);
-          }
-          to[64 * hf] = __builtin_bit_cast(u32x4, x);
-        }
+      for (int i = 0; i < NK; ++i) {
+        const int f = (tid + i * NT) / 64, op = f / 2, hf = f % 2;
+        const T* row = near_row<T, D>(step, 16 * (li / 4) + 4 * (op / KC) + li % 4, kt, kn, a.kn_st);
+        kpc[i] = __builtin_bit_cast(u32x4, tree_load8(row + 64 * (op % KC) + 16 * lg + 8 * hf));
       }
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        vch[i] = tree_load8(near_row<T, D>(step, (tid + i * NT) / CPR, vtl, vn, a.vn_st) + 8 * (tid % CPR));
+      __syncthreads();  // (the words' and the buffers' last readers are done)
+      tree_mask_words<NW>(a, b, step.j0, wave, lane, mask_words);
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) lds[tid + i * NT] = kpc[i];
+      T* vrows = reinterpret_cast<T*>(lds + kOps * 64);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        *reinterpret_cast<v8*>(vrows + (tid + i * NT) / CPR * kVPitch + 8 * (tid % CPR)) = vch[i];
+      if (__builtin_expect(near_any_odd<T>(vch), 0))
+        odd = near_take_out(vrows, kVPitch, step, NV, [&](int i, int* e, int* col) {
+          *e = (tid + i * NT) / CPR;
+          *col = 8 * (tid % CPR);
+        });
       if (odd) odd_flag = 1;
       __syncthreads();
 #pragma unroll
       for (int x = 0; x < QB; ++x)
         see_bits[x] = (uint32_t)(near_bits(step, mask_words[tq[x]]) >> (16 * lg)) & 0xffffu;
-      compute(buf, a.scale_log2, 1.f, std::true_type{}, T{});
+      compute(0, a.scale_log2, 1.f, std::true_type{});
     } while (near_next(&step, a.T));
   }
 
@@ -562,15 +642,65 @@ struct QuantPlan {
   size_t rows, bytes;
 };
 
+// An estimate of a call's time in us, from sweeps of both over calls of 4 to 512 rows
+// per KV head, 700 to 60,000 keys and 2 to 64 heads.  The sum of
+// - the longest workgroup's blocks, a block's time by the rows (narrow: a wave's, every
+//   fourth), 0.6 of it at D = 64, and longer where workgroups share a CU or take turns;
+//   or, if longer, K and V at 5.2 TB/s, where 8 MB or a quarter of them are in flight,
+//   and longer where the workgroups do not divide the CUs;
+// - the partial rows, written and read at 4 TB/s, and a round trip of the joining
+//   kernel for every 16 (D = 128) or 32 parts;
+// - the kernels' fixed part.
+struct QuantShape {
+  int rows;
+  double block_us, fixed_us, shared;  // shared: two workgroups on a CU, against one
+  int per_cu;
+};
+constexpr QuantShape kQuantShapes[] = {
+    {16, 1.6, 6.9, 1.2, 2}, {64, 1.25, 8.3, 1.45, 2}, {128, 1.45, 8.5, 1.7, 2}, {256, 2.1, 8.0, 1.0, 1}};
+
+static double quant_cost(const QuantShape& w, double heads, double M, double D, double blocks, int64_t S) {
+  const double wgs = heads * std::ceil(M / w.rows) * S, wide = D / 128;
+  const double per = std::ceil((blocks + (w.rows == 16 ? 1 : 0)) / S), load = wgs / (256.0 * w.per_cu);
+  double block = w.block_us * (wide < 1 ? 0.6 : 1);
+  if (load > 1)
+    block *= std::ceil(load) * w.shared;
+  else if (w.per_cu == 2 && load > 0.5)
+    block *= w.shared;
+  const double steps = w.rows == 16 ? std::ceil(per / kNarrowWaves) : per;
+  const double flight = std::min(wgs, 256.0 * w.per_cu) * (w.rows == 16 ? 65536 : 16384) * wide;
+  const double bytes = heads * blocks * kQBlock * D * 2;
+  double stream = bytes / 5.2e6 / std::min(1.0, flight / std::max(1.0, std::min(8e6, bytes / 4)));
+  stream *= 0.5 + 0.5 * std::ceil(wgs / 256) * 256 / wgs;
+  const double join = w.rows == 16 && S == 1 ? -2.5 : S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16);
+  return std::max(steps * block, stream) + join + w.fixed_us;
+}
+
 static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C) {
   QuantPlan p;
   p.M = (int)(Hq / Hkv * T);
   const int64_t heads = B * Hkv, blocks = C / kQBlock;
-  p.rows_wg = p.M <= 16 ? 16 : p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kTreeMaxSplits, blocks));
+  double best = 0;
+  p.S = 0;
+  for (const QuantShape& w : kQuantShapes) {
+    // Four waves of their own blocks for up to 16 rows; no shape that the rows would
+    // leave half empty.
+    if ((w.rows == 16) != (p.M <= 16) || (w.rows > 64 && p.M <= w.rows / 2)) continue;
+    const int64_t chunks = heads * ((p.M + w.rows - 1) / w.rows);
+    const int64_t tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kTreeMaxSplits, 256 / chunks, 512 / chunks};
+    for (int64_t S : tries) {
+      S = std::max<int64_t>(1, std::min(S, most));
+      const double cost = quant_cost(w, (double)heads, p.M, (double)D, (double)blocks, S);
+      if (p.S == 0 || cost < best) {
+        best = cost;
+        p.S = (int)S;
+        p.rows_wg = w.rows;
+      }
+    }
+  }
   p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
-  const int64_t want = (p.rows_wg == 16 ? 1024 : 512) / (heads * p.MC);
-  p.S = (int)std::max<int64_t>(1, std::min<int64_t>({want, kTreeMaxSplits, blocks}));
-  p.apart = p.rows_wg <= 64 || heads * p.MC * p.S < 192;
+  p.apart = p.rows_wg == 64 || (p.rows_wg > 64 && heads * p.MC * p.S < 192);
   p.P = (int)(B * (p.S + p.apart));
   p.rows = (size_t)Hkv * p.P * p.M;
   p.bytes = kSyncBytes + kTreeDealBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
@@ -586,7 +716,7 @@ static hipError_t launch_quant_t(const QuantAttnArgs& a, int rows_wg, hipStream_
   constexpr bool kLo = std::is_same<T, _Float16>::value;
   const dim3 grid(a.Hkv * a.P * a.MC);
   if (rows_wg == 16)
-    launch((quant_narrow_kernel<T, S, D>), grid, dim3(64), 0, st, a);
+    launch((quant_narrow_kernel<T, S, D>), grid, dim3(64 * kNarrowWaves), 0, st, a);
   else if (rows_wg == 64)
     launch((quant_wide_kernel<T, S, D, 1, 4, true>), grid, dim3(256), 0, st, a);
   else if (rows_wg == 128)
@@ -638,7 +768,7 @@ hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* 
   a.S = pl.S;
   a.P = pl.P;
   a.apart = pl.apart;
-  a.tail_tiles = pl.apart ? 0 : 3 + (a.T + kQBlock - 1) / kQBlock;
+  a.tail_tiles = pl.apart ? 0 : pl.rows_wg == 16 ? 2 : 3 + (a.T + kQBlock - 1) / kQBlock;
   a.ragged = p.n_sb != 0 && p.B > 1 && p.B <= kTreeRaggedB && pl.S > 1;
   a.direct = pl.S == 1 && !pl.apart;
   a.div_t = Div::of(a.T);
