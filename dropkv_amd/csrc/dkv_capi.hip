@@ -109,9 +109,10 @@ int check_quant_cache(const void* k, const void* v, const void* k_scale, const v
 int check_verify_shape(int64_t B, int64_t T, int64_t V) {
   if (B < 1 || T < 1 || V < 1) return fail(DROPKV_E_ARG, "B, T, V must be positive");
   if (T > dkv::kTreeMaxT) return fail(DROPKV_E_UNSUPPORTED, "T must be in [1, %d]", (int)dkv::kTreeMaxT);
-  if (V > kMaxLk) return fail(DROPKV_E_UNSUPPORTED, "V too large");
+  if (V > (1 << 26)) return fail(DROPKV_E_UNSUPPORTED, "V too large: it must be at most %d", 1 << 26);
   // (Up to 64 workgroups of 256 a row, and a grid holds fewer than 2^32 work-items.)
   if (B >= (1 << 17) || B * (2 * T - 1) >= (1 << 17)) return fail(DROPKV_E_UNSUPPORTED, "B*(2*T-1) too large");
+  if ((double)B * (double)V >= 8589934592.) return fail(DROPKV_E_UNSUPPORTED, "B*V too large");
   return DROPKV_OK;
 }
 

@@ -12,8 +12,12 @@
 // A random number may lie next to the border of two tokens, and p - q is a
 // difference of near values, so all weights and sums are in 64 bits: sums of two
 // orders differ by 10^-15, which moves a border past a given u_0 about once in 10^10
-// samples of a vocabulary of 150,000.  The exponential is 2^k times the Taylor sum
-// of 2^f, |f| <= 1/2, to the 11th power (2^-52 of it is left).
+// samples of a vocabulary of 150,000.  The exponential is 2^(k/32), from a table and
+// the exponent, times the Taylor sum of 2^f, |f| <= 1/64, to the 4th power, which
+// leaves 10^-12 of it, in 9 operations of 64 bits and 6 others.  (One sum over |f| <=
+// 1/2 takes 45, and the pass over 136 rows of 151936, whose bytes take 8 us, took 26.
+// 32 entries of 8 bytes are one for each pair of LDS banks: no lanes wait for one
+// another.)
 //
 // Four kernels: maximum and sum of every row in segments; the walk, a workgroup per
 // sequence; sums of the weights that are sampled, in segments of the one row of each
@@ -38,6 +42,7 @@ struct VfPart {
 };
 struct VfSeq {           // what the walk leaves of a sequence
   double p_mul, q_mul;   // 1 / sum of the sampled node's row, and of its draft's
+  double ln_s;           // ln of the former's sum
   float p_m, q_m;        // their maxima
   int last, token;       // the node; the token that failed there, or -1
 };
@@ -49,38 +54,89 @@ struct VerifyArgs {
   const int64_t* tokens;  // [B, T]
   const float* u;         // [B, T]
   int B, T, V, S, seg;    // segments per row, elements per segment (whole tiles)
+  int pieces;             // of the sampled rows
   double mul;             // log2 e / temperature
+  float deep;             // 990 / mul
   VfPart* part;           // [B, T, S], then [B, T - 1, S] of the drafts
   VfSeq* seq;             // [B]
-  double* sums;           // [B, S, 2]: of the weights, and of p alone
+  double* sums;           // [B, pieces, 2]: of the weights, and of p alone
   int64_t* choice;        // [B, T]
   int* accepted;          // [B]
   float* logprob;         // [B, T]
 };
 
 constexpr double kLn2 = 0.693147180559945309417232121458;
-struct Exp2Taylor {
-  double c[12];
-  constexpr Exp2Taylor() : c() {
-    c[0] = 1;
-    for (int i = 1; i < 12; ++i) c[i] = c[i - 1] * kLn2 / i;
+constexpr int kVfTable = 32;
+// 2^(i / 32), from products of the square roots of 2 that the bits of i name; with
+// i / 32 less in the exponent's place, so that adding 32 e + i there makes 2^e of it.
+struct Exp2Table {
+  uint64_t t[kVfTable];
+  constexpr Exp2Table() : t() {
+    double root[5] = {};
+    double x = 2.;
+    for (int b = 4; b >= 0; --b) {  // 2^(1/2), 2^(1/4), ..
+      double y = x;
+      for (int i = 0; i < 60; ++i) y = 0.5 * (y + x / y);
+      root[b] = x = y;
+    }
+    for (int i = 0; i < kVfTable; ++i) {
+      double v = 1.;
+      for (int b = 0; b < 5; ++b)
+        if (i >> b & 1) v *= root[b];
+      t[i] = __builtin_bit_cast(uint64_t, v) - ((uint64_t)i << 47);
+    }
   }
 };
-__device__ __forceinline__ double exp2_64(double z) {  // z <= 0, or NaN
-  constexpr Exp2Taylor t{};
-  const double k = __builtin_rint(z), f = z - k;
-  double p = t.c[11];
-#pragma unroll
-  for (int i = 10; i >= 0; --i) p = __builtin_fma(p, f, t.c[i]);
-  return z < -1000. ? 0. : __builtin_ldexp(p, (int)k);
+__device__ constexpr Exp2Table kExp2Table{};
+__device__ __forceinline__ void vf_table(uint64_t* lds) {  // (then a barrier)
+  if (threadIdx.x < kVfTable) lds[threadIdx.x] = kExp2Table.t[threadIdx.x];
+}
+constexpr double kVfRound = 1.5 * 140737488355328.;  // 2^47: sums with it are whole 32nds
+// 2^(d + f), |f| <= 1/64, d the whole 32nds in the last bits of t, -1000 <= d + f <= 0
+// or so; NaN where f is.
+__device__ __forceinline__ double exp2_parts(double t, double f, const uint64_t* table) {
+  constexpr double c1 = kLn2, c2 = c1 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4;
+  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);
+  const u32x2 e = __builtin_bit_cast(u32x2, table[k & (kVfTable - 1)]);
+  double p = __builtin_fma(c4, f, c3);
+  p = __builtin_fma(p, f, c2);
+  p = __builtin_fma(p, f, c1);
+  p = __builtin_fma(p, f, 1.);
+  return p * __builtin_bit_cast(double, u32x2{e[0], e[1] + (k << 15)});
+}
+__device__ __forceinline__ double exp2_64(double z, const uint64_t* table) {  // -1000 <= z <= 1, or NaN
+  const double t = z + kVfRound;
+  return exp2_parts(t, z - (t - kVfRound), table);
 }
 
-// Eight bytes from another lane.
-__device__ __forceinline__ double shfl_xor_d(double x, int o) { return __shfl_xor(x, o); }
+// DPP moves of eight bytes, sums over the wave and inclusive sums along its lanes.
+template <int kCtrl, int kRowMask, int kBankMask>
+__device__ __forceinline__ double dpp_d(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = dpp_z<kCtrl, kRowMask, kBankMask>((uint32_t)b), hi = dpp_z<kCtrl, kRowMask, kBankMask>((uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double read_lane_d(double x, int l) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), l);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum_d(double x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += shfl_xor_d(x, o);
-  return x;
+  x += dpp_d<kDppQuadSwap1, 0xf, 0xf>(x);
+  x += dpp_d<kDppQuadSwap2, 0xf, 0xf>(x);
+  x += dpp_d<kDppHalfMirror, 0xf, 0xf>(x);
+  x += dpp_d<kDppMirror, 0xf, 0xf>(x);
+  return (read_lane_d(x, 0) + read_lane_d(x, 16)) + (read_lane_d(x, 32) + read_lane_d(x, 48));
+}
+__device__ __forceinline__ double wave_scan_d(double x) {
+  double t = x + dpp_d<kDppRowShr1, 0xf, 0xf>(x);
+  t += dpp_d<kDppRowShr2, 0xf, 0xf>(x);
+  t += dpp_d<kDppRowShr3, 0xf, 0xf>(x);
+  t += dpp_d<kDppRowShr4, 0xf, 0xe>(t);
+  t += dpp_d<kDppRowShr8, 0xf, 0xc>(t);
+  t += dpp_d<kDppRowBcast15, 0xa, 0xf>(t);
+  t += dpp_d<kDppRowBcast31, 0xc, 0xf>(t);
+  return t;
 }
 
 // Elements j .. j + 16 / sizeof(T) - 1 of a row as floats, -inf from `hi` on.
@@ -100,7 +156,17 @@ __device__ __forceinline__ void vf_load(const T* x, int j, int hi, float* v) {
   }
 }
 
-__device__ __forceinline__ double vf_weight(float v, float m, double mul) { return exp2_64(((double)v - (double)m) * mul); }
+// e^((v - m) / temperature); 0 below 2^-1000.
+__device__ __forceinline__ double vf_weight(float v, float m, double mul, const uint64_t* table) {
+  const double z = ((double)v - (double)m) * mul, e = exp2_64(z, table);
+  return z < -1000. ? 0. : e;
+}
+
+// A sum of weights against m, against the larger maximum `to` (both may be -inf, where
+// nothing has been seen).
+__device__ __forceinline__ double vf_turned(double s, float m, float to, double mul, const uint64_t* table) {
+  return m == to ? s : s * vf_weight(m, to, mul, table);
+}
 
 // Maximum and sum of a segment of a row.
 template <typename T>
@@ -108,6 +174,7 @@ __global__ void __launch_bounds__(kVfThreads) verify_stats_kernel(VerifyArgs a) 
   constexpr int EPV = 16 / (int)sizeof(T), NV = kVfElems / EPV;
   __shared__ float wm[kVfThreads / 64];
   __shared__ double ws[kVfThreads / 64];
+  __shared__ uint64_t table[kVfTable];
   const int tid = threadIdx.x, sg = blockIdx.x % a.S, row = blockIdx.x / a.S;
   const T* x;
   if (row < a.B * a.T) {
@@ -117,7 +184,9 @@ __global__ void __launch_bounds__(kVfThreads) verify_stats_kernel(VerifyArgs a) 
     x = static_cast<const T*>(a.y) + (r / (a.T - 1)) * a.y_sb + (r % (a.T - 1)) * a.y_st;
   }
   const int lo = sg * a.seg, hi = min(a.V, lo + a.seg);
-  float m = -__FLT_MAX__;  // (finite, so that -inf gets no weight)
+  vf_table(table);
+  __syncthreads();
+  float m = -INFINITY;
   double s = 0.;
   for (int j0 = lo; j0 < hi; j0 += kVfTile) {
     float v[kVfElems];
@@ -127,14 +196,33 @@ __global__ void __launch_bounds__(kVfThreads) verify_stats_kernel(VerifyArgs a) 
 #pragma unroll
     for (int e = 1; e < kVfElems; ++e) top = fmaxf(top, v[e]);
     if (top > m) {
-      s *= vf_weight(m, top, a.mul);
+      s = vf_turned(s, m, top, a.mul, table);
       m = top;
     }
+    if (m == -INFINITY) {  // nothing but -inf so far, or NaN
 #pragma unroll
-    for (int e = 0; e < kVfElems; ++e) s += vf_weight(v[e], m, a.mul);
+      for (int e = 0; e < kVfElems; ++e) s += v[e] == v[e] ? 0. : (double)v[e];
+    } else if (fabs((double)m * a.mul) < 0x1p40) {
+      // Against 2^R, R the whole 32nds next to m's exponent, so that a product's 32nds
+      // and its rest (exact) take one operation each.  (2^-990 of the largest and below
+      // are all 2^-990, which no sum notices: cheaper than a zero each.  A NaN stays
+      // one.)
+      const float least = m - a.deep;
+      const double R = ((double)m * a.mul + kVfRound) - kVfRound, round = kVfRound - R;
+      double sum = 0.;
+#pragma unroll
+      for (int e = 0; e < kVfElems; ++e) {
+        const double x = __builtin_elementwise_maximum(v[e], least), t = __builtin_fma(x, a.mul, round);
+        sum += exp2_parts(t, __builtin_fma(x, a.mul, round - t), table);
+      }
+      s += sum * exp2_64(__builtin_fma(-(double)m, a.mul, R), table);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < kVfElems; ++e) s += vf_weight(v[e], m, a.mul, table);
+    }
   }
   const float wave_m = wave_max_dpp(m);
-  s = wave_sum_d(s * vf_weight(m, wave_m, a.mul));
+  s = wave_sum_d(vf_turned(s, m, wave_m, a.mul, table));
   if ((tid & 63) == 0) {
     wm[tid >> 6] = wave_m;
     ws[tid >> 6] = s;
@@ -144,25 +232,27 @@ __global__ void __launch_bounds__(kVfThreads) verify_stats_kernel(VerifyArgs a) 
     float all = wm[0];
     for (int w = 1; w < kVfThreads / 64; ++w) all = fmaxf(all, wm[w]);
     double sum = 0.;
-    for (int w = 0; w < kVfThreads / 64; ++w) sum += ws[w] * vf_weight(wm[w], all, a.mul);
+    for (int w = 0; w < kVfThreads / 64; ++w) sum += vf_turned(ws[w], wm[w], all, a.mul, table);
     a.part[(int64_t)row * a.S + sg] = VfPart{sum, all, 0};
   }
 }
 
 // A row's maximum and sum from its segments, lane s segment s.
-__device__ __forceinline__ void vf_join(const VerifyArgs& a, int64_t row, int lane, float* m, double* s) {
-  VfPart p{0., -__FLT_MAX__, 0};
+__device__ __forceinline__ void vf_join(const VerifyArgs& a, int64_t row, int lane, const uint64_t* table, float* m, double* s) {
+  VfPart p{0., -INFINITY, 0};
   if (lane < a.S) p = a.part[row * a.S + lane];
   *m = wave_max_dpp(p.m);
-  *s = wave_sum_d(p.s * vf_weight(p.m, *m, a.mul));
+  *s = wave_sum_d(vf_turned(p.s, p.m, *m, a.mul, table));
 }
 
 // One workgroup per sequence, a wave per node at a time: which nodes stand.
 template <typename T>
 __global__ void __launch_bounds__(512) verify_walk_kernel(VerifyArgs a) {
   __shared__ int first;  // the first node that does not stand
+  __shared__ uint64_t table[kVfTable];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t* tokens = a.tokens + (int64_t)b * a.T;
+  vf_table(table);
   if (tid == 0) first = a.T;
   __syncthreads();
   for (int i = 1 + wave; i < a.T; i += 8) {
@@ -172,14 +262,14 @@ __global__ void __launch_bounds__(512) verify_walk_kernel(VerifyArgs a) {
     if (token >= 0 && token < a.V) {
       float m, qm;
       double s, qs;
-      vf_join(a, (int64_t)b * a.T + i - 1, lane, &m, &s);
+      vf_join(a, (int64_t)b * a.T + i - 1, lane, table, &m, &s);
       const float x = static_cast<float>(static_cast<const T*>(a.x)[b * a.x_sb + (i - 1) * a.x_st + token]);
       double q = 1.;
       if (a.y) {
-        vf_join(a, (int64_t)a.B * a.T + (int64_t)b * (a.T - 1) + i - 1, lane, &qm, &qs);
-        q = vf_weight(static_cast<float>(static_cast<const T*>(a.y)[b * a.y_sb + (i - 1) * a.y_st + token]), qm, a.mul) / qs;
+        vf_join(a, (int64_t)a.B * a.T + (int64_t)b * (a.T - 1) + i - 1, lane, table, &qm, &qs);
+        q = vf_weight(static_cast<float>(static_cast<const T*>(a.y)[b * a.y_sb + (i - 1) * a.y_st + token]), qm, a.mul, table) / qs;
       }
-      stands = (double)a.u[(int64_t)b * a.T + i] * q < vf_weight(x, m, a.mul) / s;
+      stands = (double)a.u[(int64_t)b * a.T + i] * q < vf_weight(x, m, a.mul, table) / s;
       lp = (float)(((double)x - (double)m) * (a.mul * kLn2) - log(s));
     }
     if (lane == 0) {
@@ -198,90 +288,119 @@ __global__ void __launch_bounds__(512) verify_walk_kernel(VerifyArgs a) {
   if (wave != 0) return;
   float m, qm = 0.f;
   double s, qs = 1.;
-  vf_join(a, (int64_t)b * a.T + last, lane, &m, &s);
+  vf_join(a, (int64_t)b * a.T + last, lane, table, &m, &s);
   const int64_t failed = last + 1 < a.T ? tokens[last + 1] : -1;
   const bool real = failed >= 0 && failed < a.V;
-  if (real && a.y) vf_join(a, (int64_t)a.B * a.T + (int64_t)b * (a.T - 1) + last, lane, &qm, &qs);
+  if (real && a.y) vf_join(a, (int64_t)a.B * a.T + (int64_t)b * (a.T - 1) + last, lane, table, &qm, &qs);
   if (lane == 0) {
     a.accepted[b] = last + 1;
-    a.seq[b] = VfSeq{1. / s, 1. / qs, m, qm, last, real ? (int)failed : -1};
+    a.seq[b] = VfSeq{1. / s, 1. / qs, log(s), m, qm, last, real ? (int)failed : -1};
   }
 }
 
-// Weight of place j of the sampled row: of what is left of p, and of p.
+// Weights of N places from j on of the sampled row: of what is left of p, and of p.
 template <typename T, int N>
-__device__ __forceinline__ void vf_weights(const VerifyArgs& a, int b, const VfSeq& q, int j, int hi, double* w, double* p) {
-  float v[N], z[N];
+__device__ __forceinline__ void vf_weights(const VerifyArgs& a, int b, const VfSeq& q, int j, int hi, const uint64_t* table,
+                                           float* v, double* w, double* p) {
+  constexpr int EPV = 16 / (int)sizeof(T);
+  float z[N];
   const T* x = static_cast<const T*>(a.x) + b * a.x_sb + q.last * a.x_st;
-  vf_load<T>(x, j, hi, v);
+  const T* y = static_cast<const T*>(a.y) + b * a.y_sb + q.last * a.y_st;
   const bool rest = q.token >= 0 && a.y;
-  if (rest) vf_load<T>(static_cast<const T*>(a.y) + b * a.y_sb + q.last * a.y_st, j, hi, z);
+  if (N == 1) {
+    v[0] = j < hi ? static_cast<float>(x[j]) : -INFINITY;
+    if (rest) z[0] = j < hi ? static_cast<float>(y[j]) : -INFINITY;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += EPV) vf_load<T>(x, j + i, hi, v + i);
+    if (rest)
+#pragma unroll
+      for (int i = 0; i < N; i += EPV) vf_load<T>(y, j + i, hi, z + i);
+  }
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    p[e] = vf_weight(v[e], q.p_m, a.mul) * q.p_mul;
+    p[e] = vf_weight(v[e], q.p_m, a.mul, table) * q.p_mul;
     // (A difference that is NaN counts for nothing: with a draft row that is not
     // finite p itself is sampled.)
-    w[e] = rest ? fmax(p[e] - vf_weight(z[e], q.q_m, a.mul) * q.q_mul, 0.) : j + e == q.token ? 0. : p[e];
+    w[e] = rest ? fmax(p[e] - vf_weight(z[e], q.q_m, a.mul, table) * q.q_mul, 0.) : j + e == q.token ? 0. : p[e];
   }
 }
 
+// Sums of both over pieces of kVfPiece places, a wave each.
+constexpr int kVfPiece = 512;
 template <typename T>
 __global__ void __launch_bounds__(kVfThreads) verify_sums_kernel(VerifyArgs a) {
-  constexpr int EPV = 16 / (int)sizeof(T);
-  __shared__ double sum[2][kVfThreads / 64];
-  const int tid = threadIdx.x, sg = blockIdx.x % a.S, b = blockIdx.x / a.S;
-  const VfSeq q = a.seq[b];
-  const int lo = sg * a.seg, hi = min(a.V, lo + a.seg);
-  double sw = 0., sp = 0.;
-  for (int j = lo + tid * EPV; j < hi; j += kVfThreads * EPV) {
-    double w[EPV], p[EPV];
-    vf_weights<T, EPV>(a, b, q, j, hi, w, p);
+  __shared__ uint64_t table[kVfTable];
+  constexpr int N = kVfPiece / 64;
+  const int groups = (a.pieces + 3) / 4, b = blockIdx.x / groups, lane = threadIdx.x & 63;
+  const int piece = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
+  vf_table(table);
+  __syncthreads();
+  if (piece >= a.pieces) return;
+  float v[N];
+  double w[N], p[N], sw = 0., sp = 0.;
+  vf_weights<T, N>(a, b, a.seq[b], piece * kVfPiece + lane * N, a.V, table, v, w, p);
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) {
-      sw += w[e];
-      sp += p[e];
-    }
+  for (int e = 0; e < N; ++e) {
+    sw += w[e];
+    sp += p[e];
   }
   sw = wave_sum_d(sw);
   sp = wave_sum_d(sp);
-  if ((tid & 63) == 0) {
-    sum[0][tid >> 6] = sw;
-    sum[1][tid >> 6] = sp;
-  }
-  __syncthreads();
-  if (tid < 2) a.sums[((int64_t)b * a.S + sg) * 2 + tid] = (sum[tid][0] + sum[tid][1]) + (sum[tid][2] + sum[tid][3]);
+  if (lane < 2) a.sums[((int64_t)b * a.pieces + piece) * 2 + lane] = lane ? sp : sw;
 }
 
-// Inclusive sums along the lanes.
-__device__ __forceinline__ double wave_scan_d(double x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
+// The workgroup's first thread with a weight that is past the target, and its last
+// with a weight.
+__device__ __forceinline__ void vf_mark(bool some, bool past, int lane, int wave, int* first, int* any) {
+  const uint64_t has = __builtin_amdgcn_ballot_w64(some), hit = __builtin_amdgcn_ballot_w64(some && past);
+  if (lane != 0) return;
+  if (hit) atomicMin(first, 64 * wave + __builtin_ctzll(hit));
+  if (has) atomicMax(any, 64 * wave + 63 - __builtin_clzll(has));
 }
 
-// The token: the segment whose running sum passes u_0 times the whole, and the
-// place in it.
+// The token: the piece whose running sum passes u_0 times the whole, and the place in
+// it.  A thread holds one piece (of up to 262144 tokens), then one place.
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads) verify_token_kernel(VerifyArgs a) {
-  constexpr int EPV = 16 / (int)sizeof(T), W = kVfThreads / 64;
-  __shared__ double wsum[W];
-  __shared__ int hit, any;
+__global__ void __launch_bounds__(kVfPiece) verify_token_kernel(VerifyArgs a) {
+  constexpr int W = kVfPiece / 64;
+  __shared__ double sum_w[W], sum_p[W], base_lds;
+  __shared__ uint64_t table[kVfTable];
+  __shared__ int first, any, piece_lds;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const VfSeq q = a.seq[b];
-  const double* sums = a.sums + (int64_t)b * a.S * 2;
-  double sw = lane < a.S ? sums[2 * lane] : 0., sp = lane < a.S ? sums[2 * lane + 1] : 0.;
-  // (Where nothing is left of p, all of p.)
-  const bool left = wave_sum_d(sw) > 0.;
-  const double mine = left ? sw : sp, upto = wave_scan_d(mine, lane), total = __shfl(upto, 63);
+  const double* sums = a.sums + (int64_t)b * a.pieces * 2;
+  const int per = (a.pieces + kVfPiece - 1) / kVfPiece, p0 = tid * per, p1 = min(p0 + per, a.pieces);
+  double sw = 0., sp = 0.;
+  for (int i = p0; i < p1; ++i) {
+    sw += sums[2 * i];
+    sp += sums[2 * i + 1];
+  }
+  vf_table(table);
   if (tid == 0) {
-    hit = a.V;
+    first = kVfPiece;
     any = -1;
   }
+  double cw = wave_scan_d(sw), cp = wave_scan_d(sp);
+  if (lane == 63) {
+    sum_w[wave] = cw;
+    sum_p[wave] = cp;
+  }
   __syncthreads();
-  if (!(total > 0.) || !(total < __builtin_inf())) {  // (a row that is not finite; every wave alike)
+  double all_w = 0., all_p = 0.;
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    if (k == wave) {
+      cw += all_w;
+      cp += all_p;
+    }
+    all_w += sum_w[k];
+    all_p += sum_p[k];
+  }
+  // (Where nothing is left of p, all of p.)
+  const bool left = all_w > 0.;
+  const double mine = left ? sw : sp, upto = left ? cw : cp, total = left ? all_w : all_p;
+  if (!(total > 0.) || !(total < __builtin_inf())) {  // (a row that is not finite; every thread alike)
     if (tid == 0) {
       a.choice[(int64_t)b * a.T + q.last] = -1;
       a.logprob[(int64_t)b * a.T + q.last] = __builtin_nanf("");
@@ -289,45 +408,44 @@ __global__ void __launch_bounds__(kVfThreads) verify_token_kernel(VerifyArgs a) 
     return;
   }
   const double target = (double)a.u[(int64_t)b * a.T] * total;
-  // The first segment past the target, else the last one with any weight.
-  const uint64_t past = __builtin_amdgcn_ballot_w64(mine > 0. && upto > target), some = __builtin_amdgcn_ballot_w64(mine > 0.);
-  const int sg = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-  double base = __shfl(upto - mine, sg);
-  const int lo = sg * a.seg, hi = min(a.V, lo + a.seg);
-  for (int j0 = lo; j0 < hi; j0 += kVfThreads * EPV) {
-    const int j = j0 + tid * EPV;
-    double w[EPV], p[EPV], own = 0.;
-    vf_weights<T, EPV>(a, b, q, j, hi, w, p);
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) {
-      w[e] = left ? w[e] : p[e];
-      own += w[e];
-    }
-    const double incl = wave_scan_d(own, lane);
-    if (lane == 63) wsum[wave] = incl;
-    __syncthreads();
-    double run = base + (incl - own);
-    for (int k = 0; k < wave; ++k) run += wsum[k];
-    int at = a.V, most = -1;
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) {
-      run += w[e];
-      if (w[e] > 0.) {
-        most = j + e;
-        if (run > target && at == a.V) at = j + e;
+  // The first thread past the target, else the last one with any weight.
+  vf_mark(mine > 0., upto > target, lane, wave, &first, &any);
+  __syncthreads();
+  if (tid == (first < kVfPiece ? first : any)) {
+    double run = upto - mine, base = run;
+    int at = p0;  // the first of its pieces past the target, else its last with any weight
+    for (int i = p0; i < p1 && per > 1; ++i) {
+      const double x = left ? sums[2 * i] : sums[2 * i + 1];
+      if (x > 0.) {
+        at = i;
+        base = run;
+        if (run + x > target) break;
       }
+      run += x;
     }
-    if (at < a.V) atomicMin(&hit, at);
-    if (most >= 0) atomicMax(&any, most);
-    for (int k = 0; k < W; ++k) base += wsum[k];
-    __syncthreads();
-    if (hit < a.V) break;
+    piece_lds = at;
+    base_lds = base;
   }
+  __syncthreads();
   if (tid == 0) {
-    const int token = hit < a.V ? hit : any;
-    const float x = static_cast<float>(static_cast<const T*>(a.x)[b * a.x_sb + q.last * a.x_st + token]);
-    a.choice[(int64_t)b * a.T + q.last] = token;
-    a.logprob[(int64_t)b * a.T + q.last] = (float)(((double)x - (double)q.p_m) * (a.mul * kLn2) + log(q.p_mul));
+    first = kVfPiece;
+    any = -1;
+  }
+  const int j = piece_lds * kVfPiece + tid;
+  float x;
+  double w, p;
+  vf_weights<T, 1>(a, b, q, j, a.V, table, &x, &w, &p);
+  w = left ? w : p;
+  double run = wave_scan_d(w);
+  if (lane == 63) sum_w[wave] = run;
+  __syncthreads();
+  run += base_lds;
+  for (int k = 0; k < wave; ++k) run += sum_w[k];
+  vf_mark(w > 0., run > target, lane, wave, &first, &any);
+  __syncthreads();
+  if (tid == (first < kVfPiece ? first : any)) {
+    a.choice[(int64_t)b * a.T + q.last] = j;
+    a.logprob[(int64_t)b * a.T + q.last] = (float)(((double)x - (double)q.p_m) * (a.mul * kLn2) - q.ln_s);
   }
 }
 
@@ -340,13 +458,13 @@ struct VerifyPlan {
 };
 static VerifyPlan verify_plan(int64_t B, int64_t T, int64_t V, bool draft) {
   const int64_t rows = B * (draft ? 2 * T - 1 : T), tiles = (V + kVfTile - 1) / kVfTile;
-  // (The sampled rows, one a sequence, are cut alike.)
-  const int64_t want = std::min<int64_t>({tiles, kVfMaxSegs, std::max<int64_t>({1, kVfGroups / rows, 512 / B})});
+  const int64_t want = std::min<int64_t>({tiles, kVfMaxSegs, std::max<int64_t>(1, kVfGroups / rows)});
   const int64_t per = (tiles + want - 1) / want;
   VerifyPlan p;
   p.S = (int)((tiles + per - 1) / per);
   p.seg = (int)std::min<int64_t>(per * kVfTile, INT32_MAX - kVfTile);
-  p.bytes = kSyncBytes + 256 + (size_t)rows * p.S * sizeof(VfPart) + (size_t)B * (sizeof(VfSeq) + p.S * 16);
+  p.bytes = kSyncBytes + 256 + (size_t)rows * p.S * sizeof(VfPart) + 
+            (size_t)B * (sizeof(VfSeq) + (size_t)((V + kVfPiece - 1) / kVfPiece) * 16);
   return p;
 }
 size_t verify_workspace_bytes(int64_t B, int64_t T, int64_t V, bool draft) { return verify_plan(B, T, V, draft).bytes; }
@@ -356,8 +474,8 @@ static hipError_t launch_verify_t(const VerifyArgs& a, hipStream_t st) {
   const int rows = a.B * (a.y ? 2 * a.T - 1 : a.T);
   launch(verify_stats_kernel<T>, dim3((unsigned)(rows * a.S)), dim3(kVfThreads), 0, st, a);
   launch(verify_walk_kernel<T>, dim3(a.B), dim3(512), 0, st, a);
-  launch(verify_sums_kernel<T>, dim3((unsigned)(a.B * a.S)), dim3(kVfThreads), 0, st, a);
-  launch(verify_token_kernel<T>, dim3(a.B), dim3(kVfThreads), 0, st, a);
+  launch(verify_sums_kernel<T>, dim3((unsigned)(a.B * ((a.pieces + 3) / 4))), dim3(kVfThreads), 0, st, a);
+  launch(verify_token_kernel<T>, dim3(a.B), dim3(kVfPiece), 0, st, a);
   return hipGetLastError();
 }
 
@@ -377,7 +495,9 @@ hipError_t launch_verify_drafts(const dropkv_verify_drafts_args& p, hipStream_t 
   a.V = (int)p.V;
   a.S = pl.S;
   a.seg = pl.seg;
+  a.pieces = (int)((p.V + kVfPiece - 1) / kVfPiece);
   a.mul = 1.4426950408889634074 / p.temperature;
+  a.deep = (float)(990. / a.mul);
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15) + kSyncBytes;
   a.part = reinterpret_cast<VfPart*>(ws);
   a.seq = reinterpret_cast<VfSeq*>(a.part + (size_t)p.B * (p.draft_logits ? 2 * p.T - 1 : p.T) * pl.S);

@@ -639,22 +639,53 @@ QUANT_BLOCK = 64  # rows of a block, which has one scale for K and one for V
 _STORE_CODE = {torch.int8: _lib.DROPKV_INT8, torch.float8_e4m3fn: _lib.DROPKV_E4M3}
 
 
-class QuantCache(NamedTuple):
-    """Buffers of a cache in 8 bits (``quant_cache``).  A full block of 64 rows holds
-    ``q`` in ``k`` (row-major) and ``v`` (transposed within the block) standing for
-    ``scale * q``; the rows of the last block, while it is not full, are in the
-    tails, row r at ``r % 128``.  With ``layers`` there is an axis N in front."""
+class QuantCache:
+    """Buffers of a cache in 8 bits (``quant_cache`` makes them).  A full block of 64
+    rows holds ``q`` in ``k`` (row-major) and ``v`` (transposed within the block)
+    standing for ``scale * q``; the rows of the last block, while it is not full, are
+    in the tails, row r at ``r % 128``.  With an axis N in front they are those of N
+    layers.  Iterates over the six tensors.
 
-    k: torch.Tensor        # [B, H, capacity, D] int8 or float8_e4m3fn
-    v: torch.Tensor        # [B, H, capacity / 64, D, 64]
-    k_scale: torch.Tensor  # [B, H, capacity / 64] fp32
-    v_scale: torch.Tensor
-    k_tail: torch.Tensor   # [B, H, 128, D] bf16 or fp16
-    v_tail: torch.Tensor
+    * ``k`` [B, H, capacity, D] int8 or float8_e4m3fn, ``v`` [B, H, capacity / 64, D, 64];
+    * ``k_scale``, ``v_scale`` [B, H, capacity / 64] fp32;
+    * ``k_tail``, ``v_tail`` [B, H, 128, D] bf16 or fp16.
+    """
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "lead", "H", "capacity", "D", "layers", "dtype",
+                 "store", "index", "codes")
+
+    def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
+        kshape = k.shape
+        if len(kshape) != 4 and len(kshape) != 5:
+            raise RuntimeError("QuantCache: k must be [B, H, capacity, D] or [N, B, H, capacity, D]")
+        *lead, H, C, D = kshape
+        n, store, dtype = C // QUANT_BLOCK, k.dtype, k_tail.dtype
+        if (C % QUANT_BLOCK or v.shape != (*lead, H, n, D, QUANT_BLOCK) or k_scale.shape != (*lead, H, n)
+                or v_scale.shape != k_scale.shape or k_tail.shape != (*lead, H, 2 * QUANT_BLOCK, D)
+                or v_tail.shape != k_tail.shape):
+            raise RuntimeError("QuantCache: the buffers' shapes must be those of quant_cache")
+        if (store not in _STORE_CODE or v.dtype is not store or not k_scale.dtype is v_scale.dtype is torch.float32
+                or (dtype is not torch.bfloat16 and dtype is not torch.float16) or v_tail.dtype is not dtype):
+            raise RuntimeError("QuantCache: the buffers' dtypes must be those of quant_cache")
+        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
+        for t in self:
+            if not t.is_contiguous() or t.get_device() != k.get_device() or t.requires_grad:
+                raise RuntimeError("QuantCache: the buffers must be contiguous, on one device and without gradients")
+        self.lead, self.H, self.capacity, self.D = tuple(lead), H, C, D
+        self.layers, self.dtype, self.store = len(kshape) == 5, dtype, store
+        self.index = k.get_device()
+        self.codes = _DTYPE_CODE[dtype], _STORE_CODE[store]
+
+    def __iter__(self):
+        return iter((self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
+
+    def pointers(self):
+        return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                self.k_tail.data_ptr(), self.v_tail.data_ptr())
 
     def layer(self, i: int) -> "QuantCache":
         """Layer ``i`` of a cache of several (views)."""
-        if self.k.dim() != 5:
+        if not self.layers:
             raise RuntimeError("the cache has no axis of layers")
         return QuantCache(*(t[i] for t in self))
 
@@ -685,34 +716,25 @@ def quant_cache(B: int, H: int, capacity: int, D: int, dtype: torch.dtype = torc
                       zeros(torch.float32, n), zeros(dtype, 2 * QUANT_BLOCK, D), zeros(dtype, 2 * QUANT_BLOCK, D))
 
 
-def _quant_shape(name: str, c: QuantCache):
-    """(leading axes, H, capacity, D, layers or not) of a cache whose buffers fit one
-    another."""
-    kshape = c.k.shape
-    if len(kshape) != 4 and len(kshape) != 5:
-        raise RuntimeError(f"{name}: the cache's buffers must be those of quant_cache")
-    *lead, H, C, D = kshape
-    n, store, dtype = C // QUANT_BLOCK, c.k.dtype, c.k_tail.dtype
-    if (c.v.shape != (*lead, H, n, D, QUANT_BLOCK) or c.k_scale.shape != (*lead, H, n)
-            or c.v_scale.shape != c.k_scale.shape or c.k_tail.shape != (*lead, H, 2 * QUANT_BLOCK, D)
-            or c.v_tail.shape != c.k_tail.shape or C % QUANT_BLOCK or store not in _STORE_CODE
-            or c.v.dtype is not store or not c.k_scale.dtype is c.v_scale.dtype is torch.float32
-            or (dtype is not torch.bfloat16 and dtype is not torch.float16) or c.v_tail.dtype is not dtype):
-        raise RuntimeError(f"{name}: the cache's buffers must be those of quant_cache")
-    for t in c:
-        if not t.is_contiguous():
-            raise RuntimeError(f"{name}: the cache's buffers must be contiguous")
-    return lead, H, C, D, len(kshape) == 5
+def _quant_device(name: str, cache: QuantCache, *ts) -> int:
+    """The device that the cache and ``ts`` (None left out) are on."""
+    index = cache.index
+    if index < 0:
+        raise RuntimeError(f"{name}: all tensors must be on one ROCm (cuda) device")
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"{name}: all tensors must be on one ROCm (cuda) device")
+    return index
 
 
-def _layer_counts(name: str, n_rows: torch.Tensor, lead, layers: bool):
+def _layer_counts(name: str, n_rows: torch.Tensor, cache: QuantCache):
     """Strides {layer, batch} of the stored rows' counts."""
-    nshape, B = n_rows.shape, lead[-1]
-    if n_rows.dtype is not torch.int32 or len(nshape) != len(lead) or nshape[-1] not in (1, B) or (
-            layers and nshape[0] != lead[0]):
+    nshape, lead = n_rows.shape, cache.lead
+    if n_rows.dtype is not torch.int32 or len(nshape) != len(lead) or (nshape[-1] != 1 and nshape[-1] != lead[-1]) or (
+            cache.layers and nshape[0] != lead[0]):
         raise RuntimeError(f"{name}: n_rows must be int32, [1] or [B], or [N, 1] or [N, B]")
     ns = n_rows.stride()
-    return (ns[0] if layers else 0), (ns[-1] if nshape[-1] > 1 else 0)
+    return (ns[0] if cache.layers else 0), (ns[-1] if nshape[-1] > 1 else 0)
 
 
 _QAPPEND_ARGS = _lib.ARGS["dropkv_quant_append"].pack
@@ -727,36 +749,42 @@ def quant_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor, n_rows: to
     (else all L); ``path`` [B, L] int32: row i is row ``path[b, i]`` (what
     ``tree_commit`` returns).  Rows beyond the capacity are dropped.  k and v must
     not lie in the cache's own buffers."""
-    index = _device_index("quant_append", k, v, n_rows, path, counts, *cache)
+    index = _quant_device("quant_append", cache, k, v, n_rows, path, counts)
     if _differentiating():
         _no_grad("quant_append", k, v, *cache)
-    lead, H, C, D, layers = _quant_shape("quant_append", cache)
-    shape, dtype = k.shape, k.dtype
-    if len(shape) != len(lead) + 3 or shape[:-2] != (*lead, H) or shape[-1] != D or v.shape != shape:
+    lead, H, D, layers, dtype = cache.lead, cache.H, cache.D, cache.layers, cache.dtype
+    shape = k.shape
+    if len(shape) != len(lead) + 3 or v.shape != shape:
         raise RuntimeError("quant_append: k and v must be [B, H, L, D] or [N, B, H, L, D], as the cache")
-    if dtype is not cache.k_tail.dtype or v.dtype is not dtype:
-        raise RuntimeError("quant_append: k and v must have the cache's dtype")
     L, B = shape[-2], lead[-1]
-    n_sn, n_sb = _layer_counts("quant_append", n_rows, lead, layers)
+    if shape != (*lead, H, L, D):
+        raise RuntimeError("quant_append: k and v must be [B, H, L, D] or [N, B, H, L, D], as the cache")
+    if k.dtype is not dtype or v.dtype is not dtype:
+        raise RuntimeError("quant_append: k and v must have the cache's dtype")
+    n_sn, n_sb = _layer_counts("quant_append", n_rows, cache)
+    c_ptr = p_ptr = 0
     if counts is not None:
         if counts.dtype is not torch.int32 or counts.shape != (B,):
             raise RuntimeError("quant_append: counts must be int32 [B]")
         counts = counts.contiguous()
+        c_ptr = counts.data_ptr()
     if path is not None:
         if path.dtype is not torch.int32 or path.shape != (B, L):
             raise RuntimeError("quant_append: path must be int32 [B, L]")
         path = path.contiguous()
-    if not (L and B and H):
+        p_ptr = path.data_ptr()
+    if not L:
         return
-    k, v = _rows(k), _rows(v)
     ks, vs = k.stride(), v.stride()
+    if ks[-1] != 1:
+        ks = (k := k.contiguous()).stride()
+    if vs[-1] != 1:
+        vs = (v := v.contiguous()).stride()
     if not layers:
         ks, vs = (0, *ks), (0, *vs)
     _call("dropkv_quant_append", index, _QAPPEND_ARGS(
-        k.data_ptr(), *ks[:4], v.data_ptr(), *vs[:4], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-        cache.v_scale.data_ptr(), cache.k_tail.data_ptr(), cache.v_tail.data_ptr(), n_rows.data_ptr(), n_sn, n_sb,
-        0 if counts is None else counts.data_ptr(), 0 if path is None else path.data_ptr(), _DTYPE_CODE[dtype],
-        _STORE_CODE[cache.k.dtype], lead[0] if layers else 1, B, H, L, D, C))
+        k.data_ptr(), *ks[:4], v.data_ptr(), *vs[:4], *cache.pointers(), n_rows.data_ptr(), n_sn, n_sb, c_ptr, p_ptr,
+        *cache.codes, lead[0] if layers else 1, B, H, L, D, cache.capacity))
 
 
 _QREAD_ARGS = _lib.ARGS["dropkv_quant_read"].pack
@@ -766,20 +794,19 @@ def quant_read(cache: QuantCache, n_rows: torch.Tensor, rows: int, first: int = 
     """Rows ``first .. first + rows - 1`` of every head as new tensors ``(k, v)``
     [B, H, rows, D] (or [N, B, H, rows, D]) of the cache's 16-bit dtype
     (``dropkv_quant_read``); zeros behind the ``n_rows`` that are stored."""
-    index = _device_index("quant_read", n_rows, *cache)
+    index = _quant_device("quant_read", cache, n_rows)
     if _differentiating():
         _no_grad("quant_read", *cache)
-    lead, H, C, D, layers = _quant_shape("quant_read", cache)
-    if rows < 0 or first < 0 or first + rows > C:
-        raise RuntimeError(f"quant_read: rows must lie within the capacity of {C}")
-    n_sn, n_sb = _layer_counts("quant_read", n_rows, lead, layers)
+    lead, H, D = cache.lead, cache.H, cache.D
+    if rows < 0 or first < 0 or first + rows > cache.capacity:
+        raise RuntimeError(f"quant_read: rows must lie within the capacity of {cache.capacity}")
+    n_sn, n_sb = _layer_counts("quant_read", n_rows, cache)
     k = cache.k_tail.new_empty((*lead, H, rows, D))
     v = torch.empty_like(k)
-    if k.numel():
+    if rows:
         _call("dropkv_quant_read", index, _QREAD_ARGS(
-            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-            cache.k_tail.data_ptr(), cache.v_tail.data_ptr(), n_rows.data_ptr(), n_sn, n_sb, k.data_ptr(), v.data_ptr(),
-            _DTYPE_CODE[k.dtype], _STORE_CODE[cache.k.dtype], lead[0] if layers else 1, lead[-1], H, rows, D, C, first))
+            *cache.pointers(), n_rows.data_ptr(), n_sn, n_sb, k.data_ptr(), v.data_ptr(), *cache.codes,
+            lead[0] if cache.layers else 1, lead[-1], H, rows, D, cache.capacity, first))
     return k, v
 
 
@@ -809,19 +836,18 @@ def quant_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, c
     one layer's ``cache`` in the place of the buffers.  Returns ``out`` [B, T, Hq, D],
     which must not lie in an input.  The cache is not written: ``quant_append``
     stores the rows."""
-    index = _device_index("quant_attention", q, k_new, v_new, n_rows, out, workspace, mask, *cache)
+    index = _quant_device("quant_attention", cache, q, k_new, v_new, n_rows, out, workspace, mask)
     if _differentiating():
         _no_grad("quant_attention", q, k_new, v_new, out, *cache)
-    lead, Hkv, C, D, layers = _quant_shape("quant_attention", cache)
-    dtype, shape, kshape = q.dtype, q.shape, k_new.shape
-    if layers:
+    Hkv, C, D, dtype, shape, kshape = cache.H, cache.capacity, cache.D, cache.dtype, q.shape, k_new.shape
+    if cache.layers:
         raise RuntimeError("quant_attention: takes one layer of the cache (cache.layer(i))")
-    if not dtype is k_new.dtype is v_new.dtype is cache.k_tail.dtype:
+    if not dtype is q.dtype is k_new.dtype is v_new.dtype:
         raise RuntimeError("quant_attention: q, k_new and v_new must have the cache's dtype")
     if len(shape) != 4:
         raise RuntimeError("quant_attention: q must be [B, Hq, T, D]")
     B, Hq, T, qD = shape
-    if lead[0] != B or qD != D or kshape != (B, Hkv, T, D) or v_new.shape != kshape:
+    if cache.lead[0] != B or qD != D or kshape != (B, Hkv, T, D) or v_new.shape != kshape:
         raise RuntimeError("quant_attention: q, k_new, v_new and the cache do not fit one another")
     counts = n_rows.numel()
     if n_rows.dtype is not torch.int32 or (counts != 1 and counts != B) or not n_rows.is_contiguous():
@@ -849,17 +875,20 @@ def quant_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, c
         workspace = _stream_workspace(nbytes, q.device)
     elif not workspace.is_contiguous():
         raise RuntimeError("quant_attention: the workspace must be contiguous")
-    q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)
-    q_b, q_h, q_t, _ = q.stride()
-    kn_b, kn_h, kn_t, _ = k_new.stride()
-    vn_b, vn_h, vn_t, _ = v_new.stride()
+    q_b, q_h, q_t, q_d = q.stride()
+    if q_d != 1:
+        q_b, q_h, q_t, _ = (q := q.contiguous()).stride()
+    kn_b, kn_h, kn_t, kn_d = k_new.stride()
+    if kn_d != 1:
+        kn_b, kn_h, kn_t, _ = (k_new := k_new.contiguous()).stride()
+    vn_b, vn_h, vn_t, vn_d = v_new.stride()
+    if vn_d != 1:
+        vn_b, vn_h, vn_t, _ = (v_new := v_new.contiguous()).stride()
     o_b, o_t, o_h, _ = out.stride()
     _call("dropkv_quant_attention", index, _QATTN_ARGS(
         q.data_ptr(), q_b, q_h, q_t, k_new.data_ptr(), kn_b, kn_h, kn_t, v_new.data_ptr(), vn_b, vn_h, vn_t,
-        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-        cache.k_tail.data_ptr(), cache.v_tail.data_ptr(), n_rows.data_ptr(), counts > 1, m_ptr, m_b, m_t, m_j,
-        _DTYPE_CODE[dtype], _STORE_CODE[cache.k.dtype], B, Hq, Hkv, T, D, C, scale, out.data_ptr(), o_b, o_t, o_h,
-        workspace.data_ptr(), workspace.nbytes))
+        *cache.pointers(), n_rows.data_ptr(), counts > 1, m_ptr, m_b, m_t, m_j, *cache.codes, B, Hq, Hkv, T, D, C, scale,
+        out.data_ptr(), o_b, o_t, o_h, workspace.data_ptr(), workspace.nbytes))
     return out
 
 
@@ -1075,7 +1104,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
         d_ptr, (d_b, d_t, _) = draft_logits.data_ptr(), draft_logits.stride()
     nbytes = _verify_bytes(B, T, V, d_ptr != 0)
     if nbytes == 0:
-        raise RuntimeError("verify_drafts: T must be at most 256, V at most 2^30, B * (2 T - 1) below 2^17")
+        raise RuntimeError("verify_drafts: T must be at most 256, V at most 2^26, B * (2 T - 1) below 2^17, "
+                           "B * V below 2^33")
     ws = _stream_workspace(nbytes, logits.device)
     x_b, x_t, _ = logits.stride()
     _call("dropkv_verify_drafts", index, _VERIFY_ARGS(

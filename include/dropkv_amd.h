@@ -600,7 +600,8 @@ int dropkv_quant_attention(const dropkv_quant_attention_args* args, void* stream
  *            last the one drawn), then -1: what dropkv_tree_commit takes
  *   accepted [B] int32: how many; logprobs [B, T] fp32: ln p of each, then 0
  * A sampled row that holds +inf or NaN, or only -inf, gives -1 and NaN.
- * 1 <= T <= 256, V <= 2^30, 0 < temperature < inf, B * (2 T - 1) < 2^17.  The
+ * 1 <= T <= 256, V <= 2^26, 1e-30 < temperature < 1e30, B * (2 T - 1) < 2^17,
+ * B * V < 2^33.  The
  * workspace needs no initialisation; its first DROPKV_SYNC_BYTES are left alone. */
 typedef struct {
   const void* logits;
