@@ -101,7 +101,9 @@ int check_quant_cache(const void* k, const void* v, const void* k_scale, const v
   if (!decode_head_dim_supported(D)) return fail(DROPKV_E_UNSUPPORTED, "head dim %lld not supported", (long long)D);
   if (capacity < 64 || capacity % 64 || capacity > ((int64_t)1 << 30) / D)
     return fail(DROPKV_E_ARG, "capacity must be a multiple of 64, capacity * D at most 2^30");
-  for (const void* p : {k, v, k_scale, v_scale, k_tail, v_tail})
+  if ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 3u)
+    return fail(DROPKV_E_ARG, "the scales must be 4-byte aligned");
+  for (const void* p : {k, v, k_tail, v_tail})
     if (!aligned16(p)) return fail(DROPKV_E_ARG, "the cache's buffers must be 16-byte aligned");
   return DROPKV_OK;
 }

@@ -16,7 +16,13 @@ a tree (or chain) of them, a captured graph too, whose attention rotates
 queries and keys and lays out the drafted rows (``dropkv_norm_rope``), attends
 over the cache and the tree (``dropkv_tree_attention``), and whose end takes the
 best token at every node (``dropkv_token_logprobs``) and appends the rows of the
-path that stands to every layer's buffer (``dropkv_tree_commit``).
+path that stands to every layer's buffer (``dropkv_tree_commit``).  A chain of
+drafted tokens may be verified by sampling instead, from given random numbers
+(``dropkv_verify_drafts``).
+
+With ``cache_dtype`` the rows are held in 8 bits with a scale for each block of 64
+rows and head: half the memory, and half the bytes that a step reads
+(``dropkv_quant_append``, ``dropkv_quant_attention``).
 """
 
 from __future__ import annotations
@@ -41,7 +47,7 @@ def _decode_attention(module, query, key, value, attention_mask=None, scaling=No
     dec = getattr(_active, "decoder", None)
     if dec is None:
         raise RuntimeError("dropkv_decode attention used outside CompressedDecoder")
-    if dec.tree_size:
+    if dec.drafts:
         return dec._tree_attention(module, query, key, value, scaling, kwargs.get("sliding_window")), None
     if query.shape[2] != 1:
         raise RuntimeError("dropkv_decode attention takes one query position per step")
@@ -129,9 +135,18 @@ class CompressedDecoder:
     With ``tree_size`` T, :meth:`set_tree` and :meth:`verify` take up to T
     drafted tokens in one forward; sequences of a batch then advance by their
     own number of tokens.
+
+    With ``cache_dtype`` (``"int8"``, ``"fp8"`` or the torch dtypes) the rows are held
+    in 8 bits (``self.cache``, an :class:`ops.QuantCache` of all layers) in the place of
+    ``k_buf`` / ``v_buf``.
     """
 
-    def __init__(self, model, cache, max_new_tokens: int, use_graph: bool = True, tree_size: int = 0):
+    _STORES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn, torch.int8: torch.int8,
+               torch.float8_e4m3fn: torch.float8_e4m3fn}
+
+    def __init__(self, model, cache, max_new_tokens: int, use_graph: bool = True, tree_size: int = 0, cache_dtype=None):
+        if cache_dtype is not None and cache_dtype not in self._STORES:
+            raise ValueError(f"cache_dtype must be 'int8', 'fp8' or None, got {cache_dtype!r}")
         _register()
         self.model = model
         self.tree_size = int(tree_size)
@@ -148,39 +163,58 @@ class CompressedDecoder:
         # (A verification that starts below max_new_tokens may end past it.)
         self.capacity = (max(stored) + max_new_tokens + self.tree_size + 63) // 64 * 64
         self.max_new_tokens = max_new_tokens
+        # Rows of a forward's own, which its end appends: of drafted tokens, or, with
+        # rows in 8 bits, of a step's one token too.
+        self.drafts = self.tree_size or (1 if cache_dtype is not None else 0)
         self.k_buf, self.v_buf = [], []
-        if self.tree_size:
-            self._k_all = torch.empty(len(kv), B, Hkv, self.capacity, D, dtype=k0.dtype, device=self.device)
-            self._v_all = torch.empty_like(self._k_all)
-        for i, (k, v) in enumerate(kv):
+        self.cache: Optional[ops.QuantCache] = None
+        if cache_dtype is not None:
+            self.cache = ops.quant_cache(B, Hkv, self.capacity, D, dtype=k0.dtype, store=self._STORES[cache_dtype],
+                                         layers=len(kv), device=self.device)
+            self._layers = [self.cache.layer(i) for i in range(len(kv))]
+            empty = torch.zeros(1, dtype=torch.int32, device=self.device)
+            with torch.no_grad():
+                for one, (k, v) in zip(self._layers, kv):
+                    ops.quant_append(one, k, v, empty)
+            # (A buffer without room: which drafts stand is asked of tree_commit, their
+            # rows are appended by quant_append.)
+            self._no_room = torch.zeros(B, 1, 1, D, dtype=k0.dtype, device=self.device)
+            self._full = torch.ones(1, dtype=torch.int32, device=self.device)
+        else:
             if self.tree_size:
-                kb, vb = self._k_all[i], self._v_all[i]
-            else:
-                kb = torch.empty(B, Hkv, self.capacity, D, dtype=k.dtype, device=self.device)
-                vb = torch.empty_like(kb)
-            kb[:, :, :k.shape[2]].copy_(k)
-            vb[:, :, :v.shape[2]].copy_(v)
-            self.k_buf.append(kb)
-            self.v_buf.append(vb)
+                self._k_all = torch.empty(len(kv), B, Hkv, self.capacity, D, dtype=k0.dtype, device=self.device)
+                self._v_all = torch.empty_like(self._k_all)
+            for i, (k, v) in enumerate(kv):
+                if self.tree_size:
+                    kb, vb = self._k_all[i], self._v_all[i]
+                else:
+                    kb = torch.empty(B, Hkv, self.capacity, D, dtype=k.dtype, device=self.device)
+                    vb = torch.empty_like(kb)
+                kb[:, :, :k.shape[2]].copy_(k)
+                vb[:, :, :v.shape[2]].copy_(v)
+                self.k_buf.append(kb)
+                self.v_buf.append(vb)
         self.n_rows = torch.tensor(stored, dtype=torch.int32, device=self.device)
         Hq = model.config.num_attention_heads
         self.logical = cache.get_seq_length()
-        if self.tree_size:
-            T = self.tree_size
+        if self.drafts:
+            T = self.drafts
             self.n_rows = self.n_rows[:, None].repeat(1, B)
             self._k_draft = torch.empty(len(kv), B, Hkv, T, D, dtype=k0.dtype, device=self.device)
             self._v_draft = torch.empty_like(self._k_draft)
             # (One token takes more splits than a tree of them.)
-            self.ws = max((ops.tree_workspace(B, Hq, Hkv, D, t, self.capacity, self.device) for t in (1, T)),
+            workspace = ops.tree_workspace if self.cache is None else ops.quant_workspace
+            self.ws = max((workspace(B, Hq, Hkv, D, t, self.capacity, self.device) for t in (1, T)),
                           key=torch.Tensor.numel)
+        else:
+            self.ws = ops.decode_workspace(B, Hq, Hkv, D, self.capacity, self.device)
+        if self.tree_size:
             self._tree_tok = torch.zeros(B, T, dtype=torch.int64, device=self.device)
             self._tree_parents = torch.zeros(B, T, dtype=torch.int32, device=self.device)
             self._tree_depth = torch.zeros(B, T, dtype=torch.int64, device=self.device)
             self._tree_mask = torch.zeros(B, T, T, dtype=torch.bool, device=self.device)
             self._root = torch.zeros(1, dtype=torch.int32, device=self.device)
             self.set_tree(range(-1, T - 1))
-        else:
-            self.ws = ops.decode_workspace(B, Hq, Hkv, D, self.capacity, self.device)
         self.pos = torch.full((B, 1), self.logical, dtype=torch.int64, device=self.device)
         self.tok = torch.zeros(B, 1, dtype=torch.int64, device=self.device)
         self.steps = 0
@@ -188,6 +222,9 @@ class CompressedDecoder:
         self.logits: Optional[torch.Tensor] = None
         self.tree_graph: Optional[torch.cuda.CUDAGraph] = None
         self.verified: Optional[Verified] = None
+        self.use_graph = bool(use_graph)
+        self.logits_graph: Optional[torch.cuda.CUDAGraph] = None  # of a verification by sampling: the forward alone
+        self._tree_logits_out: Optional[torch.Tensor] = None
         if use_graph:
             self._capture()
 
@@ -197,7 +234,7 @@ class CompressedDecoder:
         _active.decoder = self
         try:
             with _own_attention(self.model.config), (
-                    rotary_deferral(self._defer) if self.tree_size else contextlib.nullcontext()):
+                    rotary_deferral(self._defer) if self.drafts else contextlib.nullcontext()):
                 yield
         finally:
             _active.decoder = prev
@@ -214,7 +251,7 @@ class CompressedDecoder:
         """One layer of a forward over T tokens: rows into the drafts' buffers,
         then attention over cache and drafts.  [B, T, Hq, D]."""
         if sliding_window is not None:
-            raise RuntimeError("a decoder with tree_size takes no layers with a sliding window")
+            raise RuntimeError("a decoder with tree_size or cache_dtype takes no layers with a sliding window")
         i = module.layer_idx
         T, D = query.shape[2], query.shape[3]
         k_new, v_new = self._k_draft[i, :, :, :T], self._v_draft[i, :, :, :T]
@@ -224,30 +261,49 @@ class CompressedDecoder:
         else:  # a layer whose rotation was not deferred
             k_new.copy_(key)
             v_new.copy_(value)
-        return ops.tree_attention(query, k_new, v_new, self.k_buf[i], self.v_buf[i], self.n_rows[i],
-                                  scaling if scaling is not None else D ** -0.5, workspace=self.ws,
-                                  mask=self._tree_mask if T > 1 else None)
+        scale, mask = scaling if scaling is not None else D ** -0.5, self._tree_mask if T > 1 else None
+        if self.cache is not None:
+            return ops.quant_attention(query, k_new, v_new, self._layers[i], self.n_rows[i], scale, workspace=self.ws,
+                                       mask=mask)
+        return ops.tree_attention(query, k_new, v_new, self.k_buf[i], self.v_buf[i], self.n_rows[i], scale,
+                                  workspace=self.ws, mask=mask)
 
     def _advance(self):
         """After a forward over one token: its row counts."""
-        if self.tree_size:
+        if self.cache is not None:
+            ops.quant_append(self.cache, self._k_draft[:, :, :, :1], self._v_draft[:, :, :, :1], self.n_rows)
+        elif self.tree_size:
             ops.tree_commit(self.tok, self._root, self.tok, self._k_draft[:, :, :, :1], self._v_draft[:, :, :, :1],
                             self._k_all, self._v_all, self.n_rows)
         self.n_rows.add_(1)
         self.pos.add_(1)
 
+    def _commit(self, tokens, choice, store: bool = True):
+        """The path of the drafted tokens that stands, its rows appended."""
+        if self.cache is None:
+            return ops.tree_commit(tokens, self._tree_parents, choice, self._k_draft, self._v_draft, self._k_all,
+                                   self._v_all, self.n_rows)
+        path, accepted = ops.tree_commit(tokens, self._tree_parents, choice, self._k_draft[0, :, :1],
+                                         self._v_draft[0, :, :1], self._no_room, self._no_room, self._full)
+        ops.quant_append(self.cache, self._k_draft, self._v_draft, self.n_rows, path=path,
+                         counts=accepted if store else torch.zeros_like(accepted))
+        return path, accepted
+
     @torch.no_grad()
-    def _tree_forward(self) -> Verified:
-        """A forward over the drafted tokens, and the path of them that stands.
-        The counts are not advanced."""
+    def _tree_logits(self) -> torch.Tensor:
         with self._active():
             # (A negative token has no embedding, and equals no best token.)
-            logits = self.model(self._tree_tok.clamp(min=0), position_ids=self.pos + self._tree_depth,
-                                past_key_values=_StepCache(self.logical), use_cache=True).logits
+            return self.model(self._tree_tok.clamp(min=0), position_ids=self.pos + self._tree_depth,
+                              past_key_values=_StepCache(self.logical), use_cache=True).logits
+
+    @torch.no_grad()
+    def _tree_forward(self, store: bool = True) -> Verified:
+        """A forward over the drafted tokens, and the path of them that stands.
+        The counts are not advanced."""
+        logits = self._tree_logits()
         best = ops.token_logprobs(logits, top=1)
         choice = best.top_ids[..., 0]
-        path, accepted = ops.tree_commit(self._tree_tok, self._tree_parents, choice, self._k_draft, self._v_draft,
-                                         self._k_all, self._v_all, self.n_rows)
+        path, accepted = self._commit(self._tree_tok, choice, store)
         on, at = path >= 0, path.clamp(min=0).long()
         return Verified(torch.where(on, choice.gather(1, at), -1),
                         torch.where(on, best.top_logprobs[..., 0].gather(1, at), 0.0), accepted, path, logits)
@@ -263,18 +319,26 @@ class CompressedDecoder:
                              use_cache=True, logits_to_keep=1)
         return out.logits
 
-    @torch.no_grad()
-    def _capture(self):
-        # One eager run on a side stream first (library workspaces, lazy
-        # initialisation); it stores a row at n that the first replay rewrites.
+    def _beside(self, run):
+        """``run()`` on a stream of its own, between two waits."""
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
-            self._forward()
-            if self.tree_size:
-                self._tree_forward()
+            run()
         torch.cuda.current_stream(self.device).wait_stream(side)
         torch.cuda.synchronize(self.device)
+
+    @torch.no_grad()
+    def _capture(self):
+        # One eager run on a side stream first (library workspaces, lazy
+        # initialisation); it stores a row at n that the first replay rewrites (in 8
+        # bits none: a block that it filled up would have lost the rows before it).
+        def once():
+            self._forward()
+            if self.tree_size:
+                self._tree_forward(store=self.cache is None)
+
+        self._beside(once)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.logits = self._forward()
@@ -335,31 +399,85 @@ class CompressedDecoder:
             depth[:, i] = torch.where(child, depth[rows, up] + 1, 0)
             mask[:, i] |= mask[rows, up] & child[:, None]
         self.tree_nodes = t
+        self._is_chain = bool((full[:, :t] == torch.arange(-1, t - 1)).all())
         self._tree_parents.copy_(full.to(torch.int32))
         self._tree_depth.copy_(depth)
         self._tree_mask.copy_(mask)
 
     @torch.no_grad()
-    def verify(self, tokens: torch.Tensor) -> Verified:
+    def verify(self, tokens: torch.Tensor, uniforms: Optional[torch.Tensor] = None,
+               draft_logits: Optional[torch.Tensor] = None, temperature: float = 1.0) -> Verified:
         """One forward over the tree: ``tokens`` [B, t], the last token of each
         sequence at node 0 and drafted ones at the others (a negative one never
         stands: it may fill a node that is left out).  From the root on the path
         follows the children that the model's best token agrees with; the rows of
         its nodes are appended and the positions advanced, by ``accepted`` tokens
-        a sequence, of which the last is the model's own."""
+        a sequence, of which the last is the model's own.
+
+        With ``uniforms`` ([B, t] fp32 in [0, 1)) the tokens are judged and drawn by
+        sampling instead, at ``temperature``, and the tree has to be a chain:
+        ``draft_logits`` [B, t - 1, vocab] is what the drafts were drawn from, without
+        it they are taken as given (:func:`ops.verify_drafts`)."""
         if not self.tree_size:
             raise RuntimeError("the decoder was made without tree_size")
-        if tuple(tokens.shape) != (self._tree_tok.shape[0], self.tree_nodes):
-            raise ValueError(f"tokens must be [{self._tree_tok.shape[0]}, {self.tree_nodes}], as the tree")
+        t = self.tree_nodes
+        if tuple(tokens.shape) != (self._tree_tok.shape[0], t):
+            raise ValueError(f"tokens must be [{self._tree_tok.shape[0]}, {t}], as the tree")
+        if uniforms is None:
+            if draft_logits is not None or temperature != 1.0:
+                raise ValueError("draft_logits and temperature go with uniforms")
+        elif not self._is_chain:
+            raise ValueError("tokens are verified by sampling along a chain (set_tree(range(-1, t - 1)))")
+        elif tuple(uniforms.shape) != tuple(tokens.shape):
+            raise ValueError("uniforms must have the tokens' shape")
         self._check_room()
-        self._tree_tok[:, :self.tree_nodes].copy_(tokens)
-        self.steps += self.tree_nodes
+        self._tree_tok[:, :t].copy_(tokens)
+        if uniforms is not None:
+            return self._verify_sampled(t, uniforms, draft_logits, temperature)
+        self.steps += t
         if self.tree_graph is not None:
             self.tree_graph.replay()
             return self.verified
         v = self._tree_forward()
         self._tree_advance(v)
         return v
+
+    def _verify_sampled(self, t: int, uniforms, draft_logits, temperature) -> Verified:
+        """The forward (a graph of its own, captured at the first call), then the chain
+        judged and its rows appended."""
+        if self.use_graph and self.logits_graph is None:
+            self._beside(self._tree_logits)
+            self.logits_graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.logits_graph):
+                self._tree_logits_out = self._tree_logits()
+        if self.logits_graph is not None:
+            self.logits_graph.replay()
+            logits = self._tree_logits_out
+        else:
+            logits = self._tree_logits()
+        tokens = self._tree_tok
+        choice, accepted, logprobs = ops.verify_drafts(logits[:, :t], tokens[:, :t], uniforms, draft_logits, temperature)
+        T = tokens.shape[1]
+        if t < T:
+            choice = torch.nn.functional.pad(choice, (0, T - t), value=-1)
+            logprobs = torch.nn.functional.pad(logprobs, (0, T - t))
+        # (The nodes that stand are known: no other equals a choice.)
+        on = torch.arange(T, device=tokens.device) < accepted[:, None]
+        path, _ = self._commit(torch.where(on, tokens, -2), choice)
+        self.steps += t
+        v = Verified(choice, logprobs, accepted, path, logits)
+        self._tree_advance(v)
+        return v
+
+    @torch.no_grad()
+    def stored(self, layer: int):
+        """Layer ``layer``'s rows (k, v) [B, Hkv, n, D], n the longest sequence's count
+        (asked of the device): views of the buffers, or new tensors read back from 8
+        bits, then zeros behind a shorter sequence's rows."""
+        n = int(self.n_rows[layer].max())
+        if self.cache is not None:
+            return ops.quant_read(self._layers[layer], self.n_rows[layer], n)
+        return self.k_buf[layer][:, :, :n], self.v_buf[layer][:, :, :n]
 
     @torch.no_grad()
     def generate(self, token: torch.Tensor, steps: int) -> torch.Tensor:

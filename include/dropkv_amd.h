@@ -486,7 +486,8 @@ int dropkv_token_logprobs(const dropkv_token_logprobs_args* args, void* stream);
  * for s q.  A block whose a is below 2^-100 is zeros; one that holds a value that is
  * not finite reads as NaN.  The rows of the last block, while it is not full, are
  * kept as they are.  Buffers (N layers, 1 where there is no such axis; capacity a
- * multiple of 64), all contiguous and 16-byte aligned, zeros at first:
+ * multiple of 64), all contiguous and (but for the scales) 16-byte aligned, zeros at
+ * first:
  *   k        [N, B, H, capacity, D] bytes
  *   v        [N, B, H, capacity / 64, D, 64] bytes: transposed within the block
  *   k_scale, v_scale  [N, B, H, capacity / 64] fp32: s
