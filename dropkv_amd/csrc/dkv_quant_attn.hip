@@ -30,6 +30,7 @@ struct QuantAttnArgs : TreeArgs {  // (kbuf, vbuf: the 8-bit blocks)
   const float* vs;
   const void* ktail;  // [B, Hkv, 128, D]
   const void* vtail;
+  uint32_t* arrived;  // [B, Hkv]: parts done, where the last one to arrive joins them; else null
 };
 
 struct QuantCut {
@@ -119,7 +120,8 @@ __device__ __forceinline__ bool near_take_out(T* rows, int pitch, const Near& s,
 // matrix operands straight into registers, the next block's loads issued as soon as
 // a block's registers are consumed.  P goes into the product in two parts, rounded
 // and remainder.  The waves' results are joined in LDS; the only part's workgroup
-// writes the output.
+// writes the output.  Of several parts the last workgroup to arrive joins them, where
+// they are few bytes (FIG1); more are joined by a second kernel.
 constexpr int kNarrowWaves = 4;
 template <typename T, typename S, int D>
 __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(QuantAttnArgs a) {
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
   __shared__ __attribute__((aligned(16))) char lds[kLds];
   __shared__ uint64_t mask_words[16];  // (T <= 16 rows)
   __shared__ float part_m[NW][16], part_l[NW][16];
-  __shared__ int odd_flag;
+  __shared__ int odd_flag, last;
 
   const TreePart part = tree_part<QuantCut>(a, hkv, slot, lane);
   const int b = part.b;
@@ -345,12 +347,12 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[d0 + e] = static_cast<T>(l == 0.f ? 0.f : acc[e] * inv);
       } else {
-        *reinterpret_cast<f32x4*>(a.part_o + base * D + d0) = acc;
+        st_dev16(make_rsrc(a.part_o + base * D, D * 4u), d0 * 4u, acc);
       }
     }
     if (!a.direct && (threadIdx.x & 15) == 0) {
-      a.part_m[base] = mx;
-      a.part_l[base] = l;
+      st_dev(a.part_m + base, mx);
+      st_dev(a.part_l + base, l);
     }
   }
   if (__builtin_expect(odd_flag, 0)) {
@@ -358,6 +360,71 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
     __syncthreads();
     tree_add_odd<T, D, 64 * NW>(a, b, hkv, slot, 0, 16);
   }
+  if (!a.arrived) return;
+  // (Every wave's stores are out first.  The counter is zero before the call and wraps
+  // to zero.)
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = atomicInc(a.arrived + bh, (uint32_t)part.count - 1u) == (uint32_t)part.count - 1u;
+    if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  }
+  __syncthreads();
+  if (!last || row >= a.M) return;
+  // 16 threads a row: 16 parts' maxima and sums a thread each, and the partial rows, in
+  // one round trip.
+  const int sub = threadIdx.x & 15;
+  const int64_t at0 = ((int64_t)hkv * a.P + part.first) * a.M + row;
+  // (Ragged sequences may have more than 16.)
+  f32x4 acc[D / 64];
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float mx = -__FLT_MAX__, l = 0.f;
+#pragma unroll 1
+  for (int s0 = 0; s0 < part.count; s0 += 16) {
+    const int s = s0 + sub;
+    const float pm = s < part.count ? a.part_m[at0 + (int64_t)s * a.M] : -__FLT_MAX__;
+    const float pl = s < part.count ? a.part_l[at0 + (int64_t)s * a.M] : 0.f;
+    f32x4 x[16][D / 64];
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        x[k][c] = *reinterpret_cast<const f32x4*>(a.part_o + (at0 + (int64_t)min(s0 + k, part.count - 1) * a.M) * D +
+                                                  4 * sub + 64 * c);
+    float top = pm;
+    top = fmaxf(top, dpp_f<kDppQuadSwap1>(top));
+    top = fmaxf(top, dpp_f<kDppQuadSwap2>(top));
+    top = fmaxf(top, dpp_f<kDppHalfMirror>(top));
+    top = fmaxf(top, dpp_f<kDppMirror>(top));
+    top = fmaxf(mx, top);
+    const float turn = __builtin_amdgcn_exp2f(mx - top), f = s < part.count ? __builtin_amdgcn_exp2f(pm - top) : 0.f;
+    mx = top;
+    float sum = pl * f;
+    sum += dpp_f<kDppQuadSwap1>(sum);
+    sum += dpp_f<kDppQuadSwap2>(sum);
+    sum += dpp_f<kDppHalfMirror>(sum);
+    sum += dpp_f<kDppMirror>(sum);
+    l = l * turn + sum;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) acc[c] *= turn;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float fk = __shfl(f, (lane & 48) | k);
+      if (s0 + k < part.count)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[c][e] = fmaf(fk, x[k][c][e], acc[c][e]);
+    }
+  }
+  const int hr = a.div_t.div(row), tr = row - hr * a.T;
+  T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)tr * a.o_st + (int64_t)(hkv * g + hr) * a.o_sh;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[4 * sub + 64 * c + e] = static_cast<T>(l == 0.f ? 0.f : acc[c][e] * inv);
 }
 
 // More than 16 rows: NW waves of QB blocks of 16 rows take the same keys, so that a
@@ -639,6 +706,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
 // sequence, and whether the 16-bit keys are parts of their own.
 struct QuantPlan {
   int M, rows_wg, MC, S, P, apart;
+  int one;  // the last workgroup of a KV head joins its parts
   size_t rows, bytes;
 };
 
@@ -647,7 +715,7 @@ struct QuantPlan {
 // - the longest workgroup's blocks, a block's time by the rows (narrow: a wave's, every
 //   fourth), 0.6 of it at D = 64, and longer where workgroups share a CU or take turns;
 //   or, if longer, K and V at 5.2 TB/s, where 8 MB or a quarter of them are in flight,
-//   and longer where the workgroups do not divide the CUs;
+//   and longer where the workgroups do not divide the CUs (of more than 30 MB);
 // - the partial rows, written and read at 4 TB/s, and a round trip of the joining
 //   kernel for every 16 (D = 128) or 32 parts;
 // - the kernels' fixed part.
@@ -658,6 +726,8 @@ struct QuantShape {
 };
 constexpr QuantShape kQuantShapes[] = {
     {16, 1.6, 6.9, 1.2, 2}, {64, 1.25, 8.3, 1.45, 2}, {128, 1.45, 8.5, 1.7, 2}, {256, 2.1, 8.0, 1.0, 1}};
+
+constexpr int64_t kOneJoin = 8192;  // elements
 
 static double quant_cost(const QuantShape& w, double heads, double M, double D, double blocks, int64_t S) {
   const double wgs = heads * std::ceil(M / w.rows) * S, wide = D / 128;
@@ -671,7 +741,7 @@ static double quant_cost(const QuantShape& w, double heads, double M, double D, 
   const double flight = std::min(wgs, 256.0 * w.per_cu) * (w.rows == 16 ? 65536 : 16384) * wide;
   const double bytes = heads * blocks * kQBlock * D * 2;
   double stream = bytes / 5.2e6 / std::min(1.0, flight / std::max(1.0, std::min(8e6, bytes / 4)));
-  stream *= 0.5 + 0.5 * std::ceil(wgs / 256) * 256 / wgs;
+  if (bytes > 3e7) stream *= 0.5 + 0.5 * std::ceil(wgs / 256) * 256 / wgs;
   const double join = w.rows == 16 && S == 1 ? -2.5 : S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16);
   return std::max(steps * block, stream) + join + w.fixed_us;
 }
@@ -702,6 +772,8 @@ static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
   p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
   p.apart = p.rows_wg == 64 || (p.rows_wg > 64 && heads * p.MC * p.S < 192);
   p.P = (int)(B * (p.S + p.apart));
+  // (What one workgroup reads in a round trip.)
+  p.one = p.rows_wg == 16 && p.S > 1 && p.S <= 16 && heads <= (int64_t)(kSyncBytes / sizeof(uint32_t)) && p.S * p.M * D <= kOneJoin;
   p.rows = (size_t)Hkv * p.P * p.M;
   p.bytes = kSyncBytes + kTreeDealBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
   return p;
@@ -723,7 +795,7 @@ static hipError_t launch_quant_t(const QuantAttnArgs& a, int rows_wg, hipStream_
     launch((quant_wide_kernel<T, S, D, 2, 4, kLo>), grid, dim3(256), 0, st, a);
   else
     launch((quant_wide_kernel<T, S, D, 2, 8, kLo>), grid, dim3(512), 0, st, a);
-  if (!a.direct)
+  if (!a.direct && !a.arrived)
     launch((tree_merge_kernel<T, D>), dim3((a.B * a.Hkv * a.M + 3) / 4), dim3(256), 0, st, static_cast<const TreeArgs&>(a));
   return hipGetLastError();
 }
@@ -774,6 +846,7 @@ hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* 
   a.div_t = Div::of(a.T);
   a.scale_log2 = (float)p.scale * 1.4426950408889634f;
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
+  if (pl.one) a.arrived = reinterpret_cast<uint32_t*>(ws);
   a.deal = reinterpret_cast<int*>(ws + kSyncBytes);
   a.part_m = reinterpret_cast<float*>(ws + kSyncBytes + kTreeDealBytes);
   a.part_l = a.part_m + pl.rows;

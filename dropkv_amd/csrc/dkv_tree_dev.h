@@ -98,15 +98,17 @@ __device__ __forceinline__ TreeParts tree_parts_ragged(const TreeArgs& a, int la
   return p;
 }
 // Part `slot` of a KV head: tiles t_lo .. t_hi of sequence b, whose stored rows
-// are n, and with `tail` the drafted keys; b < 0: none.
+// are n, and with `tail` the drafted keys; b < 0: none.  The sequence's parts are
+// `count` from `first` on.
 struct TreePart {
   int b, n, t_lo, t_hi;
   bool tail;
+  int first, count;
 };
 template <class Cut = TreeCut>
 __device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int hkv, int slot, int lane) {
   TreePart p;
-  if (slot >= a.B * a.S) return TreePart{slot - a.B * a.S, 0, 0, 0, true};
+  if (slot >= a.B * a.S) return TreePart{slot - a.B * a.S, 0, 0, 0, true, 0, 0};
   int first, count, per;
   if (a.ragged) {
     const TreeParts all = tree_parts_ragged<Cut>(a, lane);
@@ -115,7 +117,7 @@ __device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int hkv, int sl
       a.deal[2 * lane + 1] = all.count;
     }
     const uint64_t hit = __builtin_amdgcn_ballot_w64(all.first <= slot && slot < all.first + all.count);
-    if (!hit) return TreePart{-1, 0, 0, 0, false};
+    if (!hit) return TreePart{-1, 0, 0, 0, false, 0, 0};
     p.b = __builtin_ctzll(hit);
     first = __builtin_amdgcn_readlane(all.first, p.b);
     count = __builtin_amdgcn_readlane(all.count, p.b);
@@ -132,6 +134,8 @@ __device__ __forceinline__ TreePart tree_part(const TreeArgs& a, int hkv, int sl
   p.t_lo = min((slot - first) * per, tiles);
   p.t_hi = min(p.t_lo + per, tiles);
   p.tail = !a.apart && slot - first == count - 1;
+  p.first = first;
+  p.count = count;
   return p;
 }
 

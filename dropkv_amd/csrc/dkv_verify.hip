@@ -19,9 +19,9 @@
 // 32 entries of 8 bytes are one for each pair of LDS banks: no lanes wait for one
 // another.)
 //
-// Four kernels: maximum and sum of every row in segments; the walk, a workgroup per
-// sequence; sums of the weights that are sampled, in segments of the one row of each
-// sequence; and the token.
+// First the maximum and sum of every row, in segments; then the walk, the sums of the
+// weights that are sampled, over pieces of the one row of each sequence, and the token:
+// in one kernel for short chains, else in three.
 #include "dkv_common.h"
 #include "dkv_internal.h"
 #include "dkv_select_dev.h"
@@ -42,7 +42,6 @@ struct VfPart {
 };
 struct VfSeq {           // what the walk leaves of a sequence
   double p_mul, q_mul;   // 1 / sum of the sampled node's row, and of its draft's
-  double ln_s;           // ln of the former's sum
   float p_m, q_m;        // their maxima
   int last, token;       // the node; the token that failed there, or -1
 };
@@ -54,11 +53,12 @@ struct VerifyArgs {
   const int64_t* tokens;  // [B, T]
   const float* u;         // [B, T]
   int B, T, V, S, seg;    // segments per row, elements per segment (whole tiles)
-  int pieces;             // of the sampled rows
+  int pieces, groups;     // of the sampled rows: pieces, and workgroups of eight of them
   double mul;             // log2 e / temperature
   float deep;             // 990 / mul
   VfPart* part;           // [B, T, S], then [B, T - 1, S] of the drafts
   VfSeq* seq;             // [B]
+  uint32_t* arrived;      // [B]: workgroups done, of a call in two kernels
   double* sums;           // [B, pieces, 2]: of the weights, and of p alone
   int64_t* choice;        // [B, T]
   int* accepted;          // [B]
@@ -245,57 +245,60 @@ __device__ __forceinline__ void vf_join(const VerifyArgs& a, int64_t row, int la
   *s = wave_sum_d(vf_turned(p.s, p.m, *m, a.mul, table));
 }
 
-// One workgroup per sequence, a wave per node at a time: which nodes stand.
+// Which nodes of sequence b stand: a wave of the workgroup (kVfWide threads) per node at
+// a time.  With `write` the outputs of the nodes but the last that stands; returns
+// (to every thread) what the sampling needs.
+constexpr int kVfWide = 512;
+struct VfWalk {
+  double s[kTreeMaxT], qs[kTreeMaxT];
+  float m[kTreeMaxT], qm[kTreeMaxT];
+  int first;  // the first node that does not stand
+};
 template <typename T>
-__global__ void __launch_bounds__(512) verify_walk_kernel(VerifyArgs a) {
-  __shared__ int first;  // the first node that does not stand
-  __shared__ uint64_t table[kVfTable];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ VfSeq vf_walk(const VerifyArgs& a, int b, bool write, const uint64_t* table, VfWalk* sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t* tokens = a.tokens + (int64_t)b * a.T;
-  vf_table(table);
-  if (tid == 0) first = a.T;
+  if (tid == 0) sh->first = a.T;
   __syncthreads();
-  for (int i = 1 + wave; i < a.T; i += 8) {
-    const int64_t token = tokens[i];
-    bool stands = false;
-    float lp = 0.f;
-    if (token >= 0 && token < a.V) {
-      float m, qm;
-      double s, qs;
-      vf_join(a, (int64_t)b * a.T + i - 1, lane, table, &m, &s);
-      const float x = static_cast<float>(static_cast<const T*>(a.x)[b * a.x_sb + (i - 1) * a.x_st + token]);
-      double q = 1.;
-      if (a.y) {
-        vf_join(a, (int64_t)a.B * a.T + (int64_t)b * (a.T - 1) + i - 1, lane, table, &qm, &qs);
-        q = vf_weight(static_cast<float>(static_cast<const T*>(a.y)[b * a.y_sb + (i - 1) * a.y_st + token]), qm, a.mul, table) / qs;
-      }
-      stands = (double)a.u[(int64_t)b * a.T + i] * q < vf_weight(x, m, a.mul, table) / s;
-      lp = (float)(((double)x - (double)m) * (a.mul * kLn2) - log(s));
+  for (int i = 1 + wave; i <= a.T; i += kVfWide / 64) {  // (node T: its parent's row alone)
+    const int64_t token = i < a.T ? tokens[i] : -1;
+    const bool real = token >= 0 && token < a.V;
+    const int64_t at = real ? token : 0;
+    const bool draft = a.y && i < a.T;
+    const float x = static_cast<float>(static_cast<const T*>(a.x)[b * a.x_sb + (i - 1) * a.x_st + at]);
+    const float u = a.u[(int64_t)b * a.T + min(i, a.T - 1)];
+    float y = 0.f, m, qm = 0.f;
+    if (draft) y = static_cast<float>(static_cast<const T*>(a.y)[b * a.y_sb + (i - 1) * a.y_st + at]);
+    double s, qs = 1., q = 1.;
+    vf_join(a, (int64_t)b * a.T + i - 1, lane, table, &m, &s);
+    if (draft) {
+      vf_join(a, (int64_t)a.B * a.T + (int64_t)b * (a.T - 1) + i - 1, lane, table, &qm, &qs);
+      q = vf_weight(y, qm, a.mul, table) / qs;
     }
+    const bool stands = real && (double)u * q < vf_weight(x, m, a.mul, table) / s;
     if (lane == 0) {
-      if (!stands) atomicMin(&first, i);
-      // (Places past the node that is sampled are put right below.)
+      sh->m[i - 1] = m;
+      sh->s[i - 1] = s;
+      sh->qm[i - 1] = qm;
+      sh->qs[i - 1] = qs;
+      if (!stands && i < a.T) atomicMin(&sh->first, i);
+    }
+    if (write && stands && lane == 0) {
       a.choice[(int64_t)b * a.T + i - 1] = token;
-      a.logprob[(int64_t)b * a.T + i - 1] = lp;
+      a.logprob[(int64_t)b * a.T + i - 1] = (float)(((double)x - (double)m) * (a.mul * kLn2) - log(s));
     }
   }
   __syncthreads();
-  const int last = first - 1;
-  for (int i = last + tid; i < a.T; i += 512) {
-    a.choice[(int64_t)b * a.T + i] = -1;
-    a.logprob[(int64_t)b * a.T + i] = 0.f;
-  }
-  if (wave != 0) return;
-  float m, qm = 0.f;
-  double s, qs = 1.;
-  vf_join(a, (int64_t)b * a.T + last, lane, table, &m, &s);
+  const int last = sh->first - 1;
   const int64_t failed = last + 1 < a.T ? tokens[last + 1] : -1;
-  const bool real = failed >= 0 && failed < a.V;
-  if (real && a.y) vf_join(a, (int64_t)a.B * a.T + (int64_t)b * (a.T - 1) + last, lane, table, &qm, &qs);
-  if (lane == 0) {
-    a.accepted[b] = last + 1;
-    a.seq[b] = VfSeq{1. / s, 1. / qs, log(s), m, qm, last, real ? (int)failed : -1};
+  if (write) {
+    for (int i = last + 1 + tid; i < a.T; i += kVfWide) {
+      a.choice[(int64_t)b * a.T + i] = -1;
+      a.logprob[(int64_t)b * a.T + i] = 0.f;
+    }
+    if (tid == 0) a.accepted[b] = last + 1;
   }
+  return VfSeq{1. / sh->s[last], 1. / sh->qs[last], sh->m[last], sh->qm[last], last, failed >= 0 && failed < a.V ? (int)failed : -1};
 }
 
 // Weights of N places from j on of the sampled row: of what is left of p, and of p.
@@ -326,20 +329,15 @@ __device__ __forceinline__ void vf_weights(const VerifyArgs& a, int b, const VfS
   }
 }
 
-// Sums of both over pieces of kVfPiece places, a wave each.
+// Sums of both over piece `piece` of kVfPiece places, by a wave.
 constexpr int kVfPiece = 512;
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads) verify_sums_kernel(VerifyArgs a) {
-  __shared__ uint64_t table[kVfTable];
+__device__ __forceinline__ void vf_piece(const VerifyArgs& a, int b, const VfSeq& q, int piece, int lane,
+                                         const uint64_t* table, bool across) {
   constexpr int N = kVfPiece / 64;
-  const int groups = (a.pieces + 3) / 4, b = blockIdx.x / groups, lane = threadIdx.x & 63;
-  const int piece = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
-  vf_table(table);
-  __syncthreads();
-  if (piece >= a.pieces) return;
   float v[N];
   double w[N], p[N], sw = 0., sp = 0.;
-  vf_weights<T, N>(a, b, a.seq[b], piece * kVfPiece + lane * N, a.V, table, v, w, p);
+  vf_weights<T, N>(a, b, q, piece * kVfPiece + lane * N, a.V, table, v, w, p);
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     sw += w[e];
@@ -347,7 +345,12 @@ __global__ void __launch_bounds__(kVfThreads) verify_sums_kernel(VerifyArgs a) {
   }
   sw = wave_sum_d(sw);
   sp = wave_sum_d(sp);
-  if (lane < 2) a.sums[((int64_t)b * a.pieces + piece) * 2 + lane] = lane ? sp : sw;
+  double* to = a.sums + ((int64_t)b * a.pieces + piece) * 2 + lane;
+  if (lane >= 2) return;
+  if (across)
+    st_dev(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, lane ? sp : sw));
+  else
+    *to = lane ? sp : sw;
 }
 
 // The workgroup's first thread with a weight that is past the target, and its last
@@ -361,14 +364,16 @@ __device__ __forceinline__ void vf_mark(bool some, bool past, int lane, int wave
 
 // The token: the piece whose running sum passes u_0 times the whole, and the place in
 // it.  A thread holds one piece (of up to 262144 tokens), then one place.
+static_assert(kVfPiece == kVfWide, "a thread each");
+struct VfToken {
+  double sum_w[kVfWide / 64], sum_p[kVfWide / 64], base;
+  int first, any, piece;
+};
 template <typename T>
-__global__ void __launch_bounds__(kVfPiece) verify_token_kernel(VerifyArgs a) {
-  constexpr int W = kVfPiece / 64;
-  __shared__ double sum_w[W], sum_p[W], base_lds;
-  __shared__ uint64_t table[kVfTable];
-  __shared__ int first, any, piece_lds;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const VfSeq q = a.seq[b];
+__device__ __forceinline__ void vf_token(const VerifyArgs& a, int b, const VfSeq& q, const uint64_t* table, VfToken* sh) {
+  constexpr int W = kVfWide / 64;
+  double *sum_w = sh->sum_w, *sum_p = sh->sum_p;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double* sums = a.sums + (int64_t)b * a.pieces * 2;
   const int per = (a.pieces + kVfPiece - 1) / kVfPiece, p0 = tid * per, p1 = min(p0 + per, a.pieces);
   double sw = 0., sp = 0.;
@@ -376,10 +381,10 @@ __global__ void __launch_bounds__(kVfPiece) verify_token_kernel(VerifyArgs a) {
     sw += sums[2 * i];
     sp += sums[2 * i + 1];
   }
-  vf_table(table);
+  const double ln_s = -log(q.p_mul);
   if (tid == 0) {
-    first = kVfPiece;
-    any = -1;
+    sh->first = kVfPiece;
+    sh->any = -1;
   }
   double cw = wave_scan_d(sw), cp = wave_scan_d(sp);
   if (lane == 63) {
@@ -409,9 +414,9 @@ __global__ void __launch_bounds__(kVfPiece) verify_token_kernel(VerifyArgs a) {
   }
   const double target = (double)a.u[(int64_t)b * a.T] * total;
   // The first thread past the target, else the last one with any weight.
-  vf_mark(mine > 0., upto > target, lane, wave, &first, &any);
+  vf_mark(mine > 0., upto > target, lane, wave, &sh->first, &sh->any);
   __syncthreads();
-  if (tid == (first < kVfPiece ? first : any)) {
+  if (tid == (sh->first < kVfPiece ? sh->first : sh->any)) {
     double run = upto - mine, base = run;
     int at = p0;  // the first of its pieces past the target, else its last with any weight
     for (int i = p0; i < p1 && per > 1; ++i) {
@@ -423,15 +428,15 @@ __global__ void __launch_bounds__(kVfPiece) verify_token_kernel(VerifyArgs a) {
       }
       run += x;
     }
-    piece_lds = at;
-    base_lds = base;
+    sh->piece = at;
+    sh->base = base;
   }
   __syncthreads();
   if (tid == 0) {
-    first = kVfPiece;
-    any = -1;
+    sh->first = kVfPiece;
+    sh->any = -1;
   }
-  const int j = piece_lds * kVfPiece + tid;
+  const int j = sh->piece * kVfPiece + tid;
   float x;
   double w, p;
   vf_weights<T, 1>(a, b, q, j, a.V, table, &x, &w, &p);
@@ -439,18 +444,69 @@ __global__ void __launch_bounds__(kVfPiece) verify_token_kernel(VerifyArgs a) {
   double run = wave_scan_d(w);
   if (lane == 63) sum_w[wave] = run;
   __syncthreads();
-  run += base_lds;
+  run += sh->base;
   for (int k = 0; k < wave; ++k) run += sum_w[k];
-  vf_mark(w > 0., run > target, lane, wave, &first, &any);
+  vf_mark(w > 0., run > target, lane, wave, &sh->first, &sh->any);
   __syncthreads();
-  if (tid == (first < kVfPiece ? first : any)) {
+  if (tid == (sh->first < kVfPiece ? sh->first : sh->any)) {
     a.choice[(int64_t)b * a.T + q.last] = j;
-    a.logprob[(int64_t)b * a.T + q.last] = (float)(((double)x - (double)q.p_m) * (a.mul * kLn2) - q.ln_s);
+    a.logprob[(int64_t)b * a.T + q.last] = (float)(((double)x - (double)q.p_m) * (a.mul * kLn2) - ln_s);
   }
+}
+
+// The walk, the sums and the token by a kernel each.
+template <typename T>
+__global__ void __launch_bounds__(kVfWide) verify_walk_kernel(VerifyArgs a) {
+  __shared__ uint64_t table[kVfTable];
+  __shared__ VfWalk walk;
+  vf_table(table);
+  const VfSeq q = vf_walk<T>(a, blockIdx.x, true, table, &walk);
+  if (threadIdx.x == 0) a.seq[blockIdx.x] = q;
+}
+template <typename T>
+__global__ void __launch_bounds__(kVfWide) verify_sums_kernel(VerifyArgs a) {
+  __shared__ uint64_t table[kVfTable];
+  const int b = blockIdx.x / a.groups, piece = (blockIdx.x % a.groups) * (kVfWide / 64) + (threadIdx.x >> 6);
+  vf_table(table);
+  __syncthreads();
+  if (piece < a.pieces) vf_piece<T>(a, b, a.seq[b], piece, threadIdx.x & 63, table, false);
+}
+template <typename T>
+__global__ void __launch_bounds__(kVfWide) verify_token_kernel(VerifyArgs a) {
+  __shared__ uint64_t table[kVfTable];
+  __shared__ VfToken token;
+  vf_table(table);
+  vf_token<T>(a, blockIdx.x, a.seq[blockIdx.x], table, &token);
+}
+
+// The three in one, for short chains: each workgroup of a sequence makes the walk for
+// itself, and the last one to arrive draws the token (its counter is zero before the
+// call and wraps to zero).  8 nodes of one sequence: FIGURES
+template <typename T>
+__global__ void __launch_bounds__(kVfWide) verify_rest_kernel(VerifyArgs a) {
+  __shared__ uint64_t table[kVfTable];
+  __shared__ VfWalk walk;
+  __shared__ VfToken token;
+  __shared__ int last;
+  const int b = blockIdx.x / a.groups, group = blockIdx.x % a.groups, piece = group * (kVfWide / 64) + (threadIdx.x >> 6);
+  vf_table(table);
+  const VfSeq q = vf_walk<T>(a, b, group == 0, table, &walk);
+  if (piece < a.pieces) vf_piece<T>(a, b, q, piece, threadIdx.x & 63, table, true);
+  // (Every wave's sums are out first.)
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = atomicInc(a.arrived + b, (uint32_t)a.groups - 1u) == (uint32_t)a.groups - 1u;
+    if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  }
+  __syncthreads();
+  if (last) vf_token<T>(a, b, q, table, &token);
 }
 
 // Workgroups of a call: enough to fill the GPU where a row can be cut.
 constexpr int64_t kVfGroups = 2048;
+// Nodes up to which every workgroup of a sequence walks for itself (two a wave).
+constexpr int kVfShort = 16;
 
 struct VerifyPlan {
   int S, seg;
@@ -473,9 +529,13 @@ template <typename T>
 static hipError_t launch_verify_t(const VerifyArgs& a, hipStream_t st) {
   const int rows = a.B * (a.y ? 2 * a.T - 1 : a.T);
   launch(verify_stats_kernel<T>, dim3((unsigned)(rows * a.S)), dim3(kVfThreads), 0, st, a);
-  launch(verify_walk_kernel<T>, dim3(a.B), dim3(512), 0, st, a);
-  launch(verify_sums_kernel<T>, dim3((unsigned)(a.B * ((a.pieces + 3) / 4))), dim3(kVfThreads), 0, st, a);
-  launch(verify_token_kernel<T>, dim3(a.B), dim3(kVfPiece), 0, st, a);
+  if (a.T <= kVfShort && a.B <= (int)(kSyncBytes / sizeof(uint32_t))) {
+    launch(verify_rest_kernel<T>, dim3((unsigned)(a.B * a.groups)), dim3(kVfWide), 0, st, a);
+  } else {
+    launch(verify_walk_kernel<T>, dim3(a.B), dim3(kVfWide), 0, st, a);
+    launch(verify_sums_kernel<T>, dim3((unsigned)(a.B * a.groups)), dim3(kVfWide), 0, st, a);
+    launch(verify_token_kernel<T>, dim3(a.B), dim3(kVfWide), 0, st, a);
+  }
   return hipGetLastError();
 }
 
@@ -496,9 +556,12 @@ hipError_t launch_verify_drafts(const dropkv_verify_drafts_args& p, hipStream_t 
   a.S = pl.S;
   a.seg = pl.seg;
   a.pieces = (int)((p.V + kVfPiece - 1) / kVfPiece);
+  a.groups = (a.pieces + kVfWide / 64 - 1) / (kVfWide / 64);
   a.mul = 1.4426950408889634074 / p.temperature;
   a.deep = (float)(990. / a.mul);
-  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15) + kSyncBytes;
+  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
+  a.arrived = reinterpret_cast<uint32_t*>(ws);
+  ws += kSyncBytes;
   a.part = reinterpret_cast<VfPart*>(ws);
   a.seq = reinterpret_cast<VfSeq*>(a.part + (size_t)p.B * (p.draft_logits ? 2 * p.T - 1 : p.T) * pl.S);
   a.sums = reinterpret_cast<double*>(a.seq + p.B);

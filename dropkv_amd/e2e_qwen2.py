@@ -125,9 +125,10 @@ def run(args) -> dict:
             cache = make_cache("dynamic" if kind == "dynamic" else "dropkv")
             tok, t_pre = _timed(lambda: prefill(model, ids, cache))
             if kind == "dropkv":
-                dec, t_setup = _timed(lambda: CompressedDecoder(model, cache, args.decode))
+                dec, t_setup = _timed(lambda: CompressedDecoder(model, cache, args.decode,
+                                                                cache_dtype=args.cache_dtype))
                 out, t_dec = _timed(lambda: dec.generate(tok, args.decode))
-                stored, logical = int(dec.n_rows[0]), int(dec.pos[0, 0])
+                stored, logical = int(dec.n_rows.flatten()[0]), int(dec.pos[0, 0])
                 del dec
             else:
                 t_setup = 0.0
@@ -146,7 +147,9 @@ def run(args) -> dict:
             "logical_length": logical,
         }
         if kind == "dropkv":
-            res[kind]["decode"] = "CompressedDecoder: HIP graph per step, dropkv_decode_attention"
+            res[kind]["decode"] = ("CompressedDecoder: HIP graph per step, " + (
+                "dropkv_decode_attention" if args.cache_dtype is None else
+                f"dropkv_quant_attention on rows in {args.cache_dtype}"))
             res[kind]["decode_setup_ms"] = statistics.median(setup_ms)
         else:
             res[kind]["decode"] = "eager Transformers forward per step (SDPA, torch.cat append)"
@@ -173,6 +176,8 @@ def main(argv=None):
     p.add_argument("--keep-ratio", type=float, default=0.1)
     p.add_argument("--window", type=int, default=8)
     p.add_argument("--kernel-size", type=int, default=11)
+    p.add_argument("--cache-dtype", choices=("int8", "fp8"), default=None,
+                   help="hold the compressed cache in 8 bits while decoding")
     p.add_argument("--reps", type=int, default=3)
     p.add_argument("--warmup", type=int, default=1)
     p.add_argument("--seed", type=int, default=0)

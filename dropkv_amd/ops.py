@@ -37,7 +37,7 @@ def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
 
 
 def _evict_workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
-    """A new ``dropkv_scores`` / ``dropkv_evict`` workspace: its leading
+    """A new workspace of the calls that count in it: its leading
     counters (_lib.SYNC_BYTES) start at zero, and every call leaves them zero."""
     ws = _workspace(nbytes, dev)
     ws[: _lib.SYNC_BYTES].zero_()
@@ -822,7 +822,7 @@ def quant_workspace(B: int, Hq: int, Hkv: int, D: int, T: int, capacity: int, de
     nbytes = _quant_bytes(B, Hq, Hkv, D, T, (capacity + QUANT_BLOCK - 1) // QUANT_BLOCK * QUANT_BLOCK)
     if nbytes == 0:
         raise RuntimeError("unsupported geometry of a cache in 8 bits")
-    return _workspace(nbytes, torch.device(device))
+    return _evict_workspace(nbytes, torch.device(device))  # (counters at its start)
 
 
 _QATTN_ARGS = _lib.ARGS["dropkv_quant_attention"].pack

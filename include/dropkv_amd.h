@@ -551,7 +551,9 @@ int dropkv_quant_read(const dropkv_quant_read_args* args, void* stream);
  * and sums are fp32; the stored values enter the products as they are.  The weights
  * enter the product with V in two parts (16 bits or more) up to Hq / Hkv * T = 64
  * rows a KV head, and for fp16; for bf16 they may enter it rounded once beyond.
- * Values of V below 2^118.  The workspace as for dropkv_tree_attention. */
+ * Values of V below 2^118.  The workspace as for dropkv_tree_attention, but that its
+ * first DROPKV_SYNC_BYTES must be zero when it is first used; every call leaves them
+ * zero. */
 typedef struct {
   const void* q;
   int64_t q_s[3];
@@ -603,7 +605,8 @@ int dropkv_quant_attention(const dropkv_quant_attention_args* args, void* stream
  * A sampled row that holds +inf or NaN, or only -inf, gives -1 and NaN.
  * 1 <= T <= 256, V <= 2^26, 1e-30 < temperature < 1e30, B * (2 T - 1) < 2^17,
  * B * V < 2^33.  The
- * workspace needs no initialisation; its first DROPKV_SYNC_BYTES are left alone. */
+ * workspace's first DROPKV_SYNC_BYTES must be zero when it is first used, and every call
+ * leaves them zero. */
 typedef struct {
   const void* logits;
   int64_t x_s[2];
