@@ -115,27 +115,27 @@ __device__ __forceinline__ bool near_take_out(T* rows, int pitch, const Near& s,
   return odd;
 }
 
-// Up to 16 rows per KV head: workgroups of four waves, which take the blocks of a
-// part in turn, and the step of 16-bit keys as one block more.  K and V come as
+// Up to 32 rows per KV head (RT tiles of 16): workgroups of four waves, which take the
+// blocks of a part in turn, and the step of 16-bit keys as one block more.  K and V come as
 // matrix operands straight into registers, the next block's loads issued as soon as
 // a block's registers are consumed.  P goes into the product in two parts, rounded
 // and remainder.  The waves' results are joined in LDS; the only part's workgroup
 // writes the output.  Of several parts the last workgroup to arrive joins them, where
 // they are few bytes (FIG1); more are joined by a second kernel.
 constexpr int kNarrowWaves = 4;
-template <typename T, typename S, int D>
-__global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(QuantAttnArgs a) {
+template <typename T, typename S, int D, int RT>
+__global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narrow_kernel(QuantAttnArgs a) {
   typedef typename Elem<T>::v8 v8;
   typedef Elem<__bf16>::v8 b8;
-  constexpr int KC = D / 64, DT = D / 16, CPR = D / 8, GRP = 64 / CPR, NW = kNarrowWaves;
+  constexpr int KC = D / 64, DT = D / 16, CPR = D / 8, GRP = 64 / CPR, NW = kNarrowWaves, ROWS = 16 * RT;
   constexpr int kVPitch = D + 16;  // transposing reads without bank conflicts
   constexpr int kOPitch = D + 4;   // floats
-  constexpr int kLds = std::max(kQBlock * kVPitch * (int)sizeof(T), NW * 16 * kOPitch * 4);
+  constexpr int kLds = std::max(kQBlock * kVPitch * (int)sizeof(T), NW * ROWS * kOPitch * 4);
   const int slot = blockIdx.x % a.P, hkv = blockIdx.x / a.P, g = a.Hq / a.Hkv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
-  __shared__ uint64_t mask_words[16];  // (T <= 16 rows)
-  __shared__ float part_m[NW][16], part_l[NW][16];
+  __shared__ uint64_t mask_words[ROWS];  // (T <= the rows)
+  __shared__ float part_m[NW][ROWS], part_l[NW][ROWS];
   __shared__ int odd_flag, last;
 
   const TreePart part = tree_part<QuantCut>(a, hkv, slot, lane);
@@ -169,75 +169,92 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
     load_v(j);
   }
 
-  // Row li of the KV head: query head hkv g + h, token t.
-  const bool valid = li < a.M;
-  const int h = valid ? a.div_t.div(li) : 0, t = valid ? li - h * a.T : 0;
-  v8 qop[KC][2];
-  const T* qr = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hkv * g + h) * a.q_sh + (int64_t)t * a.q_st;
+  // Row 16 x + li: query head hkv g + h, token t.
+  int tq[RT];
+  v8 qop[RT][KC][2];
+  float m[RT], lsum[RT];
+  f32x4 s[RT][4], o[RT][DT];
 #pragma unroll
-  for (int c = 0; c < KC; ++c)
+  for (int x = 0; x < RT; ++x) {
+    const int row = min(16 * x + li, a.M - 1);  // (rows past the last repeat it and are not stored)
+    const int h = a.div_t.div(row), t = row - h * a.T;
+    tq[x] = t;
+    const T* qr = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hkv * g + h) * a.q_sh + (int64_t)t * a.q_st;
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) qop[c][hf] = tree_load8(qr + 64 * c + 16 * lg + 8 * hf);
-
-  float m = -__FLT_MAX__, lsum = 0.f;  // (finite, so that logits of -inf get no weight)
-  f32x4 s[4], o[DT];
+    for (int c = 0; c < KC; ++c)
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int hf = 0; hf < 2; ++hf) qop[x][c][hf] = tree_load8(qr + 64 * c + 16 * lg + 8 * hf);
+    m[x] = -__FLT_MAX__;  // (finite, so that logits of -inf get no weight)
+    lsum[x] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   // From products to weights; `seen`: a bit for each of the lane's keys.
-  auto weigh = [&](float mul, uint32_t seen) __attribute__((always_inline)) {
+  auto weigh = [&](int x, float mul, uint32_t seen) __attribute__((always_inline)) {
     float tmax = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float x = (seen >> e) & 1 ? s[e / 4][e % 4] * mul : -INFINITY;
-      s[e / 4][e % 4] = x;
-      tmax = fmaxf(tmax, x);
+      const float y = (seen >> e) & 1 ? s[x][e / 4][e % 4] * mul : -INFINITY;
+      s[x][e / 4][e % 4] = y;
+      tmax = fmaxf(tmax, y);
     }
     tmax = max_xor32(max_xor16(tmax));
-    if (wave_any(tmax > m)) {
-      const float mnew = fmaxf(m, tmax), alpha = __builtin_amdgcn_exp2f(m - mnew);
-      lsum *= alpha;
+    if (wave_any(tmax > m[x])) {
+      const float mnew = fmaxf(m[x], tmax), alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
+      lsum[x] *= alpha;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-      m = mnew;
+      for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
+      m[x] = mnew;
     }
     // (The difference of two rounded logits, the larger one itself among them: no
     // weight is above 1 however large they are.)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float p = __builtin_amdgcn_exp2f(s[e / 4][e % 4] - m);
-      s[e / 4][e % 4] = p;
-      lsum += p;
+      const float p = __builtin_amdgcn_exp2f(s[x][e / 4][e % 4] - m[x]);
+      s[x][e / 4][e % 4] = p;
+      lsum[x] += p;
     }
   };
 
   for (; j < part.t_hi; j += NW) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < RT; ++x) s[x][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < KC; ++c)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) s[i] = Elem<T>::mfma(unpack8<S, T>(kx[i][c], hf), qop[c][hf], s[i]);
+        for (int hf = 0; hf < 2; ++hf) {
+          const v8 kop = unpack8<S, T>(kx[i][c], hf);
+#pragma unroll
+          for (int x = 0; x < RT; ++x) s[x][i] = Elem<T>::mfma(kop, qop[x][c][hf], s[x][i]);
+        }
     }
     const float mul = ks * a.scale_log2, vscale = vs;
     load_k(j + NW);
-    weigh(mul, 0xffffu);
-    b8 phi[2], plo[2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
+    for (int x = 0; x < RT; ++x) weigh(x, mul, 0xffffu);
+    b8 phi[RT][2], plo[RT][2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = s[2 * hf + e / 4][e % 4] * vscale;
-        phi[hf][e] = static_cast<__bf16>(p);
-        plo[hf][e] = static_cast<__bf16>(p - static_cast<float>(phi[hf][e]));
-      }
+    for (int x = 0; x < RT; ++x)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = s[x][2 * hf + e / 4][e % 4] * vscale;
+          phi[x][hf][e] = static_cast<__bf16>(p);
+          plo[x][hf][e] = static_cast<__bf16>(p - static_cast<float>(phi[x][hf][e]));
+        }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const b8 vop = unpack8<S, __bf16>(vx[dt], hf);
-        o[dt] = Elem<__bf16>::mfma(vop, phi[hf], o[dt]);
-        o[dt] = Elem<__bf16>::mfma(vop, plo[hf], o[dt]);
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+          o[x][dt] = Elem<__bf16>::mfma(vop, phi[x][hf], o[x][dt]);
+          o[x][dt] = Elem<__bf16>::mfma(vop, plo[x][hf], o[x][dt]);
+        }
       }
     load_v(j + NW);
   }
@@ -268,13 +285,15 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
         vch[i] = tree_load8(near_row<T, D>(step, v_row + i * GRP, vtl, vn, a.vn_st) + v_col);
       tree_mask_words<1>(a, b, step.j0, 0, lane, mask_words);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
+        for (int x = 0; x < RT; ++x) {
+          s[x][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) s[i] = Elem<T>::mfma(kop[i][c][hf], qop[c][hf], s[i]);
-      }
+          for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) s[x][i] = Elem<T>::mfma(kop[i][c][hf], qop[x][c][hf], s[x][i]);
+        }
 #pragma unroll
       for (int i = 0; i < kQBlock / GRP; ++i) *reinterpret_cast<v8*>(vt + (v_row + i * GRP) * kVPitch + v_col) = vch[i];
       if (__builtin_expect(near_any_odd<T>(vch), 0))
@@ -282,45 +301,55 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
           *e = v_row + i * GRP;
           *col = v_col;
         });
-      const uint64_t bits = near_bits(step, mask_words[t]);
-      weigh(a.scale_log2, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
-      v8 phi[2], plo[2];
+      v8 phi[RT][2], plo[RT][2];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int x = 0; x < RT; ++x) {
+        const uint64_t bits = near_bits(step, mask_words[tq[x]]);
+        weigh(x, a.scale_log2, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = s[2 * hf + e / 4][e % 4];
-          phi[hf][e] = static_cast<T>(p);
-          plo[hf][e] = static_cast<T>(p - static_cast<float>(phi[hf][e]));
-        }
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p = s[x][2 * hf + e / 4][e % 4];
+            phi[x][hf][e] = static_cast<T>(p);
+            plo[x][hf][e] = static_cast<T>(p - static_cast<float>(phi[x][hf][e]));
+          }
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const v8 vop = near_v<T, D>(vt, 16 * lg + 8 * hf, 16 * dt, li, kVPitch);
-          o[dt] = Elem<T>::mfma(vop, phi[hf], o[dt]);
-          o[dt] = Elem<T>::mfma(vop, plo[hf], o[dt]);
+#pragma unroll
+          for (int x = 0; x < RT; ++x) {
+            o[x][dt] = Elem<T>::mfma(vop, phi[x][hf], o[x][dt]);
+            o[x][dt] = Elem<T>::mfma(vop, plo[x][hf], o[x][dt]);
+          }
         }
     } while (near_next(&step, a.T));
   }
 
   // The waves' results joined: 16 threads a row.
-  lsum = add_xor32(add_xor16(lsum));
   if (threadIdx.x == 0) odd_flag = 0;
   __syncthreads();  // (V's rows have been read)
-  float* ol = reinterpret_cast<float*>(lds) + (wave * 16 + li) * kOPitch + 4 * lg;
-  if (valid) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(ol + 16 * dt) = o[dt];
-  }
-  if (lg == 0) {
-    part_m[wave][li] = m;
-    part_l[wave][li] = lsum;
+  for (int x = 0; x < RT; ++x) {
+    const int at = 16 * x + li;
+    const float l = add_xor32(add_xor16(lsum[x]));
+    float* ol = reinterpret_cast<float*>(lds) + (wave * ROWS + at) * kOPitch + 4 * lg;
+    if (at < a.M) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(ol + 16 * dt) = o[x][dt];
+    }
+    if (lg == 0) {
+      part_m[wave][at] = m[x];
+      part_l[wave][at] = l;
+    }
   }
   if (wave_any(odd) && lane == 0) odd_flag = 1;
   __syncthreads();
-  const int row = threadIdx.x >> 4;
-  if (row < a.M) {
+#pragma unroll 1
+  for (int row = threadIdx.x >> 4; row < a.M; row += 16) {
     float mx = part_m[0][row], l = 0.f, f[NW];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mx = fmaxf(mx, part_m[w][row]);
@@ -332,6 +361,9 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
     const int hr = a.div_t.div(row), tr = row - hr * a.T;
     T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)tr * a.o_st + (int64_t)(hkv * g + hr) * a.o_sh;
     const int64_t base = ((int64_t)hkv * a.P + slot) * a.M + row;
+    // (The wave's four rows.)
+    const rsrc_t prs = make_rsrc(
+        a.part_o + (((int64_t)hkv * a.P + slot) * a.M + __builtin_amdgcn_readfirstlane(row & ~3)) * D, 4 * D * 4u);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
@@ -339,15 +371,15 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + (w * 16 + row) * kOPitch + d0);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) + (w * ROWS + row) * kOPitch + d0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = fmaf(f[w], x[e], acc[e]);
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(f[w], y[e], acc[e]);
       }
       if (a.direct) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[d0 + e] = static_cast<T>(l == 0.f ? 0.f : acc[e] * inv);
       } else {
-        st_dev16(make_rsrc(a.part_o + base * D, D * 4u), d0 * 4u, acc);
+        st_dev16(prs, ((row & 3) * D + d0) * 4u, acc);
       }
     }
     if (!a.direct && (threadIdx.x & 15) == 0) {
@@ -358,7 +390,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
   if (__builtin_expect(odd_flag, 0)) {
     __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    tree_add_odd<T, D, 64 * NW>(a, b, hkv, slot, 0, 16);
+    tree_add_odd<T, D, 64 * NW>(a, b, hkv, slot, 0, ROWS);
   }
   if (!a.arrived) return;
   // (Every wave's stores are out first.  The counter is zero before the call and wraps
@@ -370,64 +402,67 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, 2) quant_narrow_kernel(Quan
     if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   }
   __syncthreads();
-  if (!last || row >= a.M) return;
+  if (!last) return;
   // 16 threads a row: 16 parts' maxima and sums a thread each, and the partial rows, in
   // one round trip.
   const int sub = threadIdx.x & 15;
-  const int64_t at0 = ((int64_t)hkv * a.P + part.first) * a.M + row;
-  // (Ragged sequences may have more than 16.)
-  f32x4 acc[D / 64];
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float mx = -__FLT_MAX__, l = 0.f;
 #pragma unroll 1
-  for (int s0 = 0; s0 < part.count; s0 += 16) {
-    const int s = s0 + sub;
-    const float pm = s < part.count ? a.part_m[at0 + (int64_t)s * a.M] : -__FLT_MAX__;
-    const float pl = s < part.count ? a.part_l[at0 + (int64_t)s * a.M] : 0.f;
-    f32x4 x[16][D / 64];
+  for (int row = threadIdx.x >> 4; row < a.M; row += 16) {
+    const int64_t at0 = ((int64_t)hkv * a.P + part.first) * a.M + row;
+    // (Ragged sequences may have more than 16.)
+    f32x4 acc[D / 64];
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
+    for (int c = 0; c < D / 64; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float mx = -__FLT_MAX__, l = 0.f;
+#pragma unroll 1
+    for (int s0 = 0; s0 < part.count; s0 += 16) {
+      const int s = s0 + sub;
+      const float pm = s < part.count ? a.part_m[at0 + (int64_t)s * a.M] : -__FLT_MAX__;
+      const float pl = s < part.count ? a.part_l[at0 + (int64_t)s * a.M] : 0.f;
+      f32x4 x[16][D / 64];
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-        x[k][c] = *reinterpret_cast<const f32x4*>(a.part_o + (at0 + (int64_t)min(s0 + k, part.count - 1) * a.M) * D +
-                                                  4 * sub + 64 * c);
-    float top = pm;
-    top = fmaxf(top, dpp_f<kDppQuadSwap1>(top));
-    top = fmaxf(top, dpp_f<kDppQuadSwap2>(top));
-    top = fmaxf(top, dpp_f<kDppHalfMirror>(top));
-    top = fmaxf(top, dpp_f<kDppMirror>(top));
-    top = fmaxf(mx, top);
-    const float turn = __builtin_amdgcn_exp2f(mx - top), f = s < part.count ? __builtin_amdgcn_exp2f(pm - top) : 0.f;
-    mx = top;
-    float sum = pl * f;
-    sum += dpp_f<kDppQuadSwap1>(sum);
-    sum += dpp_f<kDppQuadSwap2>(sum);
-    sum += dpp_f<kDppHalfMirror>(sum);
-    sum += dpp_f<kDppMirror>(sum);
-    l = l * turn + sum;
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) acc[c] *= turn;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float fk = __shfl(f, (lane & 48) | k);
-      if (s0 + k < part.count)
+      for (int k = 0; k < 16; ++k)
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
+          x[k][c] = *reinterpret_cast<const f32x4*>(a.part_o + (at0 + (int64_t)min(s0 + k, part.count - 1) * a.M) * D +
+                                                    4 * sub + 64 * c);
+      float top = pm;
+      top = fmaxf(top, dpp_f<kDppQuadSwap1>(top));
+      top = fmaxf(top, dpp_f<kDppQuadSwap2>(top));
+      top = fmaxf(top, dpp_f<kDppHalfMirror>(top));
+      top = fmaxf(top, dpp_f<kDppMirror>(top));
+      top = fmaxf(mx, top);
+      const float turn = __builtin_amdgcn_exp2f(mx - top), f = s < part.count ? __builtin_amdgcn_exp2f(pm - top) : 0.f;
+      mx = top;
+      float sum = pl * f;
+      sum += dpp_f<kDppQuadSwap1>(sum);
+      sum += dpp_f<kDppQuadSwap2>(sum);
+      sum += dpp_f<kDppHalfMirror>(sum);
+      sum += dpp_f<kDppMirror>(sum);
+      l = l * turn + sum;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[c][e] = fmaf(fk, x[k][c][e], acc[c][e]);
+      for (int c = 0; c < D / 64; ++c) acc[c] *= turn;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float fk = __shfl(f, (lane & 48) | k);
+        if (s0 + k < part.count)
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][e] = fmaf(fk, x[k][c][e], acc[c][e]);
+      }
     }
+    const int hr = a.div_t.div(row), tr = row - hr * a.T;
+    T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)tr * a.o_st + (int64_t)(hkv * g + hr) * a.o_sh;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[4 * sub + 64 * c + e] = static_cast<T>(l == 0.f ? 0.f : acc[c][e] * inv);
   }
-  const int hr = a.div_t.div(row), tr = row - hr * a.T;
-  T* out = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)tr * a.o_st + (int64_t)(hkv * g + hr) * a.o_sh;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[4 * sub + 64 * c + e] = static_cast<T>(l == 0.f ? 0.f : acc[c][e] * inv);
 }
 
-// More than 16 rows: NW waves of QB blocks of 16 rows take the same keys, so that a
+// More than 32 rows: NW waves of QB blocks of 16 rows take the same keys, so that a
 // block of K and V is read, and turned into operands, once for all of them.  LDS holds
 // the operands of a stage of 64 keys as the lanes read them, 16 bytes a lane, 1 KB a
 // product; the next stage's bytes are on their way in registers while the waves
@@ -725,24 +760,25 @@ struct QuantShape {
   int per_cu;
 };
 constexpr QuantShape kQuantShapes[] = {
-    {16, 1.6, 6.9, 1.2, 2}, {64, 1.25, 8.3, 1.45, 2}, {128, 1.45, 8.5, 1.7, 2}, {256, 2.1, 8.0, 1.0, 1}};
+    {16, 1.6, 6.9, 1.2, 2}, {32, 2.1, 7.2, 1.0, 1}, {64, 1.25, 8.3, 1.45, 2}, {128, 1.45, 8.5, 1.7, 2}, {256, 2.1, 8.0, 1.0, 1}};
 
 constexpr int64_t kOneJoin = 8192;  // elements
 
 static double quant_cost(const QuantShape& w, double heads, double M, double D, double blocks, int64_t S) {
   const double wgs = heads * std::ceil(M / w.rows) * S, wide = D / 128;
-  const double per = std::ceil((blocks + (w.rows == 16 ? 1 : 0)) / S), load = wgs / (256.0 * w.per_cu);
+  const bool narrow = w.rows <= 32;
+  const double per = std::ceil((blocks + narrow) / S), load = wgs / (256.0 * w.per_cu);
   double block = w.block_us * (wide < 1 ? 0.6 : 1);
   if (load > 1)
     block *= std::ceil(load) * w.shared;
   else if (w.per_cu == 2 && load > 0.5)
     block *= w.shared;
-  const double steps = w.rows == 16 ? std::ceil(per / kNarrowWaves) : per;
-  const double flight = std::min(wgs, 256.0 * w.per_cu) * (w.rows == 16 ? 65536 : 16384) * wide;
+  const double steps = narrow ? std::ceil(per / kNarrowWaves) : per;
+  const double flight = std::min(wgs, 256.0 * w.per_cu) * (narrow ? 65536 : 16384) * wide;
   const double bytes = heads * blocks * kQBlock * D * 2;
   double stream = bytes / 5.2e6 / std::min(1.0, flight / std::max(1.0, std::min(8e6, bytes / 4)));
   if (bytes > 3e7) stream *= 0.5 + 0.5 * std::ceil(wgs / 256) * 256 / wgs;
-  const double join = w.rows == 16 && S == 1 ? -2.5 : S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16);
+  const double join = narrow && S == 1 ? -2.5 : S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16);
   return std::max(steps * block, stream) + join + w.fixed_us;
 }
 
@@ -754,9 +790,9 @@ static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
   double best = 0;
   p.S = 0;
   for (const QuantShape& w : kQuantShapes) {
-    // Four waves of their own blocks for up to 16 rows; no shape that the rows would
-    // leave half empty.
-    if ((w.rows == 16) != (p.M <= 16) || (w.rows > 64 && p.M <= w.rows / 2)) continue;
+    // No shape that the rows would leave half empty; waves of their own blocks for up to
+    // 32 rows, workgroups that share them beyond.
+    if ((w.rows > 16 && p.M <= w.rows / 2) || (w.rows <= 32 && p.M > w.rows)) continue;
     const int64_t chunks = heads * ((p.M + w.rows - 1) / w.rows);
     const int64_t tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kTreeMaxSplits, 256 / chunks, 512 / chunks};
     for (int64_t S : tries) {
@@ -773,7 +809,7 @@ static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
   p.apart = p.rows_wg == 64 || (p.rows_wg > 64 && heads * p.MC * p.S < 192);
   p.P = (int)(B * (p.S + p.apart));
   // (What one workgroup reads in a round trip.)
-  p.one = p.rows_wg == 16 && p.S > 1 && p.S <= 16 && heads <= (int64_t)(kSyncBytes / sizeof(uint32_t)) && p.S * p.M * D <= kOneJoin;
+  p.one = p.rows_wg <= 32 && p.S > 1 && p.S <= 16 && heads <= (int64_t)(kSyncBytes / sizeof(uint32_t)) && p.S * p.M * D <= kOneJoin;
   p.rows = (size_t)Hkv * p.P * p.M;
   p.bytes = kSyncBytes + kTreeDealBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
   return p;
@@ -788,7 +824,9 @@ static hipError_t launch_quant_t(const QuantAttnArgs& a, int rows_wg, hipStream_
   constexpr bool kLo = std::is_same<T, _Float16>::value;
   const dim3 grid(a.Hkv * a.P * a.MC);
   if (rows_wg == 16)
-    launch((quant_narrow_kernel<T, S, D>), grid, dim3(64 * kNarrowWaves), 0, st, a);
+    launch((quant_narrow_kernel<T, S, D, 1>), grid, dim3(64 * kNarrowWaves), 0, st, a);
+  else if (rows_wg == 32)
+    launch((quant_narrow_kernel<T, S, D, 2>), grid, dim3(64 * kNarrowWaves), 0, st, a);
   else if (rows_wg == 64)
     launch((quant_wide_kernel<T, S, D, 1, 4, true>), grid, dim3(256), 0, st, a);
   else if (rows_wg == 128)
@@ -840,7 +878,7 @@ hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* 
   a.S = pl.S;
   a.P = pl.P;
   a.apart = pl.apart;
-  a.tail_tiles = pl.apart ? 0 : pl.rows_wg == 16 ? 2 : 3 + (a.T + kQBlock - 1) / kQBlock;
+  a.tail_tiles = pl.apart ? 0 : pl.rows_wg <= 32 ? 2 : 3 + (a.T + kQBlock - 1) / kQBlock;
   a.ragged = p.n_sb != 0 && p.B > 1 && p.B <= kTreeRaggedB && pl.S > 1;
   a.direct = pl.S == 1 && !pl.apart;
   a.div_t = Div::of(a.T);
