@@ -41,6 +41,11 @@ struct QuantCut {
 // reference that its weights are taken against before it turns what it has summed.
 constexpr float kQRise = 8.f;
 
+// Weights are 2^(x mul - m + log2 vs) by one fma, vs the scale of the block's values.
+// From here on (in powers of two) m's own rounding would lift them far above 1: there the
+// difference of the two rounded logits is taken first, the larger one itself among them.
+constexpr float kQFar = 4194304.f;
+
 // A step of 16-bit keys: the `held` rows of the tail (rows first ..), then `fresh`
 // new ones from j0 on.
 struct Near {
@@ -189,16 +194,16 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // From products to weights; `seen`: a bit for each of the lane's keys.
-  auto weigh = [&](int x, float mul, uint32_t seen) __attribute__((always_inline)) {
+  // From products (times `mul`: logits) to weights times the values' scale, 2^up = 1 /
+  // down; `seen`: a bit for each of the lane's keys.
+  auto weigh = [&](int x, float mul, float up, float down, uint32_t seen) __attribute__((always_inline)) {
     float tmax = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float y = (seen >> e) & 1 ? s[x][e / 4][e % 4] * mul : -INFINITY;
-      s[x][e / 4][e % 4] = y;
-      tmax = fmaxf(tmax, y);
+      s[x][e / 4][e % 4] = (seen >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
+      tmax = fmaxf(tmax, s[x][e / 4][e % 4]);
     }
-    tmax = max_xor32(max_xor16(tmax));
+    tmax = max_xor32(max_xor16(tmax)) * mul;
     if (wave_any(tmax > m[x])) {
       const float mnew = fmaxf(m[x], tmax), alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
       lsum[x] *= alpha;
@@ -206,14 +211,21 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
       for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
       m[x] = mnew;
     }
-    // (The difference of two rounded logits, the larger one itself among them: no
-    // weight is above 1 however large they are.)
+    float by = mul, less = up - m[x];
+    if (wave_any(fabsf(m[x]) >= kQFar)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[x][e / 4][e % 4] = s[x][e / 4][e % 4] * mul - m[x];
+      by = 1.f;
+      less = up;
+    }
+    float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float p = __builtin_amdgcn_exp2f(s[x][e / 4][e % 4] - m[x]);
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[x][e / 4][e % 4], by, less));
       s[x][e / 4][e % 4] = p;
-      lsum[x] += p;
+      sum += p;
     }
+    lsum[x] = fmaf(sum, down, lsum[x]);
   };
 
   for (; j < part.t_hi; j += NW) {
@@ -230,10 +242,11 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
           for (int x = 0; x < RT; ++x) s[x][i] = Elem<T>::mfma(kop, qop[x][c][hf], s[x][i]);
         }
     }
-    const float mul = ks * a.scale_log2, vscale = vs;
+    // (A block of zeros has no scale: any will do.)
+    const float mul = ks * a.scale_log2, fold = vs == 0.f ? 1.f : vs, up = __builtin_amdgcn_logf(fold), down = 1.f / fold;
     load_k(j + NW);
 #pragma unroll
-    for (int x = 0; x < RT; ++x) weigh(x, mul, 0xffffu);
+    for (int x = 0; x < RT; ++x) weigh(x, mul, up, down, 0xffffu);
     b8 phi[RT][2], plo[RT][2];
 #pragma unroll
     for (int x = 0; x < RT; ++x)
@@ -241,7 +254,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
       for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float p = s[x][2 * hf + e / 4][e % 4] * vscale;
+          const float p = s[x][2 * hf + e / 4][e % 4];
           phi[x][hf][e] = static_cast<__bf16>(p);
           plo[x][hf][e] = static_cast<__bf16>(p - static_cast<float>(phi[x][hf][e]));
         }
@@ -305,7 +318,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
 #pragma unroll
       for (int x = 0; x < RT; ++x) {
         const uint64_t bits = near_bits(step, mask_words[tq[x]]);
-        weigh(x, a.scale_log2, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
+        weigh(x, a.scale_log2, 0.f, 1.f, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -584,15 +597,13 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     bool turn = false;
 #pragma unroll
     for (int x = 0; x < QB; ++x) {
+      if (kNear)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[x][e / 4][e % 4] *= mul;
-        if (kNear) s[x][e / 4][e % 4] = (see_bits[x] >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
-      }
+        for (int e = 0; e < 16; ++e) s[x][e / 4][e % 4] = (see_bits[x] >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
       float tmax = s[x][0][0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, s[x][e / 4][e % 4]);
-      top[x] = max_xor32(max_xor16(tmax));
+      top[x] = max_xor32(max_xor16(tmax)) * mul;
       turn |= top[x] - m[x] > kQRise;
     }
     if (wave_any(turn)) {
@@ -607,6 +618,22 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     }
     // (A block of zeros has no scale: any will do.)
     const float fold = vscale == 0.f ? 1.f : vscale, up = __builtin_amdgcn_logf(fold), down = 1.f / fold;
+    float by = mul, less[QB];
+    bool far = false;
+#pragma unroll
+    for (int x = 0; x < QB; ++x) {
+      less[x] = up - m[x];
+      far |= fabsf(m[x]) >= kQFar;
+    }
+    if (wave_any(far)) {
+#pragma unroll
+      for (int x = 0; x < QB; ++x) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[x][e / 4][e % 4] = s[x][e / 4][e % 4] * mul - m[x];
+        less[x] = up;
+      }
+      by = 1.f;
+    }
     f32x4 sum[QB];
 #pragma unroll
     for (int x = 0; x < QB; ++x) sum[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -620,7 +647,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
       for (int x = 0; x < QB; ++x)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float p = __builtin_amdgcn_exp2f((s[x][2 * hf + e / 4][e % 4] - m[x]) + up);
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[x][2 * hf + e / 4][e % 4], by, less[x]));
           phi[x][e] = static_cast<VT>(p);
           if (LO) plo[x][e] = static_cast<VT>(p - static_cast<float>(phi[x][e]));
         }
