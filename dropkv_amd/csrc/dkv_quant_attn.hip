@@ -204,9 +204,9 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       s[x][e / 4][e % 4] = (seen >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
-      tmax = fmaxf(tmax, s[x][e / 4][e % 4]);
+      tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
     }
-    tmax = max_xor32(max_xor16(tmax)) * mul;
+    tmax = maximum_xor32(maximum_xor16(tmax)) * mul;
     if (wave_any(tmax > m[x])) {
       const float mnew = fmaxf(m[x], tmax), alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
       lsum[x] *= alpha;
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
         }
     }
     // (A block of zeros has no scale: any will do.)
-    const float mul = ks * a.scale_log2, fold = vs == 0.f ? 1.f : vs, up = __builtin_amdgcn_logf(fold), down = 1.f / fold;
+    const float mul = ks * a.scale_log2, fold = vs == 0.f ? 1.f : vs, up = __builtin_amdgcn_logf(fold), down = __builtin_amdgcn_rcpf(fold);
     load_k(j + NW);
 #pragma unroll
     for (int x = 0; x < RT; ++x) weigh(x, mul, up, down, 0xffffu);
@@ -487,15 +487,16 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
 // the weights' sum.  P is rounded once for bf16 in workgroups of 128 rows and more, in
 // two parts otherwise.  Bound by the matrix cores and the ALUs in turn: 4 x 64 heads of
 // 26214 rows, 64 tokens, 221 us (995 TFLOP/s), of which 11 are the join.
-template <typename T, typename S, int D, int QB, int NW, bool LO>
+template <typename T, typename S, int D, int QB, int NW, bool LO, bool PAIR>
 __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a) {
   typedef typename Elem<T>::v8 v8;
   constexpr int KC = D / 64, DT = D / 16, NT = 64 * NW;
   constexpr int kPieces = 64 * (4 * KC), NC = 2 * kPieces / NT;  // 16-byte pieces of a block's K (or V); per thread
   constexpr int kOps = 4 * KC * 2;                               // operands of a stage's K (or V)
-  constexpr int kBuf = 2 * kOps * 64;                            // 16-byte places per buffer
-  static_assert(DT == 4 * KC && NC * NT == 2 * kPieces, "whole pieces per thread");
-  __shared__ u32x4 lds[2 * kBuf];
+  constexpr int kBuf = kOps * 64;                                // 16-byte places per buffer of K (or V)
+  constexpr int kVBufs = PAIR ? 3 : 2;                           // (of K: 2)
+  static_assert(DT == 4 * KC && NC * NT == 2 * kPieces && (!PAIR || NW == 8), "whole pieces per thread");
+  __shared__ u32x4 lds[(2 + kVBufs) * kBuf];
   __shared__ uint64_t mask_words[kTreeMaxT];
   __shared__ int odd_flag;
 
@@ -550,12 +551,12 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     ks = ksc[min(j, blocks - 1)];
     vs = vsc[min(j, blocks - 1)];
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
+  auto put = [&](int kbuf, int vbuf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       int op;
       const bool v = place(i, &op);
-      u32x4* to = lds + buf * kBuf + ((v ? kOps : 0) + 2 * op) * 64 + lane;
+      u32x4* to = lds + (v ? 2 + vbuf : kbuf) * kBuf + 2 * op * 64 + lane;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
         to[64 * hf] = v ? __builtin_bit_cast(u32x4, unpack8<S, __bf16>(piece[i], hf))
@@ -575,18 +576,16 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // The stage in buffer `buf`, the logits times `mul`, the weights times vscale; or,
-  // `near`, 16-bit keys of see_bits, their V in rows behind K's operands.
+  // A stage in three steps: products with K, weights, products with V.  Of `near` stages,
+  // 16-bit keys of see_bits, K's operands are at the start of LDS and V's rows behind.
   uint32_t see_bits[QB];
   constexpr int kVPitch = D + 16;  // transposing reads without bank conflicts
   static_assert(kOps * 64 * 16 + kQBlock * kVPitch * 2 <= (int)sizeof(lds), "a step of 16-bit keys fits");
-  auto compute = [&](int buf, float mul, float vscale, auto near) __attribute__((always_inline)) {
-    constexpr bool kNear = decltype(near)::value;
-    typedef std::conditional_t<kNear, T, __bf16> VT;
-    typedef typename Elem<VT>::v8 vv8;
+  f32x4 s[QB][4];
+  u32x4 phi[QB][2], plo[LO ? QB : 1][2];
+  float down = 1.f;
+  auto with_k = [&](int buf) __attribute__((always_inline)) {
     const u32x4* kt = lds + buf * kBuf + lane;
-    const u32x4* vt = kt + kOps * 64;
-    f32x4 s[QB][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -598,6 +597,12 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
         for (int x = 0; x < QB; ++x) s[x][i] = Elem<T>::mfma(kop, qop[x][c / 2][c % 2], s[x][i]);
       }
     }
+  };
+  // The logits are the products times `mul`; the weights come times vscale.
+  auto weigh = [&](float mul, float vscale, auto near) __attribute__((always_inline)) {
+    constexpr bool kNear = decltype(near)::value;
+    typedef std::conditional_t<kNear, T, __bf16> VT;
+    typedef typename Elem<VT>::v8 vv8;
     float top[QB];
     bool turn = false;
 #pragma unroll
@@ -607,8 +612,8 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
         for (int e = 0; e < 16; ++e) s[x][e / 4][e % 4] = (see_bits[x] >> e) & 1 ? s[x][e / 4][e % 4] : -INFINITY;
       float tmax = s[x][0][0];
 #pragma unroll
-      for (int e = 1; e < 16; ++e) tmax = fmaxf(tmax, s[x][e / 4][e % 4]);
-      top[x] = max_xor32(max_xor16(tmax)) * mul;
+      for (int e = 1; e < 16; ++e) tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
+      top[x] = maximum_xor32(maximum_xor16(tmax)) * mul;
       turn |= top[x] - m[x] > kQRise;
     }
     if (wave_any(turn)) {
@@ -622,7 +627,8 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
       }
     }
     // (A block of zeros has no scale: any will do.)
-    const float fold = vscale == 0.f ? 1.f : vscale, up = __builtin_amdgcn_logf(fold), down = 1.f / fold;
+    const float fold = vscale == 0.f ? 1.f : vscale, up = __builtin_amdgcn_logf(fold);
+    down = __builtin_amdgcn_rcpf(fold);
     float by = mul, less[QB];
     bool far = false;
 #pragma unroll
@@ -639,6 +645,26 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
       }
       by = 1.f;
     }
+#pragma unroll
+    for (int x = 0; x < QB; ++x)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        vv8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[x][2 * hf + e / 4][e % 4], by, less[x]));
+          hi[e] = static_cast<VT>(p);
+          if (LO) lo[e] = static_cast<VT>(p - static_cast<float>(hi[e]));
+        }
+        phi[x][hf] = __builtin_bit_cast(u32x4, hi);
+        if (LO) plo[x][hf] = __builtin_bit_cast(u32x4, lo);
+      }
+  };
+  auto with_v = [&](int buf, auto near) __attribute__((always_inline)) {
+    constexpr bool kNear = decltype(near)::value;
+    typedef std::conditional_t<kNear, T, __bf16> VT;
+    typedef typename Elem<VT>::v8 vv8;
+    const u32x4* vt = lds + (2 + buf) * kBuf + lane;
     f32x4 sum[QB];
 #pragma unroll
     for (int x = 0; x < QB; ++x) sum[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -647,19 +673,10 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     for (int e = 0; e < 8; ++e) ones[e] = static_cast<VT>(1.f);
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      vv8 phi[QB], plo[LO ? QB : 1];
-#pragma unroll
-      for (int x = 0; x < QB; ++x)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[x][2 * hf + e / 4][e % 4], by, less[x]));
-          phi[x][e] = static_cast<VT>(p);
-          if (LO) plo[x][e] = static_cast<VT>(p - static_cast<float>(phi[x][e]));
-        }
 #pragma unroll
       for (int x = 0; x < QB; ++x) {
-        sum[x] = Elem<VT>::mfma(ones, phi[x], sum[x]);
-        if (LO) sum[x] = Elem<VT>::mfma(ones, plo[x], sum[x]);
+        sum[x] = Elem<VT>::mfma(ones, bitcast_u4<vv8>(phi[x][hf]), sum[x]);
+        if (LO) sum[x] = Elem<VT>::mfma(ones, bitcast_u4<vv8>(plo[x][hf]), sum[x]);
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -670,8 +687,8 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
           vop = bitcast_u4<vv8>(vt[(2 * dt + hf) * 64]);
 #pragma unroll
         for (int x = 0; x < QB; ++x) {
-          o[x][dt] = Elem<VT>::mfma(vop, phi[x], o[x][dt]);
-          if (LO) o[x][dt] = Elem<VT>::mfma(vop, plo[x], o[x][dt]);
+          o[x][dt] = Elem<VT>::mfma(vop, bitcast_u4<vv8>(phi[x][hf]), o[x][dt]);
+          if (LO) o[x][dt] = Elem<VT>::mfma(vop, bitcast_u4<vv8>(plo[x][hf]), o[x][dt]);
         }
       }
     }
@@ -679,20 +696,87 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     for (int x = 0; x < QB; ++x) lsum[x] = fmaf(sum[x][0], down, lsum[x]);
   };
 
+  // Keeps kAhead operands on their way from LDS before the products that take them: left
+  // alone, the compiler has two (64 cycles of products under a latency of 130, which was
+  // 1000 of a stage's 4400 cycles).
+  auto ahead = [&](auto reads, auto products) __attribute__((always_inline)) {
+    constexpr int R = decltype(reads)::value, M = decltype(products)::value, kAhead = 8, kEach = M / R;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < R - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, M - (R - kAhead) * kEach, 0);
+  };
+
   if (tid == 0) odd_flag = 0;
-  int buf = 0, j = part.t_lo;
-  if (j < part.t_hi) {
-    fetch(j);
-    float mul = ks * a.scale_log2, vscale = vs;
-    put(0);
-    for (; j < part.t_hi; ++j) {
-      fetch(j + 1);
-      __syncthreads();
-      compute(buf, mul, vscale, std::false_type{});
-      buf ^= 1;
-      mul = ks * a.scale_log2;
-      vscale = vs;
-      put(buf);
+  if constexpr (PAIR) {
+    // Two groups of four waves, one on each SIMD, half a stage apart: while one works with
+    // the matrix cores (V of its last stage, K of this one), the other makes weights and
+    // puts operands, a barrier between the halves.  The second group is ahead by a stage
+    // with its pieces: those of stage j + 1 must lie there when the first one begins it.
+    // V is read a stage after K, so it has three buffers.
+    const int group = wave >> 2, n = part.t_hi - part.t_lo;
+    if (n > 0) {
+      auto turn_over = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      fetch(part.t_lo);
+      float mul = ks * a.scale_log2, vscale = vs;
+      put(0, 0);
+      if (group) {
+        fetch(part.t_lo + 1);
+        put(1, 1);
+      }
+      fetch(part.t_lo + 1 + group);
+      turn_over();
+      if (group) turn_over();
+      int vput = 1 + group, vget = 0;  // buffers of V: of the stage put next, and of the last one
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {  // (before the first stage there are no weights)
+          phi[x][hf] = u32x4{0u, 0u, 0u, 0u};
+          if (LO) plo[x][hf] = u32x4{0u, 0u, 0u, 0u};
+        }
+      for (int j = 0; j < n; ++j) {
+        with_v(vget, std::false_type{});
+        with_k(j & 1);
+        ahead(std::integral_constant<int, 2 * kOps>{}, std::integral_constant<int, (2 * DT + 2) * QB * (LO ? 2 : 1) + 8 * KC * QB>{});
+        vget = j == 0 ? 0 : vget == 2 ? 0 : vget + 1;
+        turn_over();
+        weigh(mul, vscale, std::false_type{});
+        put((j + 1 + group) & 1, vput);
+        vput = vput == 2 ? 0 : vput + 1;
+        fetch(part.t_lo + j + 2 + group);
+        mul = ksc[min(part.t_lo + j + 1, blocks - 1)] * a.scale_log2;
+        vscale = vsc[min(part.t_lo + j + 1, blocks - 1)];
+        turn_over();
+      }
+      with_v(vget, std::false_type{});
+      ahead(std::integral_constant<int, kOps>{}, std::integral_constant<int, (2 * DT + 2) * QB * (LO ? 2 : 1)>{});
+      if (!group) turn_over();
+    }
+  } else {
+    int buf = 0, j = part.t_lo;
+    if (j < part.t_hi) {
+      fetch(j);
+      float mul = ks * a.scale_log2, vscale = vs;
+      put(0, 0);
+      for (; j < part.t_hi; ++j) {
+        fetch(j + 1);
+        __syncthreads();
+        with_k(buf);
+        weigh(mul, vscale, std::false_type{});
+        with_v(buf, std::false_type{});
+        buf ^= 1;
+        mul = ks * a.scale_log2;
+        vscale = vs;
+        put(buf, buf);
+      }
     }
   }
   if (part.tail) {
@@ -734,7 +818,9 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
 #pragma unroll
       for (int x = 0; x < QB; ++x)
         see_bits[x] = (uint32_t)(near_bits(step, mask_words[tq[x]]) >> (16 * lg)) & 0xffffu;
-      compute(0, a.scale_log2, 1.f, std::true_type{});
+      with_k(0);
+      weigh(a.scale_log2, 1.f, std::true_type{});
+      with_v(0, std::true_type{});
     } while (near_next(&step, a.T));
   }
 
@@ -860,11 +946,11 @@ static hipError_t launch_quant_t(const QuantAttnArgs& a, int rows_wg, hipStream_
   else if (rows_wg == 32)
     launch((quant_narrow_kernel<T, S, D, 2>), grid, dim3(64 * kNarrowWaves), 0, st, a);
   else if (rows_wg == 64)
-    launch((quant_wide_kernel<T, S, D, 1, 4, true>), grid, dim3(256), 0, st, a);
+    launch((quant_wide_kernel<T, S, D, 1, 4, true, false>), grid, dim3(256), 0, st, a);
   else if (rows_wg == 128)
-    launch((quant_wide_kernel<T, S, D, 2, 4, kLo>), grid, dim3(256), 0, st, a);
+    launch((quant_wide_kernel<T, S, D, 2, 4, kLo, false>), grid, dim3(256), 0, st, a);
   else
-    launch((quant_wide_kernel<T, S, D, 2, 8, kLo>), grid, dim3(512), 0, st, a);
+    launch((quant_wide_kernel<T, S, D, 2, 8, kLo, true>), grid, dim3(512), 0, st, a);
   if (!a.direct && !a.arrived)
     launch((tree_merge_kernel<T, D>), dim3((a.B * a.Hkv * a.M + 3) / 4), dim3(256), 0, st, static_cast<const TreeArgs&>(a));
   return hipGetLastError();

@@ -51,16 +51,6 @@ constexpr float kPRise<_Float16> = 1.f;
 // (exact where they are near) and scaled after.  Below, by one fma.
 constexpr float kTreeFar = 4194304.f;
 
-// Lane i's value and lane i ^ 16's (32's), the larger; NaN where either is.
-__device__ __forceinline__ float maximum_xor16(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float maximum_xor32(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
 // Up to 16 rows per KV head: one wave per part, its own tiles.  K comes in
 // registers as the matrix operand, V through LDS for the transposing reads; the
 // next tile's loads are issued as soon as a tile's registers are consumed.

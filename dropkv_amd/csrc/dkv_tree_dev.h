@@ -58,6 +58,16 @@ __device__ __forceinline__ typename Elem<T>::v8 tree_load8(const T* p) {
   return __builtin_bit_cast(typename Elem<T>::v8, *reinterpret_cast<const Raw*>(p));
 }
 
+// Lane i's value and lane i ^ 16's (32's), the larger; NaN where either is.
+__device__ __forceinline__ float maximum_xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float maximum_xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // Sequence b's stored rows.  The host keeps 0 <= n <= C; the clamp keeps every
 // access in bounds.
 __device__ __forceinline__ int tree_rows(const TreeArgs& a, int b) {
