@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
   // alone, the compiler has two (64 cycles of products under a latency of 130, which was
   // 1000 of a stage's 4400 cycles).
   auto ahead = [&](auto reads, auto products) __attribute__((always_inline)) {
-    constexpr int R = decltype(reads)::value, M = decltype(products)::value, kAhead = 8, kEach = M / R;
+    constexpr int R = decltype(reads)::value, M = decltype(products)::value, kAhead = R < 16 ? 4 : 8, kEach = M / R;
     __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
     for (int i = 0; i < R - kAhead; ++i) {
@@ -770,8 +770,10 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
         fetch(j + 1);
         __syncthreads();
         with_k(buf);
+        ahead(std::integral_constant<int, kOps>{}, std::integral_constant<int, 8 * KC * QB>{});
         weigh(mul, vscale, std::false_type{});
         with_v(buf, std::false_type{});
+        ahead(std::integral_constant<int, kOps>{}, std::integral_constant<int, (2 * DT + 2) * QB * (LO ? 2 : 1)>{});
         buf ^= 1;
         mul = ks * a.scale_log2;
         vscale = vs;
