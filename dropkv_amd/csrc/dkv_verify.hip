@@ -204,11 +204,12 @@ __global__ void __launch_bounds__(kVfThreads) verify_stats_kernel(VerifyArgs a) 
     if (m == -INFINITY) {  // nothing but -inf so far, or NaN
 #pragma unroll
       for (int e = 0; e < kVfElems; ++e) s += v[e] == v[e] ? 0. : (double)v[e];
-    } else if (fabs((double)m * a.mul) < 0x1p40) {
+    } else if (fabs((double)m * a.mul) < 0x1p27) {
       // Against 2^R, R the whole 32nds next to m's exponent, so that a product's 32nds
       // and its rest (exact) take one operation each.  (2^-990 of the largest and below
       // are all 2^-990, which no sum notices: cheaper than a zero each.  A NaN stays
-      // one.)
+      // one.  In fp32 `least` is off by up to 2^-24 of m, 8 powers of two here; beyond,
+      // it might be m itself.)
       const float least = m - a.deep;
       const double R = ((double)m * a.mul + kVfRound) - kVfRound, round = kVfRound - R;
       double sum = 0.;
@@ -522,7 +523,7 @@ static VerifyPlan verify_plan(int64_t B, int64_t T, int64_t V, bool draft) {
   VerifyPlan p;
   p.S = (int)((tiles + per - 1) / per);
   p.seg = (int)std::min<int64_t>(per * kVfTile, INT32_MAX - kVfTile);
-  p.bytes = kSyncBytes + 256 + (size_t)rows * p.S * sizeof(VfPart) + 
+  p.bytes = kSyncBytes + 256 + (size_t)rows * p.S * sizeof(VfPart) +
             (size_t)B * (sizeof(VfSeq) + (size_t)((V + kVfPiece - 1) / kVfPiece) * 16);
   return p;
 }

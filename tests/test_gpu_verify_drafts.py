@@ -207,3 +207,27 @@ def test_graph_replays_and_streams(gpu):
             other = ops.verify_drafts(x2, tok2, u2, y2)
         torch.cuda.synchronize()
         assert torch.equal(other.choice, out.choice)
+
+
+@pytest.mark.parametrize("temperature,top", [(1e-6, 2.0 ** 17), (3e-9, 100.0), (3e-9, -100.0), (1e-12, 100.0), (1e-12, 1.0),
+                                             (1e-29, 3.0), (2e-5, 2.0 ** 12), (1e-3, 2.0 ** 17)])
+def test_temperatures_next_to_zero(gpu, temperature, top):
+    """Logits a step of fp32 below the largest, where that is thousands of powers of two:
+    the largest ones share all of the probability."""
+    from dropkv_amd import ops
+    step = abs(top) * 2.0 ** -23
+    k = torch.randint(1, 4, (4, 3, 5000), generator=torch.Generator().manual_seed(1))
+    k[:, :, 77::1000] = 0
+    x = (top - k.double() * step * 2).float().to(gpu)
+    gap = 2 * step / temperature
+    u = torch.tensor([0.0, 0.9, 0.0]).repeat(4, 1).to(gpu)
+    u[:, 0] = torch.tensor([0.0, 0.25, 0.65, 0.99])
+    tok = torch.full((4, 3), 78, device=gpu)
+    got = ops.verify_drafts(x, tok, u, None, temperature)
+    if gap > 800:
+        assert (got.accepted == 1).all() and got.choice[:, 0].tolist() == [77, 1077, 3077, 4077]
+        torch.testing.assert_close(got.logprobs[:, 0].cpu().double(), torch.full((4,), -math.log(5.0), dtype=torch.float64),
+                                   rtol=2.0 ** -22, atol=2.0 ** -22)
+    else:  # (differences of a step are exact in 64 bits)
+        lp = torch.log_softmax((x[:, 0].double() - top) / temperature, -1).gather(1, got.choice[:, :1].clamp(min=0))[:, 0]
+        torch.testing.assert_close(got.logprobs[:, 0].double(), lp, rtol=2.0 ** -22, atol=2.0 ** -22)
