@@ -264,7 +264,8 @@ int dropkv_set_tail_select(int mode, int64_t spin_polls, int64_t spin_polls_b);
  * no timers).  dropkv_timing_enable(1) makes every later dropkv_scores /
  * dropkv_select / dropkv_compact / dropkv_compact2 / dropkv_evict /
  * dropkv_evict_ld / dropkv_append / dropkv_decode_attention / dropkv_tree_* /
- * dropkv_norm_rope / dropkv_token_logprobs call on the calling thread launch its kernels with
+ * dropkv_norm_rope / dropkv_token_logprobs / dropkv_quant_* / dropkv_verify_drafts
+ * call on the calling thread launch its kernels with
  * hipExtLaunchKernel and a (start, stop) event pair each, which the runtime
  * sets to that dispatch's own begin and end time stamps.  dropkv_timing_read
  * waits for the last kernel of the most recent such call, writes the
@@ -551,9 +552,9 @@ int dropkv_quant_read(const dropkv_quant_read_args* args, void* stream);
  * and sums are fp32; the stored values enter the products as they are.  The weights
  * enter the product with V in two parts (16 bits or more) up to Hq / Hkv * T = 64
  * rows a KV head, and for fp16; for bf16 they may enter it rounded once beyond.
- * Values of V below 2^118.  The workspace as for dropkv_tree_attention, but that its
- * first DROPKV_SYNC_BYTES must be zero when it is first used; every call leaves them
- * zero. */
+ * The largest magnitude of V times the number of keys below 2^118.  The workspace as
+ * for dropkv_tree_attention, but that its first DROPKV_SYNC_BYTES must be zero when it
+ * is first used; every call leaves them zero. */
 typedef struct {
   const void* q;
   int64_t q_s[3];
@@ -604,9 +605,8 @@ int dropkv_quant_attention(const dropkv_quant_attention_args* args, void* stream
  *   accepted [B] int32: how many; logprobs [B, T] fp32: ln p of each, then 0
  * A sampled row that holds +inf or NaN, or only -inf, gives -1 and NaN.
  * 1 <= T <= 256, V <= 2^26, 1e-30 < temperature < 1e30, B * (2 T - 1) < 2^17,
- * B * V < 2^33.  The
- * workspace's first DROPKV_SYNC_BYTES must be zero when it is first used, and every call
- * leaves them zero. */
+ * B * V < 2^33.  The workspace's first DROPKV_SYNC_BYTES must be zero when it is first
+ * used, and every call leaves them zero. */
 typedef struct {
   const void* logits;
   int64_t x_s[2];
