@@ -98,6 +98,8 @@ hipError_t launch_scores(const ScorePlan& p, int dtype, int D, const void* q, in
 // (ScorePlan::off_sync): zero when a workspace is first used, and zero again
 // after every call (the DROPKV_SYNC_BYTES contract of the C ABI).
 constexpr size_t kSyncBytes = 4096;
+// The distance (in words) of `n` of them: cache lines of their own while they last.
+inline int sync_stride(int64_t n) { return n <= 32 ? 32 : n <= 1024 ? (int)(1024 / n) : 1; }
 hipError_t launch_debug_state(const ScorePlan& p, const char* ws, int D, float* lse_out, float* y_out,
                               hipStream_t st);
 // The generic scoring kernels on the same plan's workspace; no fused pooling.

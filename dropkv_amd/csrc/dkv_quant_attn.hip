@@ -30,7 +30,8 @@ struct QuantAttnArgs : TreeArgs {  // (kbuf, vbuf: the 8-bit blocks)
   const float* vs;
   const void* ktail;  // [B, Hkv, 128, D]
   const void* vtail;
-  uint32_t* arrived;  // [B, Hkv]: parts done, where the last one to arrive joins them; else null
+  uint32_t* arrived;  // [B, Hkv] at arrived_s: parts done, where the last one to arrive joins them; else null
+  int arrived_s;
 };
 
 struct QuantCut {
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
   __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    last = atomicInc(a.arrived + bh, (uint32_t)part.count - 1u) == (uint32_t)part.count - 1u;
+    last = atomicInc(a.arrived + bh * a.arrived_s, (uint32_t)part.count - 1u) == (uint32_t)part.count - 1u;
     if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   }
   __syncthreads();
@@ -1005,6 +1006,7 @@ hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* 
   a.scale_log2 = (float)p.scale * 1.4426950408889634f;
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
   if (pl.one) a.arrived = reinterpret_cast<uint32_t*>(ws);
+  a.arrived_s = sync_stride(p.B * p.Hkv);
   a.deal = reinterpret_cast<int*>(ws + kSyncBytes);
   a.part_m = reinterpret_cast<float*>(ws + kSyncBytes + kTreeDealBytes);
   a.part_l = a.part_m + pl.rows;

@@ -60,7 +60,8 @@ struct VerifyArgs {
   float deep;             // 990 / mul
   VfPart* part;           // [B, T, S], then [B, T - 1, S] of the drafts
   VfSeq* seq;             // [B]
-  uint32_t* arrived;      // [B]: workgroups done, of a call in two kernels
+  uint32_t* arrived;      // [B] at arrived_s: workgroups done, of a call in two kernels
+  int arrived_s;
   double* sums;           // [B, pieces, 2]: of the weights, and of p alone
   int64_t* choice;        // [B, T]
   int* accepted;          // [B]
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(kVfWide) verify_rest_kernel(VerifyArgs a) {
   __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    last = atomicInc(a.arrived + b, (uint32_t)a.groups - 1u) == (uint32_t)a.groups - 1u;
+    last = atomicInc(a.arrived + b * a.arrived_s, (uint32_t)a.groups - 1u) == (uint32_t)a.groups - 1u;
     if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   }
   __syncthreads();
@@ -565,6 +566,7 @@ hipError_t launch_verify_drafts(const dropkv_verify_drafts_args& p, hipStream_t 
   a.deep = (float)(990. / a.mul);
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
   a.arrived = reinterpret_cast<uint32_t*>(ws);
+  a.arrived_s = sync_stride(p.B);
   ws += kSyncBytes;
   a.part = reinterpret_cast<VfPart*>(ws);
   a.seq = reinterpret_cast<VfSeq*>(a.part + (size_t)p.B * (p.draft_logits ? 2 * p.T - 1 : p.T) * pl.S);
