@@ -7,9 +7,10 @@ Public API (same names and semantics as the reference modules
 * :class:`DropKVCache`, :func:`prefill_chunked` -- the evicting cache;
 * :mod:`dropkv_amd.ops` -- lower-level ops (scores, select, compact,
   compact2, EvictPlan for one-call layer eviction; tree_attention,
-  tree_commit, norm_rope and token_logprobs for drafted tokens);
+  tree_commit, norm_rope, token_logprobs and verify_drafts for drafted tokens;
+  quant_cache, quant_append, quant_read and quant_attention for a cache in 8 bits);
 * :class:`dropkv_amd.decode.CompressedDecoder` -- decoding on the compressed
-  cache, one token or a tree of drafted ones per forward.
+  cache, in 16 or 8 bits, one token or a tree of drafted ones per forward.
 """
 
 from .dropkv_cache import DropKVCache, prefill_chunked

@@ -483,11 +483,16 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
 // block of K and V is read, and turned into operands, once for all of them.  LDS holds
 // the operands of a stage of 64 keys as the lanes read them, 16 bytes a lane, 1 KB a
 // product; the next stage's bytes are on their way in registers while the waves
-// compute, and go to the other of two buffers: one barrier a stage.  V's scale goes
-// into the reference of the exponent (P is 2^(x - m + log2 vs)), and is taken out of
-// the weights' sum.  P is rounded once for bf16 in workgroups of 128 rows and more, in
-// two parts otherwise.  Bound by the matrix cores and the ALUs in turn: 4 x 64 heads of
-// 26214 rows, 64 tokens, 221 us (995 TFLOP/s), of which 11 are the join.
+// compute, and go to another buffer.  V's scale goes into the reference of the exponent
+// (P is 2^(x - m + log2 vs)), and is taken out of the weights' sum.  P is rounded once
+// for bf16 in workgroups of 128 rows and more, in two parts otherwise.
+// 64 or 128 rows: one barrier a stage, and the two workgroups of a CU overlap.  256 rows
+// (PAIR): two groups of four waves, half a stage apart.
+// Bound by the matrix cores and the ALUs, which share the issue of a SIMD and the clock
+// that the power leaves: 4 x 64 heads of 26214 rows, 64 tokens, 204 to 217 us by the box
+// (1080 to 1010 TFLOP/s; 231 with all waves in step), of which 11 are the join; the
+// matrix cores are busy 55% of the time, the ALUs 62%.  16 tokens of 32/8 heads over 3276
+// rows: 13 us, two kernels' latencies (9 and 4).
 template <typename T, typename S, int D, int QB, int NW, bool LO, bool PAIR>
 __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a) {
   typedef typename Elem<T>::v8 v8;

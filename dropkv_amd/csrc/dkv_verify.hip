@@ -17,9 +17,10 @@
 // bits and 8 others.  32 entries of 8 bytes are one for each pair of LDS banks: no lanes
 // wait for one another.
 //
-// Bound by that arithmetic: the pass over 136 rows of 151936 in bf16 takes 18.5 us,
-// whose bytes take 8 (26 us with one sum over |f| <= 1/2, 45 operations); over 704 rows
-// of 32003 in fp32 18.6, whose bytes take 17.
+// Bound by that arithmetic: the pass over 136 rows of 151936 in bf16 takes 18.3 us,
+// whose bytes take 8 (26 us with one sum over |f| <= 1/2, 45 operations): 25 operations
+// an element in all, of four cycles each, are 13.5 us.  Over 704 rows of 32003 in fp32 it
+// takes 19 to 21, whose bytes take 17.
 //
 // First the maximum and sum of every row, in segments; then the walk, the sums of the
 // weights that are sampled, over pieces of the one row of each sequence, and the token:
@@ -485,8 +486,9 @@ __global__ void __launch_bounds__(kVfWide) verify_token_kernel(VerifyArgs a) {
 
 // The three in one, for short chains: each workgroup of a sequence makes the walk for
 // itself, and the last one to arrive draws the token (its counter is zero before the
-// call and wraps to zero).  8 nodes of one sequence: 8.1 us
-// where the three kernels take 12 and their gaps; 8 sequences of 9 13.2 either way.
+// call and wraps to zero).  8 nodes of one sequence: 8.1 us where the three kernels take
+// 12 and their gaps, of which 3.8 are a kernel that does nothing, 1.5 the walk and the
+// sums and 2.8 the token, each step a round trip of memory; 8 sequences of 9: 12.7.
 template <typename T>
 __global__ void __launch_bounds__(kVfWide) verify_rest_kernel(VerifyArgs a) {
   __shared__ uint64_t table[kVfTable];
