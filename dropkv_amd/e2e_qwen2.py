@@ -107,6 +107,7 @@ def run(args) -> dict:
     from transformers import DynamicCache
 
     dev = torch.device("cuda:0")
+    cache_dtype = getattr(args, "cache_dtype", None)  # (callers of before have no such field)
     cfg = make_config(num_hidden_layers=args.layers)
     model = build_model(cfg, dev, seed=args.seed)
     ids = random_prompt(cfg.vocab_size, args.prompt, seed=args.seed + 1, device=dev)
@@ -126,7 +127,7 @@ def run(args) -> dict:
             tok, t_pre = _timed(lambda: prefill(model, ids, cache))
             if kind == "dropkv":
                 dec, t_setup = _timed(lambda: CompressedDecoder(model, cache, args.decode,
-                                                                cache_dtype=args.cache_dtype))
+                                                                cache_dtype=cache_dtype))
                 out, t_dec = _timed(lambda: dec.generate(tok, args.decode))
                 stored, logical = int(dec.n_rows.flatten()[0]), int(dec.pos[0, 0])
                 del dec
@@ -148,8 +149,8 @@ def run(args) -> dict:
         }
         if kind == "dropkv":
             res[kind]["decode"] = ("CompressedDecoder: HIP graph per step, " + (
-                "dropkv_decode_attention" if args.cache_dtype is None else
-                f"dropkv_quant_attention on rows in {args.cache_dtype}"))
+                "dropkv_decode_attention" if cache_dtype is None else
+                f"dropkv_quant_attention on rows in {cache_dtype}"))
             res[kind]["decode_setup_ms"] = statistics.median(setup_ms)
         else:
             res[kind]["decode"] = "eager Transformers forward per step (SDPA, torch.cat append)"

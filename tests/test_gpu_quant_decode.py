@@ -208,3 +208,14 @@ def test_refusals(gpu, tiny):
         plain.step(tok)
     with pytest.raises(RuntimeError, match="capacity"):
         plain.step(tok)
+
+
+@pytest.mark.parametrize("fields", [{}, {"cache_dtype": None}, {"cache_dtype": "int8"}])
+def test_the_command(gpu, fields):
+    """The end-to-end command's function, also from callers that name no cache dtype."""
+    import argparse
+    from dropkv_amd import e2e_qwen2
+    res = e2e_qwen2.run(argparse.Namespace(prompt=512, decode=4, layers=2, keep_ratio=0.1, window=8, kernel_size=11, reps=1,
+                                           warmup=0, seed=0, compare=False, **fields))["dropkv"]
+    assert res["logical_length"] == 516 and res["stored_kv_rows_layer0"] == 51 + 4
+    assert ("int8" in res["decode"]) == ("int8" in fields.values())
