@@ -878,7 +878,8 @@ struct QuantPlan {
 //   or, if longer, K and V at 5.2 TB/s, where 8 MB or a quarter of them are in flight,
 //   and longer where the workgroups do not divide the CUs (of more than 30 MB);
 // - the partial rows, written and read at 4 TB/s, and a round trip of the joining
-//   kernel for every 16 (D = 128) or 32 parts;
+//   kernel for every 16 (D = 128) or 32 parts; of one part, whose workgroup writes the
+//   output, neither, but the new tokens' steps behind the blocks';
 // - the kernels' fixed part.
 struct QuantShape {
   int rows;
@@ -890,7 +891,7 @@ constexpr QuantShape kQuantShapes[] = {
 
 constexpr int64_t kOneJoin = 8192;  // elements
 
-static double quant_cost(const QuantShape& w, double heads, double M, double D, double blocks, int64_t S) {
+static double quant_cost(const QuantShape& w, double heads, double M, double D, double T, double blocks, int64_t S) {
   const double wgs = heads * std::ceil(M / w.rows) * S, wide = D / 128;
   const bool narrow = w.rows <= 32;
   const double per = std::ceil((blocks + narrow) / S), load = wgs / (256.0 * w.per_cu);
@@ -904,7 +905,9 @@ static double quant_cost(const QuantShape& w, double heads, double M, double D, 
   const double bytes = heads * blocks * kQBlock * D * 2;
   double stream = bytes / 5.2e6 / std::min(1.0, flight / std::max(1.0, std::min(8e6, bytes / 4)));
   if (bytes > 3e7) stream *= 0.5 + 0.5 * std::ceil(wgs / 256) * 256 / wgs;
-  const double join = narrow && S == 1 ? -2.5 : S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16);
+  const double join = S > 1    ? S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16)
+                      : narrow ? -2.5
+                               : -2. + 2. * wide * (std::ceil(T / kQBlock) - 1);
   return std::max(steps * block, stream) + join + w.fixed_us;
 }
 
@@ -923,7 +926,7 @@ static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
     const int64_t tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kTreeMaxSplits, 256 / chunks, 512 / chunks};
     for (int64_t S : tries) {
       S = std::max<int64_t>(1, std::min(S, most));
-      const double cost = quant_cost(w, (double)heads, p.M, (double)D, (double)blocks, S);
+      const double cost = quant_cost(w, (double)heads, p.M, (double)D, (double)T, (double)blocks, S);
       if (p.S == 0 || cost < best) {
         best = cost;
         p.S = (int)S;
@@ -932,7 +935,7 @@ static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
     }
   }
   p.MC = (p.M + p.rows_wg - 1) / p.rows_wg;
-  p.apart = p.rows_wg == 64 || (p.rows_wg > 64 && heads * p.MC * p.S < 192);
+  p.apart = p.S > 1 && (p.rows_wg == 64 || (p.rows_wg > 64 && heads * p.MC * p.S < 192));
   p.P = (int)(B * (p.S + p.apart));
   // (What one workgroup reads in a round trip.)
   p.one = p.rows_wg <= 32 && p.S > 1 && p.S <= 16 && heads <= (int64_t)(kSyncBytes / sizeof(uint32_t)) && p.S * p.M * D <= kOneJoin;
