@@ -871,8 +871,9 @@ struct QuantPlan {
   size_t rows, bytes;
 };
 
-// An estimate of a call's time in us, from sweeps of both over calls of 4 to 512 rows
-// per KV head, 700 to 60,000 keys and 2 to 64 heads.  The sum of
+// An estimate of a call's time in us, from sweeps of both over calls of 1 to 512 rows
+// per KV head, 2 to 60,000 keys and 2 to 64 heads (the host knows the capacity, not
+// the rows).  The sum of
 // - the longest workgroup's blocks, a block's time by the rows (narrow: a wave's, every
 //   fourth), 0.6 of it at D = 64, and longer where workgroups share a CU or take turns;
 //   or, if longer, K and V at 5.2 TB/s, where 8 MB or a quarter of them are in flight,
@@ -907,7 +908,7 @@ static double quant_cost(const QuantShape& w, double heads, double M, double D, 
   if (bytes > 3e7) stream *= 0.5 + 0.5 * std::ceil(wgs / 256) * 256 / wgs;
   const double join = S > 1    ? S * heads * M * D * 8 / 4e6 + 0.6 * std::ceil((S + 1) * wide / 16)
                       : narrow ? -2.5
-                               : -2. + 2. * wide * (std::ceil(T / kQBlock) - 1);
+                               : -3. + 2. * wide * (std::ceil(T / kQBlock) - 1);
   return std::max(steps * block, stream) + join + w.fixed_us;
 }
 
