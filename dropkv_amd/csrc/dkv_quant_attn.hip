@@ -43,8 +43,11 @@ struct QuantCut {
 constexpr float kQRise = 8.f;
 
 // Weights are 2^(x mul - m + log2 vs) by one fma, vs the scale of the block's values.
-// From here on (in powers of two) m's own rounding would lift them far above 1: there the
-// difference of the two rounded logits is taken first, the larger one itself among them.
+// From here on (in powers of two) m's own rounding would lift them far above 1, or lose
+// them: there the difference of the two rounded logits is taken first, the larger one
+// itself among them.  (Both rounded: `weigh` is compiled without contraction, which would
+// make one fma of a logit's product and the difference, and at 2^29 the largest weight
+// anything from 2^-32 to 2^32.)
 constexpr float kQFar = 4194304.f;
 
 // A step of 16-bit keys: the `held` rows of the tail (rows first ..), then `fresh`
@@ -201,6 +204,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
   // From products (times `mul`: logits) to weights times the values' scale, 2^up = 1 /
   // down; `seen`: a bit for each of the lane's keys.
   auto weigh = [&](int x, float mul, float up, float down, uint32_t seen) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
     float tmax = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -606,6 +610,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
   };
   // The logits are the products times `mul`; the weights come times vscale.
   auto weigh = [&](float mul, float vscale, auto near) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
     constexpr bool kNear = decltype(near)::value;
     typedef std::conditional_t<kNear, T, __bf16> VT;
     typedef typename Elem<VT>::v8 vv8;
