@@ -162,6 +162,7 @@ __device__ __forceinline__ void vf_load(const T* x, int j, int hi, float* v) {
 
 // e^((v - m) / temperature); 0 below 2^-1000.
 __device__ __forceinline__ double vf_weight(float v, float m, double mul, const uint64_t* table) {
+#pragma clang fp contract(off)
   const double z = ((double)v - (double)m) * mul, e = exp2_64(z, table);
   return z < -1000. ? 0. : e;
 }
@@ -307,9 +308,14 @@ __device__ __forceinline__ VfSeq vf_walk(const VerifyArgs& a, int b, bool write,
 }
 
 // Weights of N places from j on of the sampled row: of what is left of p, and of p.
+// (Each operation rounded by itself, here and in vf_weight.  A difference of products by
+// fma would leave the rounding of one of them, 2^-54 of p, on tokens that both models
+// hold equally likely, and u_0 = 0 would draw the first of those.  And a piece that has a
+// weight here for its sum has it again where its tokens are looked at one by one.)
 template <typename T, int N>
 __device__ __forceinline__ void vf_weights(const VerifyArgs& a, int b, const VfSeq& q, int j, int hi, const uint64_t* table,
                                            float* v, double* w, double* p) {
+#pragma clang fp contract(off)
   constexpr int EPV = 16 / (int)sizeof(T);
   float z[N];
   const T* x = static_cast<const T*>(a.x) + b * a.x_sb + q.last * a.x_st;
