@@ -98,8 +98,15 @@ hipError_t launch_scores(const ScorePlan& p, int dtype, int D, const void* q, in
 // (ScorePlan::off_sync): zero when a workspace is first used, and zero again
 // after every call (the DROPKV_SYNC_BYTES contract of the C ABI).
 constexpr size_t kSyncBytes = 4096;
-// The distance (in words) of `n` of them: cache lines of their own while they last.
-inline int sync_stride(int64_t n) { return n <= 32 ? 32 : n <= 1024 ? (int)(1024 / n) : 1; }
+// `n` counters there, `stride` words apart (cache lines of their own while they last);
+// null where they do not fit.  A workspace may begin anywhere: they are what lies in
+// whole words of its first kSyncBytes, not of those behind an aligned address.
+inline uint32_t* sync_counters(const void* workspace, int64_t n, int* stride) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(workspace), at = (begin + 3) & ~(uintptr_t)3;
+  const int64_t words = (int64_t)((begin + kSyncBytes - at) / sizeof(uint32_t));
+  *stride = (int)(words / n < 32 ? words / n : 32);
+  return *stride ? reinterpret_cast<uint32_t*>(at) : nullptr;
+}
 hipError_t launch_debug_state(const ScorePlan& p, const char* ws, int D, float* lse_out, float* y_out,
                               hipStream_t st);
 // The generic scoring kernels on the same plan's workspace; no fused pooling.

@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
 // sequence, and whether the 16-bit keys are parts of their own.
 struct QuantPlan {
   int M, rows_wg, MC, S, P, apart;
-  int one;  // the last workgroup of a KV head joins its parts
+  int one;  // the last workgroup of a KV head joins its parts (where there are counters)
   size_t rows, bytes;
 };
 
@@ -944,7 +944,7 @@ static QuantPlan quant_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
   p.apart = p.S > 1 && (p.rows_wg == 64 || (p.rows_wg > 64 && heads * p.MC * p.S < 192));
   p.P = (int)(B * (p.S + p.apart));
   // (What one workgroup reads in a round trip.)
-  p.one = p.rows_wg <= 32 && p.S > 1 && p.S <= 16 && heads <= (int64_t)(kSyncBytes / sizeof(uint32_t)) && p.S * p.M * D <= kOneJoin;
+  p.one = p.rows_wg <= 32 && p.S > 1 && p.S <= 16 && p.S * p.M * D <= kOneJoin;
   p.rows = (size_t)Hkv * p.P * p.M;
   p.bytes = kSyncBytes + kTreeDealBytes + p.rows * sizeof(float) * (2 + (size_t)D) + 256;
   return p;
@@ -1019,8 +1019,7 @@ hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* 
   a.div_t = Div::of(a.T);
   a.scale_log2 = (float)p.scale * 1.4426950408889634f;
   char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
-  if (pl.one) a.arrived = reinterpret_cast<uint32_t*>(ws);
-  a.arrived_s = sync_stride(p.B * p.Hkv);
+  if (pl.one) a.arrived = sync_counters(p.workspace, p.B * p.Hkv, &a.arrived_s);
   a.deal = reinterpret_cast<int*>(ws + kSyncBytes);
   a.part_m = reinterpret_cast<float*>(ws + kSyncBytes + kTreeDealBytes);
   a.part_l = a.part_m + pl.rows;

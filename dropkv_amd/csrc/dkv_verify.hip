@@ -61,7 +61,7 @@ struct VerifyArgs {
   float deep;             // 990 / mul
   VfPart* part;           // [B, T, S], then [B, T - 1, S] of the drafts
   VfSeq* seq;             // [B]
-  uint32_t* arrived;      // [B] at arrived_s: workgroups done, of a call in two kernels
+  uint32_t* arrived;      // [B] at arrived_s: workgroups done, of a call in two kernels; null: they do not fit
   int arrived_s;
   double* sums;           // [B, pieces, 2]: of the weights, and of p alone
   int64_t* choice;        // [B, T]
@@ -542,7 +542,7 @@ template <typename T>
 static hipError_t launch_verify_t(const VerifyArgs& a, hipStream_t st) {
   const int rows = a.B * (a.y ? 2 * a.T - 1 : a.T);
   launch(verify_stats_kernel<T>, dim3((unsigned)(rows * a.S)), dim3(kVfThreads), 0, st, a);
-  if (a.T <= kVfShort && a.B <= (int)(kSyncBytes / sizeof(uint32_t))) {
+  if (a.T <= kVfShort && a.arrived) {
     launch(verify_rest_kernel<T>, dim3((unsigned)(a.B * a.groups)), dim3(kVfWide), 0, st, a);
   } else {
     launch(verify_walk_kernel<T>, dim3(a.B), dim3(kVfWide), 0, st, a);
@@ -572,10 +572,8 @@ hipError_t launch_verify_drafts(const dropkv_verify_drafts_args& p, hipStream_t 
   a.groups = (a.pieces + kVfWide / 64 - 1) / (kVfWide / 64);
   a.mul = 1.4426950408889634074 / p.temperature;
   a.deep = (float)(990. / a.mul);
-  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15);
-  a.arrived = reinterpret_cast<uint32_t*>(ws);
-  a.arrived_s = sync_stride(p.B);
-  ws += kSyncBytes;
+  a.arrived = sync_counters(p.workspace, p.B, &a.arrived_s);
+  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.workspace) + 15) & ~(uintptr_t)15) + kSyncBytes;
   a.part = reinterpret_cast<VfPart*>(ws);
   a.seq = reinterpret_cast<VfSeq*>(a.part + (size_t)p.B * (p.draft_logits ? 2 * p.T - 1 : p.T) * pl.S);
   a.sums = reinterpret_cast<double*>(a.seq + p.B);
