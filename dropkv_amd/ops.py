@@ -748,7 +748,12 @@ def quant_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor, n_rows: to
     (``dropkv_quant_append``).  ``counts`` [B] int32: so many rows of each sequence
     (else all L); ``path`` [B, L] int32: row i is row ``path[b, i]`` (what
     ``tree_commit`` returns).  Rows beyond the capacity are dropped.  k and v must
-    not lie in the cache's own buffers."""
+    not lie in the cache's own buffers.
+
+    ``n_rows`` may be set back to a multiple of 64, to a row of the block that is not
+    full, and to where the last append began if that was of 64 rows or fewer.
+    Elsewhere the block's 16-bit rows are not those of the rows before the count,
+    and nothing reports it."""
     index = _quant_device("quant_append", cache, k, v, n_rows, path, counts)
     if _differentiating():
         _no_grad("quant_append", k, v, *cache)

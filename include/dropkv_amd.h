@@ -506,7 +506,12 @@ int dropkv_token_logprobs(const dropkv_token_logprobs_args* args, void* stream);
  * Rows that would lie beyond the capacity (and all where n is negative) are left
  * out.  Blocks that are filled up are written once, from the tail and the new
  * rows.  The same call again, at the same n, gives the same cache as long as no
- * more than 64 rows are appended.  N * B * H * ceil((63 + L) / 64) < 2^23. */
+ * more than 64 rows are appended.  N * B * H * ceil((63 + L) / 64) < 2^23.
+ * A count may be set back to a multiple of 64, to a row of the block that is not
+ * full, and to where the last append began if that was of 64 rows or fewer; to no
+ * other place: the rows of a full block that came with the call that filled it are
+ * in 8 bits alone, and its 16-bit rows would be taken for others' (which nothing
+ * reports). */
 typedef struct {
   const void* k_new;
   int64_t kn_s[4];
