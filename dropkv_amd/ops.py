@@ -1078,7 +1078,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     its chain), ``uniforms`` [B, T] fp32 in [0, 1): entry i judges node i, entry 0
     draws the last token.  ``draft_logits`` [B, T - 1, V], of the logits' dtype: row i
     - 1 is what node i was drawn from; without it the drafts are taken as given (a
-    lookup's).  Both are divided by ``temperature``.  ``choice`` is what
+    lookup's).  Both are divided by ``temperature``.  (fp32 ``uniforms`` come in steps
+    of up to 2^-24, and the distribution is the model's to about that much.)  ``choice`` is what
     ``tree_commit`` takes."""
     index = _device_index("verify_drafts", logits, tokens, uniforms, draft_logits)
     if _differentiating():

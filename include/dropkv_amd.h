@@ -532,9 +532,9 @@ typedef struct {
 int dropkv_quant_append(const dropkv_quant_append_args* args, void* stream);
 
 /* dropkv_quant_read: rows row0 .. row0 + L - 1 of every head to k_out / v_out
- * [N, B, H, L, D] contiguous (16-byte aligned), of dtype: s q rounded once where the
- * row's block is full, the row as it was appended where it is not, zeros from row
- * n on.  row0 + L <= capacity. */
+ * [N, B, H, L, D] contiguous (16-byte aligned), of dtype: the fp32 product s q, rounded
+ * to dtype, where the row's block is full, the row as it was appended where it is not,
+ * zeros from row n on.  row0 + L <= capacity. */
 typedef struct {
   const void* k;
   const void* v;
@@ -557,7 +557,9 @@ int dropkv_quant_read(const dropkv_quant_read_args* args, void* stream);
  * and sums are fp32; the stored values enter the products as they are.  The weights
  * enter the product with V in two parts (16 bits or more) up to Hq / Hkv * T = 64
  * rows a KV head, and for fp16; for bf16 they may enter it rounded once beyond.
- * The largest magnitude of V times the number of keys below 2^118.  The workspace as
+ * The largest magnitude of V times the number of keys below 2^118; of a block whose
+ * values of V are all below 2^-80, weights below 2^-17 of a part's largest may be left
+ * out (fp32's range: V's scale goes into the weights).  The workspace as
  * for dropkv_tree_attention, but that its first DROPKV_SYNC_BYTES must be zero when it
  * is first used; every call leaves them zero. */
 typedef struct {
@@ -604,7 +606,8 @@ int dropkv_quant_attention(const dropkv_quant_attention_args* args, void* stream
  * while u_i q(x_i) < p(x_i).  After the last node that stands a token is drawn from
  * max(p - q, 0) where a node failed there (from p where that is 0 everywhere or NaN),
  * else from p: the lowest whose running sum, in order, exceeds u_0 times the whole.
- * Weights and sums are in 64 bits.
+ * Weights and sums are in 64 bits; the random numbers are fp32, whose steps near 1 are
+ * 2^-24: what is drawn has the model's distribution to about that much.
  *   choice   [B, T] int64: the token after each node that stands (the next node's, and
  *            last the one drawn), then -1: what dropkv_tree_commit takes
  *   accepted [B] int32: how many; logprobs [B, T] fp32: ln p of each, then 0
