@@ -157,11 +157,9 @@ int64_t logprob_max_top();
 size_t logprob_workspace_bytes(int64_t N, int64_t V, int64_t top);
 hipError_t launch_token_logprobs(const dropkv_token_logprobs_args& p, hipStream_t st);
 
-// A cache in 8 bits (dkv_quant.hip, dkv_quant_attn.hip); the workgroups of a call.
+// A cache in 8 bits (dkv_quant.hip, dkv_quant_attn.hip).
 constexpr int kStoreInt8 = 4, kStoreE4m3 = 5;
-int64_t quant_append_groups(int64_t N, int64_t B, int64_t H, int64_t L);
 hipError_t launch_quant_append(const dropkv_quant_append_args& p, hipStream_t st);
-int64_t quant_read_groups(int64_t N, int64_t B, int64_t H, int64_t L, int64_t row0);
 hipError_t launch_quant_read(const dropkv_quant_read_args& p, hipStream_t st);
 size_t quant_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t C);
 hipError_t launch_quant_attention(const dropkv_quant_attention_args& p, size_t* need, hipStream_t st);

@@ -234,9 +234,6 @@ __global__ void __launch_bounds__(256) quant_read_kernel(QuantReadArgs a) {
   }
 }
 
-int64_t quant_append_groups(int64_t N, int64_t B, int64_t H, int64_t L) {
-  return 2 * N * B * H * std::max<int64_t>(1, (kQBlock - 1 + L) / kQBlock);
-}
 hipError_t launch_quant_append(const dropkv_quant_append_args& p, hipStream_t st) {
   QuantAppendArgs a{};
   a.to = QuantStore{{static_cast<uint8_t*>(p.k), static_cast<uint8_t*>(p.v)}, {p.k_scale, p.v_scale}, {p.k_tail, p.v_tail}};
@@ -260,16 +257,13 @@ hipError_t launch_quant_append(const dropkv_quant_append_args& p, hipStream_t st
   a.C = (int)p.capacity;
   // (n % 64 rows of a block, then L: so many blocks can be filled up.)
   a.slots = (int)std::max<int64_t>(1, (kQBlock - 1 + p.L) / kQBlock);
-  const dim3 grid((unsigned)quant_append_groups(p.N, p.B, p.H, p.L));
+  const dim3 grid((unsigned)(2 * p.N * p.B * p.H * a.slots));
   return quant_types(p.dtype, p.store, p.D, [&](auto t, auto s, auto d) {
     launch((quant_append_kernel<decltype(t), decltype(s), decltype(d)::value>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
   });
 }
 
-int64_t quant_read_groups(int64_t N, int64_t B, int64_t H, int64_t L, int64_t row0) {
-  return 2 * N * B * H * ((row0 + L - 1) / kQBlock - row0 / kQBlock + 1);
-}
 hipError_t launch_quant_read(const dropkv_quant_read_args& p, hipStream_t st) {
   QuantReadArgs a{};
   a.from = QuantStore{{static_cast<uint8_t*>(const_cast<void*>(p.k)), static_cast<uint8_t*>(const_cast<void*>(p.v))},
@@ -286,7 +280,7 @@ hipError_t launch_quant_read(const dropkv_quant_read_args& p, hipStream_t st) {
   a.C = (int)p.capacity;
   a.row0 = (int)p.row0;
   a.slots = (int)((p.row0 + p.L - 1) / kQBlock - p.row0 / kQBlock + 1);
-  const dim3 grid((unsigned)quant_read_groups(p.N, p.B, p.H, p.L, p.row0));
+  const dim3 grid((unsigned)(2 * p.N * p.B * p.H * a.slots));
   return quant_types(p.dtype, p.store, p.D, [&](auto t, auto s, auto d) {
     launch((quant_read_kernel<decltype(t), decltype(s), decltype(d)::value>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
