@@ -21,8 +21,8 @@ drafted tokens may be verified by sampling instead, from given random numbers
 (``dropkv_verify_drafts``).
 
 With ``cache_dtype`` the rows are held in 8 bits with a scale for each block of 64
-rows and head: half the memory, and half the bytes that a step reads
-(``dropkv_quant_append``, ``dropkv_quant_attention``).
+rows and head: half the bytes that a step reads of the cache, and half its memory but for
+128 rows a head in 16 bits (``dropkv_quant_append``, ``dropkv_quant_attention``).
 """
 
 from __future__ import annotations
