@@ -42,6 +42,16 @@ struct QuantCut {
 // reference that its weights are taken against before it turns what it has summed.
 constexpr float kQRise = 8.f;
 
+// Weights of 16-bit keys enter their products in the element type, and fp16 ends at 2^-24:
+// there they are 2^14 times as large, so that weights from 2^-22 on hold 16 bits in two
+// parts, and the outputs' sums are for as long.  (The wide kernel's maximum may then rise
+// by no more than 1: the largest weight is 2^15.  Without it a value of 1000 at a weight
+// of 2^-19 came out up to 1% off.)
+template <typename T>
+constexpr int kNearLift = std::is_same<T, _Float16>::value ? 14 : 0;
+template <typename T>
+constexpr float kNearRise = std::is_same<T, _Float16>::value ? 1.f : kQRise;
+
 // Weights are 2^(x mul - m + log2 vs) by one fma, vs the scale of the block's values.
 // From here on (in powers of two) m's own rounding would lift them far above 1, or lose
 // them: there the difference of the two rounded logits is taken first, the larger one
@@ -290,6 +300,12 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
     const int v_row = lane / CPR, v_col = 8 * (lane % CPR);
     T* vt = reinterpret_cast<T*>(lds);
     Near step = near_begin(part.n, a.T);
+    constexpr float kLift = 1 << kNearLift<T>;
+    if (kLift != 1.f)
+#pragma unroll
+      for (int x = 0; x < RT; ++x)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= kLift;
 #pragma unroll 1
     do {  // (one wave: its own LDS operations stay in order)
       v8 kop[4][KC][2], vch[kQBlock / GRP];
@@ -326,7 +342,7 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
 #pragma unroll
       for (int x = 0; x < RT; ++x) {
         const uint64_t bits = near_bits(step, mask_words[tq[x]]);
-        weigh(x, a.scale_log2, 0.f, 1.f, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
+        weigh(x, a.scale_log2, kNearLift<T>, 1.f / kLift, (uint32_t)(bits >> (16 * lg)) & 0xffffu);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -348,6 +364,11 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
           }
         }
     } while (near_next(&step, a.T));
+    if (kLift != 1.f)
+#pragma unroll
+      for (int x = 0; x < RT; ++x)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= 1.f / kLift;
   }
 
   // The waves' results joined: 16 threads a row.
@@ -612,6 +633,7 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
   auto weigh = [&](float mul, float vscale, auto near) __attribute__((always_inline)) {
 #pragma clang fp contract(off)
     constexpr bool kNear = decltype(near)::value;
+    constexpr float kRise = kNear ? kNearRise<T> : kQRise;
     typedef std::conditional_t<kNear, T, __bf16> VT;
     typedef typename Elem<VT>::v8 vv8;
     float top[QB];
@@ -625,12 +647,12 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
 #pragma unroll
       for (int e = 1; e < 16; ++e) tmax = __builtin_elementwise_maximum(tmax, s[x][e / 4][e % 4]);
       top[x] = maximum_xor32(maximum_xor16(tmax)) * mul;
-      turn |= top[x] - m[x] > kQRise;
+      turn |= top[x] - m[x] > kRise;
     }
     if (wave_any(turn)) {
 #pragma unroll
       for (int x = 0; x < QB; ++x) {
-        const float mnew = top[x] - m[x] > kQRise ? top[x] : m[x], alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
+        const float mnew = top[x] - m[x] > kRise ? top[x] : m[x], alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
         lsum[x] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[x][dt] *= alpha;
@@ -638,8 +660,8 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
       }
     }
     // (A block of zeros has no scale: any will do.)
-    const float fold = vscale == 0.f ? 1.f : vscale, up = __builtin_amdgcn_logf(fold);
-    down = __builtin_amdgcn_rcpf(fold);
+    const float fold = vscale == 0.f ? 1.f : vscale, up = kNear ? (float)kNearLift<T> : __builtin_amdgcn_logf(fold);
+    down = kNear ? 1.f / (1 << kNearLift<T>) : __builtin_amdgcn_rcpf(fold);
     float by = mul, less[QB];
     bool far = false;
 #pragma unroll
@@ -798,6 +820,12 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
     const T* kn = static_cast<const T*>(a.kn) + (int64_t)b * a.kn_sb + (int64_t)hkv * a.kn_sh;
     const T* vn = static_cast<const T*>(a.vn) + (int64_t)b * a.vn_sb + (int64_t)hkv * a.vn_sh;
     Near step = near_begin(tree_rows(a, b), a.T);
+    constexpr float kLift = 1 << kNearLift<T>;
+    if (kLift != 1.f)
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= kLift;
     constexpr int NK = kOps * 64 / NT, CPR = D / 8, NV = kQBlock * CPR / NT;
 #pragma unroll 1
     do {
@@ -832,9 +860,14 @@ __global__ void __launch_bounds__(64 * NW, 2) quant_wide_kernel(QuantAttnArgs a)
       for (int x = 0; x < QB; ++x)
         see_bits[x] = (uint32_t)(near_bits(step, mask_words[tq[x]]) >> (16 * lg)) & 0xffffu;
       with_k(0);
-      weigh(a.scale_log2, 1.f, std::true_type{});
+      weigh(a.scale_log2, kLift, std::true_type{});
       with_v(0, std::true_type{});
     } while (near_next(&step, a.T));
+    if (kLift != 1.f)
+#pragma unroll
+      for (int x = 0; x < QB; ++x)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= 1.f / kLift;
   }
 
 #pragma unroll
