@@ -514,8 +514,8 @@ __global__ void __launch_bounds__(64 * kNarrowWaves, RT == 1 ? 2 : 1) quant_narr
 // 64 or 128 rows: one barrier a stage, and the two workgroups of a CU overlap.  256 rows
 // (PAIR): two groups of four waves, half a stage apart.
 // Bound by the matrix cores and the ALUs, which share the issue of a SIMD and the clock
-// that the power leaves: 4 x 64 heads of 26214 rows, 64 tokens, 204 to 217 us by the box
-// (1080 to 1010 TFLOP/s; 231 with all waves in step), of which 11 are the join; the
+// that the power leaves: 4 x 64 heads of 26214 rows, 64 tokens, 204 to 222 us by the box
+// (1080 to 990 TFLOP/s; 231 with all waves in step), of which 11 are the join; the
 // matrix cores are busy 55% of the time, the ALUs 62%.  16 tokens of 32/8 heads over 3276
 // rows: 13 us, two kernels' latencies (9 and 4).
 template <typename T, typename S, int D, int QB, int NW, bool LO, bool PAIR>
